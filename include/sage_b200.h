@@ -347,6 +347,87 @@ int sage_attention_varlen(const void* q, const void* k, const void* v, void* out
  * Returns the number of entries written (11). */
 int sage_workspace_layout(int64_t B, int64_t H, int64_t N, size_t offsets[11]);
 
+/* ---- A quantised, paged K/V cache ------------------------------------------------------------------
+ *
+ * For programs that generate tokens: new keys and values are quantised once, as they are written, and
+ * read by every later step in one byte per element.  The reference has no cache; its callers quantise the
+ * whole K and V again with every call.  The codes and scales are the quantiser's: the bits that
+ * sage_prologue gives for the same rows.
+ *
+ *   k_codes   (pages, Hkv, page_size, width)  int8 (SAGE_QK_INT8) or e4m3 (SAGE_QK_E4M3) codes of K
+ *   k_scale   (pages, Hkv, page_size)         fp32, one per token and head
+ *   v_codes   (pages, Hkv, page_size, width)  e4m3 codes of V
+ *   v_scale   (pages, Hkv, page_size)         fp32
+ *   k_shift   optional (Hkv, width) fp32, zero in columns past head_dim: subtracted from K before it is
+ *             quantised (smooth_k's mean, taken once and kept), added again by sage_cache_read.  Attention
+ *             does not change by it, but for the LSE, which sage_cache_attention corrects
+ * width is 64 for head_dim up to 64 and 128 above (columns past head_dim hold code 0); page_size a power of
+ * two, 16 .. 256; head_dim a multiple of 8, 8 .. 128.  The buffers are contiguous and 16-byte aligned, and
+ * zeroed once when they are made (codes that nothing wrote must not be the e4m3 NaN).  Every device array
+ * of indexes (slots, page tables, lengths) is the caller's promise, but none can lead outside the buffers. */
+
+/* New rows into the cache: token i of k and v (tokens, Hkv, head_dim), (token, head) strides in elements, goes
+ * to slot slots[i] = page * page_size + offset (int32, or int64 with slots_64).  A slot below 0 or past the
+ * last page: the token is left out (padding).  Slots of one call are distinct; where two tokens name the same
+ * one, each half of its row comes from either.  A row that holds a NaN or an infinity is stored with codes 0 and
+ * scale NaN: it reads back as NaN throughout, and no code is ever a NaN, so that a key behind a mask reaches
+ * nothing. */
+int sage_cache_write(const void* k, const void* v, const void* slots, int slots_64,
+                     void* k_codes, float* k_scale, void* v_codes, float* v_scale, const float* k_shift,
+                     int64_t tokens, int64_t Hkv, int64_t head_dim, int64_t pages, int64_t page_size,
+                     const int64_t k_strides[2], const int64_t v_strides[2], int dtype, int qk_mode, void* stream);
+
+/* Sequences of the cache, packed, in 16 bits: rows cu_seqlens[i] .. cu_seqlens[i+1] of k_out and v_out
+ * (total, Hkv, head_dim) receive the first tokens of sequence i, whose pages are page_table[i] (int32, n_seq rows
+ * of page_table_width entries, page_table_stride apart).  Value = code * scale (+ shift), rounded once.  Rows
+ * before cu_seqlens[0] and from cu_seqlens[n_seq] on are left as they are; tokens on a page that does not exist
+ * read as zeros. */
+int sage_cache_read(const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
+                    const float* k_shift, const int32_t* page_table, int64_t page_table_stride,
+                    int64_t page_table_width, const int32_t* cu_seqlens, void* k_out, void* v_out,
+                    int64_t n_seq, int64_t total, int64_t Hkv, int64_t head_dim, int64_t pages, int64_t page_size,
+                    const int64_t k_strides[2], const int64_t v_strides[2], int dtype, int qk_mode, void* stream);
+
+/* Attention of new tokens over the cache.
+ *   q, out      packed (total_q, Hq, head_dim), (token, head) strides in elements; sequence i has the rows
+ *               cu_seqlens_q[i] .. cu_seqlens_q[i+1], at most max_q of them (further rows are not written);
+ *               cu_seqlens_q null: max_q rows for every sequence
+ *   lse         optional (total_q, Hq) fp32: ln sum exp(sm_scale * q.k) over the keys a row sees
+ *   seqlens_k   (n_seq) int32: cached keys of each sequence, its new tokens' own among them (they are the last
+ *               ones, written before this call); cut off at page_table_width * page_size
+ *   tree_mask   optional (total_q, max_q) bytes, rows tree_stride apart: row t sees new token j of its sequence
+ *               where tree_mask[t, j] is not 0, and all keys before the new tokens.  Null: a chain, row t sees
+ *               the keys up to its own token's
+ * A row that sees no key is 0, its LSE -infinity.  Keys on a page that does not exist are not seen.  Scores and
+ * sums in fp32; the weights of V are rounded to fp16.  What a result depends on: the keys are walked in
+ * stretches whose ends follow from the lengths of all sequences, so that the same sequence in another batch
+ * may differ in the order of fp32 sums; the same call gives the same bits.
+ *   workspace   sage_cache_attention_workspace_bytes() bytes, 256-byte aligned; calls that may run at the same
+ *               time (on two streams, in two captured graphs) each need their own */
+size_t sage_cache_attention_workspace_bytes(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q);
+int sage_cache_attention(const void* q, void* out, float* lse,
+                         const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
+                         const float* k_shift, const int32_t* page_table, int64_t page_table_stride,
+                         int64_t page_table_width, const int32_t* seqlens_k, const int32_t* cu_seqlens_q,
+                         const void* tree_mask, int64_t tree_stride, void* workspace, size_t workspace_bytes,
+                         int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t total_q, int64_t max_q, int64_t head_dim,
+                         int64_t pages, int64_t page_size, const int64_t q_strides[2], const int64_t o_strides[2],
+                         int dtype, int qk_mode, float sm_scale, void* stream);
+
+/* Rotary positions on q (B, Hq, N, head_dim) and, if k is not null, on k (B, Hk, N, head_dim): pair i of the first
+ * rotary_dim columns (columns i and i + rotary_dim / 2, or 2i and 2i + 1 with `interleaved`) of the row at position
+ * p turns by the angle p * inv_freq[i], scaled by `magnitude`; the other columns are copied.  `backward` applies
+ * the transposed map, which takes the gradient of the outputs to that of the inputs.
+ *   positions   (B, N) int32, or int64 with positions_64; pos_strides are (batch, row), 0 allowed
+ *   inv_freq    rotary_dim / 2 doubles in device memory; angles are worked out in 64 bits
+ *   strides     (batch, head, row) in elements; the outputs may be the inputs, with the same strides
+ * rotary_dim: a multiple of 8, 8 .. head_dim. */
+int sage_rotary(const void* q, void* q_out, const void* k, void* k_out, const void* positions, int positions_64,
+                const double* inv_freq, float magnitude, int64_t B, int64_t Hq, int64_t Hk, int64_t N,
+                int64_t head_dim, int64_t rotary_dim, int interleaved, int backward,
+                const int64_t q_strides[3], const int64_t qo_strides[3], const int64_t k_strides[3],
+                const int64_t ko_strides[3], const int64_t pos_strides[2], int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

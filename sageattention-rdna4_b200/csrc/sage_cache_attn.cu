@@ -1,0 +1,740 @@
+// Attention of new tokens over a quantised, paged K/V cache (layout: sage_cache.cu): one token per
+// sequence, a chain of them (each sees the keys up to its own), or a tree of drafted tokens (a mask says
+// which of them each sees).
+//
+// Rows.  The Hq / Hkv query heads of a K/V head share its keys, so the rows of a unit are the pairs
+// (new token, query head of the group), token by token; up to 8 * NB rows make a row tile.
+//
+// Products.  The cache is read in its one-byte codes and the 16-bit products take them exactly: int8 and
+// e4m3 codes are both fp16 numbers.  Scores are transposed, S^T = K Q^T, and so is the output, O^T = V^T P^T:
+// the 16-row operand of mma.m16n8k16 is then 16 keys (or 16 columns of V), and the 8-column one is 8 query
+// rows, so that a single query row wastes 7 of 8 columns and not 15 of 16 rows.  The inner dimension of a
+// product may be walked in any order, if both operands walk it alike:
+//   S^T   lane (g = lane / 4, c = lane % 4) reads the 32 bytes c of key rows g and g + 8; its k-step s is
+//         bytes 4s .. 4s+3 of them, and Q is laid out to match
+//   O^T   lane (g, c) reads the 16 bytes g of the keys 2c, 2c+1, 2c+8, 2c+9 and pairs the bytes of two keys;
+//         its rows of step j are the columns 16g + 2j and 16g + 2j + 1 of V
+// so that every shared-memory read is 16 bytes wide and no code is moved between lanes.  16-byte pieces of a
+// row are stored at piece ^ (row & 7), which spreads both reads over all banks.
+//
+// Numerics.  Q in fp16: bf16 rows are scaled by a power of two each, which is undone in the score's factor, so
+// that no bit is lost but in elements 2^-28 below their row's largest.  Scores, maxima, sums and outputs in
+// fp32.  A weight enters the second product as fp16(p * v_scale * N), where N is a factor per row that keeps the
+// largest one seen near 1 (fp16 has 11 bits there; its relative error, 2^-11, is that of the output format).
+// The running maximum moves only when a score passes it by 2^8, and N when a product passes 2^12: p stays
+// below 2^8, the accumulator is rarely touched, and neither the sums nor the 11 bits lose anything by it.
+//
+// Work.  The tiles of 64 keys of all (sequence, K/V head, row tile) units are numbered in one line, and every CTA
+// takes an equal stretch of it, so that ragged batches and single long sequences alike fill the GPU; lengths are
+// read on the device.  A unit that lies in several stretches leaves partial rows in the workspace, which
+// cache_combine_kernel joins in the order of the keys.  Each warp walks 16 of the 64 keys of every tile by itself
+// through its own ring of cp.async stages: no barrier but at the end of a unit, and no spinning wait.
+#include <algorithm>
+
+#include "sage_common.cuh"
+#include "sage_internal.h"
+
+namespace sage {
+
+namespace {
+
+constexpr int CA_WARPS = 4, CA_THREADS = 32 * CA_WARPS;
+constexpr int CA_KEYS = 64;                    // keys of a tile: 16 per warp
+constexpr float LN2_F = 0.6931471805599453f;
+constexpr float NO_MAX = -3.0e38f;
+
+struct CacheAttnKArgs {
+  const void* q;
+  void* out;
+  float* lse;
+  const uint8_t *kc, *vc;
+  const float *ks, *vs, *shift;
+  const int *table, *seqlens, *cu_q;
+  const uint8_t* tree;
+  float* part_o;             // (2 x CTAs, rows of a tile, WIDTH)
+  float2* part_ml;           // (2 x CTAs, rows of a tile): running maximum (log2 domain), sum
+  long long q_st, q_sh, o_st, o_sh, table_st, tree_st;
+  long long total_q;
+  int n_seq, table_width, pages, page_shift, Hq, Hkv, group, max_q, D;
+  int ctas;                  // of the attention kernel: the line of tiles is cut into so many stretches
+  float sm_scale, scale_log2;
+};
+
+// A sequence as the kernels see it: lengths clamped, so that no access leaves the tensors whatever the arrays hold.
+struct Seq {
+  int q0, q_len, len;
+};
+__device__ __forceinline__ Seq seq_of(const CacheAttnKArgs& a, int b) {
+  Seq s;
+  if (a.cu_q == nullptr) {                           // max_q new tokens for every sequence
+    s.q0 = b * a.max_q;
+    s.q_len = a.max_q;
+  } else {
+    const long long q0 = min(max((long long)__ldg(a.cu_q + b), 0LL), a.total_q);
+    s.q0 = (int)q0;
+    s.q_len = (int)min(max(min((long long)__ldg(a.cu_q + b + 1), a.total_q) - q0, 0LL), (long long)a.max_q);
+  }
+  s.len = (int)min(max((long long)__ldg(a.seqlens + b), 0LL), (long long)a.table_width << a.page_shift);
+  return s;
+}
+__device__ __forceinline__ int row_tiles(const CacheAttnKArgs& a, const Seq& s, int rows) { return (s.q_len * a.group + rows - 1) / rows; }
+__device__ __forceinline__ int key_tiles(const Seq& s) { return max(1, (s.len + CA_KEYS - 1) / CA_KEYS); }   // an empty sequence's rows are written too
+
+// The line of tiles: sequence by sequence, K/V head by head, row tile by row tile, key tile by key tile.
+// All threads of a CTA call this: the length of the line, the sequence in which the CTA's stretch begins, and
+// the number of tiles before that sequence.
+struct Place {
+  long long total, before;
+  int b;
+};
+template <int THREADS>
+__device__ Place find_place(const CacheAttnKArgs& a, int rows, long long* sums, int cta) {
+  // sums: THREADS / 32 + 4 words of shared memory
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto tiles_of = [&](int b) -> long long {
+    if (b >= a.n_seq) return 0;
+    const Seq s = seq_of(a, b);
+    return (long long)a.Hkv * row_tiles(a, s, rows) * key_tiles(s);
+  };
+  long long mine = 0;
+  for (int b = tid; b < a.n_seq; b += THREADS) mine += tiles_of(b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sums[warp] = mine;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) total += sums[w];
+  __syncthreads();
+  Place p;
+  p.total = total; p.before = 0; p.b = a.n_seq;
+  const long long per = (total + a.ctas - 1) / a.ctas;
+  const long long want = (long long)cta * per;
+  if (want >= total) return p;
+  long long base = 0;
+  for (int b0 = 0; b0 < a.n_seq; b0 += THREADS) {
+    const long long n = tiles_of(b0 + tid);
+    long long upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) sums[warp] = upto;
+    if (tid == 0) sums[THREADS / 32] = -1;
+    __syncthreads();
+    long long before = base, all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += sums[w];
+      all += sums[w];
+    }
+    before += upto - n;
+    if (n > 0 && want >= before && want < before + n) { sums[THREADS / 32] = b0 + tid; sums[THREADS / 32 + 1] = before; }
+    __syncthreads();
+    const long long found = sums[THREADS / 32];
+    if (found >= 0) {
+      p.b = (int)found;
+      p.before = sums[THREADS / 32 + 1];
+      __syncthreads();
+      return p;
+    }
+    base += all;
+    __syncthreads();
+  }
+  return p;
+}
+
+// A position on the line.
+struct Cursor {
+  Seq s;
+  int b, h, rt, kt;          // sequence, K/V head, row tile, key tile
+  int n_rt, n_kt;
+};
+__device__ __forceinline__ void enter_seq(const CacheAttnKArgs& a, Cursor& c, int rows) {
+  c.s = seq_of(a, c.b);
+  c.n_rt = row_tiles(a, c.s, rows);
+  c.n_kt = key_tiles(c.s);
+}
+__device__ __forceinline__ void next_tile(const CacheAttnKArgs& a, Cursor& c, int rows) {
+  if (++c.kt < c.n_kt) return;
+  c.kt = 0;
+  if (++c.rt < c.n_rt) return;
+  c.rt = 0;
+  if (++c.h < a.Hkv) return;
+  c.h = 0;
+  do {
+    if (++c.b >= a.n_seq) return;
+    enter_seq(a, c, rows);
+  } while (c.n_rt == 0);
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  const int bytes = there ? 16 : 0;                  // 0: filled with zeros, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float lds_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float fast_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// Two e4m3 codes (the low 16 bits) -> two fp16.
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3);
+  return (uint32_t)r.x | ((uint32_t)r.y << 16);
+}
+// Four K codes -> two registers of two fp16 each.
+template <bool INT8>
+__device__ __forceinline__ void k_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (INT8) {
+    const uint32_t t = w ^ 0x80808080u;                              // code + 128 in a byte; 0x6400 + it is 1024 + it
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));     // 1024 + 128
+    uint32_t u = __byte_perm(t, 0x64646464u, 0x4140), v = __byte_perm(t, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&u), bias), y = __hsub2(*reinterpret_cast<__half2*>(&v), bias);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    lo = e4m3_pair(w & 0xFFFFu);
+    hi = e4m3_pair(w >> 16);
+  }
+}
+
+// Shared memory of a CTA.
+template <int WIDTH, int NB, int STAGES> struct CaSmem {
+  static constexpr uint32_t CODES = 16 * WIDTH;                      // 16 rows
+  static constexpr uint32_t STAGE = 2 * CODES + 128;                 // K, V, and 16 scales of each
+  static constexpr uint32_t RING = CA_WARPS * STAGES * STAGE;
+  static constexpr int ROW = WIDTH + 4;                              // floats of a merge row (padded against bank conflicts)
+  static constexpr uint32_t OFF_MERGE = RING;                        // (8 NB rows, ROW)
+  static constexpr uint32_t OFF_ML = OFF_MERGE + 8 * NB * ROW * 4;   // (warps, 8 NB rows) of {max, sum, factor}
+  static constexpr uint32_t OFF_PLACE = OFF_ML + CA_WARPS * 8 * NB * 16;
+  static constexpr uint32_t BYTES = OFF_PLACE + 8 * (CA_WARPS + 4);
+};
+
+// sm_scale * (row of Q) . (shift of the K/V head), by one warp
+template <typename T>
+__device__ __forceinline__ float shift_dot(const CacheAttnKArgs& a, const T* q, int h, int width, int lane) {
+  float d = 0.f;
+  for (int i = lane; i < a.D; i += 32) d = fmaf((float)q[i], __ldg(a.shift + (long long)h * width + i), d);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  return d * a.sm_scale;
+}
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// NB: blocks of 8 query rows in a row tile.
+template <typename T, bool INT8, int WIDTH, int NB, int STAGES, int CTAS_PER_SM>
+__global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(const CacheAttnKArgs a) {
+  using L = CaSmem<WIDTH, NB, STAGES>;
+  constexpr int ROWS = 8 * NB, KSTEPS = WIDTH / 16, PIECES = WIDTH / 16;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  allow_successor();
+  const Place place = find_place<CA_THREADS>(a, ROWS, reinterpret_cast<long long*>(smem + L::OFF_PLACE), (int)blockIdx.x);
+  if (place.b >= a.n_seq) return;
+  const long long per = (place.total + a.ctas - 1) / a.ctas, first = (long long)blockIdx.x * per;
+  const int n_tiles = (int)min(per, place.total - first);
+  Cursor cur;
+  cur.b = place.b;
+  enter_seq(a, cur, ROWS);
+  {
+    const long long rest = first - place.before, unit = rest / cur.n_kt;
+    cur.kt = (int)(rest - unit * cur.n_kt);
+    cur.h = (int)(unit / cur.n_rt);
+    cur.rt = (int)(unit - (long long)cur.h * cur.n_rt);
+  }
+  Cursor ahead = cur;                                // the tile whose loads are issued next
+  const uint32_t ring = smem_addr(smem) + warp * STAGES * L::STAGE;
+
+  // this warp's 16 keys of the tile at `ahead` into stage s
+  auto issue = [&](int s) {
+    const int key0 = ahead.kt * CA_KEYS + 16 * warp;
+    const uint32_t st = ring + s * L::STAGE;
+    const int pi = key0 >> a.page_shift;
+    int page = -1;
+    if (key0 < ahead.s.len && pi < a.table_width) page = __ldg(a.table + (long long)ahead.b * a.table_st + pi);
+    const bool there = page >= 0 && page < a.pages;
+    const long long row = there ? ((((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key0 & ((1 << a.page_shift) - 1))) : 0;
+#pragma unroll
+    for (int i = 0; i < 16 * PIECES / 32; ++i) {
+      const int r = (i * 32 + lane) / PIECES, p = (i * 32 + lane) % PIECES;
+      const int swz = WIDTH == 128 ? p ^ (r & 7) : p ^ ((r >> 1) & 3);
+      const uint32_t dst = st + r * WIDTH + 16 * swz;
+      const long long src = row * WIDTH + r * WIDTH + 16 * p;
+      copy16(dst, a.kc + src, there);
+      copy16(dst + L::CODES, a.vc + src, there);
+    }
+    if (there) {
+      if (lane < 8) copy16(st + 2 * L::CODES + 16 * lane, (lane < 4 ? a.ks : a.vs) + row + 4 * (lane & 3), true);
+    } else if (lane < 16) {                          // no such keys: a scale below zero says so
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 2 * L::CODES + 4 * lane), "f"(-1.0f) : "memory");
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 2 * L::CODES + 64 + 4 * lane), "f"(0.0f) : "memory");
+    }
+  };
+  int issued = 0;
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    if (issued < n_tiles) { issue(s); next_tile(a, ahead, ROWS); ++issued; }
+    copy_commit();
+  }
+
+  uint32_t qf[NB][KSTEPS][2];                        // Q^T: k-step s of query row 8 nb + g
+  float row_c[NB][2];                                // score factor of rows 8 nb + 2c + {0, 1}
+  int row_lim[NB][2], row_tok[NB][2];                // keys that a row may see; its token within the sequence
+  float m[NB][2], l[NB][2], nf[NB][2];               // running maximum, this lane's sum, factor N
+  float o[NB][KSTEPS][4];                            // O^T: columns 16g + 2j + {0, 1} of rows 8 nb + 2c + {0, 1}
+  int plain_end = 0;                                 // keys below this need no mask
+
+  int stage = 0;
+  bool fresh = true;
+  for (int t = 0; t < n_tiles; ++t) {
+    if (fresh) {
+      fresh = false;
+      const int live = min(ROWS, cur.s.q_len * a.group - cur.rt * ROWS);      // rows of this tile that exist
+      const int ctx = cur.s.len - cur.s.q_len;
+      const int t_first = cur.rt * ROWS / a.group;
+      plain_end = a.tree ? max(ctx, 0) : max(0, min(cur.s.len, ctx + t_first + 1));
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        // Q rows: lane (g, c) holds columns c * WIDTH / 4 .. of row 8 nb + g
+        const int r = 8 * nb + g, rr = cur.rt * ROWS + r;
+        const int tok = rr / a.group, head = cur.h * a.group + rr - tok * a.group;
+        const T* src = reinterpret_cast<const T*>(a.q) + (long long)(cur.s.q0 + tok) * a.q_st + (long long)head * a.q_sh;
+        float x[WIDTH / 4], amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < WIDTH / 32; ++i) {
+          const int col = c * (WIDTH / 4) + 8 * i;
+          uint4 u = make_uint4(0u, 0u, 0u, 0u);
+          if (r < live && col < a.D) u = __ldg(reinterpret_cast<const uint4*>(src + col));
+          unpack8<T>(u, x + 8 * i);
+        }
+        float back = 1.f;                            // what undoes the row's power of two
+        if (sizeof(T) == 2 && !__is_same(T, __half)) {
+#pragma unroll
+          for (int i = 0; i < WIDTH / 4; ++i) amax = fmaxf(amax, fabsf(x[i]));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          // amax -> [2^14, 2^15): the exponent field of 2^(14 - e) is 127 + 14 - e = 268 - field(amax)
+          const int field = (int)(__float_as_uint(amax) >> 23);
+          if (field > 14 && field < 255) {
+            const int f = min(254, 268 - field);
+            const float up = __uint_as_float((uint32_t)f << 23);
+#pragma unroll
+            for (int i = 0; i < WIDTH / 4; ++i) x[i] *= up;
+            back = f <= 253 ? __uint_as_float((uint32_t)(254 - f) << 23) : 5.877471754111438e-39f;
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s) {
+          const __half2 u = __floats2half2_rn(x[4 * s], x[4 * s + 1]), v = __floats2half2_rn(x[4 * s + 2], x[4 * s + 3]);
+          qf[nb][s][0] = *reinterpret_cast<const uint32_t*>(&u);
+          qf[nb][s][1] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          // rows 2c + e sit with lane g' = 2c + e of the Q fragments
+          row_c[nb][e] = a.scale_log2 * __shfl_sync(0xffffffffu, back, 4 * (2 * c + e));
+          const int r2 = 8 * nb + 2 * c + e, tok2 = (cur.rt * ROWS + r2) / a.group;
+          row_tok[nb][e] = tok2;
+          row_lim[nb][e] = r2 < live ? (a.tree ? cur.s.len : min(cur.s.len, ctx + tok2 + 1)) : 0;
+          m[nb][e] = NO_MAX; l[nb][e] = 0.f; nf[nb][e] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nb][j][e] = 0.f;
+      }
+    }
+
+    // the stage that was read last is free: fetch into it
+    __syncwarp();
+    if (issued < n_tiles) {
+      issue(stage == 0 ? STAGES - 1 : stage - 1);
+      next_tile(a, ahead, ROWS);
+      ++issued;
+    }
+    copy_commit();
+    copy_wait<STAGES - 1>();
+    __syncwarp();
+
+    const uint32_t st = ring + stage * L::STAGE;
+    const int key0 = cur.kt * CA_KEYS + 16 * warp;
+    // ---- S^T = K Q^T
+    float s[NB][4];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[nb][e] = 0.f;
+#pragma unroll
+    for (int half = 0; half < WIDTH / 64; ++half) {
+      // 16 bytes of rows g and g + 8: four k-steps
+      uint32_t r0[4], r1[4];
+      {
+        const int p = WIDTH == 128 ? (2 * c + half) ^ (g & 7) : c ^ ((g >> 1) & 3);
+        const uint4 u = lds16(st + g * WIDTH + 16 * p), v = lds16(st + (g + 8) * WIDTH + 16 * p);
+        r0[0] = u.x; r0[1] = u.y; r0[2] = u.z; r0[3] = u.w;
+        r1[0] = v.x; r1[1] = v.y; r1[2] = v.z; r1[3] = v.w;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t f[4];
+        k_halves<INT8>(r0[i], f[0], f[2]);
+        k_halves<INT8>(r1[i], f[1], f[3]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma16816(s[nb], f, qf[nb][4 * half + i][0], qf[nb][4 * half + i][1]);
+      }
+    }
+    // ---- weights
+    const float sk0 = lds_f32(st + 2 * L::CODES + 4 * g), sk1 = lds_f32(st + 2 * L::CODES + 4 * (g + 8));
+    const float sv0 = lds_f32(st + 2 * L::CODES + 64 + 4 * g), sv1 = lds_f32(st + 2 * L::CODES + 64 + 4 * (g + 8));
+    const bool absent = sk0 < 0.f || sk1 < 0.f;
+    float p[NB][4], w[NB][4];
+    bool over = false;
+    if (key0 + 16 > plain_end || __any_sync(0xffffffffu, absent)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + g + 8 * (e >> 1), x = e & 1;
+          bool seen = key < row_lim[nb][x] && !((e >> 1) ? sk1 < 0.f : sk0 < 0.f);
+          if (a.tree != nullptr && seen) {
+            const int j = key - (cur.s.len - cur.s.q_len);
+            if (j >= 0) seen = a.tree[(long long)(cur.s.q0 + row_tok[nb][x]) * a.tree_st + j] != 0;
+          }
+          s[nb][e] = seen ? s[nb][e] * ((e >> 1) ? sk1 : sk0) : -INFINITY;
+        }
+    } else {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) { s[nb][0] *= sk0; s[nb][1] *= sk0; s[nb][2] *= sk1; s[nb][3] *= sk1; }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int x = e & 1;
+        const float d = s[nb][e] == -INFINITY ? -INFINITY : fmaf(s[nb][e], row_c[nb][x], -m[nb][x]);
+        p[nb][e] = fast_ex2(d);
+        // (a masked weight is an exact zero whatever its key's scale holds)
+        w[nb][e] = d == -INFINITY ? 0.f : p[nb][e] * (((e >> 1) ? sv1 : sv0) * nf[nb][x]);
+        over = over || d > 8.f || w[nb][e] > 4096.f;
+      }
+    if (__any_sync(0xffffffffu, over)) {
+      // new maxima and factors; the sums and the accumulator follow
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float top = m[nb][x];
+          const bool none0 = s[nb][x] == -INFINITY, none1 = s[nb][2 + x] == -INFINITY;
+          if (!none0) top = fmaxf(top, s[nb][x] * row_c[nb][x]);
+          if (!none1) top = fmaxf(top, s[nb][2 + x] * row_c[nb][x]);
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
+          const float fade = fast_ex2(m[nb][x] - top);
+          p[nb][x] = none0 ? 0.f : fast_ex2(fmaf(s[nb][x], row_c[nb][x], -top));
+          p[nb][2 + x] = none1 ? 0.f : fast_ex2(fmaf(s[nb][2 + x], row_c[nb][x], -top));
+          float big = fmaxf(none0 ? 0.f : p[nb][x] * sv0, none1 ? 0.f : p[nb][2 + x] * sv1);
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, sh));
+          float n_new = nf[nb][x], scale = fade;
+          if (big > 0.f) {
+            n_new = __fdividef(1.f, big);
+            if (nf[nb][x] > 0.f) {
+              n_new = fminf(n_new, __fdividef(nf[nb][x], fade));       // (fade 0: infinite, the new one counts)
+              scale = fade * __fdividef(n_new, nf[nb][x]);
+            }
+          }
+          m[nb][x] = top;
+          nf[nb][x] = n_new;
+          l[nb][x] *= fade;
+#pragma unroll
+          for (int j = 0; j < KSTEPS; ++j) { o[nb][j][x] *= scale; o[nb][j][2 + x] *= scale; }
+          w[nb][x] = none0 ? 0.f : p[nb][x] * (sv0 * n_new);
+          w[nb][2 + x] = none1 ? 0.f : p[nb][2 + x] * (sv1 * n_new);
+        }
+    }
+    uint32_t pf[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      l[nb][0] += p[nb][0] + p[nb][2];
+      l[nb][1] += p[nb][1] + p[nb][3];
+      const __half2 u = __floats2half2_rn(w[nb][0], w[nb][1]), v = __floats2half2_rn(w[nb][2], w[nb][3]);
+      pf[nb][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&u));
+      pf[nb][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&v));
+    }
+    // ---- O^T += V^T P^T
+    {
+      const uint32_t vt = st + L::CODES;
+      uint32_t x[4][WIDTH / 32];                     // keys 2c, 2c+1, 2c+8, 2c+9: this lane's WIDTH / 8 columns
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 2 * c + (i & 1) + 8 * (i >> 1);
+        if (WIDTH == 128) {
+          const uint4 u = lds16(vt + r * WIDTH + 16 * (g ^ (r & 7)));
+          x[i][0] = u.x; x[i][1] = u.y; x[i][WIDTH / 32 - 2] = u.z; x[i][WIDTH / 32 - 1] = u.w;
+        } else {
+          const uint2 u = lds8(vt + r * WIDTH + 16 * ((g >> 1) ^ ((r >> 1) & 3)) + 8 * (g & 1));
+          x[i][0] = u.x; x[i][1] = u.y;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < WIDTH / 32; ++i) {
+        // bytes 4i .. 4i+3: columns paired over two keys
+        const uint32_t a01 = __byte_perm(x[0][i], x[1][i], 0x5140), a23 = __byte_perm(x[0][i], x[1][i], 0x7362);
+        const uint32_t b01 = __byte_perm(x[2][i], x[3][i], 0x5140), b23 = __byte_perm(x[2][i], x[3][i], 0x7362);
+        const uint32_t f[4] = {e4m3_pair(a01 & 0xFFFFu), e4m3_pair(a01 >> 16), e4m3_pair(b01 & 0xFFFFu), e4m3_pair(b01 >> 16)};
+        const uint32_t h[4] = {e4m3_pair(a23 & 0xFFFFu), e4m3_pair(a23 >> 16), e4m3_pair(b23 & 0xFFFFu), e4m3_pair(b23 >> 16)};
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          mma16816(o[nb][2 * i], f, pf[nb][0], pf[nb][1]);
+          mma16816(o[nb][2 * i + 1], h, pf[nb][0], pf[nb][1]);
+        }
+      }
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+
+    // ---- end of the unit, or of this CTA's stretch of it
+    const bool last_of_unit = cur.kt + 1 == cur.n_kt;
+    if (last_of_unit || t + 1 == n_tiles) {
+      float* merge = reinterpret_cast<float*>(smem + L::OFF_MERGE);
+      float4* ml = reinterpret_cast<float4*>(smem + L::OFF_ML);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float sum = l[nb][x];
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
+          if (g == 0) ml[warp * ROWS + 8 * nb + 2 * c + x] = make_float4(m[nb][x], sum, nf[nb][x], 0.f);
+        }
+      __syncthreads();
+      // the four warps add their shares, one after the other, each weighed against the common maximum
+      for (int wv = 0; wv < CA_WARPS; ++wv) {
+        if (wv == warp) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const int r = 8 * nb + 2 * c + x;
+              float top = NO_MAX;
+#pragma unroll
+              for (int i = 0; i < CA_WARPS; ++i) top = fmaxf(top, ml[i * ROWS + r].x);
+              const float weight = nf[nb][x] > 0.f ? __fdividef(fast_ex2(m[nb][x] - top), nf[nb][x]) : 0.f;
+#pragma unroll
+              for (int j = 0; j < KSTEPS; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float* at = merge + r * L::ROW + (WIDTH / 8) * g + 2 * j + e;
+                  const float v = nf[nb][x] > 0.f ? o[nb][j][2 * e + x] * weight : 0.f;
+                  *at = wv == 0 ? v : *at + v;
+                }
+            }
+        }
+        __syncthreads();
+      }
+      const bool whole = last_of_unit && t + 1 >= cur.n_kt;            // all of the unit's tiles were here
+      const int live = min(ROWS, cur.s.q_len * a.group - cur.rt * ROWS);
+      // the unit began before this stretch: its part is the stretch's first, else its last
+      const long long slot = 2LL * blockIdx.x + (t > cur.kt ? 1 : 0);
+      for (int r = warp; r < live; r += CA_WARPS) {
+        float top = NO_MAX, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < CA_WARPS; ++i) top = fmaxf(top, ml[i * ROWS + r].x);
+#pragma unroll
+        for (int i = 0; i < CA_WARPS; ++i) sum += ml[i * ROWS + r].y * fast_ex2(ml[i * ROWS + r].x - top);
+        if (whole) {
+          const int rr = cur.rt * ROWS + r, tok = rr / a.group, head = cur.h * a.group + rr - tok * a.group;
+          const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+          T* dst = reinterpret_cast<T*>(a.out) + (long long)(cur.s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
+          for (int d = lane; d < a.D; d += 32) dst[d] = from_float<T>(merge[r * L::ROW + d] * inv);
+          if (a.lse != nullptr) {
+            float v = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * LN2_F;
+            if (a.shift != nullptr)
+              v += shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(cur.s.q0 + tok) * a.q_st + (long long)head * a.q_sh, cur.h, WIDTH, lane);
+            if (lane == 0) a.lse[(long long)(cur.s.q0 + tok) * a.Hq + head] = v;
+          }
+        } else {
+          float* dst = a.part_o + (slot * ROWS + r) * WIDTH;
+          for (int d = lane; d < WIDTH; d += 32) dst[d] = merge[r * L::ROW + d];
+          if (lane == 0) a.part_ml[slot * ROWS + r] = make_float2(top, sum);
+        }
+      }
+      __syncthreads();
+      fresh = true;
+    }
+    next_tile(a, cur, ROWS);
+  }
+}
+
+// Joins the parts of the units that lie in several stretches: a CTA per (unit, row), the parts in the order of
+// the keys, four at a time over its four warps.
+template <typename T>
+__global__ void __launch_bounds__(CA_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int width, int max_rt) {
+  __shared__ long long place_s[CA_WARPS + 4];
+  __shared__ float acc_s[CA_WARPS][HD];
+  __shared__ float2 ml_s[CA_WARPS];
+  wait_for_predecessor();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // blockIdx.x = ((sequence * Hkv) + head) * max_rt + row tile; blockIdx.y = row
+  const int rt = (int)(blockIdx.x % (unsigned)max_rt), bh = (int)(blockIdx.x / (unsigned)max_rt), h = bh % a.Hkv, b = bh / a.Hkv;
+  const Seq s = seq_of(a, b);
+  const int r = blockIdx.y, rr = rt * rows + r;
+  if (rr >= s.q_len * a.group) return;
+  // tiles before this sequence, and in all
+  long long before = 0, total = 0;
+  for (int i = tid; i < a.n_seq; i += CA_THREADS) {
+    const Seq x = seq_of(a, i);
+    const long long n = (long long)a.Hkv * row_tiles(a, x, rows) * key_tiles(x);
+    total += n;
+    if (i < b) before += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  long long* place_before = reinterpret_cast<long long*>(acc_s);
+  if (lane == 0) { place_s[warp] = total; place_before[warp] = before; }
+  __syncthreads();
+  total = 0; before = 0;
+#pragma unroll
+  for (int w = 0; w < CA_WARPS; ++w) { total += place_s[w]; before += place_before[w]; }
+  __syncthreads();
+  const long long per = (total + a.ctas - 1) / a.ctas;
+  const int n_kt = key_tiles(s);
+  const long long u0 = before + ((long long)h * row_tiles(a, s, rows) + rt) * n_kt, u1 = u0 + n_kt;
+  const int c0 = (int)(u0 / per), c1 = (int)((u1 - 1) / per);
+  if (c0 == c1) return;                              // written by the CTA that had all of it
+  auto slot_of = [&](int cta) { return 2LL * cta + (u0 > (long long)cta * per ? 1 : 0); };
+  float top = NO_MAX;
+  for (int i = c0 + lane; i <= c1; i += 32) top = fmaxf(top, a.part_ml[slot_of(i) * rows + r].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  const bool mine = 4 * lane < width;
+#pragma unroll 4
+  for (int i = c0 + warp; i <= c1; i += CA_WARPS) {
+    const long long at = slot_of(i) * rows + r;
+    const float2 ml = a.part_ml[at];
+    const float weight = fast_ex2(ml.x - top);
+    sum += ml.y * weight;
+    if (mine) {
+      const float4 v = *reinterpret_cast<const float4*>(a.part_o + at * width + 4 * lane);
+      acc.x = fmaf(v.x, weight, acc.x); acc.y = fmaf(v.y, weight, acc.y); acc.z = fmaf(v.z, weight, acc.z); acc.w = fmaf(v.w, weight, acc.w);
+    }
+  }
+  if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
+  if (lane == 0) ml_s[warp] = make_float2(top, sum);
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < CA_WARPS; ++w) sum += ml_s[w].y;
+  const int tok = rr / a.group, head = h * a.group + rr - tok * a.group;
+  const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+  T* dst = reinterpret_cast<T*>(a.out) + (long long)(s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
+  for (int d = tid; d < a.D; d += CA_THREADS) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < CA_WARPS; ++w) v += acc_s[w][d];
+    dst[d] = from_float<T>(v * inv);
+  }
+  if (a.lse != nullptr && warp == 0) {
+    float v = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * LN2_F;
+    if (a.shift != nullptr)
+      v += shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(s.q0 + tok) * a.q_st + (long long)head * a.q_sh, h, width, lane);
+    if (lane == 0) a.lse[(long long)(s.q0 + tok) * a.Hq + head] = v;
+  }
+}
+
+// Row tiles: 8, 16 or 32 rows, the smallest that holds all rows of a unit.
+int rows_per_tile(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+constexpr int MAX_CTAS = 160 * 3;                    // sized without a device at hand, for the largest SM count an sm_100 part has
+
+template <typename T, bool INT8, int WIDTH, int NB, int STAGES, int CTAS_PER_SM>
+cudaError_t launch_attn(CacheAttnKArgs& a, long long tiles_bound, int max_rt, int sms, cudaStream_t st) {
+  auto kern = cache_attn_kernel<T, INT8, WIDTH, NB, STAGES, CTAS_PER_SM>;
+  constexpr uint32_t smem = CaSmem<WIDTH, NB, STAGES>::BYTES;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  a.ctas = (int)std::min<long long>(std::min(sms * CTAS_PER_SM, MAX_CTAS), tiles_bound);
+  kern<<<a.ctas, CA_THREADS, smem, st>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)((long long)a.n_seq * a.Hkv * max_rt), (unsigned)std::min((long long)8 * NB, (long long)a.max_q * a.group));
+  return launch_after_predecessor(cache_combine_kernel<T>, grid, dim3(CA_THREADS), 0, st, a, 8 * NB, WIDTH, max_rt);
+}
+
+template <typename T, bool INT8, int WIDTH>
+cudaError_t launch_rows(CacheAttnKArgs& a, int rows, long long tiles_bound, int max_rt, int sms, cudaStream_t st) {
+  if (rows == 8) return launch_attn<T, INT8, WIDTH, 1, 3, 3>(a, tiles_bound, max_rt, sms, st);
+  if (rows == 16) return launch_attn<T, INT8, WIDTH, 2, 3, 2>(a, tiles_bound, max_rt, sms, st);
+  return launch_attn<T, INT8, WIDTH, 4, 3, 2>(a, tiles_bound, max_rt, sms, st);
+}
+
+template <typename T>
+cudaError_t launch_type(CacheAttnKArgs& a, const CacheView& c, int rows, long long tiles_bound, int max_rt, int sms, cudaStream_t st) {
+  if (c.width == 64) return c.int8 ? launch_rows<T, true, 64>(a, rows, tiles_bound, max_rt, sms, st) : launch_rows<T, false, 64>(a, rows, tiles_bound, max_rt, sms, st);
+  return c.int8 ? launch_rows<T, true, 128>(a, rows, tiles_bound, max_rt, sms, st) : launch_rows<T, false, 128>(a, rows, tiles_bound, max_rt, sms, st);
+}
+
+}  // namespace
+
+size_t cache_attention_scratch(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q) {
+  (void)n_seq;
+  const size_t rows = (size_t)rows_per_tile(max_q * (Hq / Hkv));
+  return (size_t)2 * MAX_CTAS * rows * (HD * sizeof(float) + sizeof(float2));
+}
+
+cudaError_t launch_cache_attention(const CacheView& c, const CacheAttnParams& p, cudaStream_t st) {
+  CacheAttnKArgs a;
+  a.q = p.q; a.out = p.out; a.lse = p.lse; a.kc = c.k_codes; a.vc = c.v_codes; a.ks = c.k_scale; a.vs = c.v_scale; a.shift = c.k_shift;
+  a.table = p.table; a.seqlens = p.seqlens; a.cu_q = p.cu_q; a.tree = p.tree;
+  a.q_st = p.q_strides[0]; a.q_sh = p.q_strides[1]; a.o_st = p.o_strides[0]; a.o_sh = p.o_strides[1];
+  a.table_st = p.table_stride; a.tree_st = p.tree_stride; a.total_q = p.total_q;
+  a.n_seq = (int)p.n_seq; a.table_width = (int)p.table_width; a.pages = (int)c.pages; a.page_shift = c.page_shift;
+  a.Hq = (int)p.Hq; a.Hkv = (int)c.H; a.group = (int)(p.Hq / c.H); a.max_q = (int)p.max_q; a.D = (int)c.D;
+  a.sm_scale = p.sm_scale; a.scale_log2 = std::min(p.sm_scale * LOG2E_F, 3.0e38f);
+  const int rows = rows_per_tile(p.max_q * a.group);
+  a.part_o = reinterpret_cast<float*>(p.scratch);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * MAX_CTAS * rows * HD);
+  const long long max_rt = (p.max_q * a.group + rows - 1) / rows;
+  const long long tiles_bound = p.n_seq * c.H * max_rt * std::max<long long>(1, ((p.table_width << c.page_shift) + CA_KEYS - 1) / CA_KEYS);
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return p.dtype == 0 ? launch_type<__half>(a, c, rows, tiles_bound, (int)max_rt, sms, st)
+                      : launch_type<__nv_bfloat16>(a, c, rows, tiles_bound, (int)max_rt, sms, st);
+}
+
+}  // namespace sage

@@ -509,4 +509,190 @@ int sage_attention_varlen(const void* q, const void* k, const void* v, void* out
                                         dtype, qk_mode, causal, smooth_k, sm_scale, nullptr, stream);
 }
 
+// ---- the quantised cache ---------------------------------------------------------------------------
+
+// Checks what the three cache operators share and describes the cache to the kernels.
+static int cache_view(const char* who, void* kc, float* ks, void* vc, float* vs, const float* shift, int64_t Hkv, int64_t head_dim,
+                      int64_t pages, int64_t page_size, int dtype, int qk_mode, sage::CacheView* c) {
+  g_err[0] = 0;
+  if (!kc || !ks || !vc || !vs) return fail(SAGE_E_ARG, "%s: null cache pointer", who);
+  if (!aligned16(kc) || !aligned16(ks) || !aligned16(vc) || !aligned16(vs) || !aligned16(shift))
+    return fail(SAGE_E_ARG, "%s: cache pointers must be 16-byte aligned", who);
+  if (Hkv < 1 || Hkv > 65535) return fail(SAGE_E_ARG, "%s: key/value heads must be 1..65535 (got %lld)", who, (long long)Hkv);
+  if (head_dim < 8 || head_dim > sage::HD || head_dim % 8)
+    return fail(SAGE_E_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in 8..128 (got %lld)", who, (long long)head_dim);
+  if (pages < 1 || pages >= ((int64_t)1 << 31)) return fail(SAGE_E_ARG, "%s: pages must be 1..2^31-1 (got %lld)", who, (long long)pages);
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return fail(SAGE_E_UNSUPPORTED, "%s: page_size must be a power of two in 16..256 (got %lld)", who, (long long)page_size);
+  if (dtype != SAGE_F16 && dtype != SAGE_BF16) return fail(SAGE_E_ARG, "%s: dtype must be SAGE_F16 or SAGE_BF16", who);
+  if (qk_mode != SAGE_QK_INT8 && qk_mode != SAGE_QK_E4M3) return fail(SAGE_E_ARG, "%s: bad qk_mode", who);
+  c->k_codes = reinterpret_cast<uint8_t*>(kc); c->v_codes = reinterpret_cast<uint8_t*>(vc);
+  c->k_scale = ks; c->v_scale = vs; c->k_shift = shift;
+  c->pages = pages; c->H = Hkv; c->D = head_dim;
+  c->page_shift = 0;
+  while (((int64_t)1 << c->page_shift) < page_size) ++c->page_shift;
+  c->width = head_dim <= 64 ? 64 : 128;
+  c->int8 = qk_mode == SAGE_QK_INT8;
+  return SAGE_OK;
+}
+
+static int check_strides2(const char* who, const char* name, const int64_t s[2]) {
+  if (!s) return fail(SAGE_E_ARG, "%s: %s strides are null", who, name);
+  for (int i = 0; i < 2; ++i) {
+    if (s[i] <= 0) return fail(SAGE_E_ARG, "%s: %s stride %d is not positive", who, name, i);
+    if (s[i] % 8) return fail(SAGE_E_ARG, "%s: %s stride %d is not a multiple of 8 elements", who, name, i);
+    if (s[i] >= ((int64_t)1 << 39)) return fail(SAGE_E_UNSUPPORTED, "%s: %s stride %d exceeds 2^39 elements", who, name, i);
+  }
+  return SAGE_OK;
+}
+
+static int check_table(const char* who, const int32_t* table, int64_t stride, int64_t width, int64_t page_size, int64_t n_seq) {
+  if (n_seq < 1 || n_seq > 65535) return fail(SAGE_E_ARG, "%s: sequences must be 1..65535 (got %lld)", who, (long long)n_seq);
+  if (!table) return fail(SAGE_E_ARG, "%s: page_table is null", who);
+  if (reinterpret_cast<uintptr_t>(table) & 3u) return fail(SAGE_E_ARG, "%s: page_table must be 4-byte aligned", who);
+  if (width < 1 || stride < 0) return fail(SAGE_E_ARG, "%s: bad page_table width or stride", who);
+  if (width * page_size > ((int64_t)1 << 30)) return fail(SAGE_E_UNSUPPORTED, "%s: sequence length exceeds 2^30", who);
+  return SAGE_OK;
+}
+
+int sage_cache_write(const void* k, const void* v, const void* slots, int slots_64,
+                     void* k_codes, float* k_scale, void* v_codes, float* v_scale, const float* k_shift,
+                     int64_t tokens, int64_t Hkv, int64_t head_dim, int64_t pages, int64_t page_size,
+                     const int64_t k_strides[2], const int64_t v_strides[2], int dtype, int qk_mode, void* stream) {
+  const char* who = "sage_cache_write";
+  sage::CacheView c;
+  int rc = cache_view(who, k_codes, k_scale, v_codes, v_scale, k_shift, Hkv, head_dim, pages, page_size, dtype, qk_mode, &c);
+  if (rc) return rc;
+  if (tokens < 0 || tokens >= ((int64_t)1 << 31)) return fail(SAGE_E_ARG, "%s: bad token count %lld", who, (long long)tokens);
+  if (tokens == 0) return SAGE_OK;
+  if (!k || !v || !slots) return fail(SAGE_E_ARG, "%s: null pointer argument", who);
+  if ((rc = check_strides2(who, "k", k_strides)) || (rc = check_strides2(who, "v", v_strides))) return rc;
+  if (!aligned16(k) || !aligned16(v)) return fail(SAGE_E_ARG, "%s: pointers must be 16-byte aligned", who);
+  if (reinterpret_cast<uintptr_t>(slots) & (slots_64 ? 7u : 3u)) return fail(SAGE_E_ARG, "%s: slots are misaligned", who);
+  if (tokens * Hkv > ((int64_t)1 << 35)) return fail(SAGE_E_UNSUPPORTED, "%s: too many rows in one call", who);
+  sage::CacheWriteParams p;
+  p.k = k; p.v = v; p.slots = slots; p.slots64 = slots_64 != 0; p.tokens = tokens; p.dtype = dtype;
+  for (int i = 0; i < 2; ++i) { p.k_strides[i] = k_strides[i]; p.v_strides[i] = v_strides[i]; }
+  const cudaError_t e = sage::launch_cache_write(c, p, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(SAGE_E_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  return SAGE_OK;
+}
+
+int sage_cache_read(const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
+                    const float* k_shift, const int32_t* page_table, int64_t page_table_stride,
+                    int64_t page_table_width, const int32_t* cu_seqlens, void* k_out, void* v_out,
+                    int64_t n_seq, int64_t total, int64_t Hkv, int64_t head_dim, int64_t pages, int64_t page_size,
+                    const int64_t k_strides[2], const int64_t v_strides[2], int dtype, int qk_mode, void* stream) {
+  const char* who = "sage_cache_read";
+  sage::CacheView c;
+  int rc = cache_view(who, const_cast<void*>(k_codes), const_cast<float*>(k_scale), const_cast<void*>(v_codes), const_cast<float*>(v_scale),
+                      k_shift, Hkv, head_dim, pages, page_size, dtype, qk_mode, &c);
+  if (rc) return rc;
+  if ((rc = check_table(who, page_table, page_table_stride, page_table_width, page_size, n_seq))) return rc;
+  if (total < 0 || total >= ((int64_t)1 << 31)) return fail(SAGE_E_ARG, "%s: bad row count %lld", who, (long long)total);
+  if (total == 0) return SAGE_OK;
+  if (!cu_seqlens || !k_out || !v_out) return fail(SAGE_E_ARG, "%s: null pointer argument", who);
+  if (reinterpret_cast<uintptr_t>(cu_seqlens) & 3u) return fail(SAGE_E_ARG, "%s: cu_seqlens must be 4-byte aligned", who);
+  if ((rc = check_strides2(who, "k_out", k_strides)) || (rc = check_strides2(who, "v_out", v_strides))) return rc;
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(SAGE_E_ARG, "%s: pointers must be 16-byte aligned", who);
+  sage::CacheReadParams p;
+  p.table = page_table; p.cu = cu_seqlens; p.k_out = k_out; p.v_out = v_out;
+  p.table_stride = page_table_stride; p.table_width = page_table_width; p.n_seq = n_seq; p.total = total; p.dtype = dtype;
+  for (int i = 0; i < 2; ++i) { p.k_strides[i] = k_strides[i]; p.v_strides[i] = v_strides[i]; }
+  const cudaError_t e = sage::launch_cache_read(c, p, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(SAGE_E_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  return SAGE_OK;
+}
+
+size_t sage_cache_attention_workspace_bytes(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q) {
+  if (n_seq < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || max_q < 1) return 0;
+  return align256(sage::cache_attention_scratch(n_seq, Hq, Hkv, max_q));
+}
+
+int sage_cache_attention(const void* q, void* out, float* lse,
+                         const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
+                         const float* k_shift, const int32_t* page_table, int64_t page_table_stride,
+                         int64_t page_table_width, const int32_t* seqlens_k, const int32_t* cu_seqlens_q,
+                         const void* tree_mask, int64_t tree_stride, void* workspace, size_t workspace_bytes,
+                         int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t total_q, int64_t max_q, int64_t head_dim,
+                         int64_t pages, int64_t page_size, const int64_t q_strides[2], const int64_t o_strides[2],
+                         int dtype, int qk_mode, float sm_scale, void* stream) {
+  const char* who = "sage_cache_attention";
+  sage::CacheView c;
+  int rc = cache_view(who, const_cast<void*>(k_codes), const_cast<float*>(k_scale), const_cast<void*>(v_codes), const_cast<float*>(v_scale),
+                      k_shift, Hkv, head_dim, pages, page_size, dtype, qk_mode, &c);
+  if (rc) return rc;
+  if ((rc = check_table(who, page_table, page_table_stride, page_table_width, page_size, n_seq))) return rc;
+  if (Hq < 1 || Hq > 65535 || Hq % Hkv)
+    return fail(SAGE_E_ARG, "%s: query heads (%lld) must be a multiple of key/value heads (%lld), up to 65535", who, (long long)Hq, (long long)Hkv);
+  if (total_q < 0 || total_q >= ((int64_t)1 << 31)) return fail(SAGE_E_ARG, "%s: bad token count %lld", who, (long long)total_q);
+  if (total_q == 0) return SAGE_OK;
+  if (max_q < 1 || max_q > total_q) return fail(SAGE_E_ARG, "%s: max_q must be 1..total_q (got %lld)", who, (long long)max_q);
+  if (!q || !out || !seqlens_k) return fail(SAGE_E_ARG, "%s: null pointer argument", who);
+  if (!cu_seqlens_q && total_q != n_seq * max_q)
+    return fail(SAGE_E_ARG, "%s: without cu_seqlens_q every sequence has max_q new tokens", who);
+  if ((reinterpret_cast<uintptr_t>(seqlens_k) | reinterpret_cast<uintptr_t>(cu_seqlens_q) | reinterpret_cast<uintptr_t>(lse)) & 3u)
+    return fail(SAGE_E_ARG, "%s: lengths and lse must be 4-byte aligned", who);
+  if (tree_mask && tree_stride < 0) return fail(SAGE_E_ARG, "%s: negative tree_stride", who);
+  if ((rc = check_strides2(who, "q", q_strides)) || (rc = check_strides2(who, "out", o_strides))) return rc;
+  if (!aligned16(q) || !aligned16(out)) return fail(SAGE_E_ARG, "%s: pointers must be 16-byte aligned", who);
+  if (!(sm_scale > 0.f) || !(sm_scale <= 3.0e38f))
+    return fail(SAGE_E_ARG, "%s: sm_scale must be finite and positive (got %g)", who, (double)sm_scale);
+  // rows of a unit in 31 bits, and the grid of the joining kernel (a CTA per unit and eight rows at least)
+  if (max_q * (Hq / Hkv) > ((int64_t)1 << 28) || n_seq * Hkv * ((max_q * (Hq / Hkv) + 7) / 8) > ((int64_t)1 << 30))
+    return fail(SAGE_E_UNSUPPORTED, "%s: too many rows in one call", who);
+  if (!workspace) return fail(SAGE_E_ARG, "%s: workspace is null", who);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(SAGE_E_ARG, "%s: workspace must be 256-byte aligned", who);
+  const size_t need = sage_cache_attention_workspace_bytes(n_seq, Hq, Hkv, max_q);
+  if (workspace_bytes < need) return fail(SAGE_E_WORKSPACE, "%s: workspace has %zu bytes, needs %zu", who, workspace_bytes, need);
+  sage::CacheAttnParams p;
+  p.q = q; p.out = out; p.lse = lse; p.table = page_table; p.seqlens = seqlens_k; p.cu_q = cu_seqlens_q;
+  p.tree = reinterpret_cast<const uint8_t*>(tree_mask); p.tree_stride = tree_stride;
+  for (int i = 0; i < 2; ++i) { p.q_strides[i] = q_strides[i]; p.o_strides[i] = o_strides[i]; }
+  p.table_stride = page_table_stride; p.table_width = page_table_width;
+  p.n_seq = n_seq; p.Hq = Hq; p.total_q = total_q; p.max_q = max_q; p.dtype = dtype; p.sm_scale = sm_scale; p.scratch = workspace;
+  const cudaError_t e = sage::launch_cache_attention(c, p, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(SAGE_E_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  return SAGE_OK;
+}
+
+int sage_rotary(const void* q, void* q_out, const void* k, void* k_out, const void* positions, int positions_64,
+                const double* inv_freq, float magnitude, int64_t B, int64_t Hq, int64_t Hk, int64_t N,
+                int64_t head_dim, int64_t rotary_dim, int interleaved, int backward,
+                const int64_t q_strides[3], const int64_t qo_strides[3], const int64_t k_strides[3],
+                const int64_t ko_strides[3], const int64_t pos_strides[2], int dtype, void* stream) {
+  const char* who = "sage_rotary";
+  g_err[0] = 0;
+  if (!k) Hk = 0;
+  if (B < 0 || N < 0 || Hq < 1 || Hk < 0 || Hq > 65535 || Hk > 65535) return fail(SAGE_E_ARG, "%s: bad sizes", who);
+  if (head_dim < 8 || head_dim > sage::HD || head_dim % 8)
+    return fail(SAGE_E_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in 8..128 (got %lld)", who, (long long)head_dim);
+  if (rotary_dim < 8 || rotary_dim > head_dim || rotary_dim % 8)
+    return fail(SAGE_E_UNSUPPORTED, "%s: rotary_dim must be a multiple of 8 in 8..head_dim (got %lld)", who, (long long)rotary_dim);
+  if (dtype != SAGE_F16 && dtype != SAGE_BF16) return fail(SAGE_E_ARG, "%s: dtype must be SAGE_F16 or SAGE_BF16", who);
+  if (B == 0 || N == 0) return SAGE_OK;
+  if (N >= ((int64_t)1 << 31) || B * N >= ((int64_t)1 << 31)) return fail(SAGE_E_UNSUPPORTED, "%s: more than 2^31 - 1 tokens", who);
+  if (!q || !q_out || !positions || !inv_freq || !pos_strides || (k && !k_out)) return fail(SAGE_E_ARG, "%s: null pointer argument", who);
+  int rc;
+  if ((rc = check_strides("q", q_strides)) || (rc = check_strides("q_out", qo_strides))) return rc;
+  if (k && ((rc = check_strides("k", k_strides)) || (rc = check_strides("k_out", ko_strides)))) return rc;
+  if (!aligned16(q) || !aligned16(q_out) || !aligned16(k) || !aligned16(k ? k_out : nullptr))
+    return fail(SAGE_E_ARG, "%s: pointers must be 16-byte aligned", who);
+  if ((reinterpret_cast<uintptr_t>(positions) & (positions_64 ? 7u : 3u)) || (reinterpret_cast<uintptr_t>(inv_freq) & 7u))
+    return fail(SAGE_E_ARG, "%s: positions or inv_freq are misaligned", who);
+  if (pos_strides[0] < 0 || pos_strides[1] < 0) return fail(SAGE_E_ARG, "%s: negative position stride", who);
+  sage::RotaryParams p;
+  p.q = q; p.k = k; p.pos = positions; p.q_out = q_out; p.k_out = k_out; p.freq = inv_freq;
+  for (int i = 0; i < 3; ++i) {
+    p.q_strides[i] = q_strides[i]; p.qo_strides[i] = qo_strides[i];
+    p.k_strides[i] = k ? k_strides[i] : 0; p.ko_strides[i] = k ? ko_strides[i] : 0;
+  }
+  p.pos_strides[0] = pos_strides[0]; p.pos_strides[1] = pos_strides[1];
+  p.magnitude = magnitude; p.B = B; p.Hq = Hq; p.Hk = Hk; p.N = N; p.D = head_dim; p.rot = rotary_dim;
+  p.pos64 = positions_64 != 0; p.interleaved = interleaved != 0; p.backward = backward != 0; p.dtype = dtype;
+  const cudaError_t e = sage::launch_rotary(p, reinterpret_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(SAGE_E_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  return SAGE_OK;
+}
+
 }  // extern "C"

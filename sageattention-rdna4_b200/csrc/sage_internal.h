@@ -99,4 +99,59 @@ void set_tiles_per_cta(int n);
 void set_skip_log2(float t);
 int choose_tiles_per_cta(int64_t q_tiles, int64_t bhq, bool causal, int sms);
 
+// ---- a quantised, paged K/V cache (see sage_cache.cu for its layout) ------------------------------
+struct CacheView {
+  uint8_t *k_codes, *v_codes;      // (pages, H, page_size, width)
+  float *k_scale, *v_scale;        // (pages, H, page_size)
+  const float* k_shift;            // optional (H, width): what was subtracted from K before it was quantised
+  int64_t pages, H, D;             // D columns of a row exist (head_dim)
+  int page_shift, width;           // log2 of the page size; bytes of a row (64 or 128)
+  int int8;                        // K codes: 1 int8, 0 e4m3
+};
+
+struct RotaryParams {
+  const void *q, *k, *pos;
+  void *q_out, *k_out;
+  const double* freq;              // rot / 2 angles per position
+  int64_t q_strides[3], k_strides[3], qo_strides[3], ko_strides[3];   // (batch, head, row)
+  int64_t pos_strides[2];          // (batch, row)
+  float magnitude;
+  int64_t B, Hq, Hk, N, D, rot;
+  int pos64, interleaved, backward, dtype;
+};
+cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t st);
+
+struct CacheWriteParams {
+  const void *k, *v, *slots;
+  int64_t k_strides[2], v_strides[2];     // (token, head)
+  int64_t tokens;
+  int slots64, dtype;
+};
+cudaError_t launch_cache_write(const CacheView& c, const CacheWriteParams& p, cudaStream_t st);
+
+struct CacheReadParams {
+  const int32_t *table, *cu;
+  void *k_out, *v_out;
+  int64_t k_strides[2], v_strides[2];     // (token, head)
+  int64_t table_stride, table_width, n_seq, total;
+  int dtype;
+};
+cudaError_t launch_cache_read(const CacheView& c, const CacheReadParams& p, cudaStream_t st);
+
+struct CacheAttnParams {
+  const void* q;
+  void* out;
+  float* lse;                             // optional (total_q, Hq)
+  const int32_t *table, *seqlens, *cu_q;
+  const uint8_t* tree;                    // optional (total_q, max_q): which new tokens of its sequence a row sees
+  int64_t q_strides[2], o_strides[2];     // (token, head)
+  int64_t table_stride, table_width, tree_stride;
+  int64_t n_seq, Hq, total_q, max_q;
+  int dtype;
+  float sm_scale;
+  void* scratch;                          // cache_attention_scratch() bytes
+};
+size_t cache_attention_scratch(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q);
+cudaError_t launch_cache_attention(const CacheView& c, const CacheAttnParams& p, cudaStream_t st);
+
 }  // namespace sage

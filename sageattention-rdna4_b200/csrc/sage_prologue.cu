@@ -227,56 +227,6 @@ __device__ __forceinline__ uint32_t qt_try_wait(uint32_t bar, uint32_t parity) {
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok;
 }
-__device__ __forceinline__ float quarter_warp_max(float x) {
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-  return x;
-}
-// rn(a / d) for a compile-time divisor: rc = rn(1/d) is a constant, the rest is Markstein's sequence
-// (checked against true division over every mantissa of several binades for d = 127 and 448).
-template <int DIV>
-__device__ __forceinline__ float div_const(float a) {
-  constexpr float d = (float)DIV, rc = 1.0f / (float)DIV;
-  const float q0 = __fmul_rn(a, rc);
-  const float r = __fmaf_rn(-q0, d, a);
-  return __fmaf_rn(r, rc, q0);
-}
-__device__ __forceinline__ uint32_t i8x4_magic2(float2 ab, float2 cd) {
-  const float2 m = make_float2(12582912.0f, 12582912.0f);
-  const float2 u = __fadd2_rn(ab, m), v = __fadd2_rn(cd, m);
-  return __byte_perm(__byte_perm(__float_as_uint(u.x), __float_as_uint(u.y), 0x0040),
-                     __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x0040), 0x5410);
-}
-
-// Largest magnitude of eight packed 16-bit values: exact on the packed form, half the instructions.
-template <typename T> struct Packed16;
-template <> struct Packed16<__half> { typedef __half2 Pair; };
-template <> struct Packed16<__nv_bfloat16> { typedef __nv_bfloat162 Pair; };
-template <typename T>
-__device__ __forceinline__ float absmax16(const uint4& u, const uint4& v) {
-  typedef typename Packed16<T>::Pair Pair;
-  const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-  Pair m = __habs2(*reinterpret_cast<const Pair*>(&w[0]));
-#pragma unroll
-  for (int i = 1; i < 8; ++i) m = __hmax2(m, __habs2(*reinterpret_cast<const Pair*>(&w[i])));
-  const float2 f = Elem<T>::cvt2(*reinterpret_cast<const uint32_t*>(&m));
-  return fmaxf(f.x, f.y);
-}
-__device__ __forceinline__ float absmax3(float m, float2 x) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(x.x)), "f"(fabsf(x.y)));
-  return r;
-}
-// e4m3 codes of rn(x / s) for four values, given rc = rn(1/s).  The remainder is taken as q0*s - x and
-// subtracted, which keeps the sign of a zero x; the packed operations have no negation, so the
-// steps divide -x (all signs turn around, those of zeros too) and the codes' sign bits are flipped back.
-__device__ __forceinline__ uint32_t e4m3x4_quot(float2 a, float2 b, float s, float rc) {
-  const float2 nrc = make_float2(-rc, -rc), s2 = make_float2(s, s);
-  const float2 qa = __fmul2_rn(a, nrc), qb = __fmul2_rn(b, nrc);
-  const float2 ya = __ffma2_rn(__ffma2_rn(qa, s2, a), nrc, qa), yb = __ffma2_rn(__ffma2_rn(qb, s2, b), nrc, qb);
-  return e4m3x4(ya.x, ya.y, yb.x, yb.y) ^ 0x80808080u;
-}
 
 // ------------------------------------------------------------------------------------------------
 // One 128-token tile, already in shared memory (128 rows of 256 bytes), by 256 threads.  Thread

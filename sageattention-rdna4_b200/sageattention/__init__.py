@@ -17,6 +17,14 @@ from .core import (  # noqa: F401
     sageattn_varlen,
 )
 from .b200_backend import status  # noqa: F401
+from .cache import (  # noqa: F401
+    SageCache,
+    SageRotary,
+    sage_cache_read,
+    sage_cache_write,
+    sage_rotary,
+    sageattn_cached,
+)
 from .sharding import partition_units, sageattn_sharded, gather_units  # noqa: F401
 
 __version__ = "0.1.0+b200"
@@ -27,6 +35,12 @@ __all__ = [
     "sageattn_qk_int8_pv_fp8_cuda",
     "sageattn_qk_int8_pv_fp8_cuda_sm90",
     "sageattn_varlen",
+    "SageCache",
+    "SageRotary",
+    "sage_cache_read",
+    "sage_cache_write",
+    "sage_rotary",
+    "sageattn_cached",
     "partition_units",
     "sageattn_sharded",
     "gather_units",

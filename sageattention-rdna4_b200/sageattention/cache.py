@@ -1,0 +1,458 @@
+"""A quantised, paged K/V cache and the operators around it, for programs that generate tokens.
+
+    rotary = SageRotary(128, base=10000.0)
+    cache = SageCache.empty(num_pages, page_size, num_kv_heads, head_dim, dtype=torch.bfloat16)
+    q, k = sage_rotary(q, k, positions, rotary)                 # q (tokens, Hq, D), k (tokens, Hkv, D)
+    sage_cache_write(cache, k, v, slots)                        # quantised as it is written
+    out = sageattn_cached(q, cache, page_table, seqlens_k)      # one new token per sequence
+    out = sageattn_cached(q, cache, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tree_mask=mask)
+    k16, v16 = sage_cache_read(cache, page_table, cu_seqlens_k, total)      # e.g. for sageattn_varlen
+
+The reference keeps no cache: its callers hand over the whole K and V with every call, which are then
+quantised again (sageattention/core.py:1037-1252).  Codes and scales here are those of its quantiser
+(kernels/hip/h34_prologue.hip:116-211): one fp32 scale per token and head, int8 or e4m3 K, e4m3 V.
+Index tensors (slots, page tables, lengths) stay on the GPU and are never read on the host: no call
+synchronises, and every call can be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _native
+from .b200_backend import _counters, _dtype_code, _STRIDE_MAX, HEAD_DIM, packed_view_reason, strided_view_reason
+
+_E4M3 = torch.float8_e4m3fn
+
+
+def _refuse(what: str, kind=ValueError):
+    _counters["refusals"] += 1
+    raise kind("%s (B200 path)" % what)
+
+
+def _check_head_dim(d: int):
+    if d < 8 or d > HEAD_DIM or d % 8:
+        _refuse("head_dim must be a multiple of 8 in 8..128, got %d" % d, NotImplementedError)
+
+
+class _on_device:
+    """Makes `dev` the current device for the C call; nothing where it is already."""
+
+    __slots__ = ("dev", "prev")
+
+    def __init__(self, dev):
+        self.dev = dev
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.dev.index:
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.prev != self.dev.index:
+            torch.cuda.set_device(self.prev)
+
+
+class SageCache:
+    """The buffers of a paged cache, which the caller may own.
+
+    k_codes : ``(pages, Hkv, page_size, width)`` int8 or float8_e4m3fn; v_codes the same shape,
+        float8_e4m3fn; ``width`` is 64 for ``head_dim`` up to 64 and 128 above
+    k_scale, v_scale : ``(pages, Hkv, page_size)`` float32
+    k_shift : optional ``(Hkv, head_dim)`` float32 that is subtracted from K before it is quantised (the mean
+        that `smooth_k` takes off, taken once over a prompt and kept).  Attention does not change by it: all
+        keys of a head move alike.
+    page_size is a power of two, 16 .. 256.  The code buffers must start as zeros (`empty` does that): codes that
+    no write has set may be read behind a mask, and must not be the e4m3 NaN.
+    """
+
+    __slots__ = ("k_codes", "k_scale", "v_codes", "v_scale", "k_shift", "head_dim", "num_pages", "page_size",
+                 "num_kv_heads", "device", "_mode", "_args", "_sizes")
+
+    def __init__(self, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
+                 head_dim: int, k_shift: Optional[torch.Tensor] = None):
+        if k_codes.dim() != 4 or k_codes.dtype not in (torch.int8, _E4M3):
+            _refuse("k_codes must be a (pages, heads, page_size, width) tensor of int8 or float8_e4m3fn")
+        pages, heads, page, width = (int(x) for x in k_codes.shape)
+        head_dim = int(head_dim)
+        _check_head_dim(head_dim)
+        if width != (64 if head_dim <= 64 else 128):
+            _refuse("rows of a cache are 64 bytes wide for head_dim up to 64, else 128; got %d" % width)
+        if page < 16 or page > 256 or page & (page - 1):
+            _refuse("page_size must be a power of two in 16..256, got %d" % page, NotImplementedError)
+        if pages < 1 or heads < 1:
+            _refuse("a cache needs at least one page and one head")
+        if v_codes.dtype != _E4M3 or tuple(v_codes.shape) != tuple(k_codes.shape):
+            _refuse("v_codes must be float8_e4m3fn of k_codes' shape")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.dtype != torch.float32 or tuple(t.shape) != (pages, heads, page):
+                _refuse("%s must be float32 (pages, heads, page_size)" % name)
+        for t in (k_codes, k_scale, v_codes, v_scale):
+            if not t.is_cuda or t.device != k_codes.device:
+                _refuse("a cache lives on one CUDA device; there is no CPU path")
+            if not t.is_contiguous() or t.data_ptr() % 16:
+                _refuse("the buffers of a cache must be contiguous and 16-byte aligned")
+        if k_shift is not None:
+            if tuple(k_shift.shape) != (heads, head_dim) or k_shift.device != k_codes.device:
+                _refuse("k_shift must be (heads, head_dim) on the cache's device")
+            padded = torch.zeros((heads, width), dtype=torch.float32, device=k_codes.device)
+            padded[:, :head_dim] = k_shift
+            k_shift = padded
+        self.k_codes, self.k_scale, self.v_codes, self.v_scale, self.k_shift = k_codes, k_scale, v_codes, v_scale, k_shift
+        self.head_dim, self.num_pages, self.page_size, self.num_kv_heads = head_dim, pages, page, heads
+        self.device = k_codes.device
+        self._mode = _native.SAGE_QK_INT8 if k_codes.dtype == torch.int8 else _native.SAGE_QK_E4M3
+        self._args = (k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
+                      0 if k_shift is None else k_shift.data_ptr())
+        self._sizes = (pages, page)
+
+    @classmethod
+    def empty(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16,
+              int8: Optional[bool] = None, device="cuda", k_shift: Optional[torch.Tensor] = None) -> "SageCache":
+        """A cache of zeros for keys and values of `dtype`.  ``int8=None`` follows the rule of `sageattn`: int8 K
+        codes for float16, e4m3 for bfloat16."""
+        _dtype_code(dtype)
+        _check_head_dim(int(head_dim))
+        if int8 is None:
+            int8 = dtype == torch.float16
+        shape = (int(num_pages), int(num_kv_heads), int(page_size))
+        width = 64 if head_dim <= 64 else 128
+        codes = [torch.zeros(shape + (width,), dtype=torch.uint8, device=device) for _ in range(2)]
+        scales = [torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(codes[0].view(torch.int8 if int8 else _E4M3), scales[0], codes[1].view(_E4M3), scales[1], head_dim, k_shift)
+
+
+def _check_rows(name: str, t: torch.Tensor, heads: int, d: int, dev):
+    """A packed (tokens, heads, head_dim) tensor next to a cache."""
+    if t.device != dev:
+        _refuse("%s must be on the cache's device" % name)
+    if t.dtype not in (torch.float16, torch.bfloat16):
+        _refuse("%s must be float16 or bfloat16" % name)
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != d:
+        _refuse("%s must be (tokens, %d, %d), got %s" % (name, heads, d, tuple(t.shape)))
+    if t.numel():
+        reason = packed_view_reason(t)
+        if reason is not None:
+            _refuse("cannot serve %s: %s" % (name, reason))
+
+
+def _check_index(name: str, t: torch.Tensor, dev, dims: int, dtypes=(torch.int32,)):
+    if t.device != dev:
+        _refuse("%s must be on the cache's device" % name)
+    if t.dtype not in dtypes or t.dim() != dims:
+        _refuse("%s must be a %d-D tensor of %s" % (name, dims, " or ".join(str(x) for x in dtypes)))
+    if t.numel() and t.stride(-1) != 1:
+        _refuse("%s must be contiguous along its last axis" % name)
+
+
+def sage_cache_write(cache: SageCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise `k` and `v`, ``(tokens, Hkv, head_dim)`` float16 or bfloat16, into the cache.
+
+    slots : ``(tokens,)`` int32 or int64 on the GPU, ``page * page_size + offset``.  A token whose slot lies below
+    0 or past the last page is left out (the padding of a batch).  Slots of one call are distinct: of two tokens
+    with one slot, each part of the row may come from either.  A row that holds a NaN or an infinity reads back as
+    NaN throughout.
+    """
+    _counters["calls"] += 1
+    dev, heads, d = cache.device, cache.num_kv_heads, cache.head_dim
+    _check_rows("k", k, heads, d, dev)
+    _check_rows("v", v, heads, d, dev)
+    if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
+        _refuse("k and v must have the same dtype and tokens")
+    _check_index("slots", slots, dev, 1, (torch.int32, torch.int64))
+    if slots.shape[0] != k.shape[0]:
+        _refuse("slots must hold one entry per token")
+    if k.shape[0] == 0:
+        return
+    with _on_device(dev):
+        rc = _native.load().sage_cache_write(
+            k.data_ptr(), v.data_ptr(), slots.data_ptr(), slots.dtype == torch.int64, *cache._args, k.shape[0], heads, d,
+            *cache._sizes, _native.strides2(k.stride(0), k.stride(1)), _native.strides2(v.stride(0), v.stride(1)),
+            _dtype_code(k.dtype), cache._mode, torch.cuda.current_stream(dev).cuda_stream)
+    _native.check(rc, "sage_cache_write")
+
+
+def sage_cache_read(cache: SageCache, page_table: torch.Tensor, cu_seqlens: torch.Tensor, total: int,
+                    dtype: torch.dtype = torch.float16, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Sequences of the cache as packed 16-bit keys and values, each ``(total, Hkv, head_dim)``.
+
+    page_table : ``(batch, width)`` int32 page ids on the GPU; cu_seqlens : ``(batch + 1,)`` int32 prefix sums of the
+    token counts on the GPU, ``cu_seqlens[-1]`` at most `total`.  Rows from ``cu_seqlens[-1]`` on are left as they are
+    (in fresh outputs: undefined); tokens on a page that does not exist read as zeros.
+    """
+    _counters["calls"] += 1
+    dev, heads, d, total = cache.device, cache.num_kv_heads, cache.head_dim, int(total)
+    code = _dtype_code(dtype)
+    _check_index("page_table", page_table, dev, 2)
+    _check_index("cu_seqlens", cu_seqlens, dev, 1)
+    if page_table.shape[0] < 1 or page_table.shape[1] < 1 or cu_seqlens.shape[0] != page_table.shape[0] + 1:
+        _refuse("page_table and cu_seqlens must describe the same sequences, at least one")
+    if total < 0:
+        _refuse("total must not be negative")
+    if out is None:
+        k = torch.empty((total, heads, d), dtype=dtype, device=dev)
+        v = torch.empty((total, heads, d), dtype=dtype, device=dev)
+    else:
+        k, v = out
+        for name, t in (("out[0]", k), ("out[1]", v)):
+            _check_rows(name, t, heads, d, dev)
+            if t.shape[0] != total or t.dtype != dtype:
+                _refuse("%s must hold total rows of dtype" % name)
+    if total == 0:
+        return k, v
+    with _on_device(dev):
+        rc = _native.load().sage_cache_read(
+            *cache._args, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cu_seqlens.data_ptr(),
+            k.data_ptr(), v.data_ptr(), page_table.shape[0], total, heads, d, *cache._sizes,
+            _native.strides2(k.stride(0), k.stride(1)), _native.strides2(v.stride(0), v.stride(1)), code, cache._mode,
+            torch.cuda.current_stream(dev).cuda_stream)
+    _native.check(rc, "sage_cache_read")
+    return k, v
+
+
+def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor, seqlens_k: torch.Tensor,
+                    cu_seqlens_q: Optional[torch.Tensor] = None, max_seqlen_q: Optional[int] = None,
+                    tree_mask: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None,
+                    return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """Attention of new tokens over the cached keys of their sequences.
+
+    q : ``(tokens, Hq, head_dim)`` packed, float16 or bfloat16, ``Hq`` a multiple of the cache's heads.
+    page_table : ``(batch, width)`` int32; seqlens_k : ``(batch,)`` int32: cached keys of each sequence, those of its
+        new tokens among them (the last ones, written before this call).
+    cu_seqlens_q : ``(batch + 1,)`` int32 prefix sums of the new tokens per sequence, with `max_seqlen_q` the largest
+        count (a longer sequence is cut off there, as in `sageattn_varlen`).  None: ``tokens / batch`` for each.
+    tree_mask : None, and a new token sees every key up to its own (one token: all of them; several: a chain);
+        or ``(tokens, >= max_seqlen_q)`` bool (or uint8): token t sees the new token j of its sequence where
+        ``tree_mask[t, j]``, and all keys before the new tokens.  A tree of drafted tokens sets a token's
+        ancestors and itself.
+    sm_scale : default ``head_dim ** -0.5``.
+    return_lse : also return the fp32 log-sum-exp ``(tokens, Hq)`` of ``sm_scale * q.k``.
+    out : optional output of q's shape and dtype.
+    A token that sees no key gets zeros and an LSE of -infinity.  The lengths stay on the GPU; the last bits of a
+    result depend on the lengths of the other sequences of the call (fp32 sums in another order).
+    """
+    _counters["calls"] += 1
+    dev, hkv, d = cache.device, cache.num_kv_heads, cache.head_dim
+    if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % hkv:
+        _refuse("q must be (tokens, heads, head_dim) with a multiple of the cache's %d heads" % hkv)
+    tokens, hq = int(q.shape[0]), int(q.shape[1])
+    _check_rows("q", q, hq, d, dev)
+    _check_index("page_table", page_table, dev, 2)
+    _check_index("seqlens_k", seqlens_k, dev, 1)
+    batch, width = int(page_table.shape[0]), int(page_table.shape[1])
+    if batch < 1 or width < 1 or seqlens_k.shape[0] != batch:
+        _refuse("page_table and seqlens_k must describe the same sequences, at least one")
+    if cu_seqlens_q is None:
+        if tokens % batch or (max_seqlen_q is not None and int(max_seqlen_q) * batch != tokens):
+            _refuse("without cu_seqlens_q every sequence needs the same number of new tokens")
+        max_q = tokens // batch
+    else:
+        _check_index("cu_seqlens_q", cu_seqlens_q, dev, 1)
+        if cu_seqlens_q.shape[0] != batch + 1:
+            _refuse("cu_seqlens_q must have batch + 1 entries")
+        if max_seqlen_q is None or int(max_seqlen_q) < 1:
+            _refuse("cu_seqlens_q needs max_seqlen_q, at least 1")
+        max_q = min(int(max_seqlen_q), tokens)
+    if tree_mask is not None:
+        _check_index("tree_mask", tree_mask, dev, 2, (torch.bool, torch.uint8))
+        if tree_mask.shape[0] != tokens or tree_mask.shape[1] < max_q:
+            _refuse("tree_mask must be (tokens, >= max_seqlen_q)")
+    scale = d ** -0.5 if sm_scale is None else float(sm_scale)
+    if not (0.0 < scale < float("inf")):
+        _refuse("sm_scale must be finite and positive, got %r" % (sm_scale,))
+    if out is None:
+        out = torch.empty((tokens, hq, d), dtype=q.dtype, device=dev)
+    else:
+        _check_rows("out", out, hq, d, dev)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            _refuse("out must have q's shape and dtype")
+    lse = torch.empty((tokens, hq), dtype=torch.float32, device=dev) if return_lse else None
+    if tokens:
+        lib = _native.load()
+        # (from the caching allocator with every call: ordered with this stream, and a captured graph's own)
+        ws = torch.empty((lib.sage_cache_attention_workspace_bytes(batch, hq, hkv, max_q),), dtype=torch.uint8, device=dev)
+        with _on_device(dev):
+            rc = lib.sage_cache_attention(
+                q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *cache._args,
+                page_table.data_ptr(), page_table.stride(0), width, seqlens_k.data_ptr(),
+                0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
+                0 if tree_mask is None else tree_mask.data_ptr(), 0 if tree_mask is None else tree_mask.stride(0),
+                ws.data_ptr(), ws.numel(), batch, hq, hkv, tokens, max_q, d, *cache._sizes,
+                _native.strides2(q.stride(0), q.stride(1)), _native.strides2(out.stride(0), out.stride(1)),
+                _dtype_code(q.dtype), cache._mode, scale, torch.cuda.current_stream(dev).cuda_stream)
+        _native.check(rc, "sage_cache_attention")
+    return (out, lse) if return_lse else out
+
+
+# ---- rotary positions --------------------------------------------------------------------------------------------
+
+class SageRotary:
+    """The frequencies of a rotary position encoding, in 64 bits on the GPU.
+
+    rotary_dim : columns of a head that turn (default all of them), a multiple of 8
+    interleaved : pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2)
+    scaling : ``"none"``; ``"linear"``, all frequencies divided by `factor`; ``"ntk"``, the base raised to
+        ``base * factor ** (rotary_dim / (rotary_dim - 2))``; ``"parts"``: frequencies that turn more than `fast` times
+        within `original_length` positions stay, those that turn less than `slow` times are divided by `factor`, a
+        linear ramp between, and the result is scaled by ``0.1 ln(factor) + 1``.
+    """
+
+    __slots__ = ("head_dim", "rotary_dim", "interleaved", "inv_freq", "magnitude", "device")
+
+    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, interleaved: bool = False,
+                 scaling: str = "none", factor: float = 1.0, original_length: int = 4096, fast: float = 32.0, slow: float = 1.0,
+                 device="cuda"):
+        head_dim = int(head_dim)
+        _check_head_dim(head_dim)
+        rot = head_dim if rotary_dim is None else int(rotary_dim)
+        if rot < 8 or rot > head_dim or rot % 8:
+            _refuse("rotary_dim must be a multiple of 8 in 8..head_dim, got %d" % rot, NotImplementedError)
+        if scaling not in ("none", "linear", "ntk", "parts"):
+            _refuse("scaling must be 'none', 'linear', 'ntk' or 'parts'")
+        if not (base > 1.0 and math.isfinite(base)) or not (factor >= 1.0 and math.isfinite(factor)):
+            _refuse("base must be above 1 and factor at least 1")
+        if scaling == "parts" and not (original_length > 0 and fast > slow > 0):
+            _refuse("'parts' needs original_length > 0 and fast > slow > 0")
+        if scaling == "ntk":
+            base = base * factor ** (rot / (rot - 2))
+        freq = [base ** (-i / rot) for i in range(0, rot, 2)]
+        self.magnitude = 1.0
+        if scaling == "linear":
+            freq = [f / factor for f in freq]
+        elif scaling == "parts":
+            keep = [min(1.0, max(0.0, (original_length * f / (2 * math.pi) - slow) / (fast - slow))) for f in freq]
+            freq = [f * (k + (1 - k) / factor) for f, k in zip(freq, keep)]
+            self.magnitude = 0.1 * math.log(factor) + 1.0
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rot, bool(interleaved)
+        self.inv_freq = torch.tensor(freq, dtype=torch.float64).to(device)
+        self.device = self.inv_freq.device
+
+
+def _rotary_views(x, layout):
+    """A logical (B, H, N, D) view of a packed or batched tensor."""
+    if x.dim() == 3:
+        return x.unsqueeze(0).transpose(1, 2)
+    if x.dim() == 4:
+        return x if layout == "HND" else x.transpose(1, 2)
+    _refuse("rotary takes (tokens, heads, head_dim) or 4-D tensors")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two servable views share an element.  Views of one buffer with the same strides (the parts of a fused
+    projection) are told apart exactly; others that reach into one another count as sharing."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    (a0, a1), (b0, b1) = span(a), span(b)
+    if not (a0 < b1 and b0 < a1):
+        return False
+    if a.stride() != b.stride():
+        return True
+    axes = sorted(zip(a.stride(), a.shape, b.shape), reverse=True)
+
+    def reachable(rest, k):
+        # is rest = sum over the axes of (index in b - index in a) * stride?  Each stride steps over all the smaller reach.
+        if k == len(axes):
+            return rest == 0
+        stride, na, nb = axes[k]
+        near = rest // stride
+        return any(-(na - 1) <= i <= nb - 1 and reachable(rest - i * stride, k + 1) for i in (near, near + 1))
+
+    return reachable((a0 - b0) // a.element_size(), 0)
+
+
+def _rotate(q, k, positions, rotary, layout, backward, out):
+    ins = [x for x in (q, k) if x is not None]
+    views = [_rotary_views(x, layout) for x in ins]
+    dev = q.device
+    if out is None:
+        outs = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in ins]
+    else:
+        outs = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(outs) != len(ins):
+            _refuse("out must hold one tensor per input")
+        for i, (x, o) in enumerate(zip(ins, outs)):
+            if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device:
+                _refuse("out must have the inputs' shapes, dtypes and device")
+            for j, y in enumerate(ins + outs[:i]):
+                own = j == i and o.data_ptr() == y.data_ptr() and o.stride() == y.stride()
+                if x.numel() and y.numel() and not own and _overlap(o, y):
+                    _refuse("out may be its own input, and overlaps nothing else")
+    o_views = [_rotary_views(x, layout) for x in outs]
+    b, _, n, d = views[0].shape
+    for v in views + o_views:
+        if v.device != dev or not v.is_cuda:
+            _refuse("rotary needs CUDA tensors on one device; there is no CPU path")
+        if v.dtype not in (torch.float16, torch.bfloat16) or v.dtype != q.dtype:
+            _refuse("q and k must share one dtype, float16 or bfloat16")
+        if v.shape[0] != b or v.shape[2] != n or v.shape[3] != d or v.shape[1] < 1:
+            _refuse("q and k must agree in all but their heads")
+        reason = strided_view_reason(v) if v.numel() else None
+        if reason is not None:
+            _refuse("cannot serve this call: %s" % reason)
+    if d != rotary.head_dim or rotary.device != dev:
+        _refuse("the rotary was made for head_dim %d on %s" % (rotary.head_dim, rotary.device))
+    if positions.device != dev or positions.dtype not in (torch.int32, torch.int64):
+        _refuse("positions must be int32 or int64 on the tensors' device")
+    if positions.dim() == 1 and positions.shape[0] == n:
+        p2 = (0, positions.stride(0))
+    elif positions.dim() == 2 and q.dim() == 4 and tuple(positions.shape) == (b, n):
+        p2 = positions.stride()
+    else:
+        _refuse("positions must be (N,) or (B, N)")
+    if b * n:
+        s3 = [_native.strides3(v.stride(0), v.stride(1), v.stride(2)) for v in (views[0], o_views[0], views[-1], o_views[-1])]
+        two = k is not None
+        with _on_device(dev):
+            rc = _native.load().sage_rotary(
+                q.data_ptr(), outs[0].data_ptr(), k.data_ptr() if two else 0, outs[1].data_ptr() if two else 0,
+                positions.data_ptr(), positions.dtype == torch.int64, rotary.inv_freq.data_ptr(), rotary.magnitude,
+                b, views[0].shape[1], views[1].shape[1] if two else 0, n, d, rotary.rotary_dim, rotary.interleaved, backward,
+                *s3, _native.strides2(*p2), _dtype_code(q.dtype), torch.cuda.current_stream(dev).cuda_stream)
+        _native.check(rc, "sage_rotary")
+    return tuple(outs)
+
+
+class _Rotary(torch.autograd.Function):
+    """The map is linear: its gradient is the transposed map of the outputs' gradients."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, rotary, layout, backward):
+        ctx.save_for_backward(positions)
+        ctx.rest = (rotary, layout, backward)
+        res = _rotate(q, k, positions, rotary, layout, backward, None)
+        return res if k is not None else res[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        rotary, layout, backward = ctx.rest
+        res = _rotate(grads[0].contiguous(), grads[1].contiguous() if len(grads) > 1 else None, ctx.saved_tensors[0], rotary, layout,
+                      not backward, None)
+        return res[0], res[1] if len(grads) > 1 else None, None, None, None, None
+
+
+def sage_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary: SageRotary,
+                tensor_layout: str = "HND", backward: bool = False, out=None):
+    """Turn queries and keys to their positions; returns ``(q, k)``, or q alone where `k` is None.
+
+    q, k : packed ``(tokens, heads, head_dim)``, or 4-D in `tensor_layout`; float16 or bfloat16; strided views as in
+        `sageattn`.  They differ in their heads at most.
+    positions : int32 or int64 on the GPU, ``(tokens,)``, for 4-D tensors also ``(B, N)``; any value (angles are
+        worked out in 64 bits).
+    backward : the transposed map, which takes the gradient of the outputs to that of the inputs (for a magnitude
+        of 1, the inverse).  Inputs that require gradients get them by it.
+    out : optional output (for two inputs a pair), each its input itself or memory of its own; not differentiable.
+    """
+    _counters["calls"] += 1
+    if tensor_layout not in ("HND", "NHD"):
+        _refuse("tensor_layout must be 'HND' or 'NHD'")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if out is not None:
+            _refuse("out cannot be given for inputs that require gradients")
+        return _Rotary.apply(q, k, positions, rotary, tensor_layout, bool(backward))
+    res = _rotate(q, k, positions, rotary, tensor_layout, bool(backward), out)
+    return res if k is not None else res[0]

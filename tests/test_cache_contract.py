@@ -1,0 +1,194 @@
+"""What the cache operators refuse, and their host side, without a GPU: every call below must stop at validation."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import sageattention as S
+from sageattention import _native, cache as C
+
+buf = (ctypes.c_char * 4096)()
+P = (ctypes.addressof(buf) + 255) // 256 * 256
+S2, S3 = _native.strides2(1024, 128), _native.strides3(8192, 1024, 128)
+ARG, UNSUPPORTED, WORKSPACE = _native.SAGE_E_ARG, _native.SAGE_E_UNSUPPORTED, _native.SAGE_E_WORKSPACE
+
+
+def _refused(rc, code, word):
+    assert rc == code, (rc, _native.load().sage_last_error())
+    assert word.encode() in _native.load().sage_last_error(), _native.load().sage_last_error()
+
+
+def _write(k=P, v=P, slots=P, s64=1, kc=P, ks=P, vc=P, vs=P, shift=None, tokens=4, heads=8, d=128, pages=4, page=64,
+           k_st=S2, v_st=S2, dtype=0, mode=0):
+    return _native.load().sage_cache_write(k, v, slots, s64, kc, ks, vc, vs, shift, tokens, heads, d, pages, page, k_st, v_st, dtype, mode, None)
+
+
+def _read(kc=P, table=P, stride=4, width=4, cu=P, k=P, v=P, n_seq=1, total=4, heads=8, d=128, pages=4, page=64, k_st=S2, v_st=S2, dtype=0, mode=0):
+    return _native.load().sage_cache_read(kc, P, P, P, None, table, stride, width, cu, k, v, n_seq, total, heads, d, pages, page, k_st, v_st, dtype, mode, None)
+
+
+def _attend(q=P, out=P, lse=None, kc=P, table=P, stride=4, width=4, lens=P, cu=P, tree=None, tree_st=0, ws=P, ws_bytes=1 << 40, n_seq=1,
+            hq=8, hkv=8, total=4, max_q=4, d=128, pages=4, page=64, q_st=S2, o_st=S2, dtype=0, mode=0, scale=0.1):
+    return _native.load().sage_cache_attention(q, out, lse, kc, P, P, P, None, table, stride, width, lens, cu, tree, tree_st, ws, ws_bytes,
+                                               n_seq, hq, hkv, total, max_q, d, pages, page, q_st, o_st, dtype, mode, scale, None)
+
+
+def _rotary(q=P, qo=P, k=None, ko=None, pos=P, p64=1, freq=P, b=1, hq=8, hk=0, n=4, d=128, rot=128, st=S3, p2=_native.strides2(0, 1), dtype=0):
+    return _native.load().sage_rotary(q, qo, k, ko, pos, p64, freq, 1.0, b, hq, hk, n, d, rot, 0, 0, st, S3, S3, S3, p2, dtype, None)
+
+
+@pytest.mark.parametrize("call", [_write, _read, _attend])
+def test_cache_shapes(call):
+    for d in (0, 4, 12, 136):
+        _refused(call(d=d), UNSUPPORTED, "head_dim")
+    for page in (0, 8, 24, 512, -16):
+        _refused(call(page=page), UNSUPPORTED, "page_size")
+    _refused(call(pages=0), ARG, "pages")
+    _refused(call(pages=1 << 31), ARG, "pages")
+    _refused(call(dtype=2), ARG, "dtype")
+    _refused(call(mode=2), ARG, "qk_mode")
+    _refused(call(kc=None), ARG, "null")
+    _refused(call(kc=P + 8), ARG, "aligned")
+
+
+def test_write_refusals():
+    assert _write(tokens=0) == 0
+    for name in ("k", "v", "slots"):
+        _refused(_write(**{name: None}), ARG, "null")
+    _refused(_write(tokens=-1), ARG, "token")
+    _refused(_write(heads=0), ARG, "heads")
+    _refused(_write(k=P + 2), ARG, "aligned")
+    _refused(_write(slots=P + 4), ARG, "slots")
+    _refused(_write(slots=P + 2, s64=0), ARG, "slots")
+    for bad in ((0, 128), (1024, -8), (1020, 128)):
+        _refused(_write(v_st=_native.strides2(*bad)), ARG, "stride")
+    _refused(_write(k_st=_native.strides2(1 << 39, 128)), UNSUPPORTED, "2^39")
+    _refused(_write(k_st=None), ARG, "strides")
+
+
+def test_read_refusals():
+    assert _read(total=0) == 0
+    for name in ("cu", "k", "v", "table"):
+        _refused(_read(**{name: None}), ARG, "null")
+    _refused(_read(n_seq=0), ARG, "sequences")
+    _refused(_read(n_seq=65536), ARG, "sequences")
+    _refused(_read(width=0), ARG, "width")
+    _refused(_read(stride=-1), ARG, "stride")
+    _refused(_read(width=1 << 28), UNSUPPORTED, "2^30")
+    _refused(_read(total=-1), ARG, "row count")
+    _refused(_read(cu=P + 2), ARG, "aligned")
+    _refused(_read(k=P + 8), ARG, "aligned")
+
+
+def test_attention_refusals():
+    assert _attend(total=0) == 0
+    for name in ("q", "out", "lens", "table", "ws"):
+        _refused(_attend(**{name: None}), ARG, "null")
+    _refused(_attend(cu=None, n_seq=3), ARG, "max_q")
+    _refused(_attend(hq=9), ARG, "multiple")
+    _refused(_attend(hq=0), ARG, "heads")
+    _refused(_attend(max_q=0), ARG, "max_q")
+    _refused(_attend(max_q=5), ARG, "max_q")
+    _refused(_attend(lse=P + 2), ARG, "aligned")
+    _refused(_attend(q=P + 8), ARG, "aligned")
+    _refused(_attend(tree=P, tree_st=-1), ARG, "tree_stride")
+    _refused(_attend(ws=P + 16), ARG, "256")
+    _refused(_attend(ws_bytes=100), WORKSPACE, "needs")
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        _refused(_attend(scale=scale), ARG, "sm_scale")
+    _refused(_attend(total=1 << 30, max_q=1 << 30), UNSUPPORTED, "rows")
+    lib = _native.load()
+    assert lib.sage_cache_attention_workspace_bytes(1, 8, 3, 1) == 0 and lib.sage_cache_attention_workspace_bytes(0, 8, 8, 1) == 0
+    assert lib.sage_cache_attention_workspace_bytes(4, 8, 8, 1) % 256 == 0
+
+
+def test_rotary_refusals():
+    assert _rotary(n=0) == 0 and _rotary(b=0) == 0
+    for name in ("q", "qo", "pos", "freq"):
+        _refused(_rotary(**{name: None}), ARG, "null")
+    _refused(_rotary(k=P, ko=None, hk=2), ARG, "null")
+    for rot in (0, 4, 12, 136):
+        _refused(_rotary(rot=rot), UNSUPPORTED, "rotary_dim")
+    _refused(_rotary(d=64, rot=72), UNSUPPORTED, "rotary_dim")
+    _refused(_rotary(d=12), UNSUPPORTED, "head_dim")
+    _refused(_rotary(hq=0), ARG, "sizes")
+    _refused(_rotary(dtype=3), ARG, "dtype")
+    _refused(_rotary(pos=P + 4), ARG, "misaligned")
+    _refused(_rotary(freq=P + 4), ARG, "misaligned")
+    _refused(_rotary(q=P + 8), ARG, "aligned")
+    _refused(_rotary(p2=_native.strides2(-1, 1)), ARG, "position stride")
+    _refused(_rotary(st=_native.strides3(8, 8, 4)), ARG, "stride")
+    _refused(_rotary(n=1 << 31), UNSUPPORTED, "tokens")
+
+
+def test_python_layer_has_no_cpu_path():
+    codes, scale = torch.zeros((2, 1, 16, 128), dtype=torch.int8), torch.zeros((2, 1, 16))
+    with pytest.raises(ValueError, match="CUDA"):
+        S.SageCache(codes, scale, codes.view(torch.float8_e4m3fn), scale, 128)
+    with pytest.raises(ValueError, match="CUDA"):
+        S.SageCache.empty(2, 16, 1, 128, device="cpu")
+    rotary = S.SageRotary(64, device="cpu")
+    x = torch.zeros((2, 3, 64), dtype=torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        S.sage_rotary(x, None, torch.zeros(2, dtype=torch.int32), rotary)
+
+
+def test_cache_buffers_are_checked():
+    codes, scale = torch.zeros((2, 1, 16, 128), dtype=torch.int8), torch.zeros((2, 1, 16))
+    e4m3 = codes.view(torch.float8_e4m3fn)
+    for args, kind, word in (((codes[0], scale, e4m3, scale, 128), ValueError, "k_codes"), ((codes.view(torch.uint8), scale, e4m3, scale, 128), ValueError, "k_codes"),
+                             ((codes, scale, codes, scale, 128), ValueError, "v_codes"), ((codes, scale[:1], e4m3, scale, 128), ValueError, "k_scale"),
+                             ((codes, scale, e4m3, scale.half(), 128), ValueError, "v_scale"), ((codes, scale, e4m3, scale, 64), ValueError, "64 bytes"),
+                             ((codes, scale, e4m3, scale, 12), NotImplementedError, "head_dim"),
+                             ((codes[:, :, :8], scale[:, :, :8], e4m3[:, :, :8], scale[:, :, :8], 128), NotImplementedError, "page_size")):
+        with pytest.raises(kind, match=word):
+            S.SageCache(*args)
+
+
+def test_rotary_frequencies():
+    base = [10000.0 ** (-i / 64) for i in range(0, 64, 2)]
+    assert S.SageRotary(128, rotary_dim=64, device="cpu").inv_freq.tolist() == base
+    linear = S.SageRotary(64, scaling="linear", factor=4.0, device="cpu")
+    assert linear.inv_freq.tolist() == [f / 4 for f in base] and linear.magnitude == 1.0
+    ntk = S.SageRotary(64, scaling="ntk", factor=4.0, device="cpu").inv_freq
+    # the slowest pair turns `factor` times as slowly, the fastest as before
+    assert ntk[0] == 1.0 and abs(ntk[-1].item() * 4 / base[-1] - 1) < 1e-12
+    parts = S.SageRotary(64, scaling="parts", factor=4.0, original_length=4096, device="cpu")
+    turns = [4096 * f / (2 * math.pi) for f in base]
+    for f, t, got in zip(base, turns, parts.inv_freq.tolist()):
+        if t >= 32:
+            assert got == f
+        elif t <= 1:
+            assert got == f / 4
+        else:
+            assert f / 4 < got < f
+    assert abs(parts.magnitude - (0.1 * math.log(4) + 1)) < 1e-15
+    for kw, kind in ((dict(rotary_dim=12), NotImplementedError), (dict(rotary_dim=72), NotImplementedError), (dict(scaling="cubic"), ValueError),
+                     (dict(factor=0.5), ValueError), (dict(base=1.0), ValueError), (dict(scaling="parts", slow=0.0), ValueError)):
+        with pytest.raises(kind):
+            S.SageRotary(64, device="cpu", **kw)
+
+
+def test_shared_elements_of_views():
+    """The exact test for views with the same strides against an enumeration of their elements."""
+    gen = torch.Generator().manual_seed(0)
+    store = torch.zeros(4096, dtype=torch.float16)
+
+    def elements(t):
+        at = [t.data_ptr() // 2]
+        for n, s in zip(t.shape, t.stride()):
+            at = [x + i * s for x in at for i in range(n)]
+        return set(at)
+
+    seen = set()
+    for _ in range(400):
+        full = torch.randint(1, 5, (4,), generator=gen).tolist()
+        strides = [full[1] * full[2] * full[3], full[2] * full[3], full[3], 1]
+        a, b = (store.as_strided([int(torch.randint(1, n + 1, (1,), generator=gen)) for n in full], strides, int(torch.randint(0, 200, (1,), generator=gen)))
+                for _ in range(2))
+        want = bool(elements(a) & elements(b))
+        assert C._overlap(a, b) == want
+        seen.add(want)
+    assert seen == {True, False}
+    assert C._overlap(store[:64].view(8, 8), store[32:96].view(8, 8).T) and not C._overlap(store[:64].view(8, 8), store[64:128].view(4, 16))
