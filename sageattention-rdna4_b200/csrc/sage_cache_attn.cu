@@ -24,10 +24,10 @@
 // The running maximum moves only when a score passes it by 2^8, and N when a product passes 2^12: p stays
 // below 2^8, the accumulator is rarely touched, and neither the sums nor the 11 bits lose anything by it.
 //
-// Work.  The tiles of 64 keys of all (sequence, K/V head, row tile) units are numbered in one line, and every CTA
+// Work.  The tiles of 128 keys of all (sequence, K/V head, row tile) units are numbered in one line, and every CTA
 // takes an equal stretch of it, so that ragged batches and single long sequences alike fill the GPU; lengths are
 // read on the device.  A unit that lies in several stretches leaves partial rows in the workspace, which
-// cache_combine_kernel joins in the order of the keys.  Each warp walks 16 of the 64 keys of every tile by itself
+// cache_combine_kernel joins in the order of the keys.  Each warp walks 32 of the 128 keys of every tile by itself
 // through its own ring of cp.async stages: no barrier but at the end of a unit, and no spinning wait.
 #include <algorithm>
 
@@ -39,7 +39,7 @@ namespace sage {
 namespace {
 
 constexpr int CA_WARPS = 4, CA_THREADS = 32 * CA_WARPS;
-constexpr int CA_KEYS = 64;                    // keys of a tile: 16 per warp
+constexpr int CA_KEYS = 128;                   // keys of a tile: 32 per warp, two blocks of 16
 constexpr float LN2_F = 0.6931471805599453f;
 constexpr float NO_MAX = -3.0e38f;
 
@@ -207,10 +207,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// Two e4m3 codes (the low 16 bits) -> two fp16.
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3);
-  return (uint32_t)r.x | ((uint32_t)r.y << 16);
+// Four e4m3 codes -> two registers of two fp16 each.
+__device__ __forceinline__ void e4m3_quad(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
 }
 // Four K codes -> two registers of two fp16 each.
 template <bool INT8>
@@ -223,15 +224,14 @@ __device__ __forceinline__ void k_halves(uint32_t w, uint32_t& lo, uint32_t& hi)
     lo = *reinterpret_cast<const uint32_t*>(&x);
     hi = *reinterpret_cast<const uint32_t*>(&y);
   } else {
-    lo = e4m3_pair(w & 0xFFFFu);
-    hi = e4m3_pair(w >> 16);
+    e4m3_quad(w, lo, hi);
   }
 }
 
 // Shared memory of a CTA.
 template <int WIDTH, int NB, int STAGES> struct CaSmem {
-  static constexpr uint32_t CODES = 16 * WIDTH;                      // 16 rows
-  static constexpr uint32_t STAGE = 2 * CODES + 128;                 // K, V, and 16 scales of each
+  static constexpr uint32_t CODES = 32 * WIDTH;                      // 32 rows
+  static constexpr uint32_t STAGE = 2 * CODES + 256;                 // K, V, and 32 scales of each
   static constexpr uint32_t RING = CA_WARPS * STAGES * STAGE;
   static constexpr int ROW = WIDTH + 4;                              // floats of a merge row (padded against bank conflicts)
   static constexpr uint32_t OFF_MERGE = RING;                        // (8 NB rows, ROW)
@@ -277,29 +277,37 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   Cursor ahead = cur;                                // the tile whose loads are issued next
   const uint32_t ring = smem_addr(smem) + warp * STAGES * L::STAGE;
 
-  // this warp's 16 keys of the tile at `ahead` into stage s
+  // This warp's 32 keys of the tile at `ahead` into stage s.  Lane l copies piece l % PIECES of rows l / PIECES + i * RPI;
+  // (row & 7) of the swizzle is that of the lane's first row, but for a change of one bit in every other copy.
+  constexpr int RPI = 32 / PIECES;                   // rows of one copy instruction
+  const int row_l = lane / PIECES, piece_l = lane % PIECES;
+  const uint32_t dst_even = row_l * WIDTH + 16 * (WIDTH == 128 ? piece_l ^ row_l : piece_l ^ (row_l >> 1));
+  const uint8_t *k_lane = a.kc + 16 * lane, *v_lane = a.vc + 16 * lane;
+  const float* s_lane = ((lane & 7) < 4 ? a.ks : a.vs) + 4 * (lane & 3);
   auto issue = [&](int s) {
-    const int key0 = ahead.kt * CA_KEYS + 16 * warp;
     const uint32_t st = ring + s * L::STAGE;
-    const int pi = key0 >> a.page_shift;
-    int page = -1;
-    if (key0 < ahead.s.len && pi < a.table_width) page = __ldg(a.table + (long long)ahead.b * a.table_st + pi);
-    const bool there = page >= 0 && page < a.pages;
-    const long long row = there ? ((((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key0 & ((1 << a.page_shift) - 1))) : 0;
 #pragma unroll
-    for (int i = 0; i < 16 * PIECES / 32; ++i) {
-      const int r = (i * 32 + lane) / PIECES, p = (i * 32 + lane) % PIECES;
-      const int swz = WIDTH == 128 ? p ^ (r & 7) : p ^ ((r >> 1) & 3);
-      const uint32_t dst = st + r * WIDTH + 16 * swz;
-      const long long src = row * WIDTH + r * WIDTH + 16 * p;
-      copy16(dst, a.kc + src, there);
-      copy16(dst + L::CODES, a.vc + src, there);
-    }
-    if (there) {
-      if (lane < 8) copy16(st + 2 * L::CODES + 16 * lane, (lane < 4 ? a.ks : a.vs) + row + 4 * (lane & 3), true);
-    } else if (lane < 16) {                          // no such keys: a scale below zero says so
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 2 * L::CODES + 4 * lane), "f"(-1.0f) : "memory");
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 2 * L::CODES + 64 + 4 * lane), "f"(0.0f) : "memory");
+    for (int blk = 0; blk < 2; ++blk) {              // 16 keys of one page
+      const int key0 = ahead.kt * CA_KEYS + 32 * warp + 16 * blk;
+      int page = -1;
+      if (key0 < ahead.s.len) page = __ldg(a.table + ahead.b * a.table_st + (key0 >> a.page_shift));
+      const bool there = (unsigned)page < (unsigned)a.pages;
+      const long long row = there ? ((((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key0 & ((1 << a.page_shift) - 1))) : 0;
+      const uint8_t *k = k_lane + row * WIDTH, *v = v_lane + row * WIDTH;
+      const uint32_t dst = st + blk * 16 * WIDTH;
+#pragma unroll
+      for (int i = 0; i < 16 / RPI; ++i) {
+        const uint32_t to = dst + i * RPI * WIDTH + (WIDTH == 128 ? dst_even ^ (64u * (i & 1)) : dst_even);
+        copy16(to, k + i * RPI * WIDTH, there);
+        copy16(to + L::CODES, v + i * RPI * WIDTH, there);
+      }
+      // scales: 32 of K, then 32 of V
+      if (there) {
+        if (lane < 8) copy16(st + 2 * L::CODES + (lane < 4 ? 0 : 128) + 64 * blk + 16 * (lane & 3), s_lane + row, true);
+      } else if (lane < 16) {                        // no such keys: a scale below zero says so
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 2 * L::CODES + 64 * blk + 4 * lane), "f"(-1.0f) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + 2 * L::CODES + 128 + 64 * blk + 4 * lane), "f"(0.0f) : "memory");
+      }
     }
   };
   int issued = 0;
@@ -364,7 +372,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           // rows 2c + e sit with lane g' = 2c + e of the Q fragments
-          row_c[nb][e] = a.scale_log2 * __shfl_sync(0xffffffffu, back, 4 * (2 * c + e));
+          row_c[nb][e] = fmaxf(a.scale_log2 * __shfl_sync(0xffffffffu, back, 4 * (2 * c + e)), 1.17549435e-38f);   // (a masked score stays -infinity)
           const int r2 = 8 * nb + 2 * c + e, tok2 = (cur.rt * ROWS + r2) / a.group;
           row_tok[nb][e] = tok2;
           row_lim[nb][e] = r2 < live ? (a.tree ? cur.s.len : min(cur.s.len, ctx + tok2 + 1)) : 0;
@@ -388,83 +396,91 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
     copy_wait<STAGES - 1>();
     __syncwarp();
 
-    const uint32_t st = ring + stage * L::STAGE;
-    const int key0 = cur.kt * CA_KEYS + 16 * warp;
-    // ---- S^T = K Q^T
-    float s[NB][4];
+    const uint32_t st = ring + stage * L::STAGE, scales = st + 2 * L::CODES + 4 * g;
+    const int key0 = cur.kt * CA_KEYS + 32 * warp;
+    // ---- S^T = K Q^T, two blocks of 16 keys
+    float s[2][NB][4];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[nb][e] = 0.f;
-#pragma unroll
-    for (int half = 0; half < WIDTH / 64; ++half) {
-      // 16 bytes of rows g and g + 8: four k-steps
-      uint32_t r0[4], r1[4];
-      {
-        const int p = WIDTH == 128 ? (2 * c + half) ^ (g & 7) : c ^ ((g >> 1) & 3);
-        const uint4 u = lds16(st + g * WIDTH + 16 * p), v = lds16(st + (g + 8) * WIDTH + 16 * p);
-        r0[0] = u.x; r0[1] = u.y; r0[2] = u.z; r0[3] = u.w;
-        r1[0] = v.x; r1[1] = v.y; r1[2] = v.z; r1[3] = v.w;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t f[4];
-        k_halves<INT8>(r0[i], f[0], f[2]);
-        k_halves<INT8>(r1[i], f[1], f[3]);
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mma16816(s[nb], f, qf[nb][4 * half + i][0], qf[nb][4 * half + i][1]);
-      }
-    }
-    // ---- weights
-    const float sk0 = lds_f32(st + 2 * L::CODES + 4 * g), sk1 = lds_f32(st + 2 * L::CODES + 4 * (g + 8));
-    const float sv0 = lds_f32(st + 2 * L::CODES + 64 + 4 * g), sv1 = lds_f32(st + 2 * L::CODES + 64 + 4 * (g + 8));
-    const bool absent = sk0 < 0.f || sk1 < 0.f;
-    float p[NB][4], w[NB][4];
-    bool over = false;
-    if (key0 + 16 > plain_end || __any_sync(0xffffffffu, absent)) {
+    for (int blk = 0; blk < 2; ++blk) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[blk][nb][e] = 0.f;
+#pragma unroll
+      for (int half = 0; half < WIDTH / 64; ++half) {
+        // 16 bytes of rows g and g + 8: four k-steps
+        const int p = WIDTH == 128 ? (2 * c + half) ^ (g & 7) : c ^ ((g >> 1) & 3);
+        const uint4 u = lds16(st + (16 * blk + g) * WIDTH + 16 * p), v = lds16(st + (16 * blk + g + 8) * WIDTH + 16 * p);
+        const uint32_t r0[4] = {u.x, u.y, u.z, u.w}, r1[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t f[4];
+          k_halves<INT8>(r0[i], f[0], f[2]);
+          k_halves<INT8>(r1[i], f[1], f[3]);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma16816(s[blk][nb], f, qf[nb][4 * half + i][0], qf[nb][4 * half + i][1]);
+        }
+      }
+    }
+    // ---- weights: key blk * 16 + g + 8 * (e / 2), row 2c + e % 2
+    float sk[2][2], sv[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { sk[i >> 1][i & 1] = lds_f32(scales + 32 * i); sv[i >> 1][i & 1] = lds_f32(scales + 128 + 32 * i); }
+    const bool absent = fminf(fminf(sk[0][0], sk[0][1]), fminf(sk[1][0], sk[1][1])) < 0.f;
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[blk][nb][e] *= sk[blk][e >> 1];
+    const bool masked = key0 + 32 > plain_end || __any_sync(0xffffffffu, absent);
+    if (masked) {
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 16 * blk + g + 8 * (e >> 1), x = e & 1;
+            bool seen = key < row_lim[nb][x] && !(sk[blk][e >> 1] < 0.f);
+            if (a.tree != nullptr && seen) {
+              const int j = key - (cur.s.len - cur.s.q_len);
+              if (j >= 0) seen = a.tree[(long long)(cur.s.q0 + row_tok[nb][x]) * a.tree_st + j] != 0;
+            }
+            if (!seen) s[blk][nb][e] = -INFINITY;
+          }
+    }
+    uint32_t pf[2][NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float p[2][4], w[2][4];
+      float p_top = 0.f, w_top = 0.f;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = key0 + g + 8 * (e >> 1), x = e & 1;
-          bool seen = key < row_lim[nb][x] && !((e >> 1) ? sk1 < 0.f : sk0 < 0.f);
-          if (a.tree != nullptr && seen) {
-            const int j = key - (cur.s.len - cur.s.q_len);
-            if (j >= 0) seen = a.tree[(long long)(cur.s.q0 + row_tok[nb][x]) * a.tree_st + j] != 0;
-          }
-          s[nb][e] = seen ? s[nb][e] * ((e >> 1) ? sk1 : sk0) : -INFINITY;
+          p[blk][e] = fast_ex2(fmaf(s[blk][nb][e], row_c[nb][e & 1], -m[nb][e & 1]));
+          w[blk][e] = p[blk][e] * (sv[blk][e >> 1] * nf[nb][e & 1]);
+          p_top = fmaxf(p_top, p[blk][e]);
+          w_top = fmaxf(w_top, w[blk][e]);
         }
-    } else {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) { s[nb][0] *= sk0; s[nb][1] *= sk0; s[nb][2] *= sk1; s[nb][3] *= sk1; }
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int x = e & 1;
-        const float d = s[nb][e] == -INFINITY ? -INFINITY : fmaf(s[nb][e], row_c[nb][x], -m[nb][x]);
-        p[nb][e] = fast_ex2(d);
-        // (a masked weight is an exact zero whatever its key's scale holds)
-        w[nb][e] = d == -INFINITY ? 0.f : p[nb][e] * (((e >> 1) ? sv1 : sv0) * nf[nb][x]);
-        over = over || d > 8.f || w[nb][e] > 4096.f;
-      }
-    if (__any_sync(0xffffffffu, over)) {
-      // new maxima and factors; the sums and the accumulator follow
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+      if (__any_sync(0xffffffffu, fmaxf(16.f * p_top, w_top) > 4096.f)) {
+        // new maxima and factors; the sums and the accumulator follow
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           float top = m[nb][x];
-          const bool none0 = s[nb][x] == -INFINITY, none1 = s[nb][2 + x] == -INFINITY;
-          if (!none0) top = fmaxf(top, s[nb][x] * row_c[nb][x]);
-          if (!none1) top = fmaxf(top, s[nb][2 + x] * row_c[nb][x]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[i >> 1][nb][2 * (i & 1) + x] * row_c[nb][x]);
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
           const float fade = fast_ex2(m[nb][x] - top);
-          p[nb][x] = none0 ? 0.f : fast_ex2(fmaf(s[nb][x], row_c[nb][x], -top));
-          p[nb][2 + x] = none1 ? 0.f : fast_ex2(fmaf(s[nb][2 + x], row_c[nb][x], -top));
-          float big = fmaxf(none0 ? 0.f : p[nb][x] * sv0, none1 ? 0.f : p[nb][2 + x] * sv1);
+          float big = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = fast_ex2(fmaf(s[i >> 1][nb][2 * (i & 1) + x], row_c[nb][x], -top));
+            p[i >> 1][2 * (i & 1) + x] = v;
+            if (s[i >> 1][nb][2 * (i & 1) + x] != -INFINITY) big = fmaxf(big, v * sv[i >> 1][i & 1]);
+          }
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, sh));
           float n_new = nf[nb][x], scale = fade;
@@ -480,22 +496,28 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           l[nb][x] *= fade;
 #pragma unroll
           for (int j = 0; j < KSTEPS; ++j) { o[nb][j][x] *= scale; o[nb][j][2 + x] *= scale; }
-          w[nb][x] = none0 ? 0.f : p[nb][x] * (sv0 * n_new);
-          w[nb][2 + x] = none1 ? 0.f : p[nb][2 + x] * (sv1 * n_new);
-        }
-    }
-    uint32_t pf[NB][2];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      l[nb][0] += p[nb][0] + p[nb][2];
-      l[nb][1] += p[nb][1] + p[nb][3];
-      const __half2 u = __floats2half2_rn(w[nb][0], w[nb][1]), v = __floats2half2_rn(w[nb][2], w[nb][3]);
-      pf[nb][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&u));
-      pf[nb][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&v));
+          for (int i = 0; i < 4; ++i) w[i >> 1][2 * (i & 1) + x] = p[i >> 1][2 * (i & 1) + x] * (sv[i >> 1][i & 1] * n_new);
+        }
+      }
+      if (masked) {                                  // a masked weight is an exact zero whatever its key's scale holds
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (s[i >> 2][nb][i & 3] == -INFINITY) w[i >> 2][i & 3] = 0.f;
+      }
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        l[nb][0] += p[blk][0] + p[blk][2];
+        l[nb][1] += p[blk][1] + p[blk][3];
+        const __half2 u = __floats2half2_rn(w[blk][0], w[blk][1]), v = __floats2half2_rn(w[blk][2], w[blk][3]);
+        pf[blk][nb][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&u));
+        pf[blk][nb][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&v));
+      }
     }
     // ---- O^T += V^T P^T
-    {
-      const uint32_t vt = st + L::CODES;
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      const uint32_t vt = st + L::CODES + 16 * blk * WIDTH;
       uint32_t x[4][WIDTH / 32];                     // keys 2c, 2c+1, 2c+8, 2c+9: this lane's WIDTH / 8 columns
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -513,12 +535,15 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
         // bytes 4i .. 4i+3: columns paired over two keys
         const uint32_t a01 = __byte_perm(x[0][i], x[1][i], 0x5140), a23 = __byte_perm(x[0][i], x[1][i], 0x7362);
         const uint32_t b01 = __byte_perm(x[2][i], x[3][i], 0x5140), b23 = __byte_perm(x[2][i], x[3][i], 0x7362);
-        const uint32_t f[4] = {e4m3_pair(a01 & 0xFFFFu), e4m3_pair(a01 >> 16), e4m3_pair(b01 & 0xFFFFu), e4m3_pair(b01 >> 16)};
-        const uint32_t h[4] = {e4m3_pair(a23 & 0xFFFFu), e4m3_pair(a23 >> 16), e4m3_pair(b23 & 0xFFFFu), e4m3_pair(b23 >> 16)};
+        uint32_t f[4], h[4];
+        e4m3_quad(a01, f[0], f[1]);
+        e4m3_quad(b01, f[2], f[3]);
+        e4m3_quad(a23, h[0], h[1]);
+        e4m3_quad(b23, h[2], h[3]);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          mma16816(o[nb][2 * i], f, pf[nb][0], pf[nb][1]);
-          mma16816(o[nb][2 * i + 1], h, pf[nb][0], pf[nb][1]);
+          mma16816(o[nb][2 * i], f, pf[blk][nb][0], pf[blk][nb][1]);
+          mma16816(o[nb][2 * i + 1], h, pf[blk][nb][0], pf[blk][nb][1]);
         }
       }
     }
@@ -698,9 +723,9 @@ cudaError_t launch_attn(CacheAttnKArgs& a, long long tiles_bound, int max_rt, in
 
 template <typename T, bool INT8, int WIDTH>
 cudaError_t launch_rows(CacheAttnKArgs& a, int rows, long long tiles_bound, int max_rt, int sms, cudaStream_t st) {
-  if (rows == 8) return launch_attn<T, INT8, WIDTH, 1, 3, 3>(a, tiles_bound, max_rt, sms, st);
-  if (rows == 16) return launch_attn<T, INT8, WIDTH, 2, 3, 2>(a, tiles_bound, max_rt, sms, st);
-  return launch_attn<T, INT8, WIDTH, 4, 3, 2>(a, tiles_bound, max_rt, sms, st);
+  if (rows == 8) return launch_attn<T, INT8, WIDTH, 1, 2, 3>(a, tiles_bound, max_rt, sms, st);
+  if (rows == 16) return launch_attn<T, INT8, WIDTH, 2, 2, 2>(a, tiles_bound, max_rt, sms, st);
+  return launch_attn<T, INT8, WIDTH, 4, 2, 2>(a, tiles_bound, max_rt, sms, st);
 }
 
 template <typename T>
