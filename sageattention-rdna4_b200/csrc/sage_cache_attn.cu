@@ -80,40 +80,47 @@ __device__ __forceinline__ Seq seq_of(const CacheAttnKArgs& a, int b) {
 __device__ __forceinline__ int row_tiles(const CacheAttnKArgs& a, const Seq& s, int rows) { return (s.q_len * a.group + rows - 1) / rows; }
 __device__ __forceinline__ int key_tiles(const Seq& s) { return max(1, (s.len + CA_KEYS - 1) / CA_KEYS); }   // an empty sequence's rows are written too
 
-// The line of tiles: sequence by sequence, K/V head by head, row tile by row tile, key tile by key tile.
+// The line of tiles: sequence by sequence, K/V head by K/V head, row tile by row tile, key tile by key tile.  CTA x
+// takes the tiles from stretch_begin(x) up to stretch_begin(x + 1); no stretch is empty (a line of fewer tiles
+// than CTAs leaves the last ones without).
+__device__ __forceinline__ long long stretches(const CacheAttnKArgs& a, long long total) { return min((long long)a.ctas, total); }
+__device__ __forceinline__ long long stretch_begin(const CacheAttnKArgs& a, long long total, long long x) { return x * total / stretches(a, total); }
+// The CTA that has tile u: the largest x whose stretch begins at or before it.
+__device__ __forceinline__ int stretch_of(const CacheAttnKArgs& a, long long total, long long u) {
+  return (int)(((u + 1) * stretches(a, total) - 1) / total);
+}
+__device__ __forceinline__ long long tiles_of_seq(const CacheAttnKArgs& a, int b, int rows) {
+  if (b >= a.n_seq) return 0;
+  const Seq s = seq_of(a, b);
+  return (long long)a.Hkv * row_tiles(a, s, rows) * key_tiles(s);
+}
+
 // All threads of a CTA call this: the length of the line, the sequence in which the CTA's stretch begins, and
-// the number of tiles before that sequence.
+// the number of tiles before that sequence.  `sums`: THREADS / 32 + 2 words of shared memory.
 struct Place {
   long long total, before;
   int b;
 };
 template <int THREADS>
-__device__ Place find_place(const CacheAttnKArgs& a, int rows, long long* sums, int cta) {
-  // sums: THREADS / 32 + 4 words of shared memory
+__device__ __forceinline__ Place find_place(const CacheAttnKArgs& a, int rows, long long* sums, int cta) {
+  constexpr int WARPS = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  auto tiles_of = [&](int b) -> long long {
-    if (b >= a.n_seq) return 0;
-    const Seq s = seq_of(a, b);
-    return (long long)a.Hkv * row_tiles(a, s, rows) * key_tiles(s);
-  };
-  long long mine = 0;
-  for (int b = tid; b < a.n_seq; b += THREADS) mine += tiles_of(b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sums[warp] = mine;
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) total += sums[w];
-  __syncthreads();
   Place p;
-  p.total = total; p.before = 0; p.b = a.n_seq;
-  const long long per = (total + a.ctas - 1) / a.ctas;
-  const long long want = (long long)cta * per;
-  if (want >= total) return p;
+  p.total = 0; p.before = 0; p.b = a.n_seq;
+  if (a.n_seq > THREADS) {                           // the length of the line first
+    long long mine = 0;
+    for (int b = tid; b < a.n_seq; b += THREADS) mine += tiles_of_seq(a, b, rows);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) p.total += sums[w];
+    __syncthreads();
+  }
   long long base = 0;
   for (int b0 = 0; b0 < a.n_seq; b0 += THREADS) {
-    const long long n = tiles_of(b0 + tid);
+    const long long n = tiles_of_seq(a, b0 + tid, rows);
     long long upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -121,23 +128,23 @@ __device__ Place find_place(const CacheAttnKArgs& a, int rows, long long* sums, 
       if (lane >= o) upto += x;
     }
     if (lane == 31) sums[warp] = upto;
-    if (tid == 0) sums[THREADS / 32] = -1;
+    if (tid == 0) sums[WARPS] = -1;
     __syncthreads();
-    long long before = base, all = 0;
+    long long before = base + upto - n, all = 0;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       if (w < warp) before += sums[w];
       all += sums[w];
     }
-    before += upto - n;
-    if (n > 0 && want >= before && want < before + n) { sums[THREADS / 32] = b0 + tid; sums[THREADS / 32 + 1] = before; }
+    if (a.n_seq <= THREADS) p.total = all;
+    const long long want = cta < p.total ? stretch_begin(a, p.total, cta) : p.total;
+    if (n > 0 && want >= before && want < before + n) { sums[WARPS] = b0 + tid; sums[WARPS + 1] = before; }
     __syncthreads();
-    const long long found = sums[THREADS / 32];
+    const long long found = sums[WARPS];
     if (found >= 0) {
       p.b = (int)found;
-      p.before = sums[THREADS / 32 + 1];
-      __syncthreads();
-      return p;
+      p.before = sums[WARPS + 1];
+      break;
     }
     base += all;
     __syncthreads();
@@ -263,8 +270,8 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   allow_successor();
   const Place place = find_place<CA_THREADS>(a, ROWS, reinterpret_cast<long long*>(smem + L::OFF_PLACE), (int)blockIdx.x);
   if (place.b >= a.n_seq) return;
-  const long long per = (place.total + a.ctas - 1) / a.ctas, first = (long long)blockIdx.x * per;
-  const int n_tiles = (int)min(per, place.total - first);
+  const long long first = stretch_begin(a, place.total, blockIdx.x);
+  const int n_tiles = (int)(stretch_begin(a, place.total, blockIdx.x + 1LL) - first);
   Cursor cur;
   cur.b = place.b;
   enter_seq(a, cur, ROWS);
@@ -284,13 +291,19 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   const uint32_t dst_even = row_l * WIDTH + 16 * (WIDTH == 128 ? piece_l ^ row_l : piece_l ^ (row_l >> 1));
   const uint8_t *k_lane = a.kc + 16 * lane, *v_lane = a.vc + 16 * lane;
   const float* s_lane = ((lane & 7) < 4 ? a.ks : a.vs) + 4 * (lane & 3);
+  int pages[2];                                      // of the tile at `ahead`, fetched a tile early
+  auto fetch_pages = [&]() {
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      const int key0 = ahead.kt * CA_KEYS + 32 * warp + 16 * blk;
+      pages[blk] = key0 < ahead.s.len ? __ldg(a.table + ahead.b * a.table_st + (key0 >> a.page_shift)) : -1;
+    }
+  };
   auto issue = [&](int s) {
     const uint32_t st = ring + s * L::STAGE;
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {              // 16 keys of one page
-      const int key0 = ahead.kt * CA_KEYS + 32 * warp + 16 * blk;
-      int page = -1;
-      if (key0 < ahead.s.len) page = __ldg(a.table + ahead.b * a.table_st + (key0 >> a.page_shift));
+      const int key0 = ahead.kt * CA_KEYS + 32 * warp + 16 * blk, page = pages[blk];
       const bool there = (unsigned)page < (unsigned)a.pages;
       const long long row = there ? ((((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key0 & ((1 << a.page_shift) - 1))) : 0;
       const uint8_t *k = k_lane + row * WIDTH, *v = v_lane + row * WIDTH;
@@ -310,10 +323,31 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
       }
     }
   };
+  // Rows of Q of the unit at `cur`: lane (g, c) fetches columns c * WIDTH / 4 .. of rows 8 nb + g.
+  uint4 q_raw[NB][WIDTH / 32];
+  auto fetch_q = [&]() {
+    const int live = cur.s.q_len * a.group - cur.rt * ROWS;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int r = 8 * nb + g, rr = cur.rt * ROWS + r, tok = rr / a.group, head = cur.h * a.group + rr - tok * a.group;
+      const T* src = reinterpret_cast<const T*>(a.q) + (long long)(cur.s.q0 + tok) * a.q_st + (long long)head * a.q_sh;
+#pragma unroll
+      for (int i = 0; i < WIDTH / 32; ++i) {
+        const int col = c * (WIDTH / 4) + 8 * i;
+        q_raw[nb][i] = r < live && col < a.D ? __ldg(reinterpret_cast<const uint4*>(src + col)) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  };
+  fetch_pages();
+  fetch_q();
   int issued = 0;
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
-    if (issued < n_tiles) { issue(s); next_tile(a, ahead, ROWS); ++issued; }
+    if (issued < n_tiles) {
+      issue(s);
+      ++issued;
+      if (issued < n_tiles) { next_tile(a, ahead, ROWS); fetch_pages(); }
+    }
     copy_commit();
   }
 
@@ -327,6 +361,14 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   int stage = 0;
   bool fresh = true;
   for (int t = 0; t < n_tiles; ++t) {
+    // the stage that was read last is free: fetch into it
+    __syncwarp();
+    if (issued < n_tiles) {
+      issue(stage == 0 ? STAGES - 1 : stage - 1);
+      ++issued;
+      if (issued < n_tiles) { next_tile(a, ahead, ROWS); fetch_pages(); }
+    }
+    copy_commit();
     if (fresh) {
       fresh = false;
       const int live = min(ROWS, cur.s.q_len * a.group - cur.rt * ROWS);      // rows of this tile that exist
@@ -335,18 +377,9 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
       plain_end = a.tree ? max(ctx, 0) : max(0, min(cur.s.len, ctx + t_first + 1));
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        // Q rows: lane (g, c) holds columns c * WIDTH / 4 .. of row 8 nb + g
-        const int r = 8 * nb + g, rr = cur.rt * ROWS + r;
-        const int tok = rr / a.group, head = cur.h * a.group + rr - tok * a.group;
-        const T* src = reinterpret_cast<const T*>(a.q) + (long long)(cur.s.q0 + tok) * a.q_st + (long long)head * a.q_sh;
         float x[WIDTH / 4], amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < WIDTH / 32; ++i) {
-          const int col = c * (WIDTH / 4) + 8 * i;
-          uint4 u = make_uint4(0u, 0u, 0u, 0u);
-          if (r < live && col < a.D) u = __ldg(reinterpret_cast<const uint4*>(src + col));
-          unpack8<T>(u, x + 8 * i);
-        }
+        for (int i = 0; i < WIDTH / 32; ++i) unpack8<T>(q_raw[nb][i], x + 8 * i);
         float back = 1.f;                            // what undoes the row's power of two
         if (sizeof(T) == 2 && !__is_same(T, __half)) {
 #pragma unroll
@@ -385,14 +418,6 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
       }
     }
 
-    // the stage that was read last is free: fetch into it
-    __syncwarp();
-    if (issued < n_tiles) {
-      issue(stage == 0 ? STAGES - 1 : stage - 1);
-      next_tile(a, ahead, ROWS);
-      ++issued;
-    }
-    copy_commit();
     copy_wait<STAGES - 1>();
     __syncwarp();
 
@@ -564,27 +589,34 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           if (g == 0) ml[warp * ROWS + 8 * nb + 2 * c + x] = make_float4(m[nb][x], sum, nf[nb][x], 0.f);
         }
       __syncthreads();
-      // the four warps add their shares, one after the other, each weighed against the common maximum
-      for (int wv = 0; wv < CA_WARPS; ++wv) {
-        if (wv == warp) {
+      // The four warps add their shares, each weighed against the common maximum: a quarter of the columns per
+      // warp and turn, so that none waits for another.
+      float weight[NB][2];
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int r = 8 * nb + 2 * c + x;
-              float top = NO_MAX;
+        for (int x = 0; x < 2; ++x) {
+          float top = NO_MAX;
 #pragma unroll
-              for (int i = 0; i < CA_WARPS; ++i) top = fmaxf(top, ml[i * ROWS + r].x);
-              const float weight = nf[nb][x] > 0.f ? __fdividef(fast_ex2(m[nb][x] - top), nf[nb][x]) : 0.f;
+          for (int i = 0; i < CA_WARPS; ++i) top = fmaxf(top, ml[i * ROWS + 8 * nb + 2 * c + x].x);
+          weight[nb][x] = nf[nb][x] > 0.f ? __fdividef(fast_ex2(m[nb][x] - top), nf[nb][x]) : 0.f;
+        }
+#pragma unroll 1
+      for (int turn = 0; turn < CA_WARPS; ++turn) {
+        const int quarter = (warp + turn) % CA_WARPS;
 #pragma unroll
-              for (int j = 0; j < KSTEPS; ++j)
+        for (int j = 0; j < KSTEPS; ++j) {
+          if (j / (KSTEPS / CA_WARPS) == quarter) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  float* at = merge + r * L::ROW + (WIDTH / 8) * g + 2 * j + e;
-                  const float v = nf[nb][x] > 0.f ? o[nb][j][2 * e + x] * weight : 0.f;
-                  *at = wv == 0 ? v : *at + v;
-                }
-            }
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                float2* at = reinterpret_cast<float2*>(merge + (8 * nb + 2 * c + x) * L::ROW + (WIDTH / 8) * g + 2 * j);
+                float2 v = make_float2(o[nb][j][x] * weight[nb][x], o[nb][j][2 + x] * weight[nb][x]);
+                if (turn > 0) { v.x += at->x; v.y += at->y; }
+                *at = v;
+              }
+          }
         }
         __syncthreads();
       }
@@ -615,32 +647,35 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           if (lane == 0) a.part_ml[slot * ROWS + r] = make_float2(top, sum);
         }
       }
-      __syncthreads();
-      fresh = true;
+      if (t + 1 < n_tiles) {
+        __syncthreads();
+        fresh = true;
+        next_tile(a, cur, ROWS);
+        fetch_q();
+        continue;
+      }
     }
-    next_tile(a, cur, ROWS);
+    ++cur.kt;
   }
 }
 
-// Joins the parts of the units that lie in several stretches: a CTA per (unit, row), the parts in the order of
-// the keys, four at a time over its four warps.
+// Joins the parts of the units that lie in several stretches: a CTA per (unit, row), the parts spread over its
+// warps and added in a fixed order.
+constexpr int CC_WARPS = 8, CC_THREADS = 32 * CC_WARPS;
 template <typename T>
-__global__ void __launch_bounds__(CA_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int width, int max_rt) {
-  __shared__ long long place_s[CA_WARPS + 4];
-  __shared__ float acc_s[CA_WARPS][HD];
-  __shared__ float2 ml_s[CA_WARPS];
-  wait_for_predecessor();
+__global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int width, int max_rt) {
+  __shared__ long long total_s[CC_WARPS], before_s[CC_WARPS];
+  __shared__ float acc_s[CC_WARPS][HD];
+  __shared__ float2 ml_s[CC_WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // blockIdx.x = ((sequence * Hkv) + head) * max_rt + row tile; blockIdx.y = row
   const int rt = (int)(blockIdx.x % (unsigned)max_rt), bh = (int)(blockIdx.x / (unsigned)max_rt), h = bh % a.Hkv, b = bh / a.Hkv;
-  const Seq s = seq_of(a, b);
+  const Seq s = seq_of(a, b);                        // (the lengths are older than the attention kernel)
   const int r = blockIdx.y, rr = rt * rows + r;
-  if (rr >= s.q_len * a.group) return;
   // tiles before this sequence, and in all
   long long before = 0, total = 0;
-  for (int i = tid; i < a.n_seq; i += CA_THREADS) {
-    const Seq x = seq_of(a, i);
-    const long long n = (long long)a.Hkv * row_tiles(a, x, rows) * key_tiles(x);
+  for (int i = tid; i < a.n_seq; i += CC_THREADS) {
+    const long long n = tiles_of_seq(a, i, rows);
     total += n;
     if (i < b) before += n;
   }
@@ -649,53 +684,66 @@ __global__ void __launch_bounds__(CA_THREADS) cache_combine_kernel(const CacheAt
     total += __shfl_xor_sync(0xffffffffu, total, o);
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
-  long long* place_before = reinterpret_cast<long long*>(acc_s);
-  if (lane == 0) { place_s[warp] = total; place_before[warp] = before; }
+  if (lane == 0) { total_s[warp] = total; before_s[warp] = before; }
   __syncthreads();
   total = 0; before = 0;
 #pragma unroll
-  for (int w = 0; w < CA_WARPS; ++w) { total += place_s[w]; before += place_before[w]; }
-  __syncthreads();
-  const long long per = (total + a.ctas - 1) / a.ctas;
+  for (int w = 0; w < CC_WARPS; ++w) { total += total_s[w]; before += before_s[w]; }
   const int n_kt = key_tiles(s);
   const long long u0 = before + ((long long)h * row_tiles(a, s, rows) + rt) * n_kt, u1 = u0 + n_kt;
-  const int c0 = (int)(u0 / per), c1 = (int)((u1 - 1) / per);
-  if (c0 == c1) return;                              // written by the CTA that had all of it
-  auto slot_of = [&](int cta) { return 2LL * cta + (u0 > (long long)cta * per ? 1 : 0); };
-  float top = NO_MAX;
-  for (int i = c0 + lane; i <= c1; i += 32) top = fmaxf(top, a.part_ml[slot_of(i) * rows + r].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const int c0 = total > 0 ? stretch_of(a, total, u0) : 0, c1 = total > 0 ? stretch_of(a, total, u1 - 1) : 0;
+  wait_for_predecessor();
+  if (rr >= s.q_len * a.group || c0 == c1) return;   // no such row, or written by the CTA that had all of its unit
+  auto at_of = [&](int cta) { return (2LL * cta + (u0 > stretch_begin(a, total, cta) ? 1 : 0)) * rows + r; };
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
+  float sum = 0.f, top = NO_MAX;
   const bool mine = 4 * lane < width;
-#pragma unroll 4
-  for (int i = c0 + warp; i <= c1; i += CA_WARPS) {
-    const long long at = slot_of(i) * rows + r;
-    const float2 ml = a.part_ml[at];
-    const float weight = fast_ex2(ml.x - top);
-    sum += ml.y * weight;
-    if (mine) {
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + at * width + 4 * lane);
-      acc.x = fmaf(v.x, weight, acc.x); acc.y = fmaf(v.y, weight, acc.y); acc.z = fmaf(v.z, weight, acc.z); acc.w = fmaf(v.w, weight, acc.w);
+  constexpr int AT_ONCE = 8;
+  for (int i0 = c0 + warp; i0 <= c1; i0 += CC_WARPS * AT_ONCE) {
+    float2 ml[AT_ONCE];
+    float4 v[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int i = i0 + j * CC_WARPS;
+      ml[j] = make_float2(NO_MAX, 0.f);
+      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i <= c1) {
+        const long long at = at_of(i);
+        ml[j] = a.part_ml[at];
+        if (mine) v[j] = *reinterpret_cast<const float4*>(a.part_o + at * width + 4 * lane);
+      }
+    }
+    float up = top;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) up = fmaxf(up, ml[j].x);
+    const float fade = fast_ex2(top - up);
+    acc.x *= fade; acc.y *= fade; acc.z *= fade; acc.w *= fade; sum *= fade;
+    top = up;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const float weight = fast_ex2(ml[j].x - top);
+      sum = fmaf(ml[j].y, weight, sum);
+      acc.x = fmaf(v[j].x, weight, acc.x); acc.y = fmaf(v[j].y, weight, acc.y); acc.z = fmaf(v[j].z, weight, acc.z); acc.w = fmaf(v[j].w, weight, acc.w);
     }
   }
   if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
   if (lane == 0) ml_s[warp] = make_float2(top, sum);
   __syncthreads();
-  sum = 0.f;
+  top = NO_MAX; sum = 0.f;
+  float weight[CC_WARPS];
 #pragma unroll
-  for (int w = 0; w < CA_WARPS; ++w) sum += ml_s[w].y;
+  for (int w = 0; w < CC_WARPS; ++w) top = fmaxf(top, ml_s[w].x);
+#pragma unroll
+  for (int w = 0; w < CC_WARPS; ++w) { weight[w] = fast_ex2(ml_s[w].x - top); sum = fmaf(ml_s[w].y, weight[w], sum); }
   const int tok = rr / a.group, head = h * a.group + rr - tok * a.group;
   const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-  T* dst = reinterpret_cast<T*>(a.out) + (long long)(s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
-  for (int d = tid; d < a.D; d += CA_THREADS) {
+  if (tid < a.D) {
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < CA_WARPS; ++w) v += acc_s[w][d];
-    dst[d] = from_float<T>(v * inv);
+    for (int w = 0; w < CC_WARPS; ++w) v = fmaf(acc_s[w][tid], weight[w], v);
+    reinterpret_cast<T*>(a.out)[(long long)(s.q0 + tok) * a.o_st + (long long)head * a.o_sh + tid] = from_float<T>(v * inv);
   }
-  if (a.lse != nullptr && warp == 0) {
+  if (a.lse != nullptr && warp == CC_WARPS - 1) {
     float v = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * LN2_F;
     if (a.shift != nullptr)
       v += shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(s.q0 + tok) * a.q_st + (long long)head * a.q_sh, h, width, lane);
@@ -718,7 +766,7 @@ cudaError_t launch_attn(CacheAttnKArgs& a, long long tiles_bound, int max_rt, in
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)((long long)a.n_seq * a.Hkv * max_rt), (unsigned)std::min((long long)8 * NB, (long long)a.max_q * a.group));
-  return launch_after_predecessor(cache_combine_kernel<T>, grid, dim3(CA_THREADS), 0, st, a, 8 * NB, WIDTH, max_rt);
+  return launch_after_predecessor(cache_combine_kernel<T>, grid, dim3(CC_THREADS), 0, st, a, 8 * NB, WIDTH, max_rt);
 }
 
 template <typename T, bool INT8, int WIDTH>
