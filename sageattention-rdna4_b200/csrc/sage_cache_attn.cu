@@ -24,11 +24,11 @@
 // The running maximum moves only when a score passes it by 2^8, and N when a product passes 2^12: p stays
 // below 2^8, the accumulator is rarely touched, and neither the sums nor the 11 bits lose anything by it.
 //
-// Work.  The tiles of 128 keys of all (sequence, K/V head, row tile) units are numbered in one line, and every CTA
-// takes an equal stretch of it, so that ragged batches and single long sequences alike fill the GPU; lengths are
-// read on the device.  A unit that lies in several stretches leaves partial rows in the workspace, which
-// cache_combine_kernel joins in the order of the keys.  Each warp walks 32 of the 128 keys of every tile by itself
-// through its own ring of cp.async stages: no barrier but at the end of a unit, and no spinning wait.
+// Work.  The steps of 32 keys of all (sequence, K/V head, row tile) units are numbered in one line, and every
+// warp of the GPU takes an equal stretch of it, by itself: its own ring of cp.async stages, no barrier, no spinning
+// wait.  So ragged batches and single long sequences alike fill the GPU; lengths are read on the device.  A unit
+// that lies in several stretches leaves partial rows in the workspace, which cache_combine_kernel joins in the
+// order of the keys.
 #include <algorithm>
 
 #include "sage_common.cuh"
@@ -39,7 +39,7 @@ namespace sage {
 namespace {
 
 constexpr int CA_WARPS = 4, CA_THREADS = 32 * CA_WARPS;
-constexpr int CA_KEYS = 128;                   // keys of a tile: 32 per warp, two blocks of 16
+constexpr int CA_KEYS = 32;                    // keys of a step: two blocks of 16
 constexpr float LN2_F = 0.6931471805599453f;
 constexpr float NO_MAX = -3.0e38f;
 
@@ -51,12 +51,13 @@ struct CacheAttnKArgs {
   const float *ks, *vs, *shift;
   const int *table, *seqlens, *cu_q;
   const uint8_t* tree;
-  float* part_o;             // (2 x CTAs, rows of a tile, WIDTH)
-  float2* part_ml;           // (2 x CTAs, rows of a tile): running maximum (log2 domain), sum
+  float* part_o;             // (2 x stretches, part_rows, WIDTH)
+  float2* part_ml;           // (2 x stretches, part_rows): running maximum (log2 domain), sum
   long long q_st, q_sh, o_st, o_sh, table_st, tree_st;
   long long total_q;
   int n_seq, table_width, pages, page_shift, Hq, Hkv, group, max_q, D;
-  int ctas;                  // of the attention kernel: the line of tiles is cut into so many stretches
+  int warps;                 // of the attention kernel: the line of steps is cut into so many stretches
+  int part_rows;             // rows of a partial result: those of a row tile that can exist
   float sm_scale, scale_log2;
 };
 
@@ -78,92 +79,93 @@ __device__ __forceinline__ Seq seq_of(const CacheAttnKArgs& a, int b) {
   return s;
 }
 __device__ __forceinline__ int row_tiles(const CacheAttnKArgs& a, const Seq& s, int rows) { return (s.q_len * a.group + rows - 1) / rows; }
-__device__ __forceinline__ int key_tiles(const Seq& s) { return max(1, (s.len + CA_KEYS - 1) / CA_KEYS); }   // an empty sequence's rows are written too
+__device__ __forceinline__ int key_steps(const Seq& s) { return max(1, (s.len + CA_KEYS - 1) / CA_KEYS); }   // an empty sequence's rows are written too
 
-// The line of tiles: sequence by sequence, K/V head by K/V head, row tile by row tile, key tile by key tile.  CTA x
-// takes the tiles from stretch_begin(x) up to stretch_begin(x + 1); no stretch is empty (a line of fewer tiles
-// than CTAs leaves the last ones without).
-__device__ __forceinline__ long long stretches(const CacheAttnKArgs& a, long long total) { return min((long long)a.ctas, total); }
-__device__ __forceinline__ long long stretch_begin(const CacheAttnKArgs& a, long long total, long long x) { return x * total / stretches(a, total); }
-// The CTA that has tile u: the largest x whose stretch begins at or before it.
-__device__ __forceinline__ int stretch_of(const CacheAttnKArgs& a, long long total, long long u) {
-  return (int)(((u + 1) * stretches(a, total) - 1) / total);
-}
-__device__ __forceinline__ long long tiles_of_seq(const CacheAttnKArgs& a, int b, int rows) {
+// The line of steps: sequence by sequence, K/V head by K/V head, row tile by row tile, step by step (fewer than 2^31
+// of them: the host sees to that).  Its stretches differ by one step at most; a line of fewer steps than warps leaves the
+// last warps without.
+struct Line {
+  unsigned total, n, per, longer;                    // steps, stretches, steps of a stretch, stretches that have one more
+  __device__ __forceinline__ Line(unsigned steps, int warps) : total(steps) {
+    n = min((unsigned)warps, steps);
+    per = n ? steps / n : 0u;
+    longer = steps - n * per;
+  }
+  __device__ __forceinline__ unsigned begin(unsigned x) const { return x * per + min(x, longer); }
+  // the stretch that has step u
+  __device__ __forceinline__ unsigned of(unsigned u) const {
+    const unsigned in_longer = longer * (per + 1);
+    return u < in_longer ? u / (per + 1) : longer + (u - in_longer) / per;
+  }
+};
+__device__ __forceinline__ unsigned steps_of_seq(const CacheAttnKArgs& a, int b, int rows) {
   if (b >= a.n_seq) return 0;
   const Seq s = seq_of(a, b);
-  return (long long)a.Hkv * row_tiles(a, s, rows) * key_tiles(s);
+  return (unsigned)a.Hkv * row_tiles(a, s, rows) * key_steps(s);
 }
 
-// All threads of a CTA call this: the length of the line, the sequence in which the CTA's stretch begins, and
-// the number of tiles before that sequence.  `sums`: THREADS / 32 + 2 words of shared memory.
-struct Place {
-  long long total, before;
-  int b;
+// All threads of a CTA call this: the line, the sequence in which the warp's stretch begins (n_seq: it has none), and
+// the number of steps before that sequence.
+struct PlaceScratch {
+  unsigned sum[CA_WARPS], found[CA_WARPS], before[CA_WARPS];
 };
-template <int THREADS>
-__device__ __forceinline__ Place find_place(const CacheAttnKArgs& a, int rows, long long* sums, int cta) {
-  constexpr int WARPS = THREADS / 32;
+__device__ __forceinline__ Line find_place(const CacheAttnKArgs& a, int rows, PlaceScratch& sh, int& seq, unsigned& steps_before) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  Place p;
-  p.total = 0; p.before = 0; p.b = a.n_seq;
-  if (a.n_seq > THREADS) {                           // the length of the line first
-    long long mine = 0;
-    for (int b = tid; b < a.n_seq; b += THREADS) mine += tiles_of_seq(a, b, rows);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) sums[warp] = mine;
+  unsigned total = 0;
+  if (a.n_seq > CA_THREADS) {                        // the length of the line first
+    unsigned mine = 0;
+    for (int b = tid; b < a.n_seq; b += CA_THREADS) mine += steps_of_seq(a, b, rows);
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) sh.sum[warp] = mine;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) p.total += sums[w];
+    for (int w = 0; w < CA_WARPS; ++w) total += sh.sum[w];
     __syncthreads();
   }
-  long long base = 0;
-  for (int b0 = 0; b0 < a.n_seq; b0 += THREADS) {
-    const long long n = tiles_of_seq(a, b0 + tid, rows);
-    long long upto = n;
+  if (tid < CA_WARPS) sh.found[tid] = a.n_seq;
+  Line line(total, a.warps);
+  unsigned base = 0;
+  for (int b0 = 0; b0 < a.n_seq; b0 += CA_THREADS) {
+    const unsigned n = steps_of_seq(a, b0 + tid, rows);
+    unsigned upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
-    if (lane == 31) sums[warp] = upto;
-    if (tid == 0) sums[WARPS] = -1;
+    if (lane == 31) sh.sum[warp] = upto;
     __syncthreads();
-    long long before = base + upto - n, all = 0;
+    unsigned before = base + upto - n;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) before += sums[w];
-      all += sums[w];
+    for (int w = 0; w < CA_WARPS; ++w) {
+      if (w < warp) before += sh.sum[w];
+      base += sh.sum[w];
     }
-    if (a.n_seq <= THREADS) p.total = all;
-    const long long want = cta < p.total ? stretch_begin(a, p.total, cta) : p.total;
-    if (n > 0 && want >= before && want < before + n) { sums[WARPS] = b0 + tid; sums[WARPS + 1] = before; }
-    __syncthreads();
-    const long long found = sums[WARPS];
-    if (found >= 0) {
-      p.b = (int)found;
-      p.before = sums[WARPS + 1];
-      break;
+    if (a.n_seq <= CA_THREADS) line = Line(base, a.warps);
+#pragma unroll
+    for (int w = 0; w < CA_WARPS; ++w) {
+      const unsigned x = blockIdx.x * CA_WARPS + w, want = line.begin(x);
+      if (x < line.n && want >= before && want - before < n) { sh.found[w] = b0 + tid; sh.before[w] = before; }
     }
-    base += all;
     __syncthreads();
   }
-  return p;
+  seq = (int)sh.found[warp];
+  steps_before = sh.before[warp];
+  return line;
 }
 
 // A position on the line.
 struct Cursor {
   Seq s;
-  int b, h, rt, kt;          // sequence, K/V head, row tile, key tile
+  int b, h, rt, kt;          // sequence, K/V head, row tile, step
   int n_rt, n_kt;
 };
 __device__ __forceinline__ void enter_seq(const CacheAttnKArgs& a, Cursor& c, int rows) {
   c.s = seq_of(a, c.b);
   c.n_rt = row_tiles(a, c.s, rows);
-  c.n_kt = key_tiles(c.s);
+  c.n_kt = key_steps(c.s);
 }
-__device__ __forceinline__ void next_tile(const CacheAttnKArgs& a, Cursor& c, int rows) {
+__device__ __forceinline__ void next_step(const CacheAttnKArgs& a, Cursor& c, int rows) {
   if (++c.kt < c.n_kt) return;
   c.kt = 0;
   if (++c.rt < c.n_rt) return;
@@ -235,16 +237,11 @@ __device__ __forceinline__ void k_halves(uint32_t w, uint32_t& lo, uint32_t& hi)
   }
 }
 
-// Shared memory of a CTA.
-template <int WIDTH, int NB, int STAGES> struct CaSmem {
-  static constexpr uint32_t CODES = 32 * WIDTH;                      // 32 rows
-  static constexpr uint32_t STAGE = 2 * CODES + 256;                 // K, V, and 32 scales of each
-  static constexpr uint32_t RING = CA_WARPS * STAGES * STAGE;
-  static constexpr int ROW = WIDTH + 4;                              // floats of a merge row (padded against bank conflicts)
-  static constexpr uint32_t OFF_MERGE = RING;                        // (8 NB rows, ROW)
-  static constexpr uint32_t OFF_ML = OFF_MERGE + 8 * NB * ROW * 4;   // (warps, 8 NB rows) of {max, sum, factor}
-  static constexpr uint32_t OFF_PLACE = OFF_ML + CA_WARPS * 8 * NB * 16;
-  static constexpr uint32_t BYTES = OFF_PLACE + 8 * (CA_WARPS + 4);
+// Shared memory of a CTA: a ring per warp.
+template <int WIDTH, int STAGES> struct CaSmem {
+  static constexpr uint32_t CODES = CA_KEYS * WIDTH;
+  static constexpr uint32_t STAGE = 2 * CODES + 2 * CA_KEYS * 4;     // K, V, and the scales of each
+  static constexpr uint32_t BYTES = CA_WARPS * STAGES * STAGE;
 };
 
 // sm_scale * (row of Q) . (shift of the K/V head), by one warp
@@ -256,6 +253,15 @@ __device__ __forceinline__ float shift_dot(const CacheAttnKArgs& a, const T* q, 
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   return d * a.sm_scale;
 }
+template <typename T> __device__ __forceinline__ uint32_t pair16(float a, float b);
+template <> __device__ __forceinline__ uint32_t pair16<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pair16<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 template <typename T> __device__ __forceinline__ T from_float(float x);
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
@@ -263,39 +269,41 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 // NB: blocks of 8 query rows in a row tile.
 template <typename T, bool INT8, int WIDTH, int NB, int STAGES, int CTAS_PER_SM>
 __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(const CacheAttnKArgs a) {
-  using L = CaSmem<WIDTH, NB, STAGES>;
+  using L = CaSmem<WIDTH, STAGES>;
   constexpr int ROWS = 8 * NB, KSTEPS = WIDTH / 16, PIECES = WIDTH / 16;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ PlaceScratch place_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const unsigned stretch = blockIdx.x * CA_WARPS + warp;
   allow_successor();
-  const Place place = find_place<CA_THREADS>(a, ROWS, reinterpret_cast<long long*>(smem + L::OFF_PLACE), (int)blockIdx.x);
-  if (place.b >= a.n_seq) return;
-  const long long first = stretch_begin(a, place.total, blockIdx.x);
-  const int n_tiles = (int)(stretch_begin(a, place.total, blockIdx.x + 1LL) - first);
   Cursor cur;
-  cur.b = place.b;
+  unsigned before;
+  const Line line = find_place(a, ROWS, place_s, cur.b, before);
+  if (cur.b >= a.n_seq) return;
+  const unsigned first = line.begin(stretch);
+  const int n_steps = (int)(line.begin(stretch + 1) - first);
   enter_seq(a, cur, ROWS);
   {
-    const long long rest = first - place.before, unit = rest / cur.n_kt;
+    const unsigned rest = first - before, unit = rest / (unsigned)cur.n_kt;
     cur.kt = (int)(rest - unit * cur.n_kt);
-    cur.h = (int)(unit / cur.n_rt);
-    cur.rt = (int)(unit - (long long)cur.h * cur.n_rt);
+    cur.h = (int)(unit / (unsigned)cur.n_rt);
+    cur.rt = (int)unit - cur.h * cur.n_rt;
   }
-  Cursor ahead = cur;                                // the tile whose loads are issued next
+  Cursor ahead = cur;                                // the step whose loads are issued next
   const uint32_t ring = smem_addr(smem) + warp * STAGES * L::STAGE;
 
-  // This warp's 32 keys of the tile at `ahead` into stage s.  Lane l copies piece l % PIECES of rows l / PIECES + i * RPI;
+  // The 32 keys of the step at `ahead` into stage s.  Lane l copies piece l % PIECES of rows l / PIECES + i * RPI;
   // (row & 7) of the swizzle is that of the lane's first row, but for a change of one bit in every other copy.
   constexpr int RPI = 32 / PIECES;                   // rows of one copy instruction
   const int row_l = lane / PIECES, piece_l = lane % PIECES;
   const uint32_t dst_even = row_l * WIDTH + 16 * (WIDTH == 128 ? piece_l ^ row_l : piece_l ^ (row_l >> 1));
   const uint8_t *k_lane = a.kc + 16 * lane, *v_lane = a.vc + 16 * lane;
   const float* s_lane = ((lane & 7) < 4 ? a.ks : a.vs) + 4 * (lane & 3);
-  int pages[2];                                      // of the tile at `ahead`, fetched a tile early
+  int pages[2];                                      // of the step at `ahead`, fetched a step early
   auto fetch_pages = [&]() {
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
-      const int key0 = ahead.kt * CA_KEYS + 32 * warp + 16 * blk;
+      const int key0 = ahead.kt * CA_KEYS + 16 * blk;
       pages[blk] = key0 < ahead.s.len ? __ldg(a.table + ahead.b * a.table_st + (key0 >> a.page_shift)) : -1;
     }
   };
@@ -303,7 +311,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
     const uint32_t st = ring + s * L::STAGE;
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {              // 16 keys of one page
-      const int key0 = ahead.kt * CA_KEYS + 32 * warp + 16 * blk, page = pages[blk];
+      const int key0 = ahead.kt * CA_KEYS + 16 * blk, page = pages[blk];
       const bool there = (unsigned)page < (unsigned)a.pages;
       const long long row = there ? ((((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key0 & ((1 << a.page_shift) - 1))) : 0;
       const uint8_t *k = k_lane + row * WIDTH, *v = v_lane + row * WIDTH;
@@ -343,10 +351,10 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   int issued = 0;
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) {
-    if (issued < n_tiles) {
+    if (issued < n_steps) {
       issue(s);
       ++issued;
-      if (issued < n_tiles) { next_tile(a, ahead, ROWS); fetch_pages(); }
+      if (issued < n_steps) { next_step(a, ahead, ROWS); fetch_pages(); }
     }
     copy_commit();
   }
@@ -360,13 +368,13 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
 
   int stage = 0;
   bool fresh = true;
-  for (int t = 0; t < n_tiles; ++t) {
+  for (int t = 0; t < n_steps; ++t) {
     // the stage that was read last is free: fetch into it
     __syncwarp();
-    if (issued < n_tiles) {
+    if (issued < n_steps) {
       issue(stage == 0 ? STAGES - 1 : stage - 1);
       ++issued;
-      if (issued < n_tiles) { next_tile(a, ahead, ROWS); fetch_pages(); }
+      if (issued < n_steps) { next_step(a, ahead, ROWS); fetch_pages(); }
     }
     copy_commit();
     if (fresh) {
@@ -422,7 +430,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
     __syncwarp();
 
     const uint32_t st = ring + stage * L::STAGE, scales = st + 2 * L::CODES + 4 * g;
-    const int key0 = cur.kt * CA_KEYS + 32 * warp;
+    const int key0 = cur.kt * CA_KEYS;
     // ---- S^T = K Q^T, two blocks of 16 keys
     float s[2][NB][4];
 #pragma unroll
@@ -574,11 +582,13 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
 
-    // ---- end of the unit, or of this CTA's stretch of it
+    // ---- end of the unit, or of the stretch
     const bool last_of_unit = cur.kt + 1 == cur.n_kt;
-    if (last_of_unit || t + 1 == n_tiles) {
-      float* merge = reinterpret_cast<float*>(smem + L::OFF_MERGE);
-      float4* ml = reinterpret_cast<float4*>(smem + L::OFF_ML);
+    if (last_of_unit || t + 1 == n_steps) {
+      const bool whole = last_of_unit && t >= cur.kt;                  // all of the unit's steps were here
+      // a unit that began before this stretch: its part is the stretch's first, else its last
+      const long long slot = 2LL * stretch + (t > cur.kt ? 1 : 0);
+      const int live = min(ROWS, cur.s.q_len * a.group - cur.rt * ROWS);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -586,71 +596,38 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           float sum = l[nb][x];
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
-          if (g == 0) ml[warp * ROWS + 8 * nb + 2 * c + x] = make_float4(m[nb][x], sum, nf[nb][x], 0.f);
-        }
-      __syncthreads();
-      // The four warps add their shares, each weighed against the common maximum: a quarter of the columns per
-      // warp and turn, so that none waits for another.
-      float weight[NB][2];
+          const int r = 8 * nb + 2 * c + x;
+          const float inv_n = nf[nb][x] > 0.f ? __fdividef(1.f, nf[nb][x]) : 0.f;
+          if (r < live) {
+            if (whole) {
+              const int tok = row_tok[nb][x], head = cur.h * a.group + cur.rt * ROWS + r - tok * a.group;
+              const float inv = sum == 0.f ? 0.f : __fdividef(inv_n, sum);
+              T* dst = reinterpret_cast<T*>(a.out) + (long long)(cur.s.q0 + tok) * a.o_st + (long long)head * a.o_sh + (WIDTH / 8) * g;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+              for (int j = 0; j < KSTEPS; ++j)
+                if ((WIDTH / 8) * g + 2 * j < a.D) *reinterpret_cast<uint32_t*>(dst + 2 * j) = pair16<T>(o[nb][j][x] * inv, o[nb][j][2 + x] * inv);
+              if (a.lse != nullptr && g == 0) a.lse[(long long)(cur.s.q0 + tok) * a.Hq + head] = sum == 0.f ? -INFINITY : (m[nb][x] + __log2f(sum)) * LN2_F;
+            } else {
+              float* dst = a.part_o + (slot * a.part_rows + r) * WIDTH + (WIDTH / 8) * g;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float top = NO_MAX;
-#pragma unroll
-          for (int i = 0; i < CA_WARPS; ++i) top = fmaxf(top, ml[i * ROWS + 8 * nb + 2 * c + x].x);
-          weight[nb][x] = nf[nb][x] > 0.f ? __fdividef(fast_ex2(m[nb][x] - top), nf[nb][x]) : 0.f;
-        }
-#pragma unroll 1
-      for (int turn = 0; turn < CA_WARPS; ++turn) {
-        const int quarter = (warp + turn) % CA_WARPS;
-#pragma unroll
-        for (int j = 0; j < KSTEPS; ++j) {
-          if (j / (KSTEPS / CA_WARPS) == quarter) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                float2* at = reinterpret_cast<float2*>(merge + (8 * nb + 2 * c + x) * L::ROW + (WIDTH / 8) * g + 2 * j);
-                float2 v = make_float2(o[nb][j][x] * weight[nb][x], o[nb][j][2 + x] * weight[nb][x]);
-                if (turn > 0) { v.x += at->x; v.y += at->y; }
-                *at = v;
-              }
+              for (int j = 0; j < KSTEPS; j += 2)
+                *reinterpret_cast<float4*>(dst + 2 * j) = make_float4(o[nb][j][x] * inv_n, o[nb][j][2 + x] * inv_n, o[nb][j + 1][x] * inv_n, o[nb][j + 1][2 + x] * inv_n);
+              if (g == 0) a.part_ml[slot * a.part_rows + r] = make_float2(m[nb][x], sum);
+            }
           }
         }
-        __syncthreads();
-      }
-      const bool whole = last_of_unit && t + 1 >= cur.n_kt;            // all of the unit's tiles were here
-      const int live = min(ROWS, cur.s.q_len * a.group - cur.rt * ROWS);
-      // the unit began before this stretch: its part is the stretch's first, else its last
-      const long long slot = 2LL * blockIdx.x + (t > cur.kt ? 1 : 0);
-      for (int r = warp; r < live; r += CA_WARPS) {
-        float top = NO_MAX, sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < CA_WARPS; ++i) top = fmaxf(top, ml[i * ROWS + r].x);
-#pragma unroll
-        for (int i = 0; i < CA_WARPS; ++i) sum += ml[i * ROWS + r].y * fast_ex2(ml[i * ROWS + r].x - top);
-        if (whole) {
+      if (whole && a.lse != nullptr && a.shift != nullptr) {           // the keys as they were before the shift was taken off
+        __syncwarp();
+        for (int r = 0; r < live; ++r) {
           const int rr = cur.rt * ROWS + r, tok = rr / a.group, head = cur.h * a.group + rr - tok * a.group;
-          const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-          T* dst = reinterpret_cast<T*>(a.out) + (long long)(cur.s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
-          for (int d = lane; d < a.D; d += 32) dst[d] = from_float<T>(merge[r * L::ROW + d] * inv);
-          if (a.lse != nullptr) {
-            float v = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * LN2_F;
-            if (a.shift != nullptr)
-              v += shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(cur.s.q0 + tok) * a.q_st + (long long)head * a.q_sh, cur.h, WIDTH, lane);
-            if (lane == 0) a.lse[(long long)(cur.s.q0 + tok) * a.Hq + head] = v;
-          }
-        } else {
-          float* dst = a.part_o + (slot * ROWS + r) * WIDTH;
-          for (int d = lane; d < WIDTH; d += 32) dst[d] = merge[r * L::ROW + d];
-          if (lane == 0) a.part_ml[slot * ROWS + r] = make_float2(top, sum);
+          const float d = shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(cur.s.q0 + tok) * a.q_st + (long long)head * a.q_sh, cur.h, WIDTH, lane);
+          if (lane == 0) a.lse[(long long)(cur.s.q0 + tok) * a.Hq + head] += d;
         }
+        __syncwarp();
       }
-      if (t + 1 < n_tiles) {
-        __syncthreads();
+      if (t + 1 < n_steps) {
         fresh = true;
-        next_tile(a, cur, ROWS);
+        next_step(a, cur, ROWS);
         fetch_q();
         continue;
       }
@@ -664,37 +641,36 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
 constexpr int CC_WARPS = 8, CC_THREADS = 32 * CC_WARPS;
 template <typename T>
 __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int width, int max_rt) {
-  __shared__ long long total_s[CC_WARPS], before_s[CC_WARPS];
+  __shared__ unsigned total_s[CC_WARPS], before_s[CC_WARPS];
   __shared__ float acc_s[CC_WARPS][HD];
   __shared__ float2 ml_s[CC_WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // blockIdx.x = ((sequence * Hkv) + head) * max_rt + row tile; blockIdx.y = row
-  const int rt = (int)(blockIdx.x % (unsigned)max_rt), bh = (int)(blockIdx.x / (unsigned)max_rt), h = bh % a.Hkv, b = bh / a.Hkv;
+  const unsigned bh = blockIdx.x / (unsigned)max_rt;
+  const int rt = (int)(blockIdx.x - bh * max_rt), b = (int)(bh / (unsigned)a.Hkv), h = (int)(bh - (unsigned)b * a.Hkv);
   const Seq s = seq_of(a, b);                        // (the lengths are older than the attention kernel)
   const int r = blockIdx.y, rr = rt * rows + r;
-  // tiles before this sequence, and in all
-  long long before = 0, total = 0;
+  // steps before this sequence, and in all
+  unsigned before = 0, total = 0;
   for (int i = tid; i < a.n_seq; i += CC_THREADS) {
-    const long long n = tiles_of_seq(a, i, rows);
+    const unsigned n = steps_of_seq(a, i, rows);
     total += n;
     if (i < b) before += n;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-  }
+  total = __reduce_add_sync(0xffffffffu, total);
+  before = __reduce_add_sync(0xffffffffu, before);
   if (lane == 0) { total_s[warp] = total; before_s[warp] = before; }
   __syncthreads();
   total = 0; before = 0;
 #pragma unroll
   for (int w = 0; w < CC_WARPS; ++w) { total += total_s[w]; before += before_s[w]; }
-  const int n_kt = key_tiles(s);
-  const long long u0 = before + ((long long)h * row_tiles(a, s, rows) + rt) * n_kt, u1 = u0 + n_kt;
-  const int c0 = total > 0 ? stretch_of(a, total, u0) : 0, c1 = total > 0 ? stretch_of(a, total, u1 - 1) : 0;
+  const Line line(total, a.warps);
+  const int n_kt = key_steps(s);
+  const unsigned u0 = before + ((unsigned)h * row_tiles(a, s, rows) + rt) * n_kt;
+  const int c0 = total > 0 ? (int)line.of(u0) : 0, c1 = total > 0 ? (int)line.of(u0 + n_kt - 1) : 0;
   wait_for_predecessor();
-  if (rr >= s.q_len * a.group || c0 == c1) return;   // no such row, or written by the CTA that had all of its unit
-  auto at_of = [&](int cta) { return (2LL * cta + (u0 > stretch_begin(a, total, cta) ? 1 : 0)) * rows + r; };
+  if (rr >= s.q_len * a.group || c0 == c1) return;   // no such row, or written by the warp that had all of its unit
+  auto at_of = [&](int x) { return (2LL * x + (u0 > line.begin(x) ? 1 : 0)) * a.part_rows + r; };
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f, top = NO_MAX;
   const bool mine = 4 * lane < width;
@@ -753,41 +729,44 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
 
 // Row tiles: 8, 16 or 32 rows, the smallest that holds all rows of a unit.
 int rows_per_tile(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
-constexpr int MAX_CTAS = 160 * 3;                    // sized without a device at hand, for the largest SM count an sm_100 part has
+constexpr int CTAS_PER_SM = 2;
+constexpr int MAX_WARPS = 160 * CTAS_PER_SM * CA_WARPS;   // sized without a device at hand, for the largest SM count an sm_100 part has
 
-template <typename T, bool INT8, int WIDTH, int NB, int STAGES, int CTAS_PER_SM>
-cudaError_t launch_attn(CacheAttnKArgs& a, long long tiles_bound, int max_rt, int sms, cudaStream_t st) {
+template <typename T, bool INT8, int WIDTH, int NB, int STAGES>
+cudaError_t launch_attn(CacheAttnKArgs& a, long long steps_bound, int max_rt, int sms, cudaStream_t st) {
   auto kern = cache_attn_kernel<T, INT8, WIDTH, NB, STAGES, CTAS_PER_SM>;
-  constexpr uint32_t smem = CaSmem<WIDTH, NB, STAGES>::BYTES;
+  constexpr uint32_t smem = CaSmem<WIDTH, STAGES>::BYTES;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  a.ctas = (int)std::min<long long>(std::min(sms * CTAS_PER_SM, MAX_CTAS), tiles_bound);
-  kern<<<a.ctas, CA_THREADS, smem, st>>>(a);
+  const int ctas = (int)std::min<long long>(std::min(sms * CTAS_PER_SM, MAX_WARPS / CA_WARPS), (steps_bound + CA_WARPS - 1) / CA_WARPS);
+  a.warps = ctas * CA_WARPS;
+  kern<<<ctas, CA_THREADS, smem, st>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((long long)a.n_seq * a.Hkv * max_rt), (unsigned)std::min((long long)8 * NB, (long long)a.max_q * a.group));
+  const dim3 grid((unsigned)((long long)a.n_seq * a.Hkv * max_rt), (unsigned)a.part_rows);
   return launch_after_predecessor(cache_combine_kernel<T>, grid, dim3(CC_THREADS), 0, st, a, 8 * NB, WIDTH, max_rt);
 }
 
 template <typename T, bool INT8, int WIDTH>
-cudaError_t launch_rows(CacheAttnKArgs& a, int rows, long long tiles_bound, int max_rt, int sms, cudaStream_t st) {
-  if (rows == 8) return launch_attn<T, INT8, WIDTH, 1, 2, 3>(a, tiles_bound, max_rt, sms, st);
-  if (rows == 16) return launch_attn<T, INT8, WIDTH, 2, 2, 2>(a, tiles_bound, max_rt, sms, st);
-  return launch_attn<T, INT8, WIDTH, 4, 2, 2>(a, tiles_bound, max_rt, sms, st);
+cudaError_t launch_rows(CacheAttnKArgs& a, int rows, long long steps_bound, int max_rt, int sms, cudaStream_t st) {
+  if (rows == 8) return launch_attn<T, INT8, WIDTH, 1, 3>(a, steps_bound, max_rt, sms, st);
+  if (rows == 16) return launch_attn<T, INT8, WIDTH, 2, 3>(a, steps_bound, max_rt, sms, st);
+  return launch_attn<T, INT8, WIDTH, 4, 3>(a, steps_bound, max_rt, sms, st);
 }
 
 template <typename T>
-cudaError_t launch_type(CacheAttnKArgs& a, const CacheView& c, int rows, long long tiles_bound, int max_rt, int sms, cudaStream_t st) {
-  if (c.width == 64) return c.int8 ? launch_rows<T, true, 64>(a, rows, tiles_bound, max_rt, sms, st) : launch_rows<T, false, 64>(a, rows, tiles_bound, max_rt, sms, st);
-  return c.int8 ? launch_rows<T, true, 128>(a, rows, tiles_bound, max_rt, sms, st) : launch_rows<T, false, 128>(a, rows, tiles_bound, max_rt, sms, st);
+cudaError_t launch_type(CacheAttnKArgs& a, const CacheView& c, int rows, long long steps_bound, int max_rt, int sms, cudaStream_t st) {
+  if (c.width == 64) return c.int8 ? launch_rows<T, true, 64>(a, rows, steps_bound, max_rt, sms, st) : launch_rows<T, false, 64>(a, rows, steps_bound, max_rt, sms, st);
+  return c.int8 ? launch_rows<T, true, 128>(a, rows, steps_bound, max_rt, sms, st) : launch_rows<T, false, 128>(a, rows, steps_bound, max_rt, sms, st);
 }
+
+size_t part_rows(int64_t rows) { return (size_t)std::min<int64_t>(rows, rows_per_tile(rows)); }
 
 }  // namespace
 
 size_t cache_attention_scratch(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q) {
   (void)n_seq;
-  const size_t rows = (size_t)rows_per_tile(max_q * (Hq / Hkv));
-  return (size_t)2 * MAX_CTAS * rows * (HD * sizeof(float) + sizeof(float2));
+  return (size_t)2 * MAX_WARPS * part_rows(max_q * (Hq / Hkv)) * (HD * sizeof(float) + sizeof(float2));
 }
 
 cudaError_t launch_cache_attention(const CacheView& c, const CacheAttnParams& p, cudaStream_t st) {
@@ -800,14 +779,15 @@ cudaError_t launch_cache_attention(const CacheView& c, const CacheAttnParams& p,
   a.Hq = (int)p.Hq; a.Hkv = (int)c.H; a.group = (int)(p.Hq / c.H); a.max_q = (int)p.max_q; a.D = (int)c.D;
   a.sm_scale = p.sm_scale; a.scale_log2 = std::min(p.sm_scale * LOG2E_F, 3.0e38f);
   const int rows = rows_per_tile(p.max_q * a.group);
+  a.part_rows = (int)part_rows(p.max_q * a.group);
   a.part_o = reinterpret_cast<float*>(p.scratch);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * MAX_CTAS * rows * HD);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * MAX_WARPS * a.part_rows * HD);
   const long long max_rt = (p.max_q * a.group + rows - 1) / rows;
-  const long long tiles_bound = p.n_seq * c.H * max_rt * std::max<long long>(1, ((p.table_width << c.page_shift) + CA_KEYS - 1) / CA_KEYS);
+  const long long steps_bound = p.n_seq * c.H * max_rt * std::max<long long>(1, ((p.table_width << c.page_shift) + CA_KEYS - 1) / CA_KEYS);
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return p.dtype == 0 ? launch_type<__half>(a, c, rows, tiles_bound, (int)max_rt, sms, st)
-                      : launch_type<__nv_bfloat16>(a, c, rows, tiles_bound, (int)max_rt, sms, st);
+  return p.dtype == 0 ? launch_type<__half>(a, c, rows, steps_bound, (int)max_rt, sms, st)
+                      : launch_type<__nv_bfloat16>(a, c, rows, steps_bound, (int)max_rt, sms, st);
 }
 
 }  // namespace sage
