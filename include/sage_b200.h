@@ -403,7 +403,9 @@ int sage_cache_read(const void* k_codes, const float* k_scale, const void* v_cod
  * stretches whose ends follow from the lengths of all sequences, so that the same sequence in another batch
  * may differ in the order of fp32 sums; the same call gives the same bits.
  *   workspace   sage_cache_attention_workspace_bytes() bytes, 256-byte aligned; calls that may run at the same
- *               time (on two streams, in two captured graphs) each need their own */
+ *               time (on two streams, in two captured graphs) each need their own
+ *   status_host optional, as for sage_attention_reported: a pinned host word that receives a non-zero code when a
+ *               bounded wait of the kernel ran out (the output is then undefined); never written otherwise */
 size_t sage_cache_attention_workspace_bytes(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q);
 int sage_cache_attention(const void* q, void* out, float* lse,
                          const void* k_codes, const float* k_scale, const void* v_codes, const float* v_scale,
@@ -412,7 +414,7 @@ int sage_cache_attention(const void* q, void* out, float* lse,
                          const void* tree_mask, int64_t tree_stride, void* workspace, size_t workspace_bytes,
                          int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t total_q, int64_t max_q, int64_t head_dim,
                          int64_t pages, int64_t page_size, const int64_t q_strides[2], const int64_t o_strides[2],
-                         int dtype, int qk_mode, float sm_scale, void* stream);
+                         int dtype, int qk_mode, float sm_scale, int32_t* status_host, void* stream);
 
 /* Rotary positions on q (B, Hq, N, head_dim) and, if k is not null, on k (B, Hk, N, head_dim): pair i of the first
  * rotary_dim columns (columns i and i + rotary_dim / 2, or 2i and 2i + 1 with `interleaved`) of the row at position

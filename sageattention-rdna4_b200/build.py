@@ -16,8 +16,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "sageattention", "libsage_b200.so")
-SOURCES = ["sage_capi.cu", "sage_prologue.cu", "sage_attn_sm100.cu", "sage_cache.cu", "sage_cache_attn.cu"]
-HEADERS = ["sage_common.cuh", "sage_internal.h", os.path.join("..", "..", "include", "sage_b200.h")]
+SOURCES = ["sage_capi.cu", "sage_prologue.cu", "sage_attn_sm100.cu", "sage_cache.cu", "sage_cache_attn.cu", "sage_cache_tree.cu"]
+HEADERS = ["sage_common.cuh", "sage_internal.h", "sage_cache_attn.cuh", os.path.join("..", "..", "include", "sage_b200.h")]
 
 
 def nvcc_path() -> str:
@@ -40,7 +40,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return OUT
     cmd = [nvcc_path(), "-std=c++17", "-O3", "-lineinfo",
            "-gencode", "arch=compute_100a,code=sm_100a",
-           "-Xcompiler", "-fPIC", "-shared", "--threads", "5",
+           "-Xcompiler", "-fPIC", "-shared", "--threads", "6",
            "-o", OUT] + [os.path.join(CSRC, s) for s in SOURCES]
     if verbose:
         cmd.insert(1, "-Xptxas")

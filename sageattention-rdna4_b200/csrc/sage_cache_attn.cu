@@ -29,10 +29,7 @@
 // wait.  So ragged batches and single long sequences alike fill the GPU; lengths are read on the device.  A unit
 // that lies in several stretches leaves partial rows in the workspace, which cache_combine_kernel joins in the
 // order of the keys.
-#include <algorithm>
-
-#include "sage_common.cuh"
-#include "sage_internal.h"
+#include "sage_cache_attn.cuh"
 
 namespace sage {
 
@@ -40,143 +37,6 @@ namespace {
 
 constexpr int CA_WARPS = 4, CA_THREADS = 32 * CA_WARPS;
 constexpr int CA_KEYS = 32;                    // keys of a step: two blocks of 16
-constexpr float LN2_F = 0.6931471805599453f;
-constexpr float NO_MAX = -3.0e38f;
-
-struct CacheAttnKArgs {
-  const void* q;
-  void* out;
-  float* lse;
-  const uint8_t *kc, *vc;
-  const float *ks, *vs, *shift;
-  const int *table, *seqlens, *cu_q;
-  const uint8_t* tree;
-  float* part_o;             // (2 x stretches, part_rows, WIDTH)
-  float2* part_ml;           // (2 x stretches, part_rows): running maximum (log2 domain), sum
-  long long q_st, q_sh, o_st, o_sh, table_st, tree_st;
-  long long total_q;
-  int n_seq, table_width, pages, page_shift, Hq, Hkv, group, max_q, D;
-  int warps;                 // of the attention kernel: the line of steps is cut into so many stretches
-  int part_rows;             // rows of a partial result: those of a row tile that can exist
-  float sm_scale, scale_log2;
-};
-
-// A sequence as the kernels see it: lengths clamped, so that no access leaves the tensors whatever the arrays hold.
-struct Seq {
-  int q0, q_len, len;
-};
-__device__ __forceinline__ Seq seq_of(const CacheAttnKArgs& a, int b) {
-  Seq s;
-  if (a.cu_q == nullptr) {                           // max_q new tokens for every sequence
-    s.q0 = b * a.max_q;
-    s.q_len = a.max_q;
-  } else {
-    const long long q0 = min(max((long long)__ldg(a.cu_q + b), 0LL), a.total_q);
-    s.q0 = (int)q0;
-    s.q_len = (int)min(max(min((long long)__ldg(a.cu_q + b + 1), a.total_q) - q0, 0LL), (long long)a.max_q);
-  }
-  s.len = (int)min(max((long long)__ldg(a.seqlens + b), 0LL), (long long)a.table_width << a.page_shift);
-  return s;
-}
-__device__ __forceinline__ int row_tiles(const CacheAttnKArgs& a, const Seq& s, int rows) { return (s.q_len * a.group + rows - 1) / rows; }
-__device__ __forceinline__ int key_steps(const Seq& s) { return max(1, (s.len + CA_KEYS - 1) / CA_KEYS); }   // an empty sequence's rows are written too
-
-// The line of steps: sequence by sequence, K/V head by K/V head, row tile by row tile, step by step (fewer than 2^31
-// of them: the host sees to that).  Its stretches differ by one step at most; a line of fewer steps than warps leaves the
-// last warps without.
-struct Line {
-  unsigned total, n, per, longer;                    // steps, stretches, steps of a stretch, stretches that have one more
-  __device__ __forceinline__ Line(unsigned steps, int warps) : total(steps) {
-    n = min((unsigned)warps, steps);
-    per = n ? steps / n : 0u;
-    longer = steps - n * per;
-  }
-  __device__ __forceinline__ unsigned begin(unsigned x) const { return x * per + min(x, longer); }
-  // the stretch that has step u
-  __device__ __forceinline__ unsigned of(unsigned u) const {
-    const unsigned in_longer = longer * (per + 1);
-    return u < in_longer ? u / (per + 1) : longer + (u - in_longer) / per;
-  }
-};
-__device__ __forceinline__ unsigned steps_of_seq(const CacheAttnKArgs& a, int b, int rows) {
-  if (b >= a.n_seq) return 0;
-  const Seq s = seq_of(a, b);
-  return (unsigned)a.Hkv * row_tiles(a, s, rows) * key_steps(s);
-}
-
-// All threads of a CTA call this: the line, the sequence in which the warp's stretch begins (n_seq: it has none), and
-// the number of steps before that sequence.
-struct PlaceScratch {
-  unsigned sum[CA_WARPS], found[CA_WARPS], before[CA_WARPS];
-};
-__device__ __forceinline__ Line find_place(const CacheAttnKArgs& a, int rows, PlaceScratch& sh, int& seq, unsigned& steps_before) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  unsigned total = 0;
-  if (a.n_seq > CA_THREADS) {                        // the length of the line first
-    unsigned mine = 0;
-    for (int b = tid; b < a.n_seq; b += CA_THREADS) mine += steps_of_seq(a, b, rows);
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) sh.sum[warp] = mine;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < CA_WARPS; ++w) total += sh.sum[w];
-    __syncthreads();
-  }
-  if (tid < CA_WARPS) sh.found[tid] = a.n_seq;
-  Line line(total, a.warps);
-  unsigned base = 0;
-  for (int b0 = 0; b0 < a.n_seq; b0 += CA_THREADS) {
-    const unsigned n = steps_of_seq(a, b0 + tid, rows);
-    unsigned upto = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    if (lane == 31) sh.sum[warp] = upto;
-    __syncthreads();
-    unsigned before = base + upto - n;
-#pragma unroll
-    for (int w = 0; w < CA_WARPS; ++w) {
-      if (w < warp) before += sh.sum[w];
-      base += sh.sum[w];
-    }
-    if (a.n_seq <= CA_THREADS) line = Line(base, a.warps);
-#pragma unroll
-    for (int w = 0; w < CA_WARPS; ++w) {
-      const unsigned x = blockIdx.x * CA_WARPS + w, want = line.begin(x);
-      if (x < line.n && want >= before && want - before < n) { sh.found[w] = b0 + tid; sh.before[w] = before; }
-    }
-    __syncthreads();
-  }
-  seq = (int)sh.found[warp];
-  steps_before = sh.before[warp];
-  return line;
-}
-
-// A position on the line.
-struct Cursor {
-  Seq s;
-  int b, h, rt, kt;          // sequence, K/V head, row tile, step
-  int n_rt, n_kt;
-};
-__device__ __forceinline__ void enter_seq(const CacheAttnKArgs& a, Cursor& c, int rows) {
-  c.s = seq_of(a, c.b);
-  c.n_rt = row_tiles(a, c.s, rows);
-  c.n_kt = key_steps(c.s);
-}
-__device__ __forceinline__ void next_step(const CacheAttnKArgs& a, Cursor& c, int rows) {
-  if (++c.kt < c.n_kt) return;
-  c.kt = 0;
-  if (++c.rt < c.n_rt) return;
-  c.rt = 0;
-  if (++c.h < a.Hkv) return;
-  c.h = 0;
-  do {
-    if (++c.b >= a.n_seq) return;
-    enter_seq(a, c, rows);
-  } while (c.n_rt == 0);
-}
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
@@ -199,11 +59,6 @@ __device__ __forceinline__ float lds_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
-}
-__device__ __forceinline__ float fast_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -244,51 +99,23 @@ template <int WIDTH, int STAGES> struct CaSmem {
   static constexpr uint32_t BYTES = CA_WARPS * STAGES * STAGE;
 };
 
-// sm_scale * (row of Q) . (shift of the K/V head), by one warp
-template <typename T>
-__device__ __forceinline__ float shift_dot(const CacheAttnKArgs& a, const T* q, int h, int width, int lane) {
-  float d = 0.f;
-  for (int i = lane; i < a.D; i += 32) d = fmaf((float)q[i], __ldg(a.shift + (long long)h * width + i), d);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-  return d * a.sm_scale;
-}
-template <typename T> __device__ __forceinline__ uint32_t pair16(float a, float b);
-template <> __device__ __forceinline__ uint32_t pair16<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <> __device__ __forceinline__ uint32_t pair16<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <typename T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // NB: blocks of 8 query rows in a row tile.
 template <typename T, bool INT8, int WIDTH, int NB, int STAGES, int CTAS_PER_SM>
 __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(const CacheAttnKArgs a) {
   using L = CaSmem<WIDTH, STAGES>;
   constexpr int ROWS = 8 * NB, KSTEPS = WIDTH / 16, PIECES = WIDTH / 16;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ PlaceScratch place_s;
+  __shared__ PlaceScratch<CA_THREADS, CA_WARPS> place_s;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const unsigned stretch = blockIdx.x * CA_WARPS + warp;
   allow_successor();
   Cursor cur;
   unsigned before;
-  const Line line = find_place(a, ROWS, place_s, cur.b, before);
+  const Line line = find_place(a, ROWS, CA_KEYS, place_s, warp, cur.b, before);
   if (cur.b >= a.n_seq) return;
   const unsigned first = line.begin(stretch);
   const int n_steps = (int)(line.begin(stretch + 1) - first);
-  enter_seq(a, cur, ROWS);
-  {
-    const unsigned rest = first - before, unit = rest / (unsigned)cur.n_kt;
-    cur.kt = (int)(rest - unit * cur.n_kt);
-    cur.h = (int)(unit / (unsigned)cur.n_rt);
-    cur.rt = (int)unit - cur.h * cur.n_rt;
-  }
+  enter_line(a, cur, first, before, ROWS, CA_KEYS);
   Cursor ahead = cur;                                // the step whose loads are issued next
   const uint32_t ring = smem_addr(smem) + warp * STAGES * L::STAGE;
 
@@ -354,7 +181,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
     if (issued < n_steps) {
       issue(s);
       ++issued;
-      if (issued < n_steps) { next_step(a, ahead, ROWS); fetch_pages(); }
+      if (issued < n_steps) { next_step(a, ahead, ROWS, CA_KEYS); fetch_pages(); }
     }
     copy_commit();
   }
@@ -374,7 +201,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
     if (issued < n_steps) {
       issue(stage == 0 ? STAGES - 1 : stage - 1);
       ++issued;
-      if (issued < n_steps) { next_step(a, ahead, ROWS); fetch_pages(); }
+      if (issued < n_steps) { next_step(a, ahead, ROWS, CA_KEYS); fetch_pages(); }
     }
     copy_commit();
     if (fresh) {
@@ -627,7 +454,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
       }
       if (t + 1 < n_steps) {
         fresh = true;
-        next_step(a, cur, ROWS);
+        next_step(a, cur, ROWS, CA_KEYS);
         fetch_q();
         continue;
       }
@@ -636,24 +463,25 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   }
 }
 
-// Joins the parts of the units that lie in several stretches: a CTA per (unit, row), the parts spread over its
-// warps and added in a fixed order.
+// Joins the parts of the units that lie in several stretches, in a fixed order.  A CTA has 8 / WARPS_PER_ROW rows of a
+// unit: with all eight warps on a row the parts are spread over them (few rows, many parts: a step of one token), with
+// one each (hundreds of rows, two or three parts) a warp adds a row's by itself.
 constexpr int CC_WARPS = 8, CC_THREADS = 32 * CC_WARPS;
-template <typename T>
-__global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int width, int max_rt) {
+template <typename T, int WARPS_PER_ROW>
+__global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int keys, int width, int max_rt) {
   __shared__ unsigned total_s[CC_WARPS], before_s[CC_WARPS];
   __shared__ float acc_s[CC_WARPS][HD];
   __shared__ float2 ml_s[CC_WARPS];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // blockIdx.x = ((sequence * Hkv) + head) * max_rt + row tile; blockIdx.y = row
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = warp % WARPS_PER_ROW;
+  // blockIdx.x = ((sequence * Hkv) + head) * max_rt + row tile
   const unsigned bh = blockIdx.x / (unsigned)max_rt;
   const int rt = (int)(blockIdx.x - bh * max_rt), b = (int)(bh / (unsigned)a.Hkv), h = (int)(bh - (unsigned)b * a.Hkv);
   const Seq s = seq_of(a, b);                        // (the lengths are older than the attention kernel)
-  const int r = blockIdx.y, rr = rt * rows + r;
+  const int r = blockIdx.y * (CC_WARPS / WARPS_PER_ROW) + warp / WARPS_PER_ROW, rr = rt * rows + r;
   // steps before this sequence, and in all
   unsigned before = 0, total = 0;
   for (int i = tid; i < a.n_seq; i += CC_THREADS) {
-    const unsigned n = steps_of_seq(a, i, rows);
+    const unsigned n = steps_of_seq(a, i, rows, keys);
     total += n;
     if (i < b) before += n;
   }
@@ -664,23 +492,27 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
   total = 0; before = 0;
 #pragma unroll
   for (int w = 0; w < CC_WARPS; ++w) { total += total_s[w]; before += before_s[w]; }
-  const Line line(total, a.warps);
-  const int n_kt = key_steps(s);
+  const Line line(total, a.max_stretches);
+  const int n_kt = key_steps(s, keys);
   const unsigned u0 = before + ((unsigned)h * row_tiles(a, s, rows) + rt) * n_kt;
   const int c0 = total > 0 ? (int)line.of(u0) : 0, c1 = total > 0 ? (int)line.of(u0 + n_kt - 1) : 0;
   wait_for_predecessor();
-  if (rr >= s.q_len * a.group || c0 == c1) return;   // no such row, or written by the warp that had all of its unit
+  // no such row, or written by the one that had all of its unit  (the whole CTA leaves, or whole warps of rows)
+  if (rt >= row_tiles(a, s, rows) || c0 == c1) return;
+  const bool live = r < rows && rr < s.q_len * a.group;
+  if (WARPS_PER_ROW == 1 && !live) return;
+  if (WARPS_PER_ROW == CC_WARPS && !live) return;
   auto at_of = [&](int x) { return (2LL * x + (u0 > line.begin(x) ? 1 : 0)) * a.part_rows + r; };
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f, top = NO_MAX;
   const bool mine = 4 * lane < width;
   constexpr int AT_ONCE = 8;
-  for (int i0 = c0 + warp; i0 <= c1; i0 += CC_WARPS * AT_ONCE) {
+  for (int i0 = c0 + share; i0 <= c1; i0 += WARPS_PER_ROW * AT_ONCE) {
     float2 ml[AT_ONCE];
     float4 v[AT_ONCE];
 #pragma unroll
     for (int j = 0; j < AT_ONCE; ++j) {
-      const int i = i0 + j * CC_WARPS;
+      const int i = i0 + j * WARPS_PER_ROW;
       ml[j] = make_float2(NO_MAX, 0.f);
       v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i <= c1) {
@@ -702,24 +534,30 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
       acc.x = fmaf(v[j].x, weight, acc.x); acc.y = fmaf(v[j].y, weight, acc.y); acc.z = fmaf(v[j].z, weight, acc.z); acc.w = fmaf(v[j].w, weight, acc.w);
     }
   }
-  if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
-  if (lane == 0) ml_s[warp] = make_float2(top, sum);
-  __syncthreads();
-  top = NO_MAX; sum = 0.f;
-  float weight[CC_WARPS];
-#pragma unroll
-  for (int w = 0; w < CC_WARPS; ++w) top = fmaxf(top, ml_s[w].x);
-#pragma unroll
-  for (int w = 0; w < CC_WARPS; ++w) { weight[w] = fast_ex2(ml_s[w].x - top); sum = fmaf(ml_s[w].y, weight[w], sum); }
   const int tok = rr / a.group, head = h * a.group + rr - tok * a.group;
-  const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-  if (tid < a.D) {
-    float v = 0.f;
+  T* dst = reinterpret_cast<T*>(a.out) + (long long)(s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
+  if (WARPS_PER_ROW == 1) {
+    const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+    if (4 * lane < a.D) *reinterpret_cast<uint2*>(dst + 4 * lane) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
+  } else {
+    if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
+    if (lane == 0) ml_s[warp] = make_float2(top, sum);
+    __syncthreads();
+    top = NO_MAX; sum = 0.f;
+    float weight[CC_WARPS];
 #pragma unroll
-    for (int w = 0; w < CC_WARPS; ++w) v = fmaf(acc_s[w][tid], weight[w], v);
-    reinterpret_cast<T*>(a.out)[(long long)(s.q0 + tok) * a.o_st + (long long)head * a.o_sh + tid] = from_float<T>(v * inv);
+    for (int w = 0; w < CC_WARPS; ++w) top = fmaxf(top, ml_s[w].x);
+#pragma unroll
+    for (int w = 0; w < CC_WARPS; ++w) { weight[w] = fast_ex2(ml_s[w].x - top); sum = fmaf(ml_s[w].y, weight[w], sum); }
+    const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+    if (tid < a.D) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < CC_WARPS; ++w) v = fmaf(acc_s[w][tid], weight[w], v);
+      dst[tid] = from_float<T>(v * inv);
+    }
   }
-  if (a.lse != nullptr && warp == CC_WARPS - 1) {
+  if (a.lse != nullptr && share == WARPS_PER_ROW - 1) {
     float v = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * LN2_F;
     if (a.shift != nullptr)
       v += shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(s.q0 + tok) * a.q_st + (long long)head * a.q_sh, h, width, lane);
@@ -727,46 +565,58 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
   }
 }
 
-// Row tiles: 8, 16 or 32 rows, the smallest that holds all rows of a unit.
-int rows_per_tile(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 constexpr int CTAS_PER_SM = 2;
-constexpr int MAX_WARPS = 160 * CTAS_PER_SM * CA_WARPS;   // sized without a device at hand, for the largest SM count an sm_100 part has
+constexpr int SIZING_SMS = 160;                      // the workspace is sized without a device at hand, for the largest SM count an sm_100 part has
 
-template <typename T, bool INT8, int WIDTH, int NB, int STAGES>
-cudaError_t launch_attn(CacheAttnKArgs& a, long long steps_bound, int max_rt, int sms, cudaStream_t st) {
+template <typename T, bool INT8, int WIDTH, int NB>
+cudaError_t launch_attn(CacheAttnKArgs& a, int sms, cudaStream_t st) {
+  constexpr int STAGES = 3;
   auto kern = cache_attn_kernel<T, INT8, WIDTH, NB, STAGES, CTAS_PER_SM>;
   constexpr uint32_t smem = CaSmem<WIDTH, STAGES>::BYTES;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  const int ctas = (int)std::min<long long>(std::min(sms * CTAS_PER_SM, MAX_WARPS / CA_WARPS), (steps_bound + CA_WARPS - 1) / CA_WARPS);
-  a.warps = ctas * CA_WARPS;
-  kern<<<ctas, CA_THREADS, smem, st>>>(a);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((long long)a.n_seq * a.Hkv * max_rt), (unsigned)a.part_rows);
-  return launch_after_predecessor(cache_combine_kernel<T>, grid, dim3(CC_THREADS), 0, st, a, 8 * NB, WIDTH, max_rt);
+  a.max_stretches = std::min(sms, SIZING_SMS) * CTAS_PER_SM * CA_WARPS;
+  const long long steps = (long long)a.n_seq * a.Hkv * std::max<long long>(1, (((long long)a.table_width << a.page_shift) + CA_KEYS - 1) / CA_KEYS);
+  kern<<<(unsigned)std::min<long long>(a.max_stretches / CA_WARPS, (steps + CA_WARPS - 1) / CA_WARPS), CA_THREADS, smem, st>>>(a);
+  return cudaGetLastError();
 }
 
 template <typename T, bool INT8, int WIDTH>
-cudaError_t launch_rows(CacheAttnKArgs& a, int rows, long long steps_bound, int max_rt, int sms, cudaStream_t st) {
-  if (rows == 8) return launch_attn<T, INT8, WIDTH, 1, 3>(a, steps_bound, max_rt, sms, st);
-  if (rows == 16) return launch_attn<T, INT8, WIDTH, 2, 3>(a, steps_bound, max_rt, sms, st);
-  return launch_attn<T, INT8, WIDTH, 4, 3>(a, steps_bound, max_rt, sms, st);
+cudaError_t launch_rows(CacheAttnKArgs& a, int rows, int sms, cudaStream_t st) {
+  return rows == 8 ? launch_attn<T, INT8, WIDTH, 1>(a, sms, st) : launch_attn<T, INT8, WIDTH, 2>(a, sms, st);
 }
 
 template <typename T>
-cudaError_t launch_type(CacheAttnKArgs& a, const CacheView& c, int rows, long long steps_bound, int max_rt, int sms, cudaStream_t st) {
-  if (c.width == 64) return c.int8 ? launch_rows<T, true, 64>(a, rows, steps_bound, max_rt, sms, st) : launch_rows<T, false, 64>(a, rows, steps_bound, max_rt, sms, st);
-  return c.int8 ? launch_rows<T, true, 128>(a, rows, steps_bound, max_rt, sms, st) : launch_rows<T, false, 128>(a, rows, steps_bound, max_rt, sms, st);
+cudaError_t launch_type(CacheAttnKArgs& a, const CacheView& c, int rows, int sms, cudaStream_t st) {
+  if (c.width == 64) return c.int8 ? launch_rows<T, true, 64>(a, rows, sms, st) : launch_rows<T, false, 64>(a, rows, sms, st);
+  return c.int8 ? launch_rows<T, true, 128>(a, rows, sms, st) : launch_rows<T, false, 128>(a, rows, sms, st);
 }
 
-size_t part_rows(int64_t rows) { return (size_t)std::min<int64_t>(rows, rows_per_tile(rows)); }
+template <typename T>
+cudaError_t launch_combine_t(const CacheAttnKArgs& a, int rows, int keys, int width, int max_rt, cudaStream_t st) {
+  const unsigned units = (unsigned)((long long)a.n_seq * a.Hkv * max_rt);
+  if (rows <= 16)
+    return launch_after_predecessor(cache_combine_kernel<T, CC_WARPS>, dim3(units, (unsigned)a.part_rows), dim3(CC_THREADS), 0, st, a, rows, keys, width, max_rt);
+  return launch_after_predecessor(cache_combine_kernel<T, 1>, dim3(units, (unsigned)((a.part_rows + CC_WARPS - 1) / CC_WARPS)), dim3(CC_THREADS), 0, st,
+                                  a, rows, keys, width, max_rt);
+}
 
 }  // namespace
 
+cudaError_t launch_cache_combine(const CacheAttnKArgs& a, int dtype, int rows, int keys, int width, int max_rt, cudaStream_t st) {
+  return dtype == 0 ? launch_combine_t<__half>(a, rows, keys, width, max_rt, st) : launch_combine_t<__nv_bfloat16>(a, rows, keys, width, max_rt, st);
+}
+
+CacheForm cache_form(int64_t rows) {
+  if (rows <= 16) return {false, rows <= 8 ? 8 : 16, CA_KEYS, SIZING_SMS * CTAS_PER_SM * CA_WARPS};
+  return rows <= 128 ? CacheForm{true, 128, 64, 2 * SIZING_SMS} : CacheForm{true, 256, 128, SIZING_SMS};
+}
+
 size_t cache_attention_scratch(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q) {
   (void)n_seq;
-  return (size_t)2 * MAX_WARPS * part_rows(max_q * (Hq / Hkv)) * (HD * sizeof(float) + sizeof(float2));
+  const int64_t rows = max_q * (Hq / Hkv);
+  const CacheForm f = cache_form(rows);
+  return (size_t)2 * f.max_stretches * std::min<int64_t>(rows, f.rows) * (HD * sizeof(float) + sizeof(float2));
 }
 
 cudaError_t launch_cache_attention(const CacheView& c, const CacheAttnParams& p, cudaStream_t st) {
@@ -778,16 +628,17 @@ cudaError_t launch_cache_attention(const CacheView& c, const CacheAttnParams& p,
   a.n_seq = (int)p.n_seq; a.table_width = (int)p.table_width; a.pages = (int)c.pages; a.page_shift = c.page_shift;
   a.Hq = (int)p.Hq; a.Hkv = (int)c.H; a.group = (int)(p.Hq / c.H); a.max_q = (int)p.max_q; a.D = (int)c.D;
   a.sm_scale = p.sm_scale; a.scale_log2 = std::min(p.sm_scale * LOG2E_F, 3.0e38f);
-  const int rows = rows_per_tile(p.max_q * a.group);
-  a.part_rows = (int)part_rows(p.max_q * a.group);
+  const int64_t rows = p.max_q * a.group;
+  const CacheForm f = cache_form(rows);
+  a.part_rows = (int)std::min<int64_t>(rows, f.rows);
   a.part_o = reinterpret_cast<float*>(p.scratch);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * MAX_WARPS * a.part_rows * HD);
-  const long long max_rt = (p.max_q * a.group + rows - 1) / rows;
-  const long long steps_bound = p.n_seq * c.H * max_rt * std::max<long long>(1, ((p.table_width << c.page_shift) + CA_KEYS - 1) / CA_KEYS);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * f.max_stretches * a.part_rows * HD);
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return p.dtype == 0 ? launch_type<__half>(a, c, rows, steps_bound, (int)max_rt, sms, st)
-                      : launch_type<__nv_bfloat16>(a, c, rows, steps_bound, (int)max_rt, sms, st);
+  const cudaError_t e = f.tree ? launch_cache_tree(a, c, p.dtype, sms, p.status_host, st)
+                               : p.dtype == 0 ? launch_type<__half>(a, c, f.rows, sms, st) : launch_type<__nv_bfloat16>(a, c, f.rows, sms, st);
+  if (e != cudaSuccess) return e;
+  return launch_cache_combine(a, p.dtype, f.rows, f.keys, c.width, (int)((rows + f.rows - 1) / f.rows), st);
 }
 
 }  // namespace sage

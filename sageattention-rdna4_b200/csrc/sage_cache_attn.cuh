@@ -1,0 +1,198 @@
+// What the kernels of sageattn_cached share: arguments, the line of work, and its division (see sage_cache_attn.cu).
+#pragma once
+
+#include <algorithm>
+
+#include "sage_common.cuh"
+#include "sage_internal.h"
+
+namespace sage {
+
+constexpr float LN2_F = 0.6931471805599453f;
+constexpr float NO_MAX = -3.0e38f;
+
+struct CacheAttnKArgs {
+  const void* q;
+  void* out;
+  float* lse;
+  const uint8_t *kc, *vc;
+  const float *ks, *vs, *shift;
+  const int *table, *seqlens, *cu_q;
+  const uint8_t* tree;
+  float* part_o;             // (2 x stretches, part_rows, WIDTH)
+  float2* part_ml;           // (2 x stretches, part_rows): running maximum (log2 domain), sum
+  long long q_st, q_sh, o_st, o_sh, table_st, tree_st;
+  long long total_q;
+  int n_seq, table_width, pages, page_shift, Hq, Hkv, group, max_q, D;
+  int max_stretches;         // the line of steps is cut into so many stretches
+  int part_rows;             // rows of a partial result: those of a row tile that can exist
+  float sm_scale, scale_log2;
+};
+
+// A sequence as the kernels see it: lengths clamped, so that no access leaves the tensors whatever the arrays hold.
+struct Seq {
+  int q0, q_len, len;
+};
+__device__ __forceinline__ Seq seq_of(const CacheAttnKArgs& a, int b) {
+  Seq s;
+  if (a.cu_q == nullptr) {                           // max_q new tokens for every sequence
+    s.q0 = b * a.max_q;
+    s.q_len = a.max_q;
+  } else {
+    const long long q0 = min(max((long long)__ldg(a.cu_q + b), 0LL), a.total_q);
+    s.q0 = (int)q0;
+    s.q_len = (int)min(max(min((long long)__ldg(a.cu_q + b + 1), a.total_q) - q0, 0LL), (long long)a.max_q);
+  }
+  s.len = (int)min(max((long long)__ldg(a.seqlens + b), 0LL), (long long)a.table_width << a.page_shift);
+  return s;
+}
+__device__ __forceinline__ int row_tiles(const CacheAttnKArgs& a, const Seq& s, int rows) { return (s.q_len * a.group + rows - 1) / rows; }
+__device__ __forceinline__ int key_steps(const Seq& s, int keys) { return max(1, (s.len + keys - 1) / keys); }   // an empty sequence's rows are written too
+
+// The line of steps (of so many keys each): sequence by sequence, K/V head by K/V head, row tile by row tile (of so many
+// rows each), step by step; fewer than 2^31 of them, the host sees to that.  Its stretches differ by one step at most;
+// a line of fewer steps than stretches wanted leaves the last ones out.
+struct Line {
+  unsigned total, n, per, longer;                    // steps, stretches, steps of a stretch, stretches that have one more
+  __device__ __forceinline__ Line(unsigned steps, int most) : total(steps) {
+    n = min((unsigned)most, steps);
+    per = n ? steps / n : 0u;
+    longer = steps - n * per;
+  }
+  __device__ __forceinline__ unsigned begin(unsigned x) const { return x * per + min(x, longer); }
+  // the stretch that has step u
+  __device__ __forceinline__ unsigned of(unsigned u) const {
+    const unsigned in_longer = longer * (per + 1);
+    return u < in_longer ? u / (per + 1) : longer + (u - in_longer) / per;
+  }
+};
+__device__ __forceinline__ unsigned steps_of_seq(const CacheAttnKArgs& a, int b, int rows, int keys) {
+  if (b >= a.n_seq) return 0;
+  const Seq s = seq_of(a, b);
+  return (unsigned)a.Hkv * row_tiles(a, s, rows) * key_steps(s, keys);
+}
+
+// All threads of a CTA call this: the line, the sequence in which the CTA's stretch `which` (of OWN) begins (n_seq: it
+// has none), and the number of steps before that sequence.
+template <int THREADS, int OWN> struct PlaceScratch {
+  unsigned sum[THREADS / 32], found[OWN], before[OWN];
+};
+template <int THREADS, int OWN>
+__device__ __forceinline__ Line find_place(const CacheAttnKArgs& a, int rows, int keys, PlaceScratch<THREADS, OWN>& sh, int which, int& seq,
+                                           unsigned& steps_before) {
+  constexpr int WARPS = THREADS / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  unsigned total = 0;
+  if (a.n_seq > THREADS) {                           // the length of the line first
+    unsigned mine = 0;
+    for (int b = tid; b < a.n_seq; b += THREADS) mine += steps_of_seq(a, b, rows, keys);
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) sh.sum[warp] = mine;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total += sh.sum[w];
+    __syncthreads();
+  }
+  if (tid < OWN) sh.found[tid] = a.n_seq;
+  Line line(total, a.max_stretches);
+  unsigned base = 0;
+  for (int b0 = 0; b0 < a.n_seq; b0 += THREADS) {
+    const unsigned n = steps_of_seq(a, b0 + tid, rows, keys);
+    unsigned upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) sh.sum[warp] = upto;
+    __syncthreads();
+    unsigned before = base + upto - n;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before += sh.sum[w];
+      base += sh.sum[w];
+    }
+    if (a.n_seq <= THREADS) line = Line(base, a.max_stretches);
+#pragma unroll
+    for (int w = 0; w < OWN; ++w) {
+      const unsigned x = blockIdx.x * OWN + w, want = line.begin(x);
+      if (x < line.n && want >= before && want - before < n) { sh.found[w] = b0 + tid; sh.before[w] = before; }
+    }
+    __syncthreads();
+  }
+  seq = (int)sh.found[which];
+  steps_before = sh.before[which];
+  return line;
+}
+
+// A position on the line.
+struct Cursor {
+  Seq s;
+  int b, h, rt, kt;          // sequence, K/V head, row tile, step
+  int n_rt, n_kt;
+};
+__device__ __forceinline__ void enter_seq(const CacheAttnKArgs& a, Cursor& c, int rows, int keys) {
+  c.s = seq_of(a, c.b);
+  c.n_rt = row_tiles(a, c.s, rows);
+  c.n_kt = key_steps(c.s, keys);
+}
+__device__ __forceinline__ void next_step(const CacheAttnKArgs& a, Cursor& c, int rows, int keys) {
+  if (++c.kt < c.n_kt) return;
+  c.kt = 0;
+  if (++c.rt < c.n_rt) return;
+  c.rt = 0;
+  if (++c.h < a.Hkv) return;
+  c.h = 0;
+  do {
+    if (++c.b >= a.n_seq) return;
+    enter_seq(a, c, rows, keys);
+  } while (c.n_rt == 0);
+}
+// The cursor of step `first` of the line, in the sequence that find_place gave.
+__device__ __forceinline__ void enter_line(const CacheAttnKArgs& a, Cursor& c, unsigned first, unsigned before, int rows, int keys) {
+  enter_seq(a, c, rows, keys);
+  const unsigned rest = first - before, unit = rest / (unsigned)c.n_kt;
+  c.kt = (int)(rest - unit * c.n_kt);
+  c.h = (int)(unit / (unsigned)c.n_rt);
+  c.rt = (int)unit - c.h * c.n_rt;
+}
+
+__device__ __forceinline__ float fast_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// sm_scale * (row of Q) . (shift of the K/V head), by one warp
+template <typename T>
+__device__ __forceinline__ float shift_dot(const CacheAttnKArgs& a, const T* q, int h, int width, int lane) {
+  float d = 0.f;
+  for (int i = lane; i < a.D; i += 32) d = fmaf((float)q[i], __ldg(a.shift + (long long)h * width + i), d);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  return d * a.sm_scale;
+}
+template <typename T> __device__ __forceinline__ uint32_t pair16(float a, float b);
+template <> __device__ __forceinline__ uint32_t pair16<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pair16<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Joins partial results (see sage_cache_attn.cu); rows and keys are those of a row tile and of a step.
+cudaError_t launch_cache_combine(const CacheAttnKArgs& a, int dtype, int rows, int keys, int width, int max_rt, cudaStream_t st);
+// The kernel for many rows (see sage_cache_tree.cu); status_host: optional pinned word for its bounded waits.
+cudaError_t launch_cache_tree(CacheAttnKArgs& a, const CacheView& c, int dtype, int sms, int32_t* status_host, cudaStream_t st);
+// How a call is served, as host arithmetic: rows of a row tile, keys of a step, stretches at most on any device.
+struct CacheForm {
+  bool tree;
+  int rows, keys, max_stretches;
+};
+CacheForm cache_form(int64_t rows);
+
+}  // namespace sage

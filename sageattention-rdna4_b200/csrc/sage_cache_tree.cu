@@ -1,0 +1,637 @@
+// sageattn_cached for many rows: trees and chains of drafted tokens whose rows (new token x query head of the
+// group) fill the tensor core's 128-row operand.  Same formulas, line of work and partial results as
+// sage_cache_attn.cu; the products are tcgen05.mma with accumulators in TMEM.
+//
+// A CTA takes a row tile of NQ x 128 rows and walks its stretch of the keys, KT at a time:
+//   warps 0 .. 4 NQ - 1   softmax: a thread owns a row (32x32b TMEM loads: a lane is a row), so that maxima and sums
+//                         need no other lane; its weights go back to TMEM as fp16, over the scores they came from, and
+//                         are the A operand of P V from there
+//   the next four warps   fetch the one-byte codes (a tile ahead, in registers), turn them into fp16 -- exact -- and
+//                         write them to shared memory as the operands want them (128-byte swizzle), two stages deep
+//   one more warp         one thread issues every tcgen05.mma and commit (three idle warps complete its warpgroup, whose
+//                         registers the softmax takes over)
+// K is a K-major operand; V, whose rows are keys too, is the MN-major B operand of P V: both are written alike, a
+// row of 64 columns in 128 bytes.  Heads of more than 64 columns take two such halves; columns 16 p .. 16 p + 7 of a
+// row go to piece p of the first half and the next 8 to piece p of the second, for K, Q and V alike, so that the
+// eight lanes that write the pieces of a row reach all banks (the order of an inner product's columns is free, and
+// that of V's is undone where the output is written).
+//
+// NQ = 2, KT = 128 (rows beyond 128): one CTA per SM with all 512 TMEM columns, {S 128, O 128} per 128 rows; while one
+// half's softmax runs the other half's products do.  NQ = 1, KT = 64: two CTAs per SM, which overlap each other.
+// (Converting a tile costs about a fifth of one half's softmax, so rows are added to a CTA before CTAs are.)
+//
+// Every wait is bounded (about two seconds): it then leaves a code in the caller's pinned host word, the CTA drains
+// its products, frees its TMEM and returns.
+#include "sage_cache_attn.cuh"
+
+namespace sage {
+
+namespace {
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+constexpr long long WAIT_CYCLES = 4000000000LL;      // about two seconds of SM clock
+struct Watch {
+  volatile uint32_t* abort;                          // in shared memory: someone of this CTA gave up
+  int32_t* host;                                     // optional pinned word
+};
+__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, const Watch& w, int code) {
+  const long long t0 = clock64();
+  for (uint32_t it = 1;; ++it) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((it & 255u) == 0u) {
+      if (*w.abort) return false;
+      if (clock64() - t0 > WAIT_CYCLES) {
+        *w.abort = 1u;
+        if (w.host != nullptr) *reinterpret_cast<volatile int32_t*>(w.host) = code;
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Watch& w, int code) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
+  if (__builtin_expect(ok != 0u, 1)) return true;
+  return mbar_wait_slow(bar, parity, w, code);
+}
+enum { CODE_LOAD = 1, CODE_MMA = 2, CODE_SOFTMAX = 4 };   // the bits of the framework's status words
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void sts_f32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void sts_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
+// Descriptors of 128-byte rows in the 128-byte swizzle, 8-row groups 1024 bytes apart: as a K-major operand, and as
+// an MN-major one whose next 64 columns lie `lead` bytes further.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// 16 codes -> 16 fp16 in eight registers, exact.
+template <bool INT8>
+__device__ __forceinline__ void codes_to_half(const uint4& u, uint32_t (&h)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (INT8) {
+      const uint32_t t = w[i] ^ 0x80808080u;         // code + 128 in a byte; 0x6400 + it is 1024 + it
+      const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+      const uint32_t a = __byte_perm(t, 0x64646464u, 0x4140), b = __byte_perm(t, 0x64646464u, 0x4342);
+      const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+      h[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
+      h[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+      asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
+          : "=r"(h[2 * i]), "=r"(h[2 * i + 1]) : "r"(w[i]));
+    }
+  }
+}
+
+template <int WIDTH, int NQ, int KT> struct TreeShape {
+  static constexpr int SOFTMAX = 128 * NQ, LOADERS = 128, THREADS = SOFTMAX + LOADERS + 128;
+  static constexpr int CTAS_PER_SM = NQ == 1 ? 2 : 1;
+  // Registers per thread: at launch (what __launch_bounds__ leaves: 65536 / threads of the SM, in eights), and after the
+  // issuing warpgroup has handed its own to the softmax.  setmaxnreg.inc waits until the pool holds what it asks for, so
+  // that the three must not add up to more than the launch has.
+  static constexpr int REGS_LAUNCH = NQ == 1 ? 80 : 128, REGS_SOFTMAX = NQ == 1 ? 120 : 168, REGS_ISSUER = NQ == 1 ? 40 : 48;
+  static_assert(NQ * REGS_SOFTMAX + REGS_LAUNCH + REGS_ISSUER <= (NQ + 2) * REGS_LAUNCH, "setmaxnreg would wait forever");
+  static constexpr int STAGES = 2, SLOTS = 4;
+  static constexpr uint32_t HALVES = WIDTH / 64;
+  static constexpr uint32_t Q_HALF = 128 * 128, Q_TILE = HALVES * Q_HALF;             // 128 rows of 128 bytes
+  static constexpr uint32_t KV_HALF = KT * 128, KV_TILE = HALVES * KV_HALF;
+  static constexpr uint32_t OFF_Q = 0, OFF_K = NQ * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE, OFF_SC = OFF_V + STAGES * KV_TILE;
+  static constexpr uint32_t SLOT = KT * 8 + 16;                                       // scales of K, scales of V, a flag per 32 keys
+  static constexpr uint32_t OFF_BAR = OFF_SC + SLOTS * SLOT, OFF_MISC = OFF_BAR + 176, USED = OFF_MISC + 16;
+  static constexpr uint32_t BYTES = USED + 1024;                                      // slack for the 1024-byte alignment
+  static constexpr uint32_t TMEM_COLS = NQ * (KT + WIDTH) <= 128 ? 128 : NQ * (KT + WIDTH) <= 256 ? 256 : 512;
+  static constexpr int ROWS = 128 * NQ;
+};
+// Barriers: per half of the rows (QF, SF, PF, PV), per stage (KF, KE, VF, VE), per slot of scales (SC).
+enum { B_QF = 0, B_KF = 2, B_KE = 4, B_VF = 6, B_VE = 8, B_SF = 10, B_PF = 12, B_PV = 14, B_SC = 16, B_DRAIN = 20, B_COUNT = 21 };
+
+template <typename T, bool INT8, int WIDTH, int NQ, int KT>
+__global__ void __launch_bounds__(TreeShape<WIDTH, NQ, KT>::THREADS, TreeShape<WIDTH, NQ, KT>::CTAS_PER_SM)
+cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
+  using L = TreeShape<WIDTH, NQ, KT>;
+  constexpr int ROWS = L::ROWS, CHUNKS = KT / 32;
+  constexpr uint32_t IDESC_QK = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
+  constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(WIDTH >> 3) << 17) | (8u << 24);   // B is MN-major
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ PlaceScratch<L::THREADS, 1> place_s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  allow_successor();
+  Cursor cur;
+  unsigned before;
+  const Line line = find_place<L::THREADS, 1>(a, ROWS, KT, place_s, 0, cur.b, before);
+  if (cur.b >= a.n_seq) return;                      // (the whole CTA)
+  const unsigned first = line.begin(blockIdx.x);
+  const int n_tiles = (int)(line.begin(blockIdx.x + 1) - first);
+  enter_line(a, cur, first, before, ROWS, KT);
+
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = base + L::OFF_BAR;
+  uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
+  volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(gbase + L::OFF_MISC);   // [0] TMEM address, [1] abort
+  const Watch watch = {misc + 1, status_host};
+  auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(B_QF + i), 4);
+      mbar_init(bar(B_KF + i), 4); mbar_init(bar(B_KE + i), 1);
+      mbar_init(bar(B_VF + i), 4); mbar_init(bar(B_VE + i), 1);
+      mbar_init(bar(B_SF + i), 1); mbar_init(bar(B_PF + i), 4); mbar_init(bar(B_PV + i), 1);
+    }
+    for (int i = 0; i < L::SLOTS; ++i) mbar_init(bar(B_SC + i), KT / 32);
+    mbar_init(bar(B_DRAIN), 1);
+    misc[1] = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  constexpr int ISSUER = (L::SOFTMAX + L::LOADERS) / 32;
+  if (warp == ISSUER) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::OFF_MISC), "r"(L::TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = misc[0];
+  auto tmem_s = [&](int g) { return tmem + (uint32_t)(g * KT); };
+  auto tmem_o = [&](int g) { return tmem + (uint32_t)(NQ * KT + g * WIDTH); };
+  // halves of a row tile that hold rows
+  auto halves_of = [&](const Cursor& c) { return NQ == 2 && c.s.q_len * a.group - c.rt * ROWS > 128 ? 2 : 1; };
+
+  if (tid < L::SOFTMAX) {
+    // ------------------------------------------------- softmax -------------------------------------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::REGS_SOFTMAX));
+    const int g = warp >> 2, r = tid & 127;
+    const uint32_t lane_sel = (uint32_t)(warp & 3) << 21;                             // 32 lanes of TMEM per warp
+    const uint32_t s_addr = tmem_s(g) + lane_sel, o_addr = tmem_o(g) + lane_sel;
+    bool ok = true;
+    int left = n_tiles, n = 0, done = 0;             // tiles to go; tiles of the CTA, and of this half, that are behind
+    while (ok && left > 0) {
+      const int count = min(left, cur.n_kt - cur.kt), kt0 = cur.kt;
+      const int ng = halves_of(cur);
+      const int live = cur.s.q_len * a.group - cur.rt * ROWS - 128 * g;               // rows of this half that exist
+      const int rr = cur.rt * ROWS + 128 * g + r, tok = rr / a.group, head = cur.h * a.group + rr - tok * a.group;
+      const bool exists = r < live;
+      const T* q_row = reinterpret_cast<const T*>(a.q) + (long long)(cur.s.q0 + tok) * a.q_st + (long long)head * a.q_sh;
+      float row_c = a.scale_log2;
+      if (g < ng) {
+        auto q_piece = [&](int i) { return exists && 8 * i < a.D ? __ldg(reinterpret_cast<const uint4*>(q_row + 8 * i)) : make_uint4(0u, 0u, 0u, 0u); };
+        float up = 1.f;
+        if (!__is_same(T, __half)) {                 // bf16: the row's largest element to [2^14, 2^15)
+          float amax = 0.f;
+#pragma unroll 4
+          for (int i = 0; i < WIDTH / 8; ++i) {
+            float x[8];
+            unpack8<T>(q_piece(i), x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+          }
+          const int field = (int)(__float_as_uint(amax) >> 23);
+          if (field > 14 && field < 255) {
+            const int f = min(254, 268 - field);
+            up = __uint_as_float((uint32_t)f << 23);
+            row_c *= f <= 253 ? __uint_as_float((uint32_t)(254 - f) << 23) : 5.877471754111438e-39f;
+          }
+        }
+        row_c = fmaxf(row_c, 1.17549435e-38f);       // (a masked score stays -infinity)
+        const uint32_t q_smem = base + L::OFF_Q + g * L::Q_TILE + r * 128;
+#pragma unroll 4
+        for (int i = 0; i < WIDTH / 8; ++i) {
+          const uint4 raw = q_piece(i);
+          uint32_t h[4] = {raw.x, raw.y, raw.z, raw.w};
+          if (!__is_same(T, __half)) {
+            float x[8];
+            unpack8<T>(raw, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = pair16<__half>(x[2 * e] * up, x[2 * e + 1] * up);
+          }
+          const int piece = WIDTH == 128 ? i >> 1 : i;
+          sts16(q_smem + (WIDTH == 128 ? (i & 1) * L::Q_HALF : 0u) + 16 * (piece ^ (r & 7)), h[0], h[1], h[2], h[3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_QF + g));
+      }
+      const int ctx = cur.s.len - cur.s.q_len;
+      const int t_first = (cur.rt * ROWS + 128 * g) / a.group;
+      const int plain_end = a.tree ? max(ctx, 0) : max(0, min(cur.s.len, ctx + t_first + 1));   // keys below need no mask
+      const int lim = exists ? (a.tree ? cur.s.len : min(cur.s.len, ctx + tok + 1)) : 0;
+      const uint8_t* tree_row = a.tree ? a.tree + (long long)(cur.s.q0 + tok) * a.tree_st : nullptr;
+      float m = NO_MAX, l = 0.f, nf = 0.f;
+
+      if (g < ng) {
+        for (int t = 0; t < count; ++t) {
+          const uint32_t sc = base + L::OFF_SC + ((n + t) % L::SLOTS) * L::SLOT;
+          ok = mbar_wait(bar(B_SF + g), (uint32_t)(done + t) & 1u, watch, CODE_SOFTMAX);
+          if (ok && t > 0) ok = mbar_wait(bar(B_PV + g), (uint32_t)(done + t - 1) & 1u, watch, CODE_SOFTMAX);   // (issued before the scores)
+          if (ok) ok = mbar_wait(bar(B_SC + (n + t) % L::SLOTS), (uint32_t)((n + t) / L::SLOTS) & 1u, watch, CODE_SOFTMAX);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const int key0 = (kt0 + t) * KT;
+          uint32_t absent = lds_u32(sc + KT * 8) | lds_u32(sc + KT * 8 + 4);
+          if (KT == 128) absent |= lds_u32(sc + KT * 8 + 8) | lds_u32(sc + KT * 8 + 12);
+          const bool masked = key0 + KT > plain_end || absent != 0u;
+          // bit i: key key0 + 32 ch + i is seen by this row
+          auto seen_bits = [&](int ch) -> uint32_t {
+            uint32_t bits = 0u;
+            for (int i = 0; i < 32; ++i) {
+              const int key = key0 + 32 * ch + i;
+              bool seen = key < lim;
+              if (tree_row != nullptr && seen && key >= ctx) seen = tree_row[key - ctx] != 0;
+              bits |= seen ? 1u << i : 0u;
+            }
+            if (absent != 0u)
+              for (int i = 0; i < 32; ++i) {
+                float sk;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sk) : "r"(sc + 4 * (32 * ch + i)));
+                if (sk < 0.f) bits &= ~(1u << i);
+              }
+            return bits;
+          };
+          uint32_t pw[KT / 2];
+          float2 sum2 = make_float2(0.f, 0.f);
+          __half2 w_top = __float2half2_rn(0.f);
+          // weights of 32 columns against the maximum m and the factor nf
+          auto weigh = [&](int ch) {
+            const uint32_t bits = masked ? seen_bits(ch) : 0xffffffffu;
+            __syncwarp();
+            uint32_t s[32];
+            tmem_ld32(s_addr + 32 * ch, s);
+            const float2 c2 = make_float2(row_c, row_c), nm2 = make_float2(-m, -m), nf2 = make_float2(nf, nf);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 sk = lds_f4(sc + 4 * (32 * ch + i)), sv = lds_f4(sc + KT * 4 + 4 * (32 * ch + i));
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                float2 x = make_float2(__uint_as_float(s[i + e]), __uint_as_float(s[i + e + 1]));
+                x = __fmul2_rn(x, e ? make_float2(sk.z, sk.w) : make_float2(sk.x, sk.y));
+                float2 d = __ffma2_rn(x, c2, nm2);
+                if (masked) {
+                  if (!(bits >> (i + e) & 1u)) d.x = -INFINITY;
+                  if (!(bits >> (i + e + 1) & 1u)) d.y = -INFINITY;
+                }
+                const float2 p = make_float2(fast_ex2(d.x), fast_ex2(d.y));
+                sum2 = __fadd2_rn(sum2, p);
+                float2 w = __fmul2_rn(p, __fmul2_rn(e ? make_float2(sv.z, sv.w) : make_float2(sv.x, sv.y), nf2));
+                if (masked) {                        // an exact zero whatever the key's scale holds
+                  if (!(bits >> (i + e) & 1u)) w.x = 0.f;
+                  if (!(bits >> (i + e + 1) & 1u)) w.y = 0.f;
+                }
+                const __half2 h = __floats2half2_rn(w.x, w.y);
+                w_top = __hmax2(w_top, h);
+                pw[(32 * ch + i + e) / 2] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+            }
+          };
+#pragma unroll
+          for (int ch = 0; ch < CHUNKS; ++ch) weigh(ch);
+          float sum = sum2.x + sum2.y;
+          // (a weight above 2^8 shows in the sum)
+          const float2 wt = __half22float2(w_top);
+          if (__any_sync(0xffffffffu, sum > 256.f || fmaxf(wt.x, wt.y) > 4096.f)) {
+            // new maximum and factor; the sum and the accumulator follow, and the weights are worked out again
+            float top = m;
+            for (int ch = 0; ch < CHUNKS; ++ch) {
+              const uint32_t bits = masked ? seen_bits(ch) : 0xffffffffu;
+              __syncwarp();
+              uint32_t s[32];
+              tmem_ld32(s_addr + 32 * ch, s);
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 sk = lds_f4(sc + 4 * (32 * ch + i));
+                const float f[4] = {sk.x, sk.y, sk.z, sk.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (bits >> (i + e) & 1u) top = fmaxf(top, __uint_as_float(s[i + e]) * f[e] * row_c);
+              }
+            }
+            float big = 0.f;
+            for (int ch = 0; ch < CHUNKS; ++ch) {
+              const uint32_t bits = masked ? seen_bits(ch) : 0xffffffffu;
+              __syncwarp();
+              uint32_t s[32];
+              tmem_ld32(s_addr + 32 * ch, s);
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                const float4 sk = lds_f4(sc + 4 * (32 * ch + i)), sv = lds_f4(sc + KT * 4 + 4 * (32 * ch + i));
+                const float f[4] = {sk.x, sk.y, sk.z, sk.w}, v[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (bits >> (i + e) & 1u) big = fmaxf(big, fast_ex2(fmaf(__uint_as_float(s[i + e]) * f[e], row_c, -top)) * v[e]);
+              }
+            }
+            const float fade = fast_ex2(m - top);
+            float n_new = nf, scale = fade;
+            if (big > 0.f) {
+              n_new = __fdividef(1.f, big);
+              if (nf > 0.f) {
+                n_new = fminf(n_new, __fdividef(nf, fade));            // (fade 0: infinite, the new one counts)
+                scale = fade * __fdividef(n_new, nf);
+              }
+            }
+            m = top;
+            nf = n_new;
+            l *= fade;
+            if (t > 0) {                             // (the unit's first product overwrites the accumulator)
+              for (int ch = 0; ch < WIDTH / 32; ++ch) {
+                uint32_t o[32];
+                tmem_ld32(o_addr + 32 * ch, o);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
+                tmem_st32(o_addr + 32 * ch, o);
+              }
+            }
+            sum2 = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int ch = 0; ch < CHUNKS; ++ch) weigh(ch);
+            sum = sum2.x + sum2.y;
+          }
+          l += sum;
+#pragma unroll
+          for (int i = 0; i < KT / 64; ++i) tmem_st32(s_addr + 32 * i, pw + 32 * i);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_PF + g));
+        }
+        if (!ok) break;
+        done += count;
+        // ---- the rows of this stretch of the unit
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PV + g), (uint32_t)(done - 1) & 1u, watch, CODE_SOFTMAX));
+        if (!ok) break;
+        tc_fence_after();
+        const bool whole = kt0 == 0 && count == cur.n_kt;
+        const long long slot = 2LL * blockIdx.x + (n > 0 ? 1 : 0);                    // a stretch's first unit, or its last
+        const float inv_n = nf > 0.f ? __fdividef(1.f, nf) : 0.f;
+        const float inv = whole ? (l == 0.f ? 0.f : __fdividef(inv_n, l)) : inv_n;
+        T* out = reinterpret_cast<T*>(a.out) + (long long)(cur.s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
+        float* part = a.part_o + (slot * a.part_rows + 128 * g + r) * WIDTH;
+#pragma unroll 1
+        for (int ch = 0; ch < WIDTH / 32; ++ch) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + 32 * ch, o);
+          if (exists) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int at = 4 * ch + i, col = WIDTH == 128 ? 16 * (at & 7) + 8 * (at >> 3) : 8 * at;
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(o[8 * i + e]) * inv;
+              if (whole) {
+                if (col < a.D)
+                  *reinterpret_cast<uint4*>(out + col) = make_uint4(pair16<T>(x[0], x[1]), pair16<T>(x[2], x[3]), pair16<T>(x[4], x[5]), pair16<T>(x[6], x[7]));
+              } else {
+                *reinterpret_cast<float4*>(part + col) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(part + col + 4) = make_float4(x[4], x[5], x[6], x[7]);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        if (exists && !whole) a.part_ml[slot * a.part_rows + 128 * g + r] = make_float2(m, l);
+        if (exists && whole && a.lse != nullptr) {
+          float v = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2_F;
+          if (a.shift != nullptr) {                  // the keys as they were before the shift was taken off
+            float d = 0.f;
+            for (int i = 0; i < a.D; ++i) d = fmaf((float)q_row[i], __ldg(a.shift + (long long)cur.h * WIDTH + i), d);
+            v += d * a.sm_scale;
+          }
+          a.lse[(long long)(cur.s.q0 + tok) * a.Hq + head] = v;
+        }
+      }
+      n += count;
+      left -= count;
+      if (left > 0) { cur.kt = cur.n_kt - 1; next_step(a, cur, ROWS, KT); }
+    }
+  } else if (tid < L::SOFTMAX + L::LOADERS) {
+    // ------------------------------------------------- loaders -------------------------------------------------------
+    const int ct = tid - L::SOFTMAX;
+    constexpr int PIECES = WIDTH / 16, RPI = 128 / PIECES, N_CHUNK = KT / RPI;        // rows of 128 threads; chunks per thread
+    const int piece = ct % PIECES, row_l = ct / PIECES;
+    Cursor ahead = cur;
+    int pages[N_CHUNK], s_page = -1;                 // of the tile at `ahead`: the page of each chunk's row, and of the key whose scales this thread fetches
+    auto page_of = [&](int key) -> int { return key < ahead.s.len ? __ldg(a.table + ahead.b * a.table_st + (key >> a.page_shift)) : -1; };
+    auto fetch_pages = [&]() {
+#pragma unroll
+      for (int i = 0; i < N_CHUNK; ++i) pages[i] = page_of(ahead.kt * KT + ((i * RPI + row_l) & ~15));
+      if (ct < KT) s_page = page_of(ahead.kt * KT + (ct & ~15));
+    };
+    uint4 kr[N_CHUNK], vr[N_CHUNK];
+    float sk = 0.f, sv = 0.f;
+    auto row_of = [&](int page, int key) -> long long {
+      return (((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+    };
+    auto fetch = [&](const uint8_t* codes, uint4 (&to)[N_CHUNK]) {
+#pragma unroll
+      for (int i = 0; i < N_CHUNK; ++i) {
+        to[i] = make_uint4(0u, 0u, 0u, 0u);
+        if ((unsigned)pages[i] < (unsigned)a.pages)
+          to[i] = __ldcs(reinterpret_cast<const uint4*>(codes + row_of(pages[i], ahead.kt * KT + i * RPI + row_l) * WIDTH + 16 * piece));
+      }
+    };
+    auto fetch_scales = [&]() {
+      if (ct < KT) {
+        const bool there = (unsigned)s_page < (unsigned)a.pages;
+        const long long at = there ? row_of(s_page, ahead.kt * KT + ct) : 0;
+        sk = there ? __ldg(a.ks + at) : -1.f;        // below zero: no such key
+        sv = there ? __ldg(a.vs + at) : 0.f;
+      }
+    };
+    auto convert = [&](uint32_t stage, const uint4 (&from)[N_CHUNK], bool as_int8) {
+#pragma unroll
+      for (int i = 0; i < N_CHUNK; ++i) {
+        const int row = i * RPI + row_l;
+        uint32_t h[8];
+        if (as_int8) codes_to_half<true>(from[i], h); else codes_to_half<false>(from[i], h);
+        const uint32_t to = stage + row * 128;
+        if (WIDTH == 128) {
+          const uint32_t at = to + 16 * (piece ^ (row & 7));
+          sts16(at, h[0], h[1], h[2], h[3]);
+          sts16(at + L::KV_HALF, h[4], h[5], h[6], h[7]);
+        } else {
+          sts16(to + 16 * ((2 * piece) ^ (row & 7)), h[0], h[1], h[2], h[3]);
+          sts16(to + 16 * ((2 * piece + 1) ^ (row & 7)), h[4], h[5], h[6], h[7]);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+    };
+    fetch_pages();
+    fetch(a.kc, kr);
+    fetch_scales();
+    fetch(a.vc, vr);
+    bool ok = true;
+    for (int n = 0; ok && n < n_tiles; ++n) {
+      const int st = n % L::STAGES;
+      const uint32_t free_parity = ((uint32_t)(n / L::STAGES) & 1u) ^ 1u;
+      const bool more = n + 1 < n_tiles;
+      // K, the scales, and the flags of keys that do not exist
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KE + st), free_parity, watch, CODE_LOAD));
+      if (!ok) break;
+      if (ct < KT) {
+        const uint32_t sc = base + L::OFF_SC + (n % L::SLOTS) * L::SLOT;
+        sts_f32(sc + 4 * ct, sk);
+        sts_f32(sc + KT * 4 + 4 * ct, sv);
+        const uint32_t none = __ballot_sync(0xffffffffu, sk < 0.f);
+        if (lane == 0) sts_u32(sc + KT * 8 + 4 * (ct >> 5), none);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_SC + n % L::SLOTS));
+      }
+      convert(base + L::OFF_K + st * L::KV_TILE, kr, INT8);
+      if (lane == 0) mbar_arrive(bar(B_KF + st));
+      // (V of this tile is in registers; the next tile's pages and K follow)
+      if (more) {
+        next_step(a, ahead, ROWS, KT);
+        fetch_pages();
+        fetch(a.kc, kr);
+        fetch_scales();
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(B_VE + st), free_parity, watch, CODE_LOAD));
+      if (!ok) break;
+      convert(base + L::OFF_V + st * L::KV_TILE, vr, false);
+      if (lane == 0) mbar_arrive(bar(B_VF + st));
+      if (more) fetch(a.vc, vr);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_ISSUER));
+    if (warp == ISSUER && lane == 0) {
+      // ------------------------------------------------- products ------------------------------------------------------
+      bool ok = true;
+      int left = n_tiles, n = 0, done0 = 0, done1 = 0, seg0 = 0, seg1 = 0;
+      auto issue_qk = [&](int g, int st) {
+        tc_fence_after();
+  #pragma unroll
+        for (int k = 0; k < WIDTH / 16; ++k)
+          mma_ss(tmem_s(g), desc_k(base + L::OFF_Q + g * L::Q_TILE + (k >> 2) * L::Q_HALF + 32 * (k & 3)),
+                 desc_k(base + L::OFF_K + st * L::KV_TILE + (k >> 2) * L::KV_HALF + 32 * (k & 3)), IDESC_QK, k > 0);
+        tc_commit(bar(B_SF + g));
+      };
+      while (ok && left > 0) {
+        const int count = min(left, cur.n_kt - cur.kt), ng = halves_of(cur);
+        ok = mbar_wait(bar(B_QF), (uint32_t)seg0++ & 1u, watch, CODE_MMA);
+        if (ok && ng == 2) ok = mbar_wait(bar(B_QF + 1), (uint32_t)seg1++ & 1u, watch, CODE_MMA);
+        if (ok) ok = mbar_wait(bar(B_KF + n % L::STAGES), (uint32_t)(n / L::STAGES) & 1u, watch, CODE_MMA);
+        if (!ok) break;
+        for (int g = 0; g < ng; ++g) issue_qk(g, n % L::STAGES);
+        tc_commit(bar(B_KE + n % L::STAGES));
+        for (int t = 0; ok && t < count; ++t, ++n) {
+          const int st = n % L::STAGES;
+          const uint32_t par = (uint32_t)(n / L::STAGES) & 1u;
+          for (int g = 0; ok && g < ng; ++g) {
+            ok = mbar_wait(bar(B_PF + g), (uint32_t)(g ? done1 : done0) & 1u, watch, CODE_MMA);
+            if (ok && g == 0) ok = mbar_wait(bar(B_VF + st), par, watch, CODE_MMA);
+            if (!ok) break;
+            if (g) ++done1; else ++done0;
+            tc_fence_after();
+  #pragma unroll
+            for (int k = 0; k < KT / 16; ++k)
+              mma_ts(tmem_o(g), tmem_s(g) + 8 * k, desc_mn(base + L::OFF_V + st * L::KV_TILE + 2048 * k, L::KV_HALF), IDESC_PV, t > 0 || k > 0);
+            tc_commit(bar(B_PV + g));
+            if (g == ng - 1) tc_commit(bar(B_VE + st));
+            if (t + 1 < count) {
+              if (g == 0) ok = mbar_wait(bar(B_KF + (n + 1) % L::STAGES), (uint32_t)((n + 1) / L::STAGES) & 1u, watch, CODE_MMA);
+              if (!ok) break;
+              issue_qk(g, (n + 1) % L::STAGES);
+              if (g == ng - 1) tc_commit(bar(B_KE + (n + 1) % L::STAGES));
+            }
+          }
+        }
+        left -= count;
+        if (left > 0) { cur.kt = cur.n_kt - 1; next_step(a, cur, ROWS, KT); }
+      }
+      tc_commit(bar(B_DRAIN));                         // every product issued is complete before the TMEM is freed
+      mbar_wait(bar(B_DRAIN), 0, watch, CODE_MMA);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == ISSUER) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS) : "memory");
+  }
+}
+
+template <typename T, bool INT8, int WIDTH, int NQ, int KT>
+cudaError_t launch_tree(CacheAttnKArgs& a, int sms, int32_t* status_host, cudaStream_t st) {
+  using L = TreeShape<WIDTH, NQ, KT>;
+  auto kern = cache_tree_kernel<T, INT8, WIDTH, NQ, KT>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::BYTES);
+  if (e != cudaSuccess) return e;
+  const long long rows = (long long)a.max_q * a.group, rts = (rows + L::ROWS - 1) / L::ROWS;
+  const long long steps = (long long)a.n_seq * a.Hkv * rts * std::max<long long>(1, (((long long)a.table_width << a.page_shift) + KT - 1) / KT);
+  a.max_stretches = std::min(std::min(sms, 160) * L::CTAS_PER_SM, cache_form(rows).max_stretches);
+  kern<<<(unsigned)std::min<long long>(a.max_stretches, steps), L::THREADS, L::BYTES, st>>>(a, status_host);
+  return cudaGetLastError();
+}
+
+template <typename T, bool INT8, int WIDTH>
+cudaError_t launch_tree_rows(CacheAttnKArgs& a, int sms, int32_t* status_host, cudaStream_t st) {
+  return cache_form((int64_t)a.max_q * a.group).rows == 128 ? launch_tree<T, INT8, WIDTH, 1, 64>(a, sms, status_host, st)
+                                                            : launch_tree<T, INT8, WIDTH, 2, 128>(a, sms, status_host, st);
+}
+template <typename T>
+cudaError_t launch_tree_type(CacheAttnKArgs& a, const CacheView& c, int sms, int32_t* status_host, cudaStream_t st) {
+  if (c.width == 64) return c.int8 ? launch_tree_rows<T, true, 64>(a, sms, status_host, st) : launch_tree_rows<T, false, 64>(a, sms, status_host, st);
+  return c.int8 ? launch_tree_rows<T, true, 128>(a, sms, status_host, st) : launch_tree_rows<T, false, 128>(a, sms, status_host, st);
+}
+
+}  // namespace
+
+cudaError_t launch_cache_tree(CacheAttnKArgs& a, const CacheView& c, int dtype, int sms, int32_t* status_host, cudaStream_t st) {
+  return dtype == 0 ? launch_tree_type<__half>(a, c, sms, status_host, st) : launch_tree_type<__nv_bfloat16>(a, c, sms, status_host, st);
+}
+
+}  // namespace sage

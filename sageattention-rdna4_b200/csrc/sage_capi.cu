@@ -616,7 +616,7 @@ int sage_cache_attention(const void* q, void* out, float* lse,
                          const void* tree_mask, int64_t tree_stride, void* workspace, size_t workspace_bytes,
                          int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t total_q, int64_t max_q, int64_t head_dim,
                          int64_t pages, int64_t page_size, const int64_t q_strides[2], const int64_t o_strides[2],
-                         int dtype, int qk_mode, float sm_scale, void* stream) {
+                         int dtype, int qk_mode, float sm_scale, int32_t* status_host, void* stream) {
   const char* who = "sage_cache_attention";
   sage::CacheView c;
   int rc = cache_view(who, const_cast<void*>(k_codes), const_cast<float*>(k_scale), const_cast<void*>(v_codes), const_cast<float*>(v_scale),
@@ -633,6 +633,7 @@ int sage_cache_attention(const void* q, void* out, float* lse,
     return fail(SAGE_E_ARG, "%s: without cu_seqlens_q every sequence has max_q new tokens", who);
   if ((reinterpret_cast<uintptr_t>(seqlens_k) | reinterpret_cast<uintptr_t>(cu_seqlens_q) | reinterpret_cast<uintptr_t>(lse)) & 3u)
     return fail(SAGE_E_ARG, "%s: lengths and lse must be 4-byte aligned", who);
+  if (reinterpret_cast<uintptr_t>(status_host) & 3u) return fail(SAGE_E_ARG, "%s: status_host must be 4-byte aligned", who);
   if (tree_mask && tree_stride < 0) return fail(SAGE_E_ARG, "%s: negative tree_stride", who);
   if ((rc = check_strides2(who, "q", q_strides)) || (rc = check_strides2(who, "out", o_strides))) return rc;
   if (!aligned16(q) || !aligned16(out)) return fail(SAGE_E_ARG, "%s: pointers must be 16-byte aligned", who);
@@ -651,7 +652,7 @@ int sage_cache_attention(const void* q, void* out, float* lse,
   p.tree = reinterpret_cast<const uint8_t*>(tree_mask); p.tree_stride = tree_stride;
   for (int i = 0; i < 2; ++i) { p.q_strides[i] = q_strides[i]; p.o_strides[i] = o_strides[i]; }
   p.table_stride = page_table_stride; p.table_width = page_table_width;
-  p.n_seq = n_seq; p.Hq = Hq; p.total_q = total_q; p.max_q = max_q; p.dtype = dtype; p.sm_scale = sm_scale; p.scratch = workspace;
+  p.n_seq = n_seq; p.Hq = Hq; p.total_q = total_q; p.max_q = max_q; p.dtype = dtype; p.sm_scale = sm_scale; p.scratch = workspace; p.status_host = status_host;
   const cudaError_t e = sage::launch_cache_attention(c, p, reinterpret_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(SAGE_E_CUDA, "%s: %s", who, cudaGetErrorString(e));
   return SAGE_OK;

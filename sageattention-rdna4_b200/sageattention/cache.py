@@ -23,7 +23,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native
-from .b200_backend import _counters, _dtype_code, _STRIDE_MAX, HEAD_DIM, packed_view_reason, strided_view_reason
+from . import b200_backend as _be
+from .b200_backend import HEAD_DIM, _counters, _dtype_code, _report_to, _state, packed_view_reason, strided_view_reason
 
 _E4M3 = torch.float8_e4m3fn
 
@@ -275,6 +276,10 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
         lib = _native.load()
         # (from the caching allocator with every call: ordered with this stream, and a captured graph's own)
         ws = torch.empty((lib.sage_cache_attention_workspace_bytes(batch, hq, hkv, max_q),), dtype=torch.uint8, device=dev)
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        capturing = torch.cuda.is_current_stream_capturing()
+        st = _state(dev, stream)                     # (the host word that a failed call reports to, as for `sageattn`)
+        st.raise_if_failed("the next call on the stream")
         with _on_device(dev):
             rc = lib.sage_cache_attention(
                 q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *cache._args,
@@ -283,8 +288,11 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
                 0 if tree_mask is None else tree_mask.data_ptr(), 0 if tree_mask is None else tree_mask.stride(0),
                 ws.data_ptr(), ws.numel(), batch, hq, hkv, tokens, max_q, d, *cache._sizes,
                 _native.strides2(q.stride(0), q.stride(1)), _native.strides2(out.stride(0), out.stride(1)),
-                _dtype_code(q.dtype), cache._mode, scale, torch.cuda.current_stream(dev).cuda_stream)
+                _dtype_code(q.dtype), cache._mode, scale, _report_to(st, capturing), stream)
         _native.check(rc, "sage_cache_attention")
+        if _be._STRICT and not capturing:
+            torch.cuda.current_stream(dev).synchronize()
+            st.raise_if_failed("this call (strict mode)")
     return (out, lse) if return_lse else out
 
 

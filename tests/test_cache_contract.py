@@ -29,9 +29,9 @@ def _read(kc=P, table=P, stride=4, width=4, cu=P, k=P, v=P, n_seq=1, total=4, he
 
 
 def _attend(q=P, out=P, lse=None, kc=P, table=P, stride=4, width=4, lens=P, cu=P, tree=None, tree_st=0, ws=P, ws_bytes=1 << 40, n_seq=1,
-            hq=8, hkv=8, total=4, max_q=4, d=128, pages=4, page=64, q_st=S2, o_st=S2, dtype=0, mode=0, scale=0.1):
+            hq=8, hkv=8, total=4, max_q=4, d=128, pages=4, page=64, q_st=S2, o_st=S2, dtype=0, mode=0, scale=0.1, status=None):
     return _native.load().sage_cache_attention(q, out, lse, kc, P, P, P, None, table, stride, width, lens, cu, tree, tree_st, ws, ws_bytes,
-                                               n_seq, hq, hkv, total, max_q, d, pages, page, q_st, o_st, dtype, mode, scale, None)
+                                               n_seq, hq, hkv, total, max_q, d, pages, page, q_st, o_st, dtype, mode, scale, status, None)
 
 
 def _rotary(q=P, qo=P, k=None, ko=None, pos=P, p64=1, freq=P, b=1, hq=8, hk=0, n=4, d=128, rot=128, st=S3, p2=_native.strides2(0, 1), dtype=0):
@@ -92,6 +92,7 @@ def test_attention_refusals():
     _refused(_attend(max_q=5), ARG, "max_q")
     _refused(_attend(lse=P + 2), ARG, "aligned")
     _refused(_attend(q=P + 8), ARG, "aligned")
+    _refused(_attend(status=P + 2), ARG, "status_host")
     _refused(_attend(tree=P, tree_st=-1), ARG, "tree_stride")
     _refused(_attend(ws=P + 16), ARG, "256")
     _refused(_attend(ws_bytes=100), WORKSPACE, "needs")
