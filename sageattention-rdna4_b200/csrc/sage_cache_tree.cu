@@ -80,13 +80,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b_d
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                ::"r"(d), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr) : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
@@ -107,6 +107,11 @@ __device__ __forceinline__ uint32_t lds_u32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
 }
 
 // Descriptors of 128-byte rows in the 128-byte swizzle, 8-row groups 1024 bytes apart: as a K-major operand, and as
@@ -151,8 +156,10 @@ template <int WIDTH, int NQ, int KT> struct TreeShape {
   static constexpr uint32_t Q_HALF = 128 * 128, Q_TILE = HALVES * Q_HALF;             // 128 rows of 128 bytes
   static constexpr uint32_t KV_HALF = KT * 128, KV_TILE = HALVES * KV_HALF;
   static constexpr uint32_t OFF_Q = 0, OFF_K = NQ * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE, OFF_SC = OFF_V + STAGES * KV_TILE;
-  static constexpr uint32_t SLOT = KT * 8 + 16;                                       // scales of K, scales of V, a flag per 32 keys
-  static constexpr uint32_t OFF_BAR = OFF_SC + SLOTS * SLOT, OFF_MISC = OFF_BAR + 176, USED = OFF_MISC + 16;
+  // of a tile: scales of K, log2 and reciprocal of the scales of V, and a word per 32 keys with a bit for each that does not exist
+  static constexpr uint32_t SLOT_LV = KT * 4, SLOT_RV = KT * 8, SLOT_NONE = KT * 12, SLOT = SLOT_NONE + 16;
+  static constexpr uint32_t OFF_BAR = OFF_SC + SLOTS * SLOT, OFF_MISC = OFF_BAR + 176, OFF_SEEN = OFF_MISC + 16;
+  static constexpr uint32_t USED = OFF_SEEN + SOFTMAX * (KT / 32) * 4;                // which keys of a tile a row sees, where not all
   static constexpr uint32_t BYTES = USED + 1024;                                      // slack for the 1024-byte alignment
   static constexpr uint32_t TMEM_COLS = NQ * (KT + WIDTH) <= 128 ? 128 : NQ * (KT + WIDTH) <= 256 ? 256 : 512;
   static constexpr int ROWS = 128 * NQ;
@@ -269,7 +276,10 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       const int plain_end = a.tree ? max(ctx, 0) : max(0, min(cur.s.len, ctx + t_first + 1));   // keys below need no mask
       const int lim = exists ? (a.tree ? cur.s.len : min(cur.s.len, ctx + tok + 1)) : 0;
       const uint8_t* tree_row = a.tree ? a.tree + (long long)(cur.s.q0 + tok) * a.tree_st : nullptr;
-      float m = NO_MAX, l = 0.f, nf = 0.f;
+      // m: running maximum of e = score + log2(scale of V); l: sum of the weights of V over their scales
+      float m = NO_MAX, l = 0.f;
+      const float2 c2 = make_float2(row_c, row_c);
+      const uint32_t seen_at = base + L::OFF_SEEN + 4 * tid;
 
       if (g < ng) {
         for (int t = 0; t < count; ++t) {
@@ -281,127 +291,115 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
           if (!ok) break;
           tc_fence_after();
           const int key0 = (kt0 + t) * KT;
-          uint32_t absent = lds_u32(sc + KT * 8) | lds_u32(sc + KT * 8 + 4);
-          if (KT == 128) absent |= lds_u32(sc + KT * 8 + 8) | lds_u32(sc + KT * 8 + 12);
-          const bool masked = key0 + KT > plain_end || absent != 0u;
-          // bit i: key key0 + 32 ch + i is seen by this row
-          auto seen_bits = [&](int ch) -> uint32_t {
-            uint32_t bits = 0u;
-            for (int i = 0; i < 32; ++i) {
-              const int key = key0 + 32 * ch + i;
-              bool seen = key < lim;
-              if (tree_row != nullptr && seen && key >= ctx) seen = tree_row[key - ctx] != 0;
-              bits |= seen ? 1u << i : 0u;
-            }
-            if (absent != 0u)
-              for (int i = 0; i < 32; ++i) {
-                float sk;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sk) : "r"(sc + 4 * (32 * ch + i)));
-                if (sk < 0.f) bits &= ~(1u << i);
+          uint32_t none = lds_u32(sc + L::SLOT_NONE) | lds_u32(sc + L::SLOT_NONE + 4);
+          if (KT == 128) none |= lds_u32(sc + L::SLOT_NONE + 8) | lds_u32(sc + L::SLOT_NONE + 12);
+          const bool masked = key0 + KT > plain_end || none != 0u;
+          if (masked) {                              // a bit per key that this row sees, in shared memory
+#pragma unroll 1
+            for (int ch = 0; ch < CHUNKS; ++ch) {
+              const int k0 = key0 + 32 * ch, upto = lim - k0;
+              uint32_t bits = upto >= 32 ? 0xffffffffu : upto <= 0 ? 0u : (1u << upto) - 1u;
+              bits &= ~lds_u32(sc + L::SLOT_NONE + 4 * ch);
+              if (tree_row != nullptr && bits != 0u && k0 + 32 > ctx) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (k0 + i >= ctx && (bits >> i & 1u) && tree_row[k0 + i - ctx] == 0) bits &= ~(1u << i);
               }
-            return bits;
-          };
-          uint32_t pw[KT / 2];
-          float2 sum2 = make_float2(0.f, 0.f);
-          __half2 w_top = __float2half2_rn(0.f);
-          // weights of 32 columns against the maximum m and the factor nf
-          auto weigh = [&](int ch) {
-            const uint32_t bits = masked ? seen_bits(ch) : 0xffffffffu;
+              sts_u32(seen_at + 4 * L::SOFTMAX * ch, bits);
+            }
             __syncwarp();
-            uint32_t s[32];
-            tmem_ld32(s_addr + 32 * ch, s);
-            const float2 c2 = make_float2(row_c, row_c), nm2 = make_float2(-m, -m), nf2 = make_float2(nf, nf);
+          }
+          // 64 columns at a time: the largest e, then the weights
+          float top = m;
+#pragma unroll 1
+          for (int half = 0; half < KT / 64; ++half) {
+            uint32_t s[64];
+            tmem_ld32(s_addr + 64 * half, s);
+            tmem_ld32(s_addr + 64 * half + 32, s + 32);
+            tmem_ld_wait();
+            const uint32_t at = sc + 256 * half;
+            if (!masked) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 sk = lds_f4(sc + 4 * (32 * ch + i)), sv = lds_f4(sc + KT * 4 + 4 * (32 * ch + i));
-#pragma unroll
-              for (int e = 0; e < 4; e += 2) {
-                float2 x = make_float2(__uint_as_float(s[i + e]), __uint_as_float(s[i + e + 1]));
-                x = __fmul2_rn(x, e ? make_float2(sk.z, sk.w) : make_float2(sk.x, sk.y));
-                float2 d = __ffma2_rn(x, c2, nm2);
-                if (masked) {
-                  if (!(bits >> (i + e) & 1u)) d.x = -INFINITY;
-                  if (!(bits >> (i + e + 1) & 1u)) d.y = -INFINITY;
-                }
-                const float2 p = make_float2(fast_ex2(d.x), fast_ex2(d.y));
-                sum2 = __fadd2_rn(sum2, p);
-                float2 w = __fmul2_rn(p, __fmul2_rn(e ? make_float2(sv.z, sv.w) : make_float2(sv.x, sv.y), nf2));
-                if (masked) {                        // an exact zero whatever the key's scale holds
-                  if (!(bits >> (i + e) & 1u)) w.x = 0.f;
-                  if (!(bits >> (i + e + 1) & 1u)) w.y = 0.f;
-                }
-                const __half2 h = __floats2half2_rn(w.x, w.y);
-                w_top = __hmax2(w_top, h);
-                pw[(32 * ch + i + e) / 2] = *reinterpret_cast<const uint32_t*>(&h);
+              for (int i = 0; i < 64; i += 4) {
+                const float4 sk = lds_f4(at + 4 * i), lv = lds_f4(at + L::SLOT_LV + 4 * i);
+                const float2 x = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(sk.x, sk.y)), c2, make_float2(lv.x, lv.y));
+                const float2 y = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(sk.z, sk.w)), c2, make_float2(lv.z, lv.w));
+                top = max3(top, x.x, x.y);
+                top = max3(top, y.x, y.y);
               }
-            }
-          };
+            } else {
+              const uint32_t bits[2] = {lds_u32(seen_at + 4 * L::SOFTMAX * (2 * half)), lds_u32(seen_at + 4 * L::SOFTMAX * (2 * half + 1))};
 #pragma unroll
-          for (int ch = 0; ch < CHUNKS; ++ch) weigh(ch);
-          float sum = sum2.x + sum2.y;
-          // (a weight above 2^8 shows in the sum)
-          const float2 wt = __half22float2(w_top);
-          if (__any_sync(0xffffffffu, sum > 256.f || fmaxf(wt.x, wt.y) > 4096.f)) {
-            // new maximum and factor; the sum and the accumulator follow, and the weights are worked out again
-            float top = m;
-            for (int ch = 0; ch < CHUNKS; ++ch) {
-              const uint32_t bits = masked ? seen_bits(ch) : 0xffffffffu;
-              __syncwarp();
-              uint32_t s[32];
-              tmem_ld32(s_addr + 32 * ch, s);
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float4 sk = lds_f4(sc + 4 * (32 * ch + i));
-                const float f[4] = {sk.x, sk.y, sk.z, sk.w};
+              for (int i = 0; i < 64; i += 4) {
+                const float4 sk = lds_f4(at + 4 * i), lv = lds_f4(at + L::SLOT_LV + 4 * i);
+                const float f[4] = {sk.x, sk.y, sk.z, sk.w}, v[4] = {lv.x, lv.y, lv.z, lv.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                  if (bits >> (i + e) & 1u) top = fmaxf(top, __uint_as_float(s[i + e]) * f[e] * row_c);
+                  if (bits[i / 32] >> ((i + e) & 31) & 1u) top = fmaxf(top, fmaf(__uint_as_float(s[i + e]) * f[e], row_c, v[e]));
               }
             }
-            float big = 0.f;
-            for (int ch = 0; ch < CHUNKS; ++ch) {
-              const uint32_t bits = masked ? seen_bits(ch) : 0xffffffffu;
-              __syncwarp();
-              uint32_t s[32];
-              tmem_ld32(s_addr + 32 * ch, s);
-#pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float4 sk = lds_f4(sc + 4 * (32 * ch + i)), sv = lds_f4(sc + KT * 4 + 4 * (32 * ch + i));
-                const float f[4] = {sk.x, sk.y, sk.z, sk.w}, v[4] = {sv.x, sv.y, sv.z, sv.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (bits >> (i + e) & 1u) big = fmaxf(big, fast_ex2(fmaf(__uint_as_float(s[i + e]) * f[e], row_c, -top)) * v[e]);
-              }
-            }
+          }
+          if (__any_sync(0xffffffffu, top > m + 8.f)) {
+            // the maximum moves; the sum and the accumulator follow
             const float fade = fast_ex2(m - top);
-            float n_new = nf, scale = fade;
-            if (big > 0.f) {
-              n_new = __fdividef(1.f, big);
-              if (nf > 0.f) {
-                n_new = fminf(n_new, __fdividef(nf, fade));            // (fade 0: infinite, the new one counts)
-                scale = fade * __fdividef(n_new, nf);
-              }
-            }
             m = top;
-            nf = n_new;
             l *= fade;
             if (t > 0) {                             // (the unit's first product overwrites the accumulator)
+#pragma unroll 1
               for (int ch = 0; ch < WIDTH / 32; ++ch) {
                 uint32_t o[32];
                 tmem_ld32(o_addr + 32 * ch, o);
+                tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * scale);
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fade);
                 tmem_st32(o_addr + 32 * ch, o);
               }
             }
-            sum2 = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int ch = 0; ch < CHUNKS; ++ch) weigh(ch);
-            sum = sum2.x + sum2.y;
           }
-          l += sum;
+          float2 l2 = make_float2(l, 0.f);
+          const float2 nm2 = make_float2(-m, -m);
+#pragma unroll 1
+          for (int half = 0; half < KT / 64; ++half) {
+            uint32_t s[64];
+            tmem_ld32(s_addr + 64 * half, s);
+            tmem_ld32(s_addr + 64 * half + 32, s + 32);
+            tmem_ld_wait();
+            const uint32_t at = sc + 256 * half;
+            uint32_t pw[32];
+            if (!masked) {
 #pragma unroll
-          for (int i = 0; i < KT / 64; ++i) tmem_st32(s_addr + 32 * i, pw + 32 * i);
+              for (int i = 0; i < 64; i += 4) {
+                const float4 sk = lds_f4(at + 4 * i), lv = lds_f4(at + L::SLOT_LV + 4 * i), rv = lds_f4(at + L::SLOT_RV + 4 * i);
+                const float2 x = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(sk.x, sk.y)), c2,
+                                            __fadd2_rn(make_float2(lv.x, lv.y), nm2));
+                const float2 y = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(sk.z, sk.w)), c2,
+                                            __fadd2_rn(make_float2(lv.z, lv.w), nm2));
+                const float2 w = make_float2(fast_ex2(x.x), fast_ex2(x.y)), z = make_float2(fast_ex2(y.x), fast_ex2(y.y));
+                l2 = __ffma2_rn(w, make_float2(rv.x, rv.y), l2);
+                l2 = __ffma2_rn(z, make_float2(rv.z, rv.w), l2);
+                pw[i / 2] = pair16<__half>(w.x, w.y);
+                pw[i / 2 + 1] = pair16<__half>(z.x, z.y);
+              }
+            } else {
+              const uint32_t bits[2] = {lds_u32(seen_at + 4 * L::SOFTMAX * (2 * half)), lds_u32(seen_at + 4 * L::SOFTMAX * (2 * half + 1))};
+#pragma unroll
+              for (int i = 0; i < 64; i += 4) {
+                const float4 sk = lds_f4(at + 4 * i), lv = lds_f4(at + L::SLOT_LV + 4 * i), rv = lds_f4(at + L::SLOT_RV + 4 * i);
+                const float f[4] = {sk.x, sk.y, sk.z, sk.w}, v[4] = {lv.x, lv.y, lv.z, lv.w}, r4[4] = {rv.x, rv.y, rv.z, rv.w};
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {        // (nothing of a key that is not seen, whatever it holds)
+                  const bool seen = bits[i / 32] >> ((i + e) & 31) & 1u;
+                  w[e] = seen ? fast_ex2(fmaf(__uint_as_float(s[i + e]) * f[e], row_c, v[e] - m)) : 0.f;
+                  if (seen) l2.x = fmaf(w[e], r4[e], l2.x);
+                }
+                pw[i / 2] = pair16<__half>(w[0], w[1]);
+                pw[i / 2 + 1] = pair16<__half>(w[2], w[3]);
+              }
+            }
+            tmem_st32(s_addr + 32 * half, pw);       // over scores that have been read
+          }
+          l = l2.x + l2.y;
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
@@ -415,14 +413,14 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         tc_fence_after();
         const bool whole = kt0 == 0 && count == cur.n_kt;
         const long long slot = 2LL * blockIdx.x + (n > 0 ? 1 : 0);                    // a stretch's first unit, or its last
-        const float inv_n = nf > 0.f ? __fdividef(1.f, nf) : 0.f;
-        const float inv = whole ? (l == 0.f ? 0.f : __fdividef(inv_n, l)) : inv_n;
+        const float inv = !whole ? 1.f : l == 0.f ? 0.f : __fdividef(1.f, l);
         T* out = reinterpret_cast<T*>(a.out) + (long long)(cur.s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
         float* part = a.part_o + (slot * a.part_rows + 128 * g + r) * WIDTH;
 #pragma unroll 1
         for (int ch = 0; ch < WIDTH / 32; ++ch) {
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * ch, o);
+          tmem_ld_wait();
           if (exists) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -461,8 +459,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     const int ct = tid - L::SOFTMAX;
     constexpr int PIECES = WIDTH / 16, RPI = 128 / PIECES, N_CHUNK = KT / RPI;        // rows of 128 threads; chunks per thread
     const int piece = ct % PIECES, row_l = ct / PIECES;
-    Cursor ahead = cur;
-    int pages[N_CHUNK], s_page = -1;                 // of the tile at `ahead`: the page of each chunk's row, and of the key whose scales this thread fetches
+    Cursor ahead = cur;                              // the tile that is fetched next
+    int pages[N_CHUNK], s_page = -1;                 // of that tile: the page of each chunk's row, and of the key whose scales this thread fetches
     auto page_of = [&](int key) -> int { return key < ahead.s.len ? __ldg(a.table + ahead.b * a.table_st + (key >> a.page_shift)) : -1; };
     auto fetch_pages = [&]() {
 #pragma unroll
@@ -509,10 +507,18 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       fence_async_smem();
       __syncwarp();
     };
+    // on to the next tile, whose pages are asked for at once
+    auto advance = [&](int tile) {
+      if (tile + 1 < n_tiles) {
+        next_step(a, ahead, ROWS, KT);
+        fetch_pages();
+      }
+    };
     fetch_pages();
     fetch(a.kc, kr);
     fetch_scales();
     fetch(a.vc, vr);
+    advance(0);
     bool ok = true;
     for (int n = 0; ok && n < n_tiles; ++n) {
       const int st = n % L::STAGES;
@@ -523,19 +529,18 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       if (!ok) break;
       if (ct < KT) {
         const uint32_t sc = base + L::OFF_SC + (n % L::SLOTS) * L::SLOT;
+        const float v = sv == 0.f ? 1e-30f : sv;     // (a row that nothing wrote: value 0, but a part of the sum)
         sts_f32(sc + 4 * ct, sk);
-        sts_f32(sc + KT * 4 + 4 * ct, sv);
+        sts_f32(sc + L::SLOT_LV + 4 * ct, __log2f(v));
+        sts_f32(sc + L::SLOT_RV + 4 * ct, __fdividef(1.f, v));
         const uint32_t none = __ballot_sync(0xffffffffu, sk < 0.f);
-        if (lane == 0) sts_u32(sc + KT * 8 + 4 * (ct >> 5), none);
+        if (lane == 0) sts_u32(sc + L::SLOT_NONE + 4 * (ct >> 5), none);
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_SC + n % L::SLOTS));
       }
       convert(base + L::OFF_K + st * L::KV_TILE, kr, INT8);
       if (lane == 0) mbar_arrive(bar(B_KF + st));
-      // (V of this tile is in registers; the next tile's pages and K follow)
-      if (more) {
-        next_step(a, ahead, ROWS, KT);
-        fetch_pages();
+      if (more) {                                    // `ahead` is tile n + 1
         fetch(a.kc, kr);
         fetch_scales();
       }
@@ -543,7 +548,10 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       if (!ok) break;
       convert(base + L::OFF_V + st * L::KV_TILE, vr, false);
       if (lane == 0) mbar_arrive(bar(B_VF + st));
-      if (more) fetch(a.vc, vr);
+      if (more) {
+        fetch(a.vc, vr);
+        advance(n + 1);
+      }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_ISSUER));
