@@ -21,8 +21,8 @@
 // that no bit is lost but in elements 2^-28 below their row's largest.  Scores, maxima, sums and outputs in
 // fp32.  A weight enters the second product as fp16(p * v_scale * N), where N is a factor per row that keeps the
 // largest one seen near 1 (fp16 has 11 bits there; its relative error, 2^-11, is that of the output format).
-// The running maximum moves only when a score passes it by 2^8, and N when a product passes 2^12: p stays
-// below 2^8, the accumulator is rarely touched, and neither the sums nor the 11 bits lose anything by it.
+// The running maximum moves only when a score passes it by 2^14, and N when a product does: the accumulator is
+// rarely touched, weights stay below fp16's 65504 and keep its 11 bits down to 2^-14, and fp32 sums lose nothing by it.
 //
 // Work.  The steps of 32 keys of all (sequence, K/V head, row tile) units are numbered in one line, and every
 // warp of the GPU takes an equal stretch of it, by itself: its own ring of cp.async stages, no barrier, no spinning
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           p_top = fmaxf(p_top, p[blk][e]);
           w_top = fmaxf(w_top, w[blk][e]);
         }
-      if (__any_sync(0xffffffffu, fmaxf(16.f * p_top, w_top) > 4096.f)) {
+      if (__any_sync(0xffffffffu, fmaxf(p_top, w_top) > 16384.f)) {
         // new maxima and factors; the sums and the accumulator follow
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -333,8 +333,17 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           for (int i = 0; i < 4; ++i) top = fmaxf(top, s[i >> 1][nb][2 * (i & 1) + x] * row_c[nb][x]);
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
-          const float fade = fast_ex2(m[nb][x] - top);
+          // (each row by itself: what another row sees moves nothing here)
           float big = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (s[i >> 1][nb][2 * (i & 1) + x] != -INFINITY) big = fmaxf(big, w[i >> 1][2 * (i & 1) + x]);
+#pragma unroll
+          for (int sh = 4; sh < 32; sh <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, sh));
+          if (!(top > m[nb][x] + 14.f || big > 16384.f)) top = m[nb][x];
+          const bool move = top != m[nb][x] || big > 16384.f;
+          const float fade = fast_ex2(m[nb][x] - top);
+          big = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float v = fast_ex2(fmaf(s[i >> 1][nb][2 * (i & 1) + x], row_c[nb][x], -top));
@@ -344,7 +353,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, sh));
           float n_new = nf[nb][x], scale = fade;
-          if (big > 0.f) {
+          if (move && big > 0.f) {
             n_new = __fdividef(1.f, big);
             if (nf[nb][x] > 0.f) {
               n_new = fminf(n_new, __fdividef(nf[nb][x], fade));       // (fade 0: infinite, the new one counts)

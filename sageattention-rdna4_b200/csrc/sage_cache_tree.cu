@@ -92,22 +92,17 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
       ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr) : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr) : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ void sts_f32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 __device__ __forceinline__ void sts_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
-  return v;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -149,17 +144,17 @@ template <int WIDTH, int NQ, int KT> struct TreeShape {
   // Registers per thread: at launch (what __launch_bounds__ leaves: 65536 / threads of the SM, in eights), and after the
   // issuing warpgroup has handed its own to the softmax.  setmaxnreg.inc waits until the pool holds what it asks for, so
   // that the three must not add up to more than the launch has.
-  static constexpr int REGS_LAUNCH = NQ == 1 ? 80 : 128, REGS_SOFTMAX = NQ == 1 ? 120 : 168, REGS_ISSUER = NQ == 1 ? 40 : 48;
+  static constexpr int REGS_LAUNCH = NQ == 1 ? 80 : 128, REGS_SOFTMAX = NQ == 1 ? 104 : 160, REGS_ISSUER = NQ == 1 ? 56 : 64;
   static_assert(NQ * REGS_SOFTMAX + REGS_LAUNCH + REGS_ISSUER <= (NQ + 2) * REGS_LAUNCH, "setmaxnreg would wait forever");
   static constexpr int STAGES = 2, SLOTS = 4;
   static constexpr uint32_t HALVES = WIDTH / 64;
   static constexpr uint32_t Q_HALF = 128 * 128, Q_TILE = HALVES * Q_HALF;             // 128 rows of 128 bytes
   static constexpr uint32_t KV_HALF = KT * 128, KV_TILE = HALVES * KV_HALF;
   static constexpr uint32_t OFF_Q = 0, OFF_K = NQ * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE, OFF_SC = OFF_V + STAGES * KV_TILE;
-  // of a tile: scales of K, log2 and reciprocal of the scales of V, and a word per 32 keys with a bit for each that does not exist
-  static constexpr uint32_t SLOT_LV = KT * 4, SLOT_RV = KT * 8, SLOT_NONE = KT * 12, SLOT = SLOT_NONE + 16;
-  static constexpr uint32_t OFF_BAR = OFF_SC + SLOTS * SLOT, OFF_MISC = OFF_BAR + 176, OFF_SEEN = OFF_MISC + 16;
-  static constexpr uint32_t USED = OFF_SEEN + SOFTMAX * (KT / 32) * 4;                // which keys of a tile a row sees, where not all
+  // of a tile: scales of K, log2 and reciprocal of the scales of V, and for every 32 keys {a bit for each that does not
+  // exist, a bit for each that holds a NaN, the largest and the smallest log2 of a scale of V}
+  static constexpr uint32_t SLOT_LV = KT * 4, SLOT_RV = KT * 8, SLOT_SUM = KT * 12, SLOT = SLOT_SUM + KT / 2;
+  static constexpr uint32_t OFF_BAR = OFF_SC + SLOTS * SLOT, OFF_MISC = OFF_BAR + 176, USED = OFF_MISC + 16;
   static constexpr uint32_t BYTES = USED + 1024;                                      // slack for the 1024-byte alignment
   static constexpr uint32_t TMEM_COLS = NQ * (KT + WIDTH) <= 128 ? 128 : NQ * (KT + WIDTH) <= 256 ? 256 : 512;
   static constexpr int ROWS = 128 * NQ;
@@ -279,7 +274,6 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       // m: running maximum of e = score + log2(scale of V); l: sum of the weights of V over their scales
       float m = NO_MAX, l = 0.f;
       const float2 c2 = make_float2(row_c, row_c);
-      const uint32_t seen_at = base + L::OFF_SEEN + 4 * tid;
 
       if (g < ng) {
         for (int t = 0; t < count; ++t) {
@@ -291,56 +285,82 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
           if (!ok) break;
           tc_fence_after();
           const int key0 = (kt0 + t) * KT;
-          uint32_t none = lds_u32(sc + L::SLOT_NONE) | lds_u32(sc + L::SLOT_NONE + 4);
-          if (KT == 128) none |= lds_u32(sc + L::SLOT_NONE + 8) | lds_u32(sc + L::SLOT_NONE + 12);
-          const bool masked = key0 + KT > plain_end || none != 0u;
-          if (masked) {                              // a bit per key that this row sees, in shared memory
+          const float* vec = reinterpret_cast<const float*>(gbase + (sc - base));
+          const uint4* sums = reinterpret_cast<const uint4*>(gbase + (sc - base) + L::SLOT_SUM);
+          uint32_t any_odd = 0u;
+          float lv_top = -INFINITY, lv_low = INFINITY;
+#pragma unroll
+          for (int ch = 0; ch < CHUNKS; ++ch) {
+            const uint4 u = sums[ch];
+            any_odd |= u.x | u.y;
+            lv_top = fmaxf(lv_top, __uint_as_float(u.z));
+            lv_low = fminf(lv_low, __uint_as_float(u.w));
+          }
+          const bool masked = key0 + KT > plain_end || any_odd != 0u;
+          if (masked) {
+            // What this row does not see becomes -infinity before anything is made of it, what it sees of a key that holds
+            // a NaN becomes one (such keys' scales stand at 1, so that they reach no other row).
 #pragma unroll 1
             for (int ch = 0; ch < CHUNKS; ++ch) {
               const int k0 = key0 + 32 * ch, upto = lim - k0;
+              const uint2 not_there = make_uint2(sums[ch].x, sums[ch].y);
               uint32_t bits = upto >= 32 ? 0xffffffffu : upto <= 0 ? 0u : (1u << upto) - 1u;
-              bits &= ~lds_u32(sc + L::SLOT_NONE + 4 * ch);
+              bits &= ~not_there.x;
               if (tree_row != nullptr && bits != 0u && k0 + 32 > ctx) {
-#pragma unroll
+#pragma unroll 8
                 for (int i = 0; i < 32; ++i)
                   if (k0 + i >= ctx && (bits >> i & 1u) && tree_row[k0 + i - ctx] == 0) bits &= ~(1u << i);
               }
-              sts_u32(seen_at + 4 * L::SOFTMAX * ch, bits);
+              __syncwarp();
+              uint32_t x[32];
+              tmem_ld32(s_addr + 32 * ch, x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = !(bits >> i & 1u) ? 0xff800000u : (not_there.y >> i & 1u) ? 0x7fffffffu : x[i];
+              tmem_st32(s_addr + 32 * ch, x);
             }
-            __syncwarp();
+            tmem_st_wait();
           }
-          // 64 columns at a time: the largest e, then the weights
-          float top = m;
+          // A bound of the row's largest e: the largest score, and the largest log2 of a scale of V; where those scales
+          // differ by more than 2^8 within the tile, or some are not this row's to see, the largest e itself.
+          float top = -INFINITY;
+          {
+            uint32_t x0[32], x1[32];
+            auto take = [&](const uint32_t* x, int ch) {
+              const float4* at = reinterpret_cast<const float4*>(vec + 32 * ch);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 sk = at[i];
+                const float2 u = __fmul2_rn(make_float2(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1])), make_float2(sk.x, sk.y));
+                const float2 v = __fmul2_rn(make_float2(__uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3])), make_float2(sk.z, sk.w));
+                top = max3(max3(top, u.x, u.y), v.x, v.y);
+              }
+            };
+            tmem_ld32(s_addr, x0);
 #pragma unroll 1
-          for (int half = 0; half < KT / 64; ++half) {
-            uint32_t s[64];
-            tmem_ld32(s_addr + 64 * half, s);
-            tmem_ld32(s_addr + 64 * half + 32, s + 32);
-            tmem_ld_wait();
-            const uint32_t at = sc + 256 * half;
-            if (!masked) {
+            for (int ch = 0; ch < CHUNKS; ch += 2) {
+              tmem_ld_wait();
+              tmem_ld32(s_addr + 32 * ch + 32, x1);
+              take(x0, ch);
+              tmem_ld_wait();
+              if (ch + 2 < CHUNKS) tmem_ld32(s_addr + 32 * ch + 64, x0);
+              take(x1, ch + 1);
+            }
+            top = fmaf(top, row_c, lv_top);
+            if (masked || lv_top - lv_low > 8.f) {
+              top = -INFINITY;
+#pragma unroll 1
+              for (int ch = 0; ch < CHUNKS; ++ch) {
+                tmem_ld32(s_addr + 32 * ch, x0);
+                tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 64; i += 4) {
-                const float4 sk = lds_f4(at + 4 * i), lv = lds_f4(at + L::SLOT_LV + 4 * i);
-                const float2 x = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(sk.x, sk.y)), c2, make_float2(lv.x, lv.y));
-                const float2 y = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(sk.z, sk.w)), c2, make_float2(lv.z, lv.w));
-                top = max3(top, x.x, x.y);
-                top = max3(top, y.x, y.y);
-              }
-            } else {
-              const uint32_t bits[2] = {lds_u32(seen_at + 4 * L::SOFTMAX * (2 * half)), lds_u32(seen_at + 4 * L::SOFTMAX * (2 * half + 1))};
-#pragma unroll
-              for (int i = 0; i < 64; i += 4) {
-                const float4 sk = lds_f4(at + 4 * i), lv = lds_f4(at + L::SLOT_LV + 4 * i);
-                const float f[4] = {sk.x, sk.y, sk.z, sk.w}, v[4] = {lv.x, lv.y, lv.z, lv.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (bits[i / 32] >> ((i + e) & 31) & 1u) top = fmaxf(top, fmaf(__uint_as_float(s[i + e]) * f[e], row_c, v[e]));
+                for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaf(__uint_as_float(x0[i]) * vec[32 * ch + i], row_c, vec[KT + 32 * ch + i]));
               }
             }
           }
-          if (__any_sync(0xffffffffu, top > m + 8.f)) {
-            // the maximum moves; the sum and the accumulator follow
+          if (__any_sync(0xffffffffu, top > m + 14.f)) {
+            // the maximum moves; the sum and the accumulator follow (weights stay below 2^14: fp16 keeps 11 bits from there to 2^-14)
+            top = top > m + 14.f ? top : m;          // (each row by itself)
             const float fade = fast_ex2(m - top);
             m = top;
             l *= fade;
@@ -356,50 +376,40 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
               }
             }
           }
-          float2 l2 = make_float2(l, 0.f);
-          const float2 nm2 = make_float2(-m, -m);
-#pragma unroll 1
-          for (int half = 0; half < KT / 64; ++half) {
-            uint32_t s[64];
-            tmem_ld32(s_addr + 64 * half, s);
-            tmem_ld32(s_addr + 64 * half + 32, s + 32);
-            tmem_ld_wait();
-            const uint32_t at = sc + 256 * half;
-            uint32_t pw[32];
-            if (!masked) {
+          {
+            float2 l2 = make_float2(l, 0.f);
+            const float2 nm2 = make_float2(-m, -m);
+            uint32_t x0[32], x1[32];
+            auto weigh = [&](const uint32_t* x, int ch) {
+              const float4* at = reinterpret_cast<const float4*>(vec + 32 * ch);
+              uint32_t pw[16];
 #pragma unroll
-              for (int i = 0; i < 64; i += 4) {
-                const float4 sk = lds_f4(at + 4 * i), lv = lds_f4(at + L::SLOT_LV + 4 * i), rv = lds_f4(at + L::SLOT_RV + 4 * i);
-                const float2 x = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(sk.x, sk.y)), c2,
+              for (int i = 0; i < 8; ++i) {
+                const float4 sk = at[i], lv = at[KT / 4 + i], rv = at[KT / 2 + i];
+                const float2 u = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1])), make_float2(sk.x, sk.y)), c2,
                                             __fadd2_rn(make_float2(lv.x, lv.y), nm2));
-                const float2 y = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(sk.z, sk.w)), c2,
+                const float2 v = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3])), make_float2(sk.z, sk.w)), c2,
                                             __fadd2_rn(make_float2(lv.z, lv.w), nm2));
-                const float2 w = make_float2(fast_ex2(x.x), fast_ex2(x.y)), z = make_float2(fast_ex2(y.x), fast_ex2(y.y));
+                const float2 w = make_float2(fast_ex2(u.x), fast_ex2(u.y)), z = make_float2(fast_ex2(v.x), fast_ex2(v.y));
                 l2 = __ffma2_rn(w, make_float2(rv.x, rv.y), l2);
                 l2 = __ffma2_rn(z, make_float2(rv.z, rv.w), l2);
-                pw[i / 2] = pair16<__half>(w.x, w.y);
-                pw[i / 2 + 1] = pair16<__half>(z.x, z.y);
+                pw[2 * i] = pair16<__half>(w.x, w.y);
+                pw[2 * i + 1] = pair16<__half>(z.x, z.y);
               }
-            } else {
-              const uint32_t bits[2] = {lds_u32(seen_at + 4 * L::SOFTMAX * (2 * half)), lds_u32(seen_at + 4 * L::SOFTMAX * (2 * half + 1))};
-#pragma unroll
-              for (int i = 0; i < 64; i += 4) {
-                const float4 sk = lds_f4(at + 4 * i), lv = lds_f4(at + L::SLOT_LV + 4 * i), rv = lds_f4(at + L::SLOT_RV + 4 * i);
-                const float f[4] = {sk.x, sk.y, sk.z, sk.w}, v[4] = {lv.x, lv.y, lv.z, lv.w}, r4[4] = {rv.x, rv.y, rv.z, rv.w};
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {        // (nothing of a key that is not seen, whatever it holds)
-                  const bool seen = bits[i / 32] >> ((i + e) & 31) & 1u;
-                  w[e] = seen ? fast_ex2(fmaf(__uint_as_float(s[i + e]) * f[e], row_c, v[e] - m)) : 0.f;
-                  if (seen) l2.x = fmaf(w[e], r4[e], l2.x);
-                }
-                pw[i / 2] = pair16<__half>(w[0], w[1]);
-                pw[i / 2 + 1] = pair16<__half>(w[2], w[3]);
-              }
+              tmem_st16(s_addr + 16 * ch, pw);       // over scores that have been read
+            };
+            tmem_ld32(s_addr, x0);
+#pragma unroll 1
+            for (int ch = 0; ch < CHUNKS; ch += 2) {
+              tmem_ld_wait();
+              tmem_ld32(s_addr + 32 * ch + 32, x1);
+              weigh(x0, ch);
+              tmem_ld_wait();
+              if (ch + 2 < CHUNKS) tmem_ld32(s_addr + 32 * ch + 64, x0);
+              weigh(x1, ch + 1);
             }
-            tmem_st32(s_addr + 32 * half, pw);       // over scores that have been read
+            l = l2.x + l2.y;
           }
-          l = l2.x + l2.y;
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
@@ -529,12 +539,15 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       if (!ok) break;
       if (ct < KT) {
         const uint32_t sc = base + L::OFF_SC + (n % L::SLOTS) * L::SLOT;
-        const float v = sv == 0.f ? 1e-30f : sv;     // (a row that nothing wrote: value 0, but a part of the sum)
-        sts_f32(sc + 4 * ct, sk);
+        const bool none = sk < 0.f, nan = isnan(sk) || isnan(sv);
+        const float v = none || nan ? 1.f : fmaxf(sv, 1e-30f);       // (0: a row that nothing wrote, all codes 0; a part of the sum)
+        sts_f32(sc + 4 * ct, none || nan ? 1.f : fmaxf(sk, 1e-30f));
         sts_f32(sc + L::SLOT_LV + 4 * ct, __log2f(v));
         sts_f32(sc + L::SLOT_RV + 4 * ct, __fdividef(1.f, v));
-        const uint32_t none = __ballot_sync(0xffffffffu, sk < 0.f);
-        if (lane == 0) sts_u32(sc + L::SLOT_NONE + 4 * (ct >> 5), none);
+        const uint32_t none32 = __ballot_sync(0xffffffffu, none), nan32 = __ballot_sync(0xffffffffu, nan);
+        // (positive floats are ordered as their bits are)
+        const float big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))), small = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(v)));
+        if (lane == 0) sts16(sc + L::SLOT_SUM + 16 * (ct >> 5), none32, nan32, __float_as_uint(__log2f(big)), __float_as_uint(__log2f(small)));
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_SC + n % L::SLOTS));
       }
