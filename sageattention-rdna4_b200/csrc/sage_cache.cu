@@ -7,6 +7,7 @@
 // rows are 64 bytes wide for heads of up to 64 columns and 128 bytes otherwise, zero-filled; the code
 // of column d is byte d.  Value = code * scale, plus the shift of K if the cache has one.
 #include <algorithm>
+#include <atomic>
 
 #include "sage_common.cuh"
 #include "sage_internal.h"
@@ -313,12 +314,6 @@ __global__ void __launch_bounds__(CACHE_THREADS) cache_read_kernel(const ReadKAr
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 template <typename T>
 cudaError_t launch_rotary_t(const RotaryKArgs& a, bool interleaved, long long blocks, cudaStream_t st) {
   const int half = a.rot / 2;
@@ -354,6 +349,16 @@ cudaError_t launch_read_t(const ReadKArgs& a, int width, cudaStream_t st) {
 }
 
 }  // namespace
+
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  return sms;
+}
 
 cudaError_t launch_rotary(const RotaryParams& p, cudaStream_t st) {
   RotaryKArgs a;

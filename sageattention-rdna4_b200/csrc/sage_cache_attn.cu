@@ -582,7 +582,8 @@ cudaError_t launch_attn(CacheAttnKArgs& a, int sms, cudaStream_t st) {
   constexpr int STAGES = 3;
   auto kern = cache_attn_kernel<T, INT8, WIDTH, NB, STAGES, CTAS_PER_SM>;
   constexpr uint32_t smem = CaSmem<WIDTH, STAGES>::BYTES;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static DeviceOnce once;
+  cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
   if (e != cudaSuccess) return e;
   a.max_stretches = std::min(sms, SIZING_SMS) * CTAS_PER_SM * CA_WARPS;
   const long long steps = (long long)a.n_seq * a.Hkv * std::max<long long>(1, (((long long)a.table_width << a.page_shift) + CA_KEYS - 1) / CA_KEYS);
@@ -642,8 +643,7 @@ cudaError_t launch_cache_attention(const CacheView& c, const CacheAttnParams& p,
   a.part_rows = (int)std::min<int64_t>(rows, f.rows);
   a.part_o = reinterpret_cast<float*>(p.scratch);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * f.max_stretches * a.part_rows * HD);
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = sm_count();
   const cudaError_t e = f.tree ? launch_cache_tree(a, c, p.dtype, sms, p.status_host, st)
                                : p.dtype == 0 ? launch_type<__half>(a, c, f.rows, sms, st) : launch_type<__nv_bfloat16>(a, c, f.rows, sms, st);
   if (e != cudaSuccess) return e;

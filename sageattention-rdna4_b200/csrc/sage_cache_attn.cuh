@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 
 #include "sage_common.cuh"
 #include "sage_internal.h"
@@ -184,6 +185,20 @@ template <typename T> __device__ __forceinline__ T from_float(float x);
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Runs something once per device (a kernel's attributes; doing it twice at the same time does no harm).
+struct DeviceOnce {
+  std::atomic<unsigned long long> done{0};           // a bit per device; further ones ask every time
+  template <typename F> cudaError_t run(F&& f) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = f();
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+};
 // Joins partial results (see sage_cache_attn.cu); rows and keys are those of a row tile and of a step.
 cudaError_t launch_cache_combine(const CacheAttnKArgs& a, int dtype, int rows, int keys, int width, int max_rt, cudaStream_t st);
 // The kernel for many rows (see sage_cache_tree.cu); status_host: optional pinned word for its bounded waits.

@@ -629,7 +629,8 @@ template <typename T, bool INT8, int WIDTH, int NQ, int KT>
 cudaError_t launch_tree(CacheAttnKArgs& a, int sms, int32_t* status_host, cudaStream_t st) {
   using L = TreeShape<WIDTH, NQ, KT>;
   auto kern = cache_tree_kernel<T, INT8, WIDTH, NQ, KT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::BYTES);
+  static DeviceOnce once;
+  cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::BYTES); });
   if (e != cudaSuccess) return e;
   const long long rows = (long long)a.max_q * a.group, rts = (rows + L::ROWS - 1) / L::ROWS;
   const long long steps = (long long)a.n_seq * a.Hkv * rts * std::max<long long>(1, (((long long)a.table_width << a.page_shift) + KT - 1) / KT);

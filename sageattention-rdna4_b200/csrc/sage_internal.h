@@ -99,6 +99,9 @@ void set_tiles_per_cta(int n);
 void set_skip_log2(float t);
 int choose_tiles_per_cta(int64_t q_tiles, int64_t bhq, bool causal, int sms);
 
+// SMs of the current device (asked for once per device).
+int sm_count();
+
 // ---- a quantised, paged K/V cache (see sage_cache.cu for its layout) ------------------------------
 struct CacheView {
   uint8_t *k_codes, *v_codes;      // (pages, H, page_size, width)

@@ -24,7 +24,7 @@ import torch
 
 from . import _native
 from . import b200_backend as _be
-from .b200_backend import HEAD_DIM, _counters, _dtype_code, _report_to, _state, packed_view_reason, strided_view_reason
+from .b200_backend import HEAD_DIM, _counters, _dtype_code, _grow, _report_to, _state, packed_view_reason, strided_view_reason
 
 _E4M3 = torch.float8_e4m3fn
 
@@ -39,22 +39,35 @@ def _check_head_dim(d: int):
         _refuse("head_dim must be a multiple of 8 in 8..128, got %d" % d, NotImplementedError)
 
 
-class _on_device:
-    """Makes `dev` the current device for the C call; nothing where it is already."""
+def _call(fn, dev, args):
+    """The C call, on `dev` as the current device."""
+    prev = torch.cuda.current_device()
+    if prev == dev.index:
+        return fn(*args)
+    torch.cuda.set_device(dev)
+    try:
+        return fn(*args)
+    finally:
+        torch.cuda.set_device(prev)
 
-    __slots__ = ("dev", "prev")
 
-    def __init__(self, dev):
-        self.dev = dev
+# A step of generation is a handful of calls whose GPU work takes a few microseconds each, so that the host path must
+# not take longer.  A call signature (shapes, strides, dtypes, devices, alignment) that has passed the checks once is
+# remembered with what the C call is given for it, as for `sageattn`.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_PLANS = 256
 
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.dev.index:
-            torch.cuda.set_device(self.dev)
 
-    def __exit__(self, *exc):
-        if self.prev != self.dev.index:
-            torch.cuda.set_device(self.prev)
+def _sig(t: torch.Tensor):
+    return t.shape, t.stride(), t.dtype, t.device, t.data_ptr() & 15
+
+
+def _remember(plans: dict, key, plan):
+    if len(plans) >= _PLANS:
+        plans.clear()
+    plans[key] = plan
+    return plan
 
 
 class SageCache:
@@ -71,7 +84,7 @@ class SageCache:
     """
 
     __slots__ = ("k_codes", "k_scale", "v_codes", "v_scale", "k_shift", "head_dim", "num_pages", "page_size",
-                 "num_kv_heads", "device", "_mode", "_args", "_sizes")
+                 "num_kv_heads", "device", "_mode", "_args", "_sizes", "_plans")
 
     def __init__(self, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
                  head_dim: int, k_shift: Optional[torch.Tensor] = None):
@@ -109,6 +122,7 @@ class SageCache:
         self._args = (k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
                       0 if k_shift is None else k_shift.data_ptr())
         self._sizes = (pages, page)
+        self._plans = {}                             # call signature -> what the C call is given for it
 
     @classmethod
     def empty(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16,
@@ -158,6 +172,19 @@ def sage_cache_write(cache: SageCache, k: torch.Tensor, v: torch.Tensor, slots: 
     NaN throughout.
     """
     _counters["calls"] += 1
+    key = ("write", _sig(k), _sig(v), _sig(slots))
+    plan = cache._plans.get(key)
+    if plan is None:
+        plan = _remember(cache._plans, key, _plan_write(cache, k, v, slots))
+    if plan:
+        dev = cache.device
+        rc = _call(_native.load().sage_cache_write, dev, (
+            k.data_ptr(), v.data_ptr(), slots.data_ptr(), plan[0], *cache._args, *plan[1:], _raw_stream(dev.index)))
+        if rc:
+            _native.check(rc, "sage_cache_write")
+
+
+def _plan_write(cache, k, v, slots):
     dev, heads, d = cache.device, cache.num_kv_heads, cache.head_dim
     _check_rows("k", k, heads, d, dev)
     _check_rows("v", v, heads, d, dev)
@@ -167,13 +194,9 @@ def sage_cache_write(cache: SageCache, k: torch.Tensor, v: torch.Tensor, slots: 
     if slots.shape[0] != k.shape[0]:
         _refuse("slots must hold one entry per token")
     if k.shape[0] == 0:
-        return
-    with _on_device(dev):
-        rc = _native.load().sage_cache_write(
-            k.data_ptr(), v.data_ptr(), slots.data_ptr(), slots.dtype == torch.int64, *cache._args, k.shape[0], heads, d,
-            *cache._sizes, _native.strides2(k.stride(0), k.stride(1)), _native.strides2(v.stride(0), v.stride(1)),
-            _dtype_code(k.dtype), cache._mode, torch.cuda.current_stream(dev).cuda_stream)
-    _native.check(rc, "sage_cache_write")
+        return ()
+    return (slots.dtype == torch.int64, k.shape[0], heads, d, *cache._sizes, _native.strides2(k.stride(0), k.stride(1)),
+            _native.strides2(v.stride(0), v.stride(1)), _dtype_code(k.dtype), cache._mode)
 
 
 def sage_cache_read(cache: SageCache, page_table: torch.Tensor, cu_seqlens: torch.Tensor, total: int,
@@ -186,33 +209,46 @@ def sage_cache_read(cache: SageCache, page_table: torch.Tensor, cu_seqlens: torc
     (in fresh outputs: undefined); tokens on a page that does not exist read as zeros.
     """
     _counters["calls"] += 1
-    dev, heads, d, total = cache.device, cache.num_kv_heads, cache.head_dim, int(total)
-    code = _dtype_code(dtype)
-    _check_index("page_table", page_table, dev, 2)
-    _check_index("cu_seqlens", cu_seqlens, dev, 1)
-    if page_table.shape[0] < 1 or page_table.shape[1] < 1 or cu_seqlens.shape[0] != page_table.shape[0] + 1:
-        _refuse("page_table and cu_seqlens must describe the same sequences, at least one")
-    if total < 0:
-        _refuse("total must not be negative")
+    dev, heads, d = cache.device, cache.num_kv_heads, cache.head_dim
+    key = ("read", _sig(page_table), _sig(cu_seqlens), total, dtype, None if out is None else tuple(_sig(t) for t in out))
+    plan = cache._plans.get(key)
+    if plan is None:
+        plan = _remember(cache._plans, key, _plan_read(cache, page_table, cu_seqlens, total, dtype, out))
     if out is None:
         k = torch.empty((total, heads, d), dtype=dtype, device=dev)
         v = torch.empty((total, heads, d), dtype=dtype, device=dev)
     else:
         k, v = out
-        for name, t in (("out[0]", k), ("out[1]", v)):
+    if plan:
+        rc = _call(_native.load().sage_cache_read, dev, (
+            *cache._args, page_table.data_ptr(), plan[0], plan[1], cu_seqlens.data_ptr(), k.data_ptr(), v.data_ptr(), *plan[2:],
+            _raw_stream(dev.index)))
+        if rc:
+            _native.check(rc, "sage_cache_read")
+    return k, v
+
+
+def _plan_read(cache, page_table, cu_seqlens, total, dtype, out):
+    dev, heads, d = cache.device, cache.num_kv_heads, cache.head_dim
+    code = _dtype_code(dtype)
+    _check_index("page_table", page_table, dev, 2)
+    _check_index("cu_seqlens", cu_seqlens, dev, 1)
+    if page_table.shape[0] < 1 or page_table.shape[1] < 1 or cu_seqlens.shape[0] != page_table.shape[0] + 1:
+        _refuse("page_table and cu_seqlens must describe the same sequences, at least one")
+    if not isinstance(total, int) or total < 0:
+        _refuse("total must be an int, not negative")
+    strides = [_native.strides2(heads * d, d)] * 2
+    if out is not None:
+        if len(out) != 2:
+            _refuse("out must be a pair")
+        for name, t in (("out[0]", out[0]), ("out[1]", out[1])):
             _check_rows(name, t, heads, d, dev)
             if t.shape[0] != total or t.dtype != dtype:
                 _refuse("%s must hold total rows of dtype" % name)
+        strides = [_native.strides2(t.stride(0), t.stride(1)) for t in out]
     if total == 0:
-        return k, v
-    with _on_device(dev):
-        rc = _native.load().sage_cache_read(
-            *cache._args, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cu_seqlens.data_ptr(),
-            k.data_ptr(), v.data_ptr(), page_table.shape[0], total, heads, d, *cache._sizes,
-            _native.strides2(k.stride(0), k.stride(1)), _native.strides2(v.stride(0), v.stride(1)), code, cache._mode,
-            torch.cuda.current_stream(dev).cuda_stream)
-    _native.check(rc, "sage_cache_read")
-    return k, v
+        return ()
+    return (page_table.stride(0), page_table.shape[1], page_table.shape[0], total, heads, d, *cache._sizes, *strides, code, cache._mode)
 
 
 def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor, seqlens_k: torch.Tensor,
@@ -237,6 +273,39 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
     result depend on the lengths of the other sequences of the call (fp32 sums in another order).
     """
     _counters["calls"] += 1
+    dev = cache.device
+    key = ("attend", _sig(q), _sig(page_table), _sig(seqlens_k), None if cu_seqlens_q is None else _sig(cu_seqlens_q), max_seqlen_q,
+           None if tree_mask is None else _sig(tree_mask), sm_scale, None if out is None else _sig(out))
+    plan = cache._plans.get(key)
+    if plan is None:
+        plan = _remember(cache._plans, key, _plan_attend(cache, q, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tree_mask, sm_scale, out))
+    if out is None:
+        out = q.new_empty(q.shape)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+    if plan:
+        ws_bytes, table_stride, width, tree_stride, rest = plan
+        stream = _raw_stream(dev.index)
+        capturing = torch.cuda.is_current_stream_capturing()
+        st = _state(dev, stream)                     # workspace and host word of the stream, as for `sageattn`
+        if st.host_word is not None and st.host_word.value:
+            st.raise_if_failed("the next call on the stream")
+        if capturing:                                # a captured call has memory of its graph's own: two graphs may run at once
+            ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+        else:
+            ws = st.ws if st.ws is not None and st.ws.numel() >= ws_bytes else _grow(st, dev, ws_bytes)
+        rc = _call(_native.load().sage_cache_attention, dev, (
+            q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *cache._args, page_table.data_ptr(), table_stride, width,
+            seqlens_k.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(),
+            tree_stride, ws.data_ptr(), ws_bytes, *rest, _report_to(st, capturing), stream))
+        if rc:
+            _native.check(rc, "sage_cache_attention")
+        if _be._STRICT and not capturing:
+            torch.cuda.current_stream(dev).synchronize()
+            st.raise_if_failed("this call (strict mode)")
+    return (out, lse) if return_lse else out
+
+
+def _plan_attend(cache, q, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tree_mask, sm_scale, out):
     dev, hkv, d = cache.device, cache.num_kv_heads, cache.head_dim
     if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % hkv:
         _refuse("q must be (tokens, heads, head_dim) with a multiple of the cache's %d heads" % hkv)
@@ -265,35 +334,16 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
     scale = d ** -0.5 if sm_scale is None else float(sm_scale)
     if not (0.0 < scale < float("inf")):
         _refuse("sm_scale must be finite and positive, got %r" % (sm_scale,))
-    if out is None:
-        out = torch.empty((tokens, hq, d), dtype=q.dtype, device=dev)
-    else:
+    if out is not None:
         _check_rows("out", out, hq, d, dev)
         if out.shape != q.shape or out.dtype != q.dtype:
             _refuse("out must have q's shape and dtype")
-    lse = torch.empty((tokens, hq), dtype=torch.float32, device=dev) if return_lse else None
-    if tokens:
-        lib = _native.load()
-        # (from the caching allocator with every call: ordered with this stream, and a captured graph's own)
-        ws = torch.empty((lib.sage_cache_attention_workspace_bytes(batch, hq, hkv, max_q),), dtype=torch.uint8, device=dev)
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        capturing = torch.cuda.is_current_stream_capturing()
-        st = _state(dev, stream)                     # (the host word that a failed call reports to, as for `sageattn`)
-        st.raise_if_failed("the next call on the stream")
-        with _on_device(dev):
-            rc = lib.sage_cache_attention(
-                q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *cache._args,
-                page_table.data_ptr(), page_table.stride(0), width, seqlens_k.data_ptr(),
-                0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
-                0 if tree_mask is None else tree_mask.data_ptr(), 0 if tree_mask is None else tree_mask.stride(0),
-                ws.data_ptr(), ws.numel(), batch, hq, hkv, tokens, max_q, d, *cache._sizes,
-                _native.strides2(q.stride(0), q.stride(1)), _native.strides2(out.stride(0), out.stride(1)),
-                _dtype_code(q.dtype), cache._mode, scale, _report_to(st, capturing), stream)
-        _native.check(rc, "sage_cache_attention")
-        if _be._STRICT and not capturing:
-            torch.cuda.current_stream(dev).synchronize()
-            st.raise_if_failed("this call (strict mode)")
-    return (out, lse) if return_lse else out
+    if tokens == 0:
+        return ()
+    o2 = _native.strides2(hq * d, d) if out is None else _native.strides2(out.stride(0), out.stride(1))
+    rest = (batch, hq, hkv, tokens, max_q, d, *cache._sizes, _native.strides2(q.stride(0), q.stride(1)), o2, _dtype_code(q.dtype), cache._mode, scale)
+    return (int(_native.load().sage_cache_attention_workspace_bytes(batch, hq, hkv, max_q)), page_table.stride(0), width,
+            0 if tree_mask is None else tree_mask.stride(0), rest)
 
 
 # ---- rotary positions --------------------------------------------------------------------------------------------
@@ -309,7 +359,7 @@ class SageRotary:
         linear ramp between, and the result is scaled by ``0.1 ln(factor) + 1``.
     """
 
-    __slots__ = ("head_dim", "rotary_dim", "interleaved", "inv_freq", "magnitude", "device")
+    __slots__ = ("head_dim", "rotary_dim", "interleaved", "inv_freq", "magnitude", "device", "_plans")
 
     def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, interleaved: bool = False,
                  scaling: str = "none", factor: float = 1.0, original_length: int = 4096, fast: float = 32.0, slow: float = 1.0,
@@ -338,6 +388,7 @@ class SageRotary:
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, rot, bool(interleaved)
         self.inv_freq = torch.tensor(freq, dtype=torch.float64).to(device)
         self.device = self.inv_freq.device
+        self._plans = {}
 
 
 def _rotary_views(x, layout):
@@ -373,12 +424,36 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _rotate(q, k, positions, rotary, layout, backward, out):
+    # (an output that is its input needs no more of a plan than that the two inputs share nothing: their distance)
+    in_place = out is not None and (out is q if k is None else len(out) == 2 and out[0] is q and out[1] is k)
+    key = (_sig(q), None if k is None else _sig(k), _sig(positions), layout, in_place and (0 if k is None else k.data_ptr() - q.data_ptr()))
+    kept = out is None or in_place
+    plan = rotary._plans.get(key) if kept else None
+    if plan is None:
+        plan = _plan_rotary(q, k, positions, rotary, layout, out)
+        if kept:
+            _remember(rotary._plans, key, plan)
+    dev = rotary.device
+    if out is None:
+        outs = (q.new_empty(q.shape),) if k is None else (q.new_empty(q.shape), k.new_empty(k.shape))
+    else:
+        outs = (out,) if isinstance(out, torch.Tensor) else tuple(out)
+    if plan:
+        k_ptrs = (0, 0) if k is None else (k.data_ptr(), outs[1].data_ptr())
+        rc = _call(_native.load().sage_rotary, dev, (
+            q.data_ptr(), outs[0].data_ptr(), *k_ptrs, positions.data_ptr(), positions.dtype == torch.int64, rotary.inv_freq.data_ptr(),
+            rotary.magnitude, *plan[0], rotary.rotary_dim, rotary.interleaved, backward, *plan[1], _raw_stream(dev.index)))
+        if rc:
+            _native.check(rc, "sage_rotary")
+    return outs
+
+
+def _plan_rotary(q, k, positions, rotary, layout, out):
     ins = [x for x in (q, k) if x is not None]
     views = [_rotary_views(x, layout) for x in ins]
     dev = q.device
-    if out is None:
-        outs = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in ins]
-    else:
+    o_views = []
+    if out is not None:
         outs = [out] if isinstance(out, torch.Tensor) else list(out)
         if len(outs) != len(ins):
             _refuse("out must hold one tensor per input")
@@ -389,7 +464,7 @@ def _rotate(q, k, positions, rotary, layout, backward, out):
                 own = j == i and o.data_ptr() == y.data_ptr() and o.stride() == y.stride()
                 if x.numel() and y.numel() and not own and _overlap(o, y):
                     _refuse("out may be its own input, and overlaps nothing else")
-    o_views = [_rotary_views(x, layout) for x in outs]
+        o_views = [_rotary_views(x, layout) for x in outs]
     b, _, n, d = views[0].shape
     for v in views + o_views:
         if v.device != dev or not v.is_cuda:
@@ -411,17 +486,19 @@ def _rotate(q, k, positions, rotary, layout, backward, out):
         p2 = positions.stride()
     else:
         _refuse("positions must be (N,) or (B, N)")
-    if b * n:
-        s3 = [_native.strides3(v.stride(0), v.stride(1), v.stride(2)) for v in (views[0], o_views[0], views[-1], o_views[-1])]
-        two = k is not None
-        with _on_device(dev):
-            rc = _native.load().sage_rotary(
-                q.data_ptr(), outs[0].data_ptr(), k.data_ptr() if two else 0, outs[1].data_ptr() if two else 0,
-                positions.data_ptr(), positions.dtype == torch.int64, rotary.inv_freq.data_ptr(), rotary.magnitude,
-                b, views[0].shape[1], views[1].shape[1] if two else 0, n, d, rotary.rotary_dim, rotary.interleaved, backward,
-                *s3, _native.strides2(*p2), _dtype_code(q.dtype), torch.cuda.current_stream(dev).cuda_stream)
-        _native.check(rc, "sage_rotary")
-    return tuple(outs)
+    if not b * n:
+        return ()
+
+    def triple(v):
+        return _native.strides3(v.stride(0), v.stride(1), v.stride(2))
+
+    def fresh(v):                                    # of a contiguous tensor in the inputs' layout
+        h = v.shape[1]
+        return _native.strides3(n * h * d, d, h * d) if q.dim() == 3 or layout == "NHD" else _native.strides3(h * n * d, n * d, d)
+    s3 = []
+    for i in (0, len(ins) - 1):
+        s3 += [triple(views[i]), triple(o_views[i]) if o_views else fresh(views[i])]
+    return ((b, views[0].shape[1], views[1].shape[1] if k is not None else 0, n, d), (*s3, _native.strides2(*p2), _dtype_code(q.dtype)))
 
 
 class _Rotary(torch.autograd.Function):
