@@ -547,7 +547,9 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
   T* dst = reinterpret_cast<T*>(a.out) + (long long)(s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
   if (WARPS_PER_ROW == 1) {
     const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-    if (4 * lane < a.D) *reinterpret_cast<uint2*>(dst + 4 * lane) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
+    // (the many-row kernel leaves the columns of wide heads in the order of its accumulator)
+    const int n = 4 * lane, col = width == 128 ? 16 * ((n >> 3) & 7) + 8 * (n >> 6) + (n & 7) : n;
+    if (mine && col < a.D) *reinterpret_cast<uint2*>(dst + col) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
   } else {
     if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
     if (lane == 0) ml_s[warp] = make_float2(top, sum);
@@ -619,7 +621,7 @@ cudaError_t launch_cache_combine(const CacheAttnKArgs& a, int dtype, int rows, i
 
 CacheForm cache_form(int64_t rows) {
   if (rows <= 16) return {false, rows <= 8 ? 8 : 16, CA_KEYS, SIZING_SMS * CTAS_PER_SM * CA_WARPS};
-  return rows <= 128 ? CacheForm{true, 128, 64, 2 * SIZING_SMS} : CacheForm{true, 256, 128, SIZING_SMS};
+  return rows <= 128 ? CacheForm{true, 128, 64, 2 * SIZING_SMS} : CacheForm{true, 256, 64, SIZING_SMS};
 }
 
 size_t cache_attention_scratch(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q) {

@@ -2,23 +2,26 @@
 // group) fill the tensor core's 128-row operand.  Same formulas, line of work and partial results as
 // sage_cache_attn.cu; the products are tcgen05.mma with accumulators in TMEM.
 //
-// A CTA takes a row tile of NQ x 128 rows and walks its stretch of the keys, KT at a time:
+// A CTA takes a row tile of NQ x 128 rows and walks its stretch of the keys, 64 at a time:
 //   warps 0 .. 4 NQ - 1   softmax: a thread owns a row (32x32b TMEM loads: a lane is a row), so that maxima and sums
 //                         need no other lane; its weights go back to TMEM as fp16, over the scores they came from, and
 //                         are the A operand of P V from there
 //   the next four warps   fetch the one-byte codes (a tile ahead, in registers), turn them into fp16 -- exact -- and
-//                         write them to shared memory as the operands want them (128-byte swizzle), two stages deep
-//   one more warp         one thread issues every tcgen05.mma and commit (three idle warps complete its warpgroup, whose
+//                         write them to shared memory as the operands want them (128-byte swizzle)
+//   NQ more warps         a thread each that issues the products of 128 rows (idle warps complete the warpgroup, whose
 //                         registers the softmax takes over)
-// K is a K-major operand; V, whose rows are keys too, is the MN-major B operand of P V: both are written alike, a
-// row of 64 columns in 128 bytes.  Heads of more than 64 columns take two such halves; columns 16 p .. 16 p + 7 of a
-// row go to piece p of the first half and the next 8 to piece p of the second, for K, Q and V alike, so that the
-// eight lanes that write the pieces of a row reach all banks (the order of an inner product's columns is free, and
-// that of V's is undone where the output is written).
+// Scores have two buffers in TMEM: those of the next tile are under way while the softmax works on a tile, and P V
+// follows behind.  K is a K-major operand; V, whose rows are keys too, is the MN-major B operand of P V: both are
+// written alike, a row of 64 columns in 128 bytes.  Heads of more than 64 columns take two such halves; columns 16 p ..
+// 16 p + 7 of a row go to piece p of the first half and the next 8 to piece p of the second, for K, Q and V alike, so
+// that the eight lanes that write the pieces of a row reach all banks (the order of an inner product's columns is
+// free, and that of V's is undone where the output is written).
 //
-// NQ = 2, KT = 128 (rows beyond 128): one CTA per SM with all 512 TMEM columns, {S 128, O 128} per 128 rows; while one
-// half's softmax runs the other half's products do.  NQ = 1, KT = 64: two CTAs per SM, which overlap each other.
-// (Converting a tile costs about a fifth of one half's softmax, so rows are added to a CTA before CTAs are.)
+// The scale of V goes into the exponent: e = score + log2(scale), the weight is 2^(e - m) and the row's sum takes the weight
+// over the scale, so that one maximum serves both the softmax and fp16's range.
+//
+// NQ = 2 (rows beyond 128): one CTA per SM with all 512 TMEM columns.  NQ = 1: two CTAs per SM.  (Rows are added to a
+// CTA before CTAs are: a tile's codes are fetched and converted once per CTA.)
 //
 // Every wait is bounded (about two seconds): it then leaves a code in the caller's pinned host word, the CTA drains
 // its products, frees its TMEM and returns.
@@ -86,12 +89,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
-      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr) : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
@@ -138,15 +142,20 @@ __device__ __forceinline__ void codes_to_half(const uint4& u, uint32_t (&h)[8]) 
   }
 }
 
-template <int WIDTH, int NQ, int KT> struct TreeShape {
+constexpr int KT = 64;                               // keys of a tile
+template <int WIDTH, int NQ> struct TreeShape {
   static constexpr int SOFTMAX = 128 * NQ, LOADERS = 128, THREADS = SOFTMAX + LOADERS + 128;
   static constexpr int CTAS_PER_SM = NQ == 1 ? 2 : 1;
   // Registers per thread: at launch (what __launch_bounds__ leaves: 65536 / threads of the SM, in eights), and after the
-  // issuing warpgroup has handed its own to the softmax.  setmaxnreg.inc waits until the pool holds what it asks for, so
-  // that the three must not add up to more than the launch has.
-  static constexpr int REGS_LAUNCH = NQ == 1 ? 80 : 128, REGS_SOFTMAX = NQ == 1 ? 104 : 160, REGS_ISSUER = NQ == 1 ? 56 : 64;
-  static_assert(NQ * REGS_SOFTMAX + REGS_LAUNCH + REGS_ISSUER <= (NQ + 2) * REGS_LAUNCH, "setmaxnreg would wait forever");
-  static constexpr int STAGES = 2, SLOTS = 4;
+  // warpgroups have shared them out.  setmaxnreg.inc waits until the pool holds what it asks for, so that the shares
+  // must not add up to more than the launch has.
+  static constexpr int REGS_LAUNCH = NQ == 1 ? 80 : 128, REGS_SOFTMAX = NQ == 1 ? 120 : 168, REGS_LOADER = NQ == 1 ? 72 : 112,
+                       REGS_ISSUER = NQ == 1 ? 48 : 64;
+  static_assert(NQ * REGS_SOFTMAX + REGS_LOADER + REGS_ISSUER <= (NQ + 2) * REGS_LAUNCH, "setmaxnreg would wait forever");
+  // Stages of K and V; slots of scales.  A slot is written once the scores STAGES tiles back are complete, which means that
+  // the softmax is done with the tile two before that.
+  static constexpr int STAGES = NQ == 1 ? 2 : 4, SLOTS = NQ == 1 ? 4 : 8;
+  static_assert(SLOTS >= STAGES + 2, "");
   static constexpr uint32_t HALVES = WIDTH / 64;
   static constexpr uint32_t Q_HALF = 128 * 128, Q_TILE = HALVES * Q_HALF;             // 128 rows of 128 bytes
   static constexpr uint32_t KV_HALF = KT * 128, KV_TILE = HALVES * KV_HALF;
@@ -154,19 +163,24 @@ template <int WIDTH, int NQ, int KT> struct TreeShape {
   // of a tile: scales of K, log2 and reciprocal of the scales of V, and for every 32 keys {a bit for each that does not
   // exist, a bit for each that holds a NaN, the largest and the smallest log2 of a scale of V}
   static constexpr uint32_t SLOT_LV = KT * 4, SLOT_RV = KT * 8, SLOT_SUM = KT * 12, SLOT = SLOT_SUM + KT / 2;
-  static constexpr uint32_t OFF_BAR = OFF_SC + SLOTS * SLOT, OFF_MISC = OFF_BAR + 176, USED = OFF_MISC + 16;
+  static constexpr uint32_t OFF_ROW = OFF_SC + SLOTS * SLOT;                          // a float per row
+  static constexpr uint32_t OFF_BAR = OFF_ROW + SOFTMAX * 4;
+  // Barriers: per half of the rows (QF) and score buffer (SF, PF, PV), per stage (KF, KE, VF, VE), per slot (SC).  What is
+  // waited for is never more than one phase away from where its barrier stands: the scores of a tile are issued after P V of
+  // the tile two before, which waited for that tile's weights.
+  static constexpr int B_QF = 0, B_PV = 2, B_SF = 6, B_PF = 10, B_DRAIN = 14, B_KF = 15, B_KE = B_KF + STAGES, B_VF = B_KE + STAGES,
+                       B_VE = B_VF + STAGES, B_SC = B_VE + STAGES, B_COUNT = B_SC + SLOTS;
+  static constexpr uint32_t OFF_MISC = OFF_BAR + (B_COUNT * 8 + 15) / 16 * 16, USED = OFF_MISC + 16;
   static constexpr uint32_t BYTES = USED + 1024;                                      // slack for the 1024-byte alignment
-  static constexpr uint32_t TMEM_COLS = NQ * (KT + WIDTH) <= 128 ? 128 : NQ * (KT + WIDTH) <= 256 ? 256 : 512;
+  static constexpr uint32_t TMEM_COLS = NQ * (2 * KT + WIDTH) <= 256 ? 256 : 512;
   static constexpr int ROWS = 128 * NQ;
 };
-// Barriers: per half of the rows (QF, SF, PF, PV), per stage (KF, KE, VF, VE), per slot of scales (SC).
-enum { B_QF = 0, B_KF = 2, B_KE = 4, B_VF = 6, B_VE = 8, B_SF = 10, B_PF = 12, B_PV = 14, B_SC = 16, B_DRAIN = 20, B_COUNT = 21 };
 
-template <typename T, bool INT8, int WIDTH, int NQ, int KT>
-__global__ void __launch_bounds__(TreeShape<WIDTH, NQ, KT>::THREADS, TreeShape<WIDTH, NQ, KT>::CTAS_PER_SM)
+template <typename T, bool INT8, int WIDTH, int NQ>
+__global__ void __launch_bounds__(TreeShape<WIDTH, NQ>::THREADS, TreeShape<WIDTH, NQ>::CTAS_PER_SM)
 cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
-  using L = TreeShape<WIDTH, NQ, KT>;
-  constexpr int ROWS = L::ROWS, CHUNKS = KT / 32;
+  using L = TreeShape<WIDTH, NQ>;
+  constexpr int ROWS = L::ROWS;
   constexpr uint32_t IDESC_QK = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
   constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | ((uint32_t)(WIDTH >> 3) << 17) | (8u << 24);   // B is MN-major
   extern __shared__ uint8_t smem_raw[];
@@ -187,14 +201,14 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
   const Watch watch = {misc + 1, status_host};
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(B_QF + i), 4);
-      mbar_init(bar(B_KF + i), 4); mbar_init(bar(B_KE + i), 1);
-      mbar_init(bar(B_VF + i), 4); mbar_init(bar(B_VE + i), 1);
-      mbar_init(bar(B_SF + i), 1); mbar_init(bar(B_PF + i), 4); mbar_init(bar(B_PV + i), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(bar(L::B_QF + i), 4);
+    for (int i = 0; i < 4; ++i) { mbar_init(bar(L::B_SF + i), 1); mbar_init(bar(L::B_PF + i), 4); mbar_init(bar(L::B_PV + i), 1); }
+    for (int i = 0; i < L::STAGES; ++i) {
+      mbar_init(bar(L::B_KF + i), 4); mbar_init(bar(L::B_KE + i), NQ);
+      mbar_init(bar(L::B_VF + i), 4); mbar_init(bar(L::B_VE + i), NQ);
     }
-    for (int i = 0; i < L::SLOTS; ++i) mbar_init(bar(B_SC + i), KT / 32);
-    mbar_init(bar(B_DRAIN), 1);
+    for (int i = 0; i < L::SLOTS; ++i) mbar_init(bar(L::B_SC + i), KT / 32);
+    mbar_init(bar(L::B_DRAIN), NQ);
     misc[1] = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -207,8 +221,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = misc[0];
-  auto tmem_s = [&](int g) { return tmem + (uint32_t)(g * KT); };
-  auto tmem_o = [&](int g) { return tmem + (uint32_t)(NQ * KT + g * WIDTH); };
+  auto tmem_s = [&](int g, int buf) { return tmem + (uint32_t)((2 * g + buf) * KT); };
+  auto tmem_o = [&](int g) { return tmem + (uint32_t)(2 * NQ * KT + g * WIDTH); };
   // halves of a row tile that hold rows
   auto halves_of = [&](const Cursor& c) { return NQ == 2 && c.s.q_len * a.group - c.rt * ROWS > 128 ? 2 : 1; };
 
@@ -217,146 +231,128 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::REGS_SOFTMAX));
     const int g = warp >> 2, r = tid & 127;
     const uint32_t lane_sel = (uint32_t)(warp & 3) << 21;                             // 32 lanes of TMEM per warp
-    const uint32_t s_addr = tmem_s(g) + lane_sel, o_addr = tmem_o(g) + lane_sel;
+    const uint32_t o_addr = tmem_o(g) + lane_sel;
+    float* row_at = reinterpret_cast<float*>(gbase + L::OFF_ROW) + 128 * g;
+    // Rows of 2 * WIDTH bytes in this half's Q tile: piece c of row r, where Q goes and outputs pass through.
+    uint8_t* q_tile = gbase + L::OFF_Q + g * L::Q_TILE;
+    auto staged = [&](int row, int c) { return reinterpret_cast<uint4*>(q_tile + (c >> 3) * L::Q_HALF + row * 128 + 16 * ((c & 7) ^ (row & 7))); };
+    // A warp moves whole rows of its 32: PIECES lanes a row, RPI rows at a time.
+    constexpr int PIECES = WIDTH / 8, RPI = 32 / PIECES;
+    const int c_l = lane % PIECES, row_l = 32 * (warp & 3) + lane / PIECES;
     bool ok = true;
     int left = n_tiles, n = 0, done = 0;             // tiles to go; tiles of the CTA, and of this half, that are behind
     while (ok && left > 0) {
       const int count = min(left, cur.n_kt - cur.kt), kt0 = cur.kt;
-      const int ng = halves_of(cur);
-      const int live = cur.s.q_len * a.group - cur.rt * ROWS - 128 * g;               // rows of this half that exist
-      const int rr = cur.rt * ROWS + 128 * g + r, tok = rr / a.group, head = cur.h * a.group + rr - tok * a.group;
+      const int first_row = cur.rt * ROWS + 128 * g, live = cur.s.q_len * a.group - first_row;   // rows of this half that exist
+      const int rr = first_row + r, tok = rr / a.group;
       const bool exists = r < live;
-      const T* q_row = reinterpret_cast<const T*>(a.q) + (long long)(cur.s.q0 + tok) * a.q_st + (long long)head * a.q_sh;
-      float row_c = a.scale_log2;
-      if (g < ng) {
-        auto q_piece = [&](int i) { return exists && 8 * i < a.D ? __ldg(reinterpret_cast<const uint4*>(q_row + 8 * i)) : make_uint4(0u, 0u, 0u, 0u); };
-        float up = 1.f;
-        if (!__is_same(T, __half)) {                 // bf16: the row's largest element to [2^14, 2^15)
-          float amax = 0.f;
+      // (offset of a row of q or out in elements)
+      auto row_of = [&](int row, long long st, long long sh) -> long long {
+        const int x = first_row + row, token = x / a.group;
+        return (long long)(cur.s.q0 + token) * st + (long long)(cur.h * a.group + x - token * a.group) * sh;
+      };
+      if (g < halves_of(cur)) {
 #pragma unroll 4
-          for (int i = 0; i < WIDTH / 8; ++i) {
-            float x[8];
-            unpack8<T>(q_piece(i), x);
+        for (int i = 0; i < 32 / RPI; ++i) {
+          const int row = row_l + i * RPI;
+          uint4 u = make_uint4(0u, 0u, 0u, 0u);
+          if (row < live && 8 * c_l < a.D) u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + row_of(row, a.q_st, a.q_sh) + 8 * c_l));
+          float back = 1.f;                          // what undoes the row's power of two
+          if (!__is_same(T, __half)) {               // bf16: the row's largest element to [2^14, 2^15)
+            float x[8], amax = 0.f;
+            unpack8<T>(u, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
-          }
-          const int field = (int)(__float_as_uint(amax) >> 23);
-          if (field > 14 && field < 255) {
-            const int f = min(254, 268 - field);
-            up = __uint_as_float((uint32_t)f << 23);
-            row_c *= f <= 253 ? __uint_as_float((uint32_t)(254 - f) << 23) : 5.877471754111438e-39f;
-          }
-        }
-        row_c = fmaxf(row_c, 1.17549435e-38f);       // (a masked score stays -infinity)
-        const uint32_t q_smem = base + L::OFF_Q + g * L::Q_TILE + r * 128;
-#pragma unroll 4
-        for (int i = 0; i < WIDTH / 8; ++i) {
-          const uint4 raw = q_piece(i);
-          uint32_t h[4] = {raw.x, raw.y, raw.z, raw.w};
-          if (!__is_same(T, __half)) {
-            float x[8];
-            unpack8<T>(raw, x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = pair16<__half>(x[2 * e] * up, x[2 * e + 1] * up);
+            for (int o = PIECES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            const int field = (int)(__float_as_uint(amax) >> 23);
+            float up = 1.f;
+            if (field > 14 && field < 255) {
+              const int f = min(254, 268 - field);
+              up = __uint_as_float((uint32_t)f << 23);
+              back = f <= 253 ? __uint_as_float((uint32_t)(254 - f) << 23) : 5.877471754111438e-39f;
+            }
+            u = make_uint4(pair16<__half>(x[0] * up, x[1] * up), pair16<__half>(x[2] * up, x[3] * up), pair16<__half>(x[4] * up, x[5] * up),
+                           pair16<__half>(x[6] * up, x[7] * up));
           }
-          const int piece = WIDTH == 128 ? i >> 1 : i;
-          sts16(q_smem + (WIDTH == 128 ? (i & 1) * L::Q_HALF : 0u) + 16 * (piece ^ (r & 7)), h[0], h[1], h[2], h[3]);
+          *staged(row, WIDTH == 128 ? (c_l & 1) * 8 + (c_l >> 1) : c_l) = u;
+          if (c_l == 0) row_at[row] = fmaxf(a.scale_log2 * back, 1.17549435e-38f);    // (a masked score stays -infinity)
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_QF + g));
-      }
-      const int ctx = cur.s.len - cur.s.q_len;
-      const int t_first = (cur.rt * ROWS + 128 * g) / a.group;
-      const int plain_end = a.tree ? max(ctx, 0) : max(0, min(cur.s.len, ctx + t_first + 1));   // keys below need no mask
-      const int lim = exists ? (a.tree ? cur.s.len : min(cur.s.len, ctx + tok + 1)) : 0;
-      const uint8_t* tree_row = a.tree ? a.tree + (long long)(cur.s.q0 + tok) * a.tree_st : nullptr;
-      // m: running maximum of e = score + log2(scale of V); l: sum of the weights of V over their scales
-      float m = NO_MAX, l = 0.f;
-      const float2 c2 = make_float2(row_c, row_c);
+        if (lane == 0) mbar_arrive(bar(L::B_QF + g));
+        const float row_c = row_at[r];
+        const int ctx = cur.s.len - cur.s.q_len;
+        const int plain_end = a.tree ? max(ctx, 0) : max(0, min(cur.s.len, ctx + first_row / a.group + 1));   // keys below need no mask
+        const int lim = exists ? (a.tree ? cur.s.len : min(cur.s.len, ctx + tok + 1)) : 0;
+        const uint8_t* tree_row = a.tree ? a.tree + (long long)(cur.s.q0 + tok) * a.tree_st : nullptr;
+        // m: running maximum of e; l: sum of the weights of V over their scales
+        float m = NO_MAX, l = 0.f;
+        const float2 c2 = make_float2(row_c, row_c);
 
-      if (g < ng) {
         for (int t = 0; t < count; ++t) {
-          const uint32_t sc = base + L::OFF_SC + ((n + t) % L::SLOTS) * L::SLOT;
-          ok = mbar_wait(bar(B_SF + g), (uint32_t)(done + t) & 1u, watch, CODE_SOFTMAX);
-          if (ok && t > 0) ok = mbar_wait(bar(B_PV + g), (uint32_t)(done + t - 1) & 1u, watch, CODE_SOFTMAX);   // (issued before the scores)
-          if (ok) ok = mbar_wait(bar(B_SC + (n + t) % L::SLOTS), (uint32_t)((n + t) / L::SLOTS) & 1u, watch, CODE_SOFTMAX);
+          const int k = done + t, buf = k & 1;       // tiles of this half so far
+          ok = mbar_wait(bar(L::B_SC + (n + t) % L::SLOTS), (uint32_t)((n + t) / L::SLOTS) & 1u, watch, CODE_SOFTMAX) &&
+               mbar_wait(bar(L::B_SF + 2 * g + buf), (uint32_t)(k >> 1) & 1u, watch, CODE_SOFTMAX);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
+          const uint32_t s_addr = tmem_s(g, buf) + lane_sel;
+          uint32_t x[64];
+          tmem_ld32(s_addr, x);
+          tmem_ld32(s_addr + 32, x + 32);
+          const uint8_t* slot_at = gbase + L::OFF_SC + ((n + t) % L::SLOTS) * L::SLOT;
+          const float4* sk4 = reinterpret_cast<const float4*>(slot_at);
+          const float4* lv4 = reinterpret_cast<const float4*>(slot_at + L::SLOT_LV);
+          const float4* rv4 = reinterpret_cast<const float4*>(slot_at + L::SLOT_RV);
+          const uint4* sums = reinterpret_cast<const uint4*>(slot_at + L::SLOT_SUM);
+          const uint4 sum0 = sums[0], sum1 = sums[1];
           const int key0 = (kt0 + t) * KT;
-          const float* vec = reinterpret_cast<const float*>(gbase + (sc - base));
-          const uint4* sums = reinterpret_cast<const uint4*>(gbase + (sc - base) + L::SLOT_SUM);
-          uint32_t any_odd = 0u;
-          float lv_top = -INFINITY, lv_low = INFINITY;
+          const bool masked = key0 + KT > plain_end || (sum0.x | sum0.y | sum1.x | sum1.y) != 0u;
+          const float lv_top = fmaxf(__uint_as_float(sum0.z), __uint_as_float(sum1.z)), lv_low = fminf(__uint_as_float(sum0.w), __uint_as_float(sum1.w));
+          uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+          if (masked) {                              // a bit per key that this row sees
 #pragma unroll
-          for (int ch = 0; ch < CHUNKS; ++ch) {
-            const uint4 u = sums[ch];
-            any_odd |= u.x | u.y;
-            lv_top = fmaxf(lv_top, __uint_as_float(u.z));
-            lv_low = fminf(lv_low, __uint_as_float(u.w));
+            for (int ch = 0; ch < 2; ++ch) {
+              const int k0 = key0 + 32 * ch, upto = lim - k0;
+              uint32_t b = upto >= 32 ? 0xffffffffu : upto <= 0 ? 0u : (1u << upto) - 1u;
+              b &= ~(ch ? sum1.x : sum0.x);
+              if (tree_row != nullptr && b != 0u && k0 + 32 > ctx) {
+#pragma unroll 4
+                for (int i = 0; i < 32; ++i)
+                  if (k0 + i >= ctx && (b >> i & 1u) && tree_row[k0 + i - ctx] == 0) b &= ~(1u << i);
+              }
+              bits[ch] = b;
+            }
+            __syncwarp();
           }
-          const bool masked = key0 + KT > plain_end || any_odd != 0u;
+          tmem_ld_wait();
           if (masked) {
             // What this row does not see becomes -infinity before anything is made of it, what it sees of a key that holds
             // a NaN becomes one (such keys' scales stand at 1, so that they reach no other row).
-#pragma unroll 1
-            for (int ch = 0; ch < CHUNKS; ++ch) {
-              const int k0 = key0 + 32 * ch, upto = lim - k0;
-              const uint2 not_there = make_uint2(sums[ch].x, sums[ch].y);
-              uint32_t bits = upto >= 32 ? 0xffffffffu : upto <= 0 ? 0u : (1u << upto) - 1u;
-              bits &= ~not_there.x;
-              if (tree_row != nullptr && bits != 0u && k0 + 32 > ctx) {
-#pragma unroll 8
-                for (int i = 0; i < 32; ++i)
-                  if (k0 + i >= ctx && (bits >> i & 1u) && tree_row[k0 + i - ctx] == 0) bits &= ~(1u << i);
-              }
-              __syncwarp();
-              uint32_t x[32];
-              tmem_ld32(s_addr + 32 * ch, x);
-              tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] = !(bits >> i & 1u) ? 0xff800000u : (not_there.y >> i & 1u) ? 0x7fffffffu : x[i];
-              tmem_st32(s_addr + 32 * ch, x);
+            for (int i = 0; i < 64; ++i) {
+              const uint32_t nan = i < 32 ? sum0.y : sum1.y;
+              x[i] = !(bits[i / 32] >> (i & 31) & 1u) ? 0xff800000u : (nan >> (i & 31) & 1u) ? 0x7fffffffu : x[i];
             }
-            tmem_st_wait();
           }
           // A bound of the row's largest e: the largest score, and the largest log2 of a scale of V; where those scales
           // differ by more than 2^8 within the tile, or some are not this row's to see, the largest e itself.
+          float2* x2 = reinterpret_cast<float2*>(x);
           float top = -INFINITY;
-          {
-            uint32_t x0[32], x1[32];
-            auto take = [&](const uint32_t* x, int ch) {
-              const float4* at = reinterpret_cast<const float4*>(vec + 32 * ch);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 sk = at[i];
-                const float2 u = __fmul2_rn(make_float2(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1])), make_float2(sk.x, sk.y));
-                const float2 v = __fmul2_rn(make_float2(__uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3])), make_float2(sk.z, sk.w));
-                top = max3(max3(top, u.x, u.y), v.x, v.y);
-              }
-            };
-            tmem_ld32(s_addr, x0);
-#pragma unroll 1
-            for (int ch = 0; ch < CHUNKS; ch += 2) {
-              tmem_ld_wait();
-              tmem_ld32(s_addr + 32 * ch + 32, x1);
-              take(x0, ch);
-              tmem_ld_wait();
-              if (ch + 2 < CHUNKS) tmem_ld32(s_addr + 32 * ch + 64, x0);
-              take(x1, ch + 1);
-            }
-            top = fmaf(top, row_c, lv_top);
-            if (masked || lv_top - lv_low > 8.f) {
-              top = -INFINITY;
-#pragma unroll 1
-              for (int ch = 0; ch < CHUNKS; ++ch) {
-                tmem_ld32(s_addr + 32 * ch, x0);
-                tmem_ld_wait();
+          for (int i = 0; i < 16; ++i) {
+            const float4 sk = sk4[i];
+            x2[2 * i] = __fmul2_rn(x2[2 * i], make_float2(sk.x, sk.y));
+            x2[2 * i + 1] = __fmul2_rn(x2[2 * i + 1], make_float2(sk.z, sk.w));
+            top = max3(max3(top, x2[2 * i].x, x2[2 * i].y), x2[2 * i + 1].x, x2[2 * i + 1].y);
+          }
+          top = fmaf(top, row_c, lv_top);
+          if (masked || lv_top - lv_low > 8.f) {
+            const float* lv = reinterpret_cast<const float*>(lv4);
+            top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) top = fmaxf(top, fmaf(__uint_as_float(x0[i]) * vec[32 * ch + i], row_c, vec[KT + 32 * ch + i]));
-              }
-            }
+            for (int i = 0; i < 64; ++i) top = fmaxf(top, fmaf(__uint_as_float(x[i]), row_c, lv[i]));
           }
           if (__any_sync(0xffffffffu, top > m + 14.f)) {
             // the maximum moves; the sum and the accumulator follow (weights stay below 2^14: fp16 keeps 11 bits from there to 2^-14)
@@ -365,100 +361,108 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
             m = top;
             l *= fade;
             if (t > 0) {                             // (the unit's first product overwrites the accumulator)
+              ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_PV + 2 * g + (buf ^ 1)), (uint32_t)((k - 1) >> 1) & 1u, watch, CODE_SOFTMAX));
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll 1
-              for (int ch = 0; ch < WIDTH / 32; ++ch) {
-                uint32_t o[32];
-                tmem_ld32(o_addr + 32 * ch, o);
+              for (int ch = 0; ch < WIDTH / 16; ++ch) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + 16 * ch, o);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fade);
-                tmem_st32(o_addr + 32 * ch, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fade);
+                tmem_st16(o_addr + 16 * ch, o);
               }
             }
           }
-          {
-            float2 l2 = make_float2(l, 0.f);
-            const float2 nm2 = make_float2(-m, -m);
-            uint32_t x0[32], x1[32];
-            auto weigh = [&](const uint32_t* x, int ch) {
-              const float4* at = reinterpret_cast<const float4*>(vec + 32 * ch);
-              uint32_t pw[16];
+          float2 l2 = make_float2(l, 0.f);
+          const float2 nm2 = make_float2(-m, -m);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 sk = at[i], lv = at[KT / 4 + i], rv = at[KT / 2 + i];
-                const float2 u = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1])), make_float2(sk.x, sk.y)), c2,
-                                            __fadd2_rn(make_float2(lv.x, lv.y), nm2));
-                const float2 v = __ffma2_rn(__fmul2_rn(make_float2(__uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3])), make_float2(sk.z, sk.w)), c2,
-                                            __fadd2_rn(make_float2(lv.z, lv.w), nm2));
-                const float2 w = make_float2(fast_ex2(u.x), fast_ex2(u.y)), z = make_float2(fast_ex2(v.x), fast_ex2(v.y));
-                l2 = __ffma2_rn(w, make_float2(rv.x, rv.y), l2);
-                l2 = __ffma2_rn(z, make_float2(rv.z, rv.w), l2);
-                pw[2 * i] = pair16<__half>(w.x, w.y);
-                pw[2 * i + 1] = pair16<__half>(z.x, z.y);
-              }
-              tmem_st16(s_addr + 16 * ch, pw);       // over scores that have been read
-            };
-            tmem_ld32(s_addr, x0);
-#pragma unroll 1
-            for (int ch = 0; ch < CHUNKS; ch += 2) {
-              tmem_ld_wait();
-              tmem_ld32(s_addr + 32 * ch + 32, x1);
-              weigh(x0, ch);
-              tmem_ld_wait();
-              if (ch + 2 < CHUNKS) tmem_ld32(s_addr + 32 * ch + 64, x0);
-              weigh(x1, ch + 1);
+          for (int ch = 0; ch < 2; ++ch) {
+            uint32_t pw[16];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int j = 8 * ch + i;
+              const float4 lv = lv4[j], rv = rv4[j];
+              const float2 u = __ffma2_rn(x2[2 * j], c2, __fadd2_rn(make_float2(lv.x, lv.y), nm2));
+              const float2 v = __ffma2_rn(x2[2 * j + 1], c2, __fadd2_rn(make_float2(lv.z, lv.w), nm2));
+              const float2 w = make_float2(fast_ex2(u.x), fast_ex2(u.y)), z = make_float2(fast_ex2(v.x), fast_ex2(v.y));
+              l2 = __ffma2_rn(w, make_float2(rv.x, rv.y), l2);
+              l2 = __ffma2_rn(z, make_float2(rv.z, rv.w), l2);
+              pw[2 * i] = pair16<__half>(w.x, w.y);
+              pw[2 * i + 1] = pair16<__half>(z.x, z.y);
             }
-            l = l2.x + l2.y;
+            tmem_st16(s_addr + 16 * ch, pw);         // over the scores, which are in registers
           }
+          l = l2.x + l2.y;
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(B_PF + g));
+          if (lane == 0) mbar_arrive(bar(L::B_PF + 2 * g + buf));
         }
         if (!ok) break;
         done += count;
-        // ---- the rows of this stretch of the unit
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(B_PV + g), (uint32_t)(done - 1) & 1u, watch, CODE_SOFTMAX));
+        // ---- the rows of this stretch of the unit, through shared memory to whole rows
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_PV + 2 * g + ((done - 1) & 1)), (uint32_t)((done - 1) >> 1) & 1u, watch, CODE_SOFTMAX));
         if (!ok) break;
         tc_fence_after();
         const bool whole = kt0 == 0 && count == cur.n_kt;
-        const long long slot = 2LL * blockIdx.x + (n > 0 ? 1 : 0);                    // a stretch's first unit, or its last
-        const float inv = !whole ? 1.f : l == 0.f ? 0.f : __fdividef(1.f, l);
-        T* out = reinterpret_cast<T*>(a.out) + (long long)(cur.s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
-        float* part = a.part_o + (slot * a.part_rows + 128 * g + r) * WIDTH;
+        const long long part_row = (2LL * blockIdx.x + (n > 0 ? 1 : 0)) * a.part_rows + 128 * g;      // a stretch's first unit, or its last
+        if (whole) {
+          const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
 #pragma unroll 1
-        for (int ch = 0; ch < WIDTH / 32; ++ch) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + 32 * ch, o);
-          tmem_ld_wait();
-          if (exists) {
+          for (int ch = 0; ch < WIDTH / 16; ++ch) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + 16 * ch, o);
+            tmem_ld_wait();
+            uint32_t h[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int at = 4 * ch + i, col = WIDTH == 128 ? 16 * (at & 7) + 8 * (at >> 3) : 8 * at;
-              float x[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(o[8 * i + e]) * inv;
-              if (whole) {
-                if (col < a.D)
-                  *reinterpret_cast<uint4*>(out + col) = make_uint4(pair16<T>(x[0], x[1]), pair16<T>(x[2], x[3]), pair16<T>(x[4], x[5]), pair16<T>(x[6], x[7]));
-              } else {
-                *reinterpret_cast<float4*>(part + col) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4*>(part + col + 4) = make_float4(x[4], x[5], x[6], x[7]);
-              }
-            }
+            for (int i = 0; i < 8; ++i) h[i] = pair16<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            *staged(r, 2 * ch) = make_uint4(h[0], h[1], h[2], h[3]);
+            *staged(r, 2 * ch + 1) = make_uint4(h[4], h[5], h[6], h[7]);
           }
+          __syncwarp();
+          const int col = WIDTH == 128 ? 16 * (c_l & 7) + 8 * (c_l >> 3) : 8 * c_l;
+#pragma unroll 4
+          for (int i = 0; i < 32 / RPI; ++i) {
+            const int row = row_l + i * RPI;
+            if (row < live && col < a.D)
+              *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + row_of(row, a.o_st, a.o_sh) + col) = *staged(row, c_l);
+          }
+        } else {
+          // (the columns stay in the order of the accumulator: cache_combine_kernel puts them right)
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+#pragma unroll 1
+            for (int ch = 0; ch < WIDTH / 32; ++ch) {
+              uint32_t o[16];
+              tmem_ld16(o_addr + half * (WIDTH / 2) + 16 * ch, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) *staged(r, 4 * ch + i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+            __syncwarp();
+#pragma unroll 4
+            for (int i = 0; i < 32 / RPI; ++i) {
+              const int row = row_l + i * RPI;
+              if (row < live) *reinterpret_cast<uint4*>(a.part_o + (part_row + row) * WIDTH + half * (WIDTH / 2) + 4 * c_l) = *staged(row, c_l);
+            }
+            __syncwarp();
+          }
+          if (exists) a.part_ml[part_row + r] = make_float2(m, l);
         }
         tc_fence_before();
-        if (exists && !whole) a.part_ml[slot * a.part_rows + 128 * g + r] = make_float2(m, l);
         if (exists && whole && a.lse != nullptr) {
           float v = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2_F;
           if (a.shift != nullptr) {                  // the keys as they were before the shift was taken off
+            const T* q_row = reinterpret_cast<const T*>(a.q) + row_of(r, a.q_st, a.q_sh);
             float d = 0.f;
             for (int i = 0; i < a.D; ++i) d = fmaf((float)q_row[i], __ldg(a.shift + (long long)cur.h * WIDTH + i), d);
             v += d * a.sm_scale;
           }
-          a.lse[(long long)(cur.s.q0 + tok) * a.Hq + head] = v;
+          a.lse[(long long)(cur.s.q0 + tok) * a.Hq + cur.h * a.group + rr - tok * a.group] = v;
         }
+        __syncwarp();                                // (the rows that passed through are read before the next Q is written)
       }
       n += count;
       left -= count;
@@ -466,6 +470,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     }
   } else if (tid < L::SOFTMAX + L::LOADERS) {
     // ------------------------------------------------- loaders -------------------------------------------------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_LOADER));
     const int ct = tid - L::SOFTMAX;
     constexpr int PIECES = WIDTH / 16, RPI = 128 / PIECES, N_CHUNK = KT / RPI;        // rows of 128 threads; chunks per thread
     const int piece = ct % PIECES, row_l = ct / PIECES;
@@ -535,7 +540,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       const uint32_t free_parity = ((uint32_t)(n / L::STAGES) & 1u) ^ 1u;
       const bool more = n + 1 < n_tiles;
       // K, the scales, and the flags of keys that do not exist
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(B_KE + st), free_parity, watch, CODE_LOAD));
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_KE + st), free_parity, watch, CODE_LOAD));
       if (!ok) break;
       if (ct < KT) {
         const uint32_t sc = base + L::OFF_SC + (n % L::SLOTS) * L::SLOT;
@@ -549,18 +554,18 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         const float big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))), small = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(v)));
         if (lane == 0) sts16(sc + L::SLOT_SUM + 16 * (ct >> 5), none32, nan32, __float_as_uint(__log2f(big)), __float_as_uint(__log2f(small)));
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_SC + n % L::SLOTS));
+        if (lane == 0) mbar_arrive(bar(L::B_SC + n % L::SLOTS));
       }
       convert(base + L::OFF_K + st * L::KV_TILE, kr, INT8);
-      if (lane == 0) mbar_arrive(bar(B_KF + st));
+      if (lane == 0) mbar_arrive(bar(L::B_KF + st));
       if (more) {                                    // `ahead` is tile n + 1
         fetch(a.kc, kr);
         fetch_scales();
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(B_VE + st), free_parity, watch, CODE_LOAD));
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_VE + st), free_parity, watch, CODE_LOAD));
       if (!ok) break;
       convert(base + L::OFF_V + st * L::KV_TILE, vr, false);
-      if (lane == 0) mbar_arrive(bar(B_VF + st));
+      if (lane == 0) mbar_arrive(bar(L::B_VF + st));
       if (more) {
         fetch(a.vc, vr);
         advance(n + 1);
@@ -568,53 +573,59 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_ISSUER));
-    if (warp == ISSUER && lane == 0) {
+    const int g = warp - ISSUER;
+    if (g < NQ && lane == 0) {
       // ------------------------------------------------- products ------------------------------------------------------
       bool ok = true;
-      int left = n_tiles, n = 0, done0 = 0, done1 = 0, seg0 = 0, seg1 = 0;
-      auto issue_qk = [&](int g, int st) {
+      int left = n_tiles, n = 0, k = 0, segments = 0;                                 // k: tiles of this half so far
+      // scores of tile n into buffer `to`
+      auto issue_qk = [&](int to) -> bool {
+        const int st = n % L::STAGES;
+        if (!mbar_wait(bar(L::B_KF + st), (uint32_t)(n / L::STAGES) & 1u, watch, CODE_MMA)) return false;
         tc_fence_after();
-  #pragma unroll
-        for (int k = 0; k < WIDTH / 16; ++k)
-          mma_ss(tmem_s(g), desc_k(base + L::OFF_Q + g * L::Q_TILE + (k >> 2) * L::Q_HALF + 32 * (k & 3)),
-                 desc_k(base + L::OFF_K + st * L::KV_TILE + (k >> 2) * L::KV_HALF + 32 * (k & 3)), IDESC_QK, k > 0);
-        tc_commit(bar(B_SF + g));
+#pragma unroll
+        for (int i = 0; i < WIDTH / 16; ++i)
+          mma_ss(tmem_s(g, to), desc_k(base + L::OFF_Q + g * L::Q_TILE + (i >> 2) * L::Q_HALF + 32 * (i & 3)),
+                 desc_k(base + L::OFF_K + st * L::KV_TILE + (i >> 2) * L::KV_HALF + 32 * (i & 3)), IDESC_QK, i > 0);
+        tc_commit(bar(L::B_SF + 2 * g + to));
+        tc_commit(bar(L::B_KE + st));
+        ++n;
+        return true;
       };
       while (ok && left > 0) {
-        const int count = min(left, cur.n_kt - cur.kt), ng = halves_of(cur);
-        ok = mbar_wait(bar(B_QF), (uint32_t)seg0++ & 1u, watch, CODE_MMA);
-        if (ok && ng == 2) ok = mbar_wait(bar(B_QF + 1), (uint32_t)seg1++ & 1u, watch, CODE_MMA);
-        if (ok) ok = mbar_wait(bar(B_KF + n % L::STAGES), (uint32_t)(n / L::STAGES) & 1u, watch, CODE_MMA);
-        if (!ok) break;
-        for (int g = 0; g < ng; ++g) issue_qk(g, n % L::STAGES);
-        tc_commit(bar(B_KE + n % L::STAGES));
-        for (int t = 0; ok && t < count; ++t, ++n) {
-          const int st = n % L::STAGES;
-          const uint32_t par = (uint32_t)(n / L::STAGES) & 1u;
-          for (int g = 0; ok && g < ng; ++g) {
-            ok = mbar_wait(bar(B_PF + g), (uint32_t)(g ? done1 : done0) & 1u, watch, CODE_MMA);
-            if (ok && g == 0) ok = mbar_wait(bar(B_VF + st), par, watch, CODE_MMA);
+        const int count = min(left, cur.n_kt - cur.kt), n0 = n;
+        if (g < halves_of(cur)) {
+          ok = mbar_wait(bar(L::B_QF + g), (uint32_t)segments & 1u, watch, CODE_MMA);
+          ++segments;
+          ok = ok && issue_qk(k & 1);
+          for (int t = 0; ok && t < count; ++t, ++k) {
+            // (the buffer of the tile before: its P V is ahead of these products in this thread's order)
+            if (t + 1 < count && !issue_qk((k + 1) & 1)) { ok = false; break; }
+            const int st = (n0 + t) % L::STAGES;
+            ok = mbar_wait(bar(L::B_VF + st), (uint32_t)((n0 + t) / L::STAGES) & 1u, watch, CODE_MMA) &&
+                 mbar_wait(bar(L::B_PF + 2 * g + (k & 1)), (uint32_t)(k >> 1) & 1u, watch, CODE_MMA);
             if (!ok) break;
-            if (g) ++done1; else ++done0;
             tc_fence_after();
-  #pragma unroll
-            for (int k = 0; k < KT / 16; ++k)
-              mma_ts(tmem_o(g), tmem_s(g) + 8 * k, desc_mn(base + L::OFF_V + st * L::KV_TILE + 2048 * k, L::KV_HALF), IDESC_PV, t > 0 || k > 0);
-            tc_commit(bar(B_PV + g));
-            if (g == ng - 1) tc_commit(bar(B_VE + st));
-            if (t + 1 < count) {
-              if (g == 0) ok = mbar_wait(bar(B_KF + (n + 1) % L::STAGES), (uint32_t)((n + 1) / L::STAGES) & 1u, watch, CODE_MMA);
-              if (!ok) break;
-              issue_qk(g, (n + 1) % L::STAGES);
-              if (g == ng - 1) tc_commit(bar(B_KE + (n + 1) % L::STAGES));
-            }
+#pragma unroll
+            for (int i = 0; i < KT / 16; ++i)
+              mma_ts(tmem_o(g), tmem_s(g, k & 1) + 8 * i, desc_mn(base + L::OFF_V + st * L::KV_TILE + 2048 * i, L::KV_HALF), IDESC_PV, t > 0 || i > 0);
+            tc_commit(bar(L::B_PV + 2 * g + (k & 1)));
+            tc_commit(bar(L::B_VE + st));
+          }
+        } else {                                     // no rows here: the stages are free as far as this half goes
+          for (int t = 0; ok && t < count; ++t, ++n) {
+            const int st = n % L::STAGES;
+            ok = mbar_wait(bar(L::B_KF + st), (uint32_t)(n / L::STAGES) & 1u, watch, CODE_MMA);
+            if (ok) mbar_arrive(bar(L::B_KE + st));
+            ok = ok && mbar_wait(bar(L::B_VF + st), (uint32_t)(n / L::STAGES) & 1u, watch, CODE_MMA);
+            if (ok) mbar_arrive(bar(L::B_VE + st));
           }
         }
         left -= count;
         if (left > 0) { cur.kt = cur.n_kt - 1; next_step(a, cur, ROWS, KT); }
       }
-      tc_commit(bar(B_DRAIN));                         // every product issued is complete before the TMEM is freed
-      mbar_wait(bar(B_DRAIN), 0, watch, CODE_MMA);
+      tc_commit(bar(L::B_DRAIN));                    // every product issued is complete before the TMEM is freed
+      mbar_wait(bar(L::B_DRAIN), 0, watch, CODE_MMA);
     }
   }
   tc_fence_before();
@@ -625,10 +636,10 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
   }
 }
 
-template <typename T, bool INT8, int WIDTH, int NQ, int KT>
+template <typename T, bool INT8, int WIDTH, int NQ>
 cudaError_t launch_tree(CacheAttnKArgs& a, int sms, int32_t* status_host, cudaStream_t st) {
-  using L = TreeShape<WIDTH, NQ, KT>;
-  auto kern = cache_tree_kernel<T, INT8, WIDTH, NQ, KT>;
+  using L = TreeShape<WIDTH, NQ>;
+  auto kern = cache_tree_kernel<T, INT8, WIDTH, NQ>;
   static DeviceOnce once;
   cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::BYTES); });
   if (e != cudaSuccess) return e;
@@ -641,8 +652,8 @@ cudaError_t launch_tree(CacheAttnKArgs& a, int sms, int32_t* status_host, cudaSt
 
 template <typename T, bool INT8, int WIDTH>
 cudaError_t launch_tree_rows(CacheAttnKArgs& a, int sms, int32_t* status_host, cudaStream_t st) {
-  return cache_form((int64_t)a.max_q * a.group).rows == 128 ? launch_tree<T, INT8, WIDTH, 1, 64>(a, sms, status_host, st)
-                                                            : launch_tree<T, INT8, WIDTH, 2, 128>(a, sms, status_host, st);
+  return cache_form((int64_t)a.max_q * a.group).rows == 128 ? launch_tree<T, INT8, WIDTH, 1>(a, sms, status_host, st)
+                                                            : launch_tree<T, INT8, WIDTH, 2>(a, sms, status_host, st);
 }
 template <typename T>
 cudaError_t launch_tree_type(CacheAttnKArgs& a, const CacheView& c, int sms, int32_t* status_host, cudaStream_t st) {
