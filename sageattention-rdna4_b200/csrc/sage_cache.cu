@@ -22,6 +22,30 @@ constexpr int CACHE_THREADS = 256;
 __device__ __forceinline__ uint4 ld_stream(const void* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }
 __device__ __forceinline__ void st_stream(void* p, const uint4& v) { __stcs(reinterpret_cast<uint4*>(p), v); }
 
+// 32 bytes in one access where WIDE says that the address is a multiple of 32, in two of 16 otherwise (every sector of
+// 32 bytes is then written twice in halves: 27 280 x 48 heads read back 258 us, 196 in one).
+template <bool WIDE> __device__ __forceinline__ void ld_stream32(const void* p, uint4& a, uint4& b, bool lo, bool hi) {
+  a = b = make_uint4(0u, 0u, 0u, 0u);
+  if (WIDE) {
+    if (lo)
+      asm volatile("ld.global.cs.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p));
+  } else {
+    if (lo) a = ld_stream(p);
+    if (hi) b = ld_stream(reinterpret_cast<const uint8_t*>(p) + 16);
+  }
+}
+template <bool WIDE> __device__ __forceinline__ void st_stream32(void* p, const uint4& a, const uint4& b, bool lo, bool hi) {
+  if (WIDE) {
+    if (lo)
+      asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                   ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+  } else {
+    if (lo) st_stream(p, a);
+    if (hi) st_stream(reinterpret_cast<uint8_t*>(p) + 16, b);
+  }
+}
+
 template <typename T> __device__ __forceinline__ uint32_t to_pair(float a, float b);
 template <> __device__ __forceinline__ uint32_t to_pair<__half>(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -82,51 +106,64 @@ __global__ void __launch_bounds__(CACHE_THREADS) rotary_kernel(const RotaryKArgs
   const int item = (int)threadIdx.x % items, r0 = (int)threadIdx.x / items;
   if (r0 >= per) return;
   const int rows = a.Hq + a.Hk;
-#pragma unroll 4
-  for (int r = r0; r < rows; r += per) {
-    const bool is_q = r < a.Hq;
-    const int h = is_q ? r : r - a.Hq;
-    const T* src = reinterpret_cast<const T*>(is_q ? a.q : a.k) +
-                   (is_q ? b * a.q_s[0] + h * a.q_s[1] + n * a.q_s[2] : b * a.k_s[0] + h * a.k_s[1] + n * a.k_s[2]);
-    T* dst = reinterpret_cast<T*>(is_q ? a.q_out : a.k_out) +
-             (is_q ? b * a.qo_s[0] + h * a.qo_s[1] + n * a.qo_s[2] : b * a.ko_s[0] + h * a.ko_s[1] + n * a.ko_s[2]);
-    if (item >= turning) {
-      const int at = a.rot + 8 * (item - turning);
-      if (is_q ? a.copy_q : a.copy_k) st_stream(dst + at, ld_stream(src + at));
-    } else if (INTERLEAVED) {
-      float x[8];
-      unpack8<T>(ld_stream(src + 8 * item), x);
-      uint32_t w[4];
+  const long long q_in = b * a.q_s[0] + n * a.q_s[2], q_to = b * a.qo_s[0] + n * a.qo_s[2];
+  const long long k_in = b * a.k_s[0] + n * a.k_s[2], k_to = b * a.ko_s[0] + n * a.ko_s[2];
+  // four rows at a time, all of their loads before the first store
+  constexpr int BATCH = 4;
+  const int at = item >= turning ? a.rot + 8 * (item - turning) : VEC * item;
+  for (int r1 = r0; r1 < rows; r1 += BATCH * per) {
+    uint4 u[BATCH], w[BATCH];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 t = cs[4 * item + e];
-        w[e] = to_pair<T>(x[2 * e] * t.x - x[2 * e + 1] * t.y, x[2 * e + 1] * t.x + x[2 * e] * t.y);
-      }
-      st_stream(dst + 8 * item, make_uint4(w[0], w[1], w[2], w[3]));
-    } else {
-      float x[8], y[8];
-      uint32_t u[4], w[4];
-      if (VEC == 8) {
-        unpack8<T>(ld_stream(src + 8 * item), x);
-        unpack8<T>(ld_stream(src + half + 8 * item), y);
+    for (int i = 0; i < BATCH; ++i) {
+      const int r = r1 + i * per;
+      const bool is_q = r < a.Hq;
+      if (r >= rows || (item >= turning && !(is_q ? a.copy_q : a.copy_k))) continue;
+      const T* src = is_q ? reinterpret_cast<const T*>(a.q) + q_in + r * a.q_s[1] : reinterpret_cast<const T*>(a.k) + k_in + (r - a.Hq) * a.k_s[1];
+      if (INTERLEAVED || VEC == 8 || item >= turning) {
+        u[i] = ld_stream(src + at);
+        if (!INTERLEAVED && item < turning) w[i] = ld_stream(src + half + at);
       } else {
-        const uint2 lo = __ldcs(reinterpret_cast<const uint2*>(src + 4 * item));
-        const uint2 hi = __ldcs(reinterpret_cast<const uint2*>(src + half + 4 * item));
-        unpack8<T>(make_uint4(lo.x, lo.y, 0u, 0u), x);
-        unpack8<T>(make_uint4(hi.x, hi.y, 0u, 0u), y);
+        const uint2 lo = __ldcs(reinterpret_cast<const uint2*>(src + at)), hi = __ldcs(reinterpret_cast<const uint2*>(src + half + at));
+        u[i] = make_uint4(lo.x, lo.y, 0u, 0u);
+        w[i] = make_uint4(hi.x, hi.y, 0u, 0u);
       }
+    }
 #pragma unroll
-      for (int e = 0; e < VEC / 2; ++e) {
-        const float2 t0 = cs[VEC * item + 2 * e], t1 = cs[VEC * item + 2 * e + 1];
-        u[e] = to_pair<T>(x[2 * e] * t0.x - y[2 * e] * t0.y, x[2 * e + 1] * t1.x - y[2 * e + 1] * t1.y);
-        w[e] = to_pair<T>(y[2 * e] * t0.x + x[2 * e] * t0.y, y[2 * e + 1] * t1.x + x[2 * e + 1] * t1.y);
-      }
-      if (VEC == 8) {
-        st_stream(dst + 8 * item, make_uint4(u[0], u[1], u[2], u[3]));
-        st_stream(dst + half + 8 * item, make_uint4(w[0], w[1], w[2], w[3]));
+    for (int i = 0; i < BATCH; ++i) {
+      const int r = r1 + i * per;
+      const bool is_q = r < a.Hq;
+      if (r >= rows || (item >= turning && !(is_q ? a.copy_q : a.copy_k))) continue;
+      T* dst = is_q ? reinterpret_cast<T*>(a.q_out) + q_to + r * a.qo_s[1] : reinterpret_cast<T*>(a.k_out) + k_to + (r - a.Hq) * a.ko_s[1];
+      if (item >= turning) {
+        st_stream(dst + at, u[i]);
+      } else if (INTERLEAVED) {
+        float x[8];
+        unpack8<T>(u[i], x);
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 t = cs[4 * item + e];
+          o[e] = to_pair<T>(x[2 * e] * t.x - x[2 * e + 1] * t.y, x[2 * e + 1] * t.x + x[2 * e] * t.y);
+        }
+        st_stream(dst + at, make_uint4(o[0], o[1], o[2], o[3]));
       } else {
-        __stcs(reinterpret_cast<uint2*>(dst + 4 * item), make_uint2(u[0], u[1]));
-        __stcs(reinterpret_cast<uint2*>(dst + half + 4 * item), make_uint2(w[0], w[1]));
+        float x[8], y[8];
+        uint32_t o[4], p[4];
+        unpack8<T>(u[i], x);
+        unpack8<T>(w[i], y);
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) {
+          const float2 t0 = cs[VEC * item + 2 * e], t1 = cs[VEC * item + 2 * e + 1];
+          o[e] = to_pair<T>(x[2 * e] * t0.x - y[2 * e] * t0.y, x[2 * e + 1] * t1.x - y[2 * e + 1] * t1.y);
+          p[e] = to_pair<T>(y[2 * e] * t0.x + x[2 * e] * t0.y, y[2 * e + 1] * t1.x + x[2 * e + 1] * t1.y);
+        }
+        if (VEC == 8) {
+          st_stream(dst + at, make_uint4(o[0], o[1], o[2], o[3]));
+          st_stream(dst + half + at, make_uint4(p[0], p[1], p[2], p[3]));
+        } else {
+          __stcs(reinterpret_cast<uint2*>(dst + at), make_uint2(o[0], o[1]));
+          __stcs(reinterpret_cast<uint2*>(dst + half + at), make_uint2(p[0], p[1]));
+        }
       }
     }
   }
@@ -187,7 +224,7 @@ __device__ __forceinline__ float quant_row16(const uint4& u0, const uint4& u1, c
   return s;
 }
 
-template <typename T, bool INT8, int WIDTH>
+template <typename T, bool INT8, int WIDTH, bool WIDE>
 __global__ void __launch_bounds__(CACHE_THREADS) cache_write_kernel(const WriteKArgs a) {
   constexpr int LANES = WIDTH / 16, ROWS = CACHE_THREADS / LANES;
   const int c = (int)threadIdx.x % LANES, col = 16 * c;
@@ -196,14 +233,13 @@ __global__ void __launch_bounds__(CACHE_THREADS) cache_write_kernel(const WriteK
   const long long token = live ? row / a.H : 0;
   const int h = live ? (int)(row - token * a.H) : 0;
   const long long slot = !live ? -1 : a.slots64 ? reinterpret_cast<const long long*>(a.slots)[token] : (long long)reinterpret_cast<const int*>(a.slots)[token];
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   const bool store = live && slot >= 0 && slot < a.total_slots;
   const T* k = reinterpret_cast<const T*>(a.k) + token * a.k_st + h * a.k_sh + col;
   const T* v = reinterpret_cast<const T*>(a.v) + token * a.v_st + h * a.v_sh + col;
   const bool lo = live && col < a.D, hi = live && col + 8 < a.D;
-  const uint4 k0 = lo ? ld_stream(k) : zero, v0 = lo ? ld_stream(v) : zero;
-  const uint4 k1 = hi ? ld_stream(k + 8) : zero, v1 = hi ? ld_stream(v + 8) : zero;
-  uint4 kw, vw;
+  uint4 k0, k1, v0, v1, kw, vw;
+  ld_stream32<WIDE>(k, k0, k1, lo, hi);
+  ld_stream32<WIDE>(v, v0, v1, lo, hi);
   // (the shift is padded to the row's width with zeros)
   const float ks = quant_row16<T, INT8, true>(k0, k1, a.shift ? a.shift + (long long)h * WIDTH : nullptr, col, LANES, &kw);
   const float vs = quant_row16<T, INT8, false>(v0, v1, nullptr, col, LANES, &vw);
@@ -247,15 +283,16 @@ __device__ __forceinline__ void decode16(const uint4& u, float* x) {
   }
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 __device__ __forceinline__ void store16(T* dst, const float* x, bool lo, bool hi) {
-  if (lo) st_stream(dst, make_uint4(to_pair<T>(x[0], x[1]), to_pair<T>(x[2], x[3]), to_pair<T>(x[4], x[5]), to_pair<T>(x[6], x[7])));
-  if (hi) st_stream(dst + 8, make_uint4(to_pair<T>(x[8], x[9]), to_pair<T>(x[10], x[11]), to_pair<T>(x[12], x[13]), to_pair<T>(x[14], x[15])));
+  st_stream32<WIDE>(dst, make_uint4(to_pair<T>(x[0], x[1]), to_pair<T>(x[2], x[3]), to_pair<T>(x[4], x[5]), to_pair<T>(x[6], x[7])),
+                    make_uint4(to_pair<T>(x[8], x[9]), to_pair<T>(x[10], x[11]), to_pair<T>(x[12], x[13]), to_pair<T>(x[14], x[15])), lo, hi);
 }
 
-template <typename T, bool INT8, int WIDTH>
-__global__ void __launch_bounds__(CACHE_THREADS) cache_read_kernel(const ReadKArgs a) {
+template <typename T, bool INT8, int WIDTH, bool WIDE>
+__global__ void __launch_bounds__(CACHE_THREADS, 3) cache_read_kernel(const ReadKArgs a) {
   constexpr int LANES = WIDTH / 16, ROWS = CACHE_THREADS / LANES;
+  constexpr int BATCH = 4;                           // heads whose codes are in flight together
   __shared__ long long where[ROWS];                  // first row of the token's page in head 0, plus its offset; -1: none
   const long long row0 = (long long)blockIdx.x * ROWS;
   if (threadIdx.x < ROWS) {
@@ -283,35 +320,51 @@ __global__ void __launch_bounds__(CACHE_THREADS) cache_read_kernel(const ReadKAr
   const bool lo = col < a.D, hi = col + 8 < a.D;
   T* k_out = reinterpret_cast<T*>(a.k_out) + row * a.k_st + col;
   T* v_out = reinterpret_cast<T*>(a.v_out) + row * a.v_st + col;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 2
-  for (int h = blockIdx.y; h < a.H; h += gridDim.y) {
-    uint4 kw = zero, vw = zero;
-    float ks = 0.f, vs = 0.f;
-    if (at0 >= 0) {
-      const long long at = at0 + ((long long)h << a.page_shift);
-      kw = ld_stream(a.kc + at * WIDTH + col);
-      vw = ld_stream(a.vc + at * WIDTH + col);
-      ks = __ldg(a.ks + at);
-      vs = __ldg(a.vs + at);
-    }
-    float x[16];
-    decode16<INT8>(kw, x);
+  const int step = (int)gridDim.y;
+  for (int h0 = blockIdx.y; h0 < a.H; h0 += BATCH * step) {
+    uint4 kw[BATCH], vw[BATCH];
+    float ks[BATCH], vs[BATCH];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], ks);
-    if (a.shift != nullptr && at0 >= 0) {
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const float4 m = __ldg(reinterpret_cast<const float4*>(a.shift + (long long)h * WIDTH + col + e));
-        x[e] = __fadd_rn(x[e], m.x); x[e + 1] = __fadd_rn(x[e + 1], m.y); x[e + 2] = __fadd_rn(x[e + 2], m.z); x[e + 3] = __fadd_rn(x[e + 3], m.w);
+    for (int i = 0; i < BATCH; ++i) {
+      const int h = h0 + i * step;
+      kw[i] = vw[i] = make_uint4(0u, 0u, 0u, 0u);
+      ks[i] = vs[i] = 0.f;
+      if (h < a.H && at0 >= 0) {
+        const long long at = at0 + ((long long)h << a.page_shift);
+        kw[i] = ld_stream(a.kc + at * WIDTH + col);
+        vw[i] = ld_stream(a.vc + at * WIDTH + col);
+        ks[i] = __ldg(a.ks + at);
+        vs[i] = __ldg(a.vs + at);
       }
     }
-    store16<T>(k_out + h * a.k_sh, x, lo, hi);
-    decode16<false>(vw, x);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], vs);
-    store16<T>(v_out + h * a.v_sh, x, lo, hi);
+    for (int i = 0; i < BATCH; ++i) {
+      const int h = h0 + i * step;
+      if (h < a.H) {
+        float x[16];
+        decode16<INT8>(kw[i], x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], ks[i]);
+        if (a.shift != nullptr && at0 >= 0) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const float4 m = __ldg(reinterpret_cast<const float4*>(a.shift + (long long)h * WIDTH + col + e));
+            x[e] = __fadd_rn(x[e], m.x); x[e + 1] = __fadd_rn(x[e + 1], m.y); x[e + 2] = __fadd_rn(x[e + 2], m.z); x[e + 3] = __fadd_rn(x[e + 3], m.w);
+          }
+        }
+        store16<T, WIDE>(k_out + h * a.k_sh, x, lo, hi);
+        decode16<false>(vw[i], x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], vs[i]);
+        store16<T, WIDE>(v_out + h * a.v_sh, x, lo, hi);
+      }
+    }
   }
+}
+
+// Whether every run of 16 columns of the rows lies on a multiple of 32 bytes, and none is cut off.
+bool in_32s(const void* p, long long s0, long long s1, int d) {
+  return (reinterpret_cast<uintptr_t>(p) & 31u) == 0 && s0 % 16 == 0 && s1 % 16 == 0 && d % 16 == 0;
 }
 
 template <typename T>
@@ -332,8 +385,10 @@ cudaError_t launch_rotary_t(const RotaryKArgs& a, bool interleaved, long long bl
 template <typename T, bool INT8>
 cudaError_t launch_write_t(const WriteKArgs& a, int width, cudaStream_t st) {
   const long long per = CACHE_THREADS / (width / 16), blocks = (a.tokens * a.H + per - 1) / per;
-  if (width == 64) cache_write_kernel<T, INT8, 64><<<(unsigned)blocks, CACHE_THREADS, 0, st>>>(a);
-  else cache_write_kernel<T, INT8, 128><<<(unsigned)blocks, CACHE_THREADS, 0, st>>>(a);
+  const dim3 grid((unsigned)blocks);
+  const bool wide = in_32s(a.k, a.k_st, a.k_sh, a.D) && in_32s(a.v, a.v_st, a.v_sh, a.D);
+  if (width == 64) (wide ? cache_write_kernel<T, INT8, 64, true> : cache_write_kernel<T, INT8, 64, false>)<<<grid, CACHE_THREADS, 0, st>>>(a);
+  else (wide ? cache_write_kernel<T, INT8, 128, true> : cache_write_kernel<T, INT8, 128, false>)<<<grid, CACHE_THREADS, 0, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -343,8 +398,9 @@ cudaError_t launch_read_t(const ReadKArgs& a, int width, cudaStream_t st) {
   // heads shared out until there are a few CTAs per SM
   const long long want = 8LL * sm_count();
   const dim3 grid((unsigned)blocks, (unsigned)std::max(1LL, std::min((long long)a.H, want / blocks)));
-  if (width == 64) cache_read_kernel<T, INT8, 64><<<grid, CACHE_THREADS, 0, st>>>(a);
-  else cache_read_kernel<T, INT8, 128><<<grid, CACHE_THREADS, 0, st>>>(a);
+  const bool wide = in_32s(a.k_out, a.k_st, a.k_sh, a.D) && in_32s(a.v_out, a.v_st, a.v_sh, a.D);
+  if (width == 64) (wide ? cache_read_kernel<T, INT8, 64, true> : cache_read_kernel<T, INT8, 64, false>)<<<grid, CACHE_THREADS, 0, st>>>(a);
+  else (wide ? cache_read_kernel<T, INT8, 128, true> : cache_read_kernel<T, INT8, 128, false>)<<<grid, CACHE_THREADS, 0, st>>>(a);
   return cudaGetLastError();
 }
 

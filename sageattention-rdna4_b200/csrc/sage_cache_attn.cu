@@ -113,9 +113,8 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   unsigned before;
   const Line line = find_place(a, ROWS, CA_KEYS, place_s, warp, cur.b, before);
   if (cur.b >= a.n_seq) return;
-  const unsigned first = line.begin(stretch);
-  const int n_steps = (int)(line.begin(stretch + 1) - first);
-  enter_line(a, cur, first, before, ROWS, CA_KEYS);
+  enter_line(a, cur, line.begin(stretch), line.begin(stretch + 1), before, ROWS, CA_KEYS);
+  if (cur.left <= 0) return;
   Cursor ahead = cur;                                // the step whose loads are issued next
   const uint32_t ring = smem_addr(smem) + warp * STAGES * L::STAGE;
 
@@ -175,16 +174,17 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   };
   fetch_pages();
   fetch_q();
-  int issued = 0;
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
-    if (issued < n_steps) {
+  // the step at `ahead` into stage s, and on to the next one
+  auto issue_next = [&](int s) {
+    if (ahead.left > 0) {
       issue(s);
-      ++issued;
-      if (issued < n_steps) { next_step(a, ahead, ROWS, CA_KEYS); fetch_pages(); }
+      next_step(a, ahead, ROWS, CA_KEYS);
+      if (ahead.left > 0) fetch_pages();
     }
     copy_commit();
-  }
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) issue_next(s);
 
   uint32_t qf[NB][KSTEPS][2];                        // Q^T: k-step s of query row 8 nb + g
   float row_c[NB][2];                                // score factor of rows 8 nb + 2c + {0, 1}
@@ -195,15 +195,10 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
 
   int stage = 0;
   bool fresh = true;
-  for (int t = 0; t < n_steps; ++t) {
+  for (;;) {
     // the stage that was read last is free: fetch into it
     __syncwarp();
-    if (issued < n_steps) {
-      issue(stage == 0 ? STAGES - 1 : stage - 1);
-      ++issued;
-      if (issued < n_steps) { next_step(a, ahead, ROWS, CA_KEYS); fetch_pages(); }
-    }
-    copy_commit();
+    issue_next(stage == 0 ? STAGES - 1 : stage - 1);
     if (fresh) {
       fresh = false;
       const int live = min(ROWS, cur.s.q_len * a.group - cur.rt * ROWS);      // rows of this tile that exist
@@ -420,10 +415,10 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
 
     // ---- end of the unit, or of the stretch
     const bool last_of_unit = cur.kt + 1 == cur.n_kt;
-    if (last_of_unit || t + 1 == n_steps) {
-      const bool whole = last_of_unit && t >= cur.kt;                  // all of the unit's steps were here
-      // a unit that began before this stretch: its part is the stretch's first, else its last
-      const long long slot = 2LL * stretch + (t > cur.kt ? 1 : 0);
+    if (last_of_unit || cur.left == 1) {
+      const bool whole = last_of_unit && cur.into >= 0;                // all of the unit's steps were here
+      // a unit that began before this stretch, or with it: its part is the stretch's first, else its last
+      const long long slot = 2LL * stretch + (cur.into > 0 ? 1 : 0);
       const int live = min(ROWS, cur.s.q_len * a.group - cur.rt * ROWS);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
@@ -461,14 +456,14 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
         }
         __syncwarp();
       }
-      if (t + 1 < n_steps) {
-        fresh = true;
-        next_step(a, cur, ROWS, CA_KEYS);
-        fetch_q();
-        continue;
-      }
+      next_step(a, cur, ROWS, CA_KEYS);
+      if (cur.left <= 0) return;
+      fresh = true;
+      fetch_q();
+      continue;
     }
     ++cur.kt;
+    --cur.left;
   }
 }
 
@@ -487,10 +482,10 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
   const int rt = (int)(blockIdx.x - bh * max_rt), b = (int)(bh / (unsigned)a.Hkv), h = (int)(bh - (unsigned)b * a.Hkv);
   const Seq s = seq_of(a, b);                        // (the lengths are older than the attention kernel)
   const int r = blockIdx.y * (CC_WARPS / WARPS_PER_ROW) + warp / WARPS_PER_ROW, rr = rt * rows + r;
-  // steps before this sequence, and in all
+  // places before this sequence, and in all
   unsigned before = 0, total = 0;
   for (int i = tid; i < a.n_seq; i += CC_THREADS) {
-    const unsigned n = steps_of_seq(a, i, rows, keys);
+    const unsigned n = places_of_seq(a, i, rows, keys);
     total += n;
     if (i < b) before += n;
   }
@@ -503,7 +498,7 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
   for (int w = 0; w < CC_WARPS; ++w) { total += total_s[w]; before += before_s[w]; }
   const Line line(total, a.max_stretches);
   const int n_kt = key_steps(s, keys);
-  const unsigned u0 = before + ((unsigned)h * row_tiles(a, s, rows) + rt) * n_kt;
+  const unsigned u0 = before + ((unsigned)h * row_tiles(a, s, rows) + rt) * (n_kt + UNIT_STEPS);
   const int c0 = total > 0 ? (int)line.of(u0) : 0, c1 = total > 0 ? (int)line.of(u0 + n_kt - 1) : 0;
   wait_for_predecessor();
   // no such row, or written by the one that had all of its unit  (the whole CTA leaves, or whole warps of rows)
@@ -588,7 +583,7 @@ cudaError_t launch_attn(CacheAttnKArgs& a, int sms, cudaStream_t st) {
   cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
   if (e != cudaSuccess) return e;
   a.max_stretches = std::min(sms, SIZING_SMS) * CTAS_PER_SM * CA_WARPS;
-  const long long steps = (long long)a.n_seq * a.Hkv * std::max<long long>(1, (((long long)a.table_width << a.page_shift) + CA_KEYS - 1) / CA_KEYS);
+  const long long steps = (long long)a.n_seq * a.Hkv * (UNIT_STEPS + std::max<long long>(1, (((long long)a.table_width << a.page_shift) + CA_KEYS - 1) / CA_KEYS));
   kern<<<(unsigned)std::min<long long>(a.max_stretches / CA_WARPS, (steps + CA_WARPS - 1) / CA_WARPS), CA_THREADS, smem, st>>>(a);
   return cudaGetLastError();
 }

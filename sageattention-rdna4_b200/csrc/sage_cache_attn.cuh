@@ -51,42 +51,45 @@ __device__ __forceinline__ int row_tiles(const CacheAttnKArgs& a, const Seq& s, 
 __device__ __forceinline__ int key_steps(const Seq& s, int keys) { return max(1, (s.len + keys - 1) / keys); }   // an empty sequence's rows are written too
 
 // The line of steps (of so many keys each): sequence by sequence, K/V head by K/V head, row tile by row tile (of so many
-// rows each), step by step; fewer than 2^31 of them, the host sees to that.  Its stretches differ by one step at most;
-// a line of fewer steps than stretches wanted leaves the last ones out.
+// rows each), step by step, and behind every unit UNIT_STEPS more places that stand for what a unit costs beyond its keys
+// (fetching Q, writing the rows): without them a stretch through many short sequences takes several times as long as one
+// through a long one.  Fewer than 2^31 places, the host sees to that.  Its stretches differ by one place at most; a line
+// of fewer places than stretches wanted leaves the last ones out.
+constexpr int UNIT_STEPS = 4;
 struct Line {
-  unsigned total, n, per, longer;                    // steps, stretches, steps of a stretch, stretches that have one more
-  __device__ __forceinline__ Line(unsigned steps, int most) : total(steps) {
-    n = min((unsigned)most, steps);
-    per = n ? steps / n : 0u;
-    longer = steps - n * per;
+  unsigned total, n, per, longer;                    // places, stretches, places of a stretch, stretches that have one more
+  __device__ __forceinline__ Line(unsigned places, int most) : total(places) {
+    n = min((unsigned)most, places);
+    per = n ? places / n : 0u;
+    longer = places - n * per;
   }
   __device__ __forceinline__ unsigned begin(unsigned x) const { return x * per + min(x, longer); }
-  // the stretch that has step u
+  // the stretch that has place u
   __device__ __forceinline__ unsigned of(unsigned u) const {
     const unsigned in_longer = longer * (per + 1);
     return u < in_longer ? u / (per + 1) : longer + (u - in_longer) / per;
   }
 };
-__device__ __forceinline__ unsigned steps_of_seq(const CacheAttnKArgs& a, int b, int rows, int keys) {
+__device__ __forceinline__ unsigned places_of_seq(const CacheAttnKArgs& a, int b, int rows, int keys) {
   if (b >= a.n_seq) return 0;
   const Seq s = seq_of(a, b);
-  return (unsigned)a.Hkv * row_tiles(a, s, rows) * key_steps(s, keys);
+  return (unsigned)a.Hkv * row_tiles(a, s, rows) * (key_steps(s, keys) + UNIT_STEPS);
 }
 
 // All threads of a CTA call this: the line, the sequence in which the CTA's stretch `which` (of OWN) begins (n_seq: it
-// has none), and the number of steps before that sequence.
+// has none), and the number of places before that sequence.
 template <int THREADS, int OWN> struct PlaceScratch {
   unsigned sum[THREADS / 32], found[OWN], before[OWN];
 };
 template <int THREADS, int OWN>
 __device__ __forceinline__ Line find_place(const CacheAttnKArgs& a, int rows, int keys, PlaceScratch<THREADS, OWN>& sh, int which, int& seq,
-                                           unsigned& steps_before) {
+                                           unsigned& places_before) {
   constexpr int WARPS = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   unsigned total = 0;
   if (a.n_seq > THREADS) {                           // the length of the line first
     unsigned mine = 0;
-    for (int b = tid; b < a.n_seq; b += THREADS) mine += steps_of_seq(a, b, rows, keys);
+    for (int b = tid; b < a.n_seq; b += THREADS) mine += places_of_seq(a, b, rows, keys);
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) sh.sum[warp] = mine;
     __syncthreads();
@@ -98,7 +101,7 @@ __device__ __forceinline__ Line find_place(const CacheAttnKArgs& a, int rows, in
   Line line(total, a.max_stretches);
   unsigned base = 0;
   for (int b0 = 0; b0 < a.n_seq; b0 += THREADS) {
-    const unsigned n = steps_of_seq(a, b0 + tid, rows, keys);
+    const unsigned n = places_of_seq(a, b0 + tid, rows, keys);
     unsigned upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -122,40 +125,57 @@ __device__ __forceinline__ Line find_place(const CacheAttnKArgs& a, int rows, in
     __syncthreads();
   }
   seq = (int)sh.found[which];
-  steps_before = sh.before[which];
+  places_before = sh.before[which];
   return line;
 }
 
-// A position on the line.
+// A position on the line, within a stretch.
 struct Cursor {
   Seq s;
   int b, h, rt, kt;          // sequence, K/V head, row tile, step
   int n_rt, n_kt;
+  int left;                  // places of the stretch from this one on; the walk is over when none is
+  int into;                  // places of the stretch before the unit's first (below 0: the unit began before the stretch)
 };
 __device__ __forceinline__ void enter_seq(const CacheAttnKArgs& a, Cursor& c, int rows, int keys) {
   c.s = seq_of(a, c.b);
   c.n_rt = row_tiles(a, c.s, rows);
   c.n_kt = key_steps(c.s, keys);
 }
-__device__ __forceinline__ void next_step(const CacheAttnKArgs& a, Cursor& c, int rows, int keys) {
-  if (++c.kt < c.n_kt) return;
+// From any place of a unit (`at` of them into it) to the first of the next one.
+__device__ __forceinline__ void next_unit(const CacheAttnKArgs& a, Cursor& c, int at, int rows, int keys) {
+  const int rest = c.n_kt + UNIT_STEPS - at;
+  c.left -= rest;
+  c.into += c.n_kt + UNIT_STEPS;
   c.kt = 0;
-  if (++c.rt < c.n_rt) return;
+  if (c.left <= 0 || ++c.rt < c.n_rt) return;
   c.rt = 0;
   if (++c.h < a.Hkv) return;
   c.h = 0;
   do {
-    if (++c.b >= a.n_seq) return;
+    if (++c.b >= a.n_seq) { c.left = 0; return; }
     enter_seq(a, c, rows, keys);
   } while (c.n_rt == 0);
 }
-// The cursor of step `first` of the line, in the sequence that find_place gave.
-__device__ __forceinline__ void enter_line(const CacheAttnKArgs& a, Cursor& c, unsigned first, unsigned before, int rows, int keys) {
+__device__ __forceinline__ void next_step(const CacheAttnKArgs& a, Cursor& c, int rows, int keys) {
+  if (c.kt + 1 < c.n_kt) {
+    ++c.kt;
+    --c.left;
+  } else {
+    next_unit(a, c, c.kt, rows, keys);
+  }
+}
+// The first step of the stretch from place `first` on, in the sequence that find_place gave.
+__device__ __forceinline__ void enter_line(const CacheAttnKArgs& a, Cursor& c, unsigned first, unsigned end, unsigned before, int rows, int keys) {
   enter_seq(a, c, rows, keys);
-  const unsigned rest = first - before, unit = rest / (unsigned)c.n_kt;
-  c.kt = (int)(rest - unit * c.n_kt);
+  const unsigned rest = first - before, per = (unsigned)(c.n_kt + UNIT_STEPS), unit = rest / per;
+  const int at = (int)(rest - unit * per);
   c.h = (int)(unit / (unsigned)c.n_rt);
   c.rt = (int)unit - c.h * c.n_rt;
+  c.kt = at;
+  c.left = (int)(end - first);
+  c.into = -at;
+  if (at >= c.n_kt) next_unit(a, c, at, rows, keys);
 }
 
 __device__ __forceinline__ float fast_ex2(float x) {

@@ -191,9 +191,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
   unsigned before;
   const Line line = find_place<L::THREADS, 1>(a, ROWS, KT, place_s, 0, cur.b, before);
   if (cur.b >= a.n_seq) return;                      // (the whole CTA)
-  const unsigned first = line.begin(blockIdx.x);
-  const int n_tiles = (int)(line.begin(blockIdx.x + 1) - first);
-  enter_line(a, cur, first, before, ROWS, KT);
+  enter_line(a, cur, line.begin(blockIdx.x), line.begin(blockIdx.x + 1), before, ROWS, KT);
+  if (cur.left <= 0) return;
 
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = base + L::OFF_BAR;
   uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
@@ -240,9 +239,9 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     constexpr int PIECES = WIDTH / 8, RPI = 32 / PIECES;
     const int c_l = lane % PIECES, row_l = 32 * (warp & 3) + lane / PIECES;
     bool ok = true;
-    int left = n_tiles, n = 0, done = 0;             // tiles to go; tiles of the CTA, and of this half, that are behind
-    while (ok && left > 0) {
-      const int count = min(left, cur.n_kt - cur.kt), kt0 = cur.kt;
+    int n = 0, done = 0;                             // tiles of the CTA, and of this half, that are behind
+    while (ok && cur.left > 0) {
+      const int count = min(cur.left, cur.n_kt - cur.kt), kt0 = cur.kt;
       const int first_row = cur.rt * ROWS + 128 * g, live = cur.s.q_len * a.group - first_row;   // rows of this half that exist
       const int rr = first_row + r, tok = rr / a.group;
       const bool exists = r < live;
@@ -407,7 +406,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         if (!ok) break;
         tc_fence_after();
         const bool whole = kt0 == 0 && count == cur.n_kt;
-        const long long part_row = (2LL * blockIdx.x + (n > 0 ? 1 : 0)) * a.part_rows + 128 * g;      // a stretch's first unit, or its last
+        // a unit that began before this stretch, or with it: its part is the stretch's first, else its last
+        const long long part_row = (2LL * blockIdx.x + (cur.into > 0 ? 1 : 0)) * a.part_rows + 128 * g;
         if (whole) {
           const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
 #pragma unroll 1
@@ -465,8 +465,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         __syncwarp();                                // (the rows that passed through are read before the next Q is written)
       }
       n += count;
-      left -= count;
-      if (left > 0) { cur.kt = cur.n_kt - 1; next_step(a, cur, ROWS, KT); }
+      next_unit(a, cur, cur.kt, ROWS, KT);
     }
   } else if (tid < L::SOFTMAX + L::LOADERS) {
     // ------------------------------------------------- loaders -------------------------------------------------------
@@ -523,22 +522,21 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       __syncwarp();
     };
     // on to the next tile, whose pages are asked for at once
-    auto advance = [&](int tile) {
-      if (tile + 1 < n_tiles) {
-        next_step(a, ahead, ROWS, KT);
-        fetch_pages();
-      }
+    auto advance = [&]() {
+      next_step(a, ahead, ROWS, KT);
+      if (ahead.left > 0) fetch_pages();
     };
     fetch_pages();
     fetch(a.kc, kr);
     fetch_scales();
     fetch(a.vc, vr);
-    advance(0);
+    advance();
     bool ok = true;
-    for (int n = 0; ok && n < n_tiles; ++n) {
+    bool more = true;
+    for (int n = 0; more; ++n) {
       const int st = n % L::STAGES;
       const uint32_t free_parity = ((uint32_t)(n / L::STAGES) & 1u) ^ 1u;
-      const bool more = n + 1 < n_tiles;
+      more = ahead.left > 0;
       // K, the scales, and the flags of keys that do not exist
       ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_KE + st), free_parity, watch, CODE_LOAD));
       if (!ok) break;
@@ -568,7 +566,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       if (lane == 0) mbar_arrive(bar(L::B_VF + st));
       if (more) {
         fetch(a.vc, vr);
-        advance(n + 1);
+        advance();
       }
     }
   } else {
@@ -577,7 +575,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     if (g < NQ && lane == 0) {
       // ------------------------------------------------- products ------------------------------------------------------
       bool ok = true;
-      int left = n_tiles, n = 0, k = 0, segments = 0;                                 // k: tiles of this half so far
+      int n = 0, k = 0, segments = 0;                                 // k: tiles of this half so far
       // scores of tile n into buffer `to`
       auto issue_qk = [&](int to) -> bool {
         const int st = n % L::STAGES;
@@ -592,8 +590,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         ++n;
         return true;
       };
-      while (ok && left > 0) {
-        const int count = min(left, cur.n_kt - cur.kt), n0 = n;
+      while (ok && cur.left > 0) {
+        const int count = min(cur.left, cur.n_kt - cur.kt), n0 = n;
         if (g < halves_of(cur)) {
           ok = mbar_wait(bar(L::B_QF + g), (uint32_t)segments & 1u, watch, CODE_MMA);
           ++segments;
@@ -621,8 +619,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
             if (ok) mbar_arrive(bar(L::B_VE + st));
           }
         }
-        left -= count;
-        if (left > 0) { cur.kt = cur.n_kt - 1; next_step(a, cur, ROWS, KT); }
+        next_unit(a, cur, cur.kt, ROWS, KT);
       }
       tc_commit(bar(L::B_DRAIN));                    // every product issued is complete before the TMEM is freed
       mbar_wait(bar(L::B_DRAIN), 0, watch, CODE_MMA);
@@ -644,7 +641,7 @@ cudaError_t launch_tree(CacheAttnKArgs& a, int sms, int32_t* status_host, cudaSt
   cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::BYTES); });
   if (e != cudaSuccess) return e;
   const long long rows = (long long)a.max_q * a.group, rts = (rows + L::ROWS - 1) / L::ROWS;
-  const long long steps = (long long)a.n_seq * a.Hkv * rts * std::max<long long>(1, (((long long)a.table_width << a.page_shift) + KT - 1) / KT);
+  const long long steps = (long long)a.n_seq * a.Hkv * rts * (UNIT_STEPS + std::max<long long>(1, (((long long)a.table_width << a.page_shift) + KT - 1) / KT));
   a.max_stretches = std::min(std::min(sms, 160) * L::CTAS_PER_SM, cache_form(rows).max_stretches);
   kern<<<(unsigned)std::min<long long>(a.max_stretches, steps), L::THREADS, L::BYTES, st>>>(a, status_host);
   return cudaGetLastError();

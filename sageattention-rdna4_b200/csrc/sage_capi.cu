@@ -640,7 +640,7 @@ int sage_cache_attention(const void* q, void* out, float* lse,
   if (!(sm_scale > 0.f) || !(sm_scale <= 3.0e38f))
     return fail(SAGE_E_ARG, "%s: sm_scale must be finite and positive (got %g)", who, (double)sm_scale);
   // what the kernels count in 31 bits: runs of 32 keys of all sequences, K/V heads and groups of eight rows
-  const int64_t row_groups = (max_q * (Hq / Hkv) + 7) / 8, runs = (page_table_width * page_size + 31) / 32;
+  const int64_t row_groups = (max_q * (Hq / Hkv) + 7) / 8, runs = (page_table_width * page_size + 31) / 32 + 4;
   if (max_q * (Hq / Hkv) > ((int64_t)1 << 28) || n_seq * Hkv > ((int64_t)1 << 30) / row_groups || n_seq * Hkv * row_groups > (((int64_t)1 << 31) - 1) / runs)
     return fail(SAGE_E_UNSUPPORTED, "%s: too many rows and keys in one call", who);
   if (!workspace) return fail(SAGE_E_ARG, "%s: workspace is null", who);

@@ -16,6 +16,13 @@ import cache_reference as R
 import sageattention as S
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _seed():
+    torch.manual_seed(0)
+
+
 DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
 
 
@@ -297,4 +304,6 @@ def test_page_of_a_cache_beyond_32_bits():
     _close(out, lse, want, want_lse, cache, [1000], table)
     cu = torch.tensor([0, 1000], dtype=torch.int32, device="cuda")
     k16, _ = S.sage_cache_read(cache, table, cu, 1000)
-    assert (k16.float() - k.float()).abs().max() <= k.float().abs().max() / 127 * 0.51
+    # half a code's step of the row's largest / 127, then half a step of fp16 on the value that is read back
+    top = k.float().abs().max()
+    assert (k16.float() - k.float()).abs().max() <= top / 127 * 0.5 * (1 + 2.0 ** -20) + top * 2.0 ** -11

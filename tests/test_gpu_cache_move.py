@@ -9,6 +9,13 @@ import sageattention as S
 from sageattention import b200_backend as be
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _seed():
+    torch.manual_seed(0)
+
+
 DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
 
 
