@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(CACHE_THREADS) rotary_kernel(const RotaryKArgs
   const int rows = a.Hq + a.Hk;
   const long long q_in = b * a.q_s[0] + n * a.q_s[2], q_to = b * a.qo_s[0] + n * a.qo_s[2];
   const long long k_in = b * a.k_s[0] + n * a.k_s[2], k_to = b * a.ko_s[0] + n * a.ko_s[2];
-  // four rows at a time, all of their loads before the first store
-  constexpr int BATCH = 4;
+  // four 16-byte loads at a time before the first store
+  constexpr int BATCH = INTERLEAVED ? 4 : 2;
   const int at = item >= turning ? a.rot + 8 * (item - turning) : VEC * item;
   for (int r1 = r0; r1 < rows; r1 += BATCH * per) {
     uint4 u[BATCH], w[BATCH];
@@ -175,6 +175,18 @@ __global__ void __launch_bounds__(CACHE_THREADS) rotary_kernel(const RotaryKArgs
 // quantiser's (codes and scales are the bits that sage_prologue gives for the same rows): scale =
 // max(amax / 127 or 448, 1e-12), code = rne(x / scale).  A row that holds a NaN or an infinity gets the scale
 // NaN and codes of 0, so that no code is ever a NaN: a key that a mask hides cannot reach a product.
+// Largest magnitude of sixteen packed values, NaN if one is.
+template <typename T>
+__device__ __forceinline__ float absmax16_nan(const uint4& u, const uint4& v) {
+  typedef typename Packed16<T>::Pair Pair;
+  const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+  Pair m = __habs2(*reinterpret_cast<const Pair*>(&w[0]));
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const Pair*>(&w[i])));
+  const float2 f = Elem<T>::cvt2(*reinterpret_cast<const uint32_t*>(&m));
+  return max_nan(f.x, f.y);
+}
+
 struct WriteKArgs {
   const void *k, *v, *slots;
   uint8_t *kc, *vc;
@@ -199,8 +211,12 @@ __device__ __forceinline__ float quant_row16(const uint4& u0, const uint4& u1, c
     }
   }
   float amax = 0.f;
+  if (IS_K && shift != nullptr) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) amax = max_nan(amax, fabsf(x[e]));
+    for (int e = 0; e < 16; ++e) amax = max_nan(amax, fabsf(x[e]));
+  } else {
+    amax = absmax16_nan<T>(u0, u1);
+  }
   for (int o = lanes / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (!(amax <= 3.402823466e38f)) {                  // a NaN or an infinity somewhere in the row
     *codes = make_uint4(0u, 0u, 0u, 0u);
@@ -228,10 +244,11 @@ template <typename T, bool INT8, int WIDTH, bool WIDE>
 __global__ void __launch_bounds__(CACHE_THREADS) cache_write_kernel(const WriteKArgs a) {
   constexpr int LANES = WIDTH / 16, ROWS = CACHE_THREADS / LANES;
   const int c = (int)threadIdx.x % LANES, col = 16 * c;
-  const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / LANES;
-  const bool live = row < a.tokens * a.H;
-  const long long token = live ? row / a.H : 0;
-  const int h = live ? (int)(row - token * a.H) : 0;
+  const unsigned row = blockIdx.x * ROWS + threadIdx.x / LANES;     // (fewer than 2^31 rows: the host sees to that)
+  const bool live = row < (unsigned)a.tokens * a.H;
+  const unsigned token32 = live ? row / (unsigned)a.H : 0u;
+  const long long token = token32;
+  const int h = live ? (int)(row - token32 * a.H) : 0;
   const long long slot = !live ? -1 : a.slots64 ? reinterpret_cast<const long long*>(a.slots)[token] : (long long)reinterpret_cast<const int*>(a.slots)[token];
   const bool store = live && slot >= 0 && slot < a.total_slots;
   const T* k = reinterpret_cast<const T*>(a.k) + token * a.k_st + h * a.k_sh + col;
@@ -264,29 +281,32 @@ struct ReadKArgs {
   int n_seq, table_width, pages, H, D, page_shift;
 };
 
-// 16 codes -> 16 values
+// 16 codes -> 16 values, in pairs
 template <bool INT8>
-__device__ __forceinline__ void decode16(const uint4& u, float* x) {
+__device__ __forceinline__ void decode16(const uint4& u, float2* x) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (INT8) {
       const uint32_t t = w[i] ^ 0x80808080u;         // code + 128, then 2^23 + it as a float
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * i + e] = __uint_as_float(__byte_perm(t, 0x4B000000u, 0x7440 + e)) - 8388736.0f;
+      const float2 bias = make_float2(-8388736.0f, -8388736.0f);
+      x[2 * i] = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(t, 0x4B000000u, 0x7440)), __uint_as_float(__byte_perm(t, 0x4B000000u, 0x7441))), bias);
+      x[2 * i + 1] = __fadd2_rn(make_float2(__uint_as_float(__byte_perm(t, 0x4B000000u, 0x7442)), __uint_as_float(__byte_perm(t, 0x4B000000u, 0x7443))), bias);
     } else {
       const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] & 0xFFFFu), __NV_E4M3);
       const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] >> 16), __NV_E4M3);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&lo)), g = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-      x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = g.x; x[4 * i + 3] = g.y;
+      x[2 * i] = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+      x[2 * i + 1] = __half22float2(*reinterpret_cast<const __half2*>(&hi));
     }
   }
 }
 
 template <typename T, bool WIDE>
-__device__ __forceinline__ void store16(T* dst, const float* x, bool lo, bool hi) {
-  st_stream32<WIDE>(dst, make_uint4(to_pair<T>(x[0], x[1]), to_pair<T>(x[2], x[3]), to_pair<T>(x[4], x[5]), to_pair<T>(x[6], x[7])),
-                    make_uint4(to_pair<T>(x[8], x[9]), to_pair<T>(x[10], x[11]), to_pair<T>(x[12], x[13]), to_pair<T>(x[14], x[15])), lo, hi);
+__device__ __forceinline__ void store16(T* dst, const float2* x, bool lo, bool hi) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = to_pair<T>(x[i].x, x[i].y);
+  st_stream32<WIDE>(dst, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]), lo, hi);
 }
 
 template <typename T, bool INT8, int WIDTH, bool WIDE>
@@ -341,21 +361,24 @@ __global__ void __launch_bounds__(CACHE_THREADS, 3) cache_read_kernel(const Read
     for (int i = 0; i < BATCH; ++i) {
       const int h = h0 + i * step;
       if (h < a.H) {
-        float x[16];
+        float2 x[8];
+        const float2 k2 = make_float2(ks[i], ks[i]), v2 = make_float2(vs[i], vs[i]);
         decode16<INT8>(kw[i], x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], ks[i]);
+        for (int e = 0; e < 8; ++e) x[e] = __fmul2_rn(x[e], k2);
         if (a.shift != nullptr && at0 >= 0) {
+          const float4* m4 = reinterpret_cast<const float4*>(a.shift + h * WIDTH + col);
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const float4 m = __ldg(reinterpret_cast<const float4*>(a.shift + (long long)h * WIDTH + col + e));
-            x[e] = __fadd_rn(x[e], m.x); x[e + 1] = __fadd_rn(x[e + 1], m.y); x[e + 2] = __fadd_rn(x[e + 2], m.z); x[e + 3] = __fadd_rn(x[e + 3], m.w);
+          for (int e = 0; e < 4; ++e) {
+            const float4 m = __ldg(m4 + e);
+            x[2 * e] = __fadd2_rn(x[2 * e], make_float2(m.x, m.y));
+            x[2 * e + 1] = __fadd2_rn(x[2 * e + 1], make_float2(m.z, m.w));
           }
         }
         store16<T, WIDE>(k_out + h * a.k_sh, x, lo, hi);
         decode16<false>(vw[i], x);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = __fmul_rn(x[e], vs[i]);
+        for (int e = 0; e < 8; ++e) x[e] = __fmul2_rn(x[e], v2);
         store16<T, WIDE>(v_out + h * a.v_sh, x, lo, hi);
       }
     }

@@ -569,7 +569,7 @@ int sage_cache_write(const void* k, const void* v, const void* slots, int slots_
   if ((rc = check_strides2(who, "k", k_strides)) || (rc = check_strides2(who, "v", v_strides))) return rc;
   if (!aligned16(k) || !aligned16(v)) return fail(SAGE_E_ARG, "%s: pointers must be 16-byte aligned", who);
   if (reinterpret_cast<uintptr_t>(slots) & (slots_64 ? 7u : 3u)) return fail(SAGE_E_ARG, "%s: slots are misaligned", who);
-  if (tokens * Hkv > ((int64_t)1 << 35)) return fail(SAGE_E_UNSUPPORTED, "%s: too many rows in one call", who);
+  if (tokens * Hkv >= ((int64_t)1 << 31)) return fail(SAGE_E_UNSUPPORTED, "%s: too many rows in one call", who);
   sage::CacheWriteParams p;
   p.k = k; p.v = v; p.slots = slots; p.slots64 = slots_64 != 0; p.tokens = tokens; p.dtype = dtype;
   for (int i = 0; i < 2; ++i) { p.k_strides[i] = k_strides[i]; p.v_strides[i] = v_strides[i]; }
