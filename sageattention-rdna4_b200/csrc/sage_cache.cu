@@ -244,11 +244,13 @@ template <typename T, bool INT8, int WIDTH, bool WIDE>
 __global__ void __launch_bounds__(CACHE_THREADS) cache_write_kernel(const WriteKArgs a) {
   constexpr int LANES = WIDTH / 16, ROWS = CACHE_THREADS / LANES;
   const int c = (int)threadIdx.x % LANES, col = 16 * c;
-  const unsigned row = blockIdx.x * ROWS + threadIdx.x / LANES;     // (fewer than 2^31 rows: the host sees to that)
-  const bool live = row < (unsigned)a.tokens * a.H;
-  const unsigned token32 = live ? row / (unsigned)a.H : 0u;
-  const long long token = token32;
-  const int h = live ? (int)(row - token32 * a.H) : 0;
+  // ROWS neighbouring tokens of one head: their codes and scales lie next to each other in a page (token by token and
+  // head by head every scale would be a write of 4 bytes to a sector of its own)
+  const unsigned block = blockIdx.x / (unsigned)a.H;
+  const int h = (int)(blockIdx.x - block * a.H);
+  long long token = (long long)block * ROWS + threadIdx.x / LANES;
+  const bool live = token < a.tokens;
+  token = live ? token : 0;
   const long long slot = !live ? -1 : a.slots64 ? reinterpret_cast<const long long*>(a.slots)[token] : (long long)reinterpret_cast<const int*>(a.slots)[token];
   const bool store = live && slot >= 0 && slot < a.total_slots;
   const T* k = reinterpret_cast<const T*>(a.k) + token * a.k_st + h * a.k_sh + col;
@@ -407,7 +409,7 @@ cudaError_t launch_rotary_t(const RotaryKArgs& a, bool interleaved, long long bl
 
 template <typename T, bool INT8>
 cudaError_t launch_write_t(const WriteKArgs& a, int width, cudaStream_t st) {
-  const long long per = CACHE_THREADS / (width / 16), blocks = (a.tokens * a.H + per - 1) / per;
+  const long long per = CACHE_THREADS / (width / 16), blocks = (a.tokens + per - 1) / per * a.H;
   const dim3 grid((unsigned)blocks);
   const bool wide = in_32s(a.k, a.k_st, a.k_sh, a.D) && in_32s(a.v, a.v_st, a.v_sh, a.D);
   if (width == 64) (wide ? cache_write_kernel<T, INT8, 64, true> : cache_write_kernel<T, INT8, 64, false>)<<<grid, CACHE_THREADS, 0, st>>>(a);
