@@ -6,8 +6,9 @@
 //   warps 0 .. 4 NQ - 1   softmax: a thread owns a row (32x32b TMEM loads: a lane is a row), so that maxima and sums
 //                         need no other lane; its weights go back to TMEM as fp16, over the scores they came from, and
 //                         are the A operand of P V from there
-//   the next four warps   fetch the one-byte codes (a tile ahead, in registers), turn them into fp16 -- exact -- and
-//                         write them to shared memory as the operands want them (128-byte swizzle)
+//   the next four warps   fetch the one-byte codes (cp.async, some tiles ahead; every thread reads back only what it
+//                         fetched), turn them into fp16 -- exact -- and write them to shared memory as the operands
+//                         want them (128-byte swizzle)
 //   NQ more warps         a thread each that issues the products of 128 rows (idle warps complete the warpgroup, whose
 //                         registers the softmax takes over)
 // Scores have two buffers in TMEM: those of the next tile are under way while the softmax works on a tile, and P V
@@ -31,7 +32,6 @@ namespace sage {
 
 namespace {
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -154,12 +154,14 @@ template <int WIDTH, int NQ> struct TreeShape {
   static_assert(NQ * REGS_SOFTMAX + REGS_LOADER + REGS_ISSUER <= (NQ + 2) * REGS_LAUNCH, "setmaxnreg would wait forever");
   // Stages of K and V; slots of scales.  A slot is written once the scores STAGES tiles back are complete, which means that
   // the softmax is done with the tile two before that.
-  static constexpr int STAGES = NQ == 1 ? 2 : 4, SLOTS = NQ == 1 ? 4 : 8;
+  static constexpr int STAGES = NQ == 1 ? 1 : 2, SLOTS = 4, RAW_STAGES = NQ == 1 ? 2 : 4;
   static_assert(SLOTS >= STAGES + 2, "");
   static constexpr uint32_t HALVES = WIDTH / 64;
   static constexpr uint32_t Q_HALF = 128 * 128, Q_TILE = HALVES * Q_HALF;             // 128 rows of 128 bytes
   static constexpr uint32_t KV_HALF = KT * 128, KV_TILE = HALVES * KV_HALF;
-  static constexpr uint32_t OFF_Q = 0, OFF_K = NQ * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE, OFF_SC = OFF_V + STAGES * KV_TILE;
+  static constexpr uint32_t RAW_TILE = 2 * KT * WIDTH + 2 * KT * 4;                   // codes and scales of K and V as they come
+  static constexpr uint32_t OFF_Q = 0, OFF_K = NQ * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE, OFF_RAW = OFF_V + STAGES * KV_TILE;
+  static constexpr uint32_t OFF_SC = OFF_RAW + RAW_STAGES * RAW_TILE;
   // of a tile: scales of K, log2 and reciprocal of the scales of V, and for every 32 keys {a bit for each that does not
   // exist, a bit for each that holds a NaN, the largest and the smallest log2 of a scale of V}
   static constexpr uint32_t SLOT_LV = KT * 4, SLOT_RV = KT * 8, SLOT_SUM = KT * 12, SLOT = SLOT_SUM + KT / 2;
@@ -194,8 +196,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
   enter_line(a, cur, line.begin(blockIdx.x), line.begin(blockIdx.x + 1), before, ROWS, KT);
   if (cur.left <= 0) return;
 
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = base + L::OFF_BAR;
-  uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u, bar0 = base + L::OFF_BAR;
+  uint8_t* gbase = smem_raw + (base - smem_addr(smem_raw));
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(gbase + L::OFF_MISC);   // [0] TMEM address, [1] abort
   const Watch watch = {misc + 1, status_host};
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
@@ -474,40 +476,69 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     constexpr int PIECES = WIDTH / 16, RPI = 128 / PIECES, N_CHUNK = KT / RPI;        // rows of 128 threads; chunks per thread
     const int piece = ct % PIECES, row_l = ct / PIECES;
     Cursor ahead = cur;                              // the tile that is fetched next
-    int pages[N_CHUNK], s_page = -1;                 // of that tile: the page of each chunk's row, and of the key whose scales this thread fetches
-    auto page_of = [&](int key) -> int { return key < ahead.s.len ? __ldg(a.table + ahead.b * a.table_st + (key >> a.page_shift)) : -1; };
-    auto fetch_pages = [&]() {
-#pragma unroll
-      for (int i = 0; i < N_CHUNK; ++i) pages[i] = page_of(ahead.kt * KT + ((i * RPI + row_l) & ~15));
-      if (ct < KT) s_page = page_of(ahead.kt * KT + (ct & ~15));
+    // Page ids: every warp keeps 32 of the sequence's, one per lane, and the 32 behind them, asked for long before
+    // they are needed.
+    int window = -1, window_next = -1, window_first = 0, window_b = -1;
+    auto ids_from = [&](int first) -> int {
+      return first + lane < a.table_width ? __ldg(a.table + ahead.b * a.table_st + first + lane) : -1;
     };
-    uint4 kr[N_CHUNK], vr[N_CHUNK];
-    float sk = 0.f, sv = 0.f;
-    auto row_of = [&](int page, int key) -> long long {
-      return (((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-    };
-    auto fetch = [&](const uint8_t* codes, uint4 (&to)[N_CHUNK]) {
-#pragma unroll
-      for (int i = 0; i < N_CHUNK; ++i) {
-        to[i] = make_uint4(0u, 0u, 0u, 0u);
-        if ((unsigned)pages[i] < (unsigned)a.pages)
-          to[i] = __ldcs(reinterpret_cast<const uint4*>(codes + row_of(pages[i], ahead.kt * KT + i * RPI + row_l) * WIDTH + 16 * piece));
+    auto find_window = [&]() {
+      const int first = (ahead.kt * KT) >> a.page_shift;                              // (a tile's pages never lie in two windows)
+      if (ahead.b == window_b && first >= window_first && first < window_first + 32) return;
+      if (ahead.b == window_b && first == window_first + 32) {
+        window = window_next;
+        window_first += 32;
+      } else {
+        window_b = ahead.b;
+        window_first = first & ~31;
+        window = ids_from(window_first);
       }
+      window_next = ids_from(window_first + 32);
     };
-    auto fetch_scales = [&]() {
-      if (ct < KT) {
-        const bool there = (unsigned)s_page < (unsigned)a.pages;
-        const long long at = there ? row_of(s_page, ahead.kt * KT + ct) : 0;
-        sk = there ? __ldg(a.ks + at) : -1.f;        // below zero: no such key
-        sv = there ? __ldg(a.vs + at) : 0.f;
+    // The next tile's codes and scales into the ring: this thread's 16-byte pieces of K, of V, and the scales of key ct.
+    const uint32_t raw = base + L::OFF_RAW + 16 * ct, raw_scales = base + L::OFF_RAW + 2 * KT * WIDTH + 4 * ct;
+    int issued = 0;
+    auto issue_next = [&]() {
+      if (ahead.left > 0) {
+        find_window();
+        const uint32_t slot = (uint32_t)(issued % L::RAW_STAGES) * L::RAW_TILE;
+        auto place_of = [&](int row, bool& there) -> long long {
+          const int key = ahead.kt * KT + row, block = key & ~15;
+          const int page = __shfl_sync(0xffffffffu, window, ((block >> a.page_shift) - window_first) & 31);
+          there = block < ahead.s.len && (unsigned)page < (unsigned)a.pages;
+          return there ? (((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key & ((1 << a.page_shift) - 1)) : 0;
+        };
+        bool there;
+#pragma unroll
+        for (int i = 0; i < N_CHUNK; ++i) {
+          const long long at = place_of(i * RPI + row_l, there) * WIDTH + 16 * piece;
+          copy16(raw + slot + i * 2048, a.kc + at, there);
+          copy16(raw + slot + (N_CHUNK + i) * 2048, a.vc + at, there);
+        }
+        const long long at = place_of(ct & (KT - 1), there);
+        if (ct < KT) {
+          if (there) {
+            copy4(raw_scales + slot, a.ks + at);
+            copy4(raw_scales + slot + KT * 4, a.vs + at);
+          } else {                                   // no such key: a scale below zero says so
+            sts_f32(raw_scales + slot, -1.f);
+            sts_f32(raw_scales + slot + KT * 4, 0.f);
+          }
+        }
+        ++issued;
+        next_step(a, ahead, ROWS, KT);
       }
+      copy_commit();
     };
-    auto convert = [&](uint32_t stage, const uint4 (&from)[N_CHUNK], bool as_int8) {
+    auto convert = [&](uint32_t from, uint32_t stage, bool as_int8) {
+      uint4 codes[N_CHUNK];
+#pragma unroll
+      for (int i = 0; i < N_CHUNK; ++i) codes[i] = lds16(from + i * 2048);
 #pragma unroll
       for (int i = 0; i < N_CHUNK; ++i) {
         const int row = i * RPI + row_l;
         uint32_t h[8];
-        if (as_int8) codes_to_half<true>(from[i], h); else codes_to_half<false>(from[i], h);
+        if (as_int8) codes_to_half<true>(codes[i], h); else codes_to_half<false>(codes[i], h);
         const uint32_t to = stage + row * 128;
         if (WIDTH == 128) {
           const uint32_t at = to + 16 * (piece ^ (row & 7));
@@ -521,27 +552,19 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       fence_async_smem();
       __syncwarp();
     };
-    // on to the next tile, whose pages are asked for at once
-    auto advance = [&]() {
-      next_step(a, ahead, ROWS, KT);
-      if (ahead.left > 0) fetch_pages();
-    };
-    fetch_pages();
-    fetch(a.kc, kr);
-    fetch_scales();
-    fetch(a.vc, vr);
-    advance();
+#pragma unroll 1
+    for (int i = 0; i < L::RAW_STAGES; ++i) issue_next();
     bool ok = true;
-    bool more = true;
-    for (int n = 0; more; ++n) {
+    for (int n = 0; n < issued; ++n) {
       const int st = n % L::STAGES;
-      const uint32_t free_parity = ((uint32_t)(n / L::STAGES) & 1u) ^ 1u;
-      more = ahead.left > 0;
+      const uint32_t free_parity = ((uint32_t)(n / L::STAGES) & 1u) ^ 1u, slot = (uint32_t)(n % L::RAW_STAGES) * L::RAW_TILE;
+      copy_wait<L::RAW_STAGES - 1>();
       // K, the scales, and the flags of keys that do not exist
       ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_KE + st), free_parity, watch, CODE_LOAD));
       if (!ok) break;
       if (ct < KT) {
         const uint32_t sc = base + L::OFF_SC + (n % L::SLOTS) * L::SLOT;
+        const float sk = lds_f32(raw_scales + slot), sv = lds_f32(raw_scales + slot + KT * 4);
         const bool none = sk < 0.f, nan = isnan(sk) || isnan(sv);
         const float v = none || nan ? 1.f : fmaxf(sv, 1e-30f);       // (0: a row that nothing wrote, all codes 0; a part of the sum)
         sts_f32(sc + 4 * ct, none || nan ? 1.f : fmaxf(sk, 1e-30f));
@@ -554,21 +577,15 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(L::B_SC + n % L::SLOTS));
       }
-      convert(base + L::OFF_K + st * L::KV_TILE, kr, INT8);
+      convert(raw + slot, base + L::OFF_K + st * L::KV_TILE, INT8);
       if (lane == 0) mbar_arrive(bar(L::B_KF + st));
-      if (more) {                                    // `ahead` is tile n + 1
-        fetch(a.kc, kr);
-        fetch_scales();
-      }
       ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_VE + st), free_parity, watch, CODE_LOAD));
       if (!ok) break;
-      convert(base + L::OFF_V + st * L::KV_TILE, vr, false);
+      convert(raw + slot + N_CHUNK * 2048, base + L::OFF_V + st * L::KV_TILE, false);
       if (lane == 0) mbar_arrive(bar(L::B_VF + st));
-      if (more) {
-        fetch(a.vc, vr);
-        advance();
-      }
+      issue_next();
     }
+    copy_wait<0>();                                  // (a wait that gave up leaves none of its own copies in flight)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_ISSUER));
     const int g = warp - ISSUER;
