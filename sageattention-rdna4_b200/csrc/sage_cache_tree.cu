@@ -154,7 +154,7 @@ template <int WIDTH, int NQ> struct TreeShape {
   static_assert(NQ * REGS_SOFTMAX + REGS_LOADER + REGS_ISSUER <= (NQ + 2) * REGS_LAUNCH, "setmaxnreg would wait forever");
   // Stages of K and V; slots of scales.  A slot is written once the scores STAGES tiles back are complete, which means that
   // the softmax is done with the tile two before that.
-  static constexpr int STAGES = NQ == 1 ? 1 : 2, SLOTS = 4, RAW_STAGES = NQ == 1 ? 2 : 4;
+  static constexpr int STAGES = 2, SLOTS = 4, RAW_STAGES = NQ == 1 ? 0 : 4;
   static_assert(SLOTS >= STAGES + 2, "");
   static constexpr uint32_t HALVES = WIDTH / 64;
   static constexpr uint32_t Q_HALF = 128 * 128, Q_TILE = HALVES * Q_HALF;             // 128 rows of 128 bytes
@@ -476,64 +476,28 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     constexpr int PIECES = WIDTH / 16, RPI = 128 / PIECES, N_CHUNK = KT / RPI;        // rows of 128 threads; chunks per thread
     const int piece = ct % PIECES, row_l = ct / PIECES;
     Cursor ahead = cur;                              // the tile that is fetched next
-    // Page ids: every warp keeps 32 of the sequence's, one per lane, and the 32 behind them, asked for long before
-    // they are needed.
-    int window = -1, window_next = -1, window_first = 0, window_b = -1;
-    auto ids_from = [&](int first) -> int {
-      return first + lane < a.table_width ? __ldg(a.table + ahead.b * a.table_st + first + lane) : -1;
+    auto row_of = [&](int page, int key) -> long long {
+      return (((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
     };
-    auto find_window = [&]() {
-      const int first = (ahead.kt * KT) >> a.page_shift;                              // (a tile's pages never lie in two windows)
-      if (ahead.b == window_b && first >= window_first && first < window_first + 32) return;
-      if (ahead.b == window_b && first == window_first + 32) {
-        window = window_next;
-        window_first += 32;
-      } else {
-        window_b = ahead.b;
-        window_first = first & ~31;
-        window = ids_from(window_first);
+    // The scales of this thread's key of tile n: a scale of K below zero says that there is no such key.
+    auto store_scales = [&](int n, float sk, float sv) {
+      if (ct < KT) {
+        const uint32_t sc = base + L::OFF_SC + (n % L::SLOTS) * L::SLOT;
+        const bool none = sk < 0.f, nan = isnan(sk) || isnan(sv);
+        const float v = none || nan ? 1.f : fmaxf(sv, 1e-30f);       // (0: a row that nothing wrote, all codes 0; a part of the sum)
+        sts_f32(sc + 4 * ct, none || nan ? 1.f : fmaxf(sk, 1e-30f));
+        sts_f32(sc + L::SLOT_LV + 4 * ct, __log2f(v));
+        sts_f32(sc + L::SLOT_RV + 4 * ct, __fdividef(1.f, v));
+        const uint32_t none32 = __ballot_sync(0xffffffffu, none), nan32 = __ballot_sync(0xffffffffu, nan);
+        // (positive floats are ordered as their bits are)
+        const float big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))), small = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(v)));
+        if (lane == 0) sts16(sc + L::SLOT_SUM + 16 * (ct >> 5), none32, nan32, __float_as_uint(__log2f(big)), __float_as_uint(__log2f(small)));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::B_SC + n % L::SLOTS));
       }
-      window_next = ids_from(window_first + 32);
     };
-    // The next tile's codes and scales into the ring: this thread's 16-byte pieces of K, of V, and the scales of key ct.
-    const uint32_t raw = base + L::OFF_RAW + 16 * ct, raw_scales = base + L::OFF_RAW + 2 * KT * WIDTH + 4 * ct;
-    int issued = 0;
-    auto issue_next = [&]() {
-      if (ahead.left > 0) {
-        find_window();
-        const uint32_t slot = (uint32_t)(issued % L::RAW_STAGES) * L::RAW_TILE;
-        auto place_of = [&](int row, bool& there) -> long long {
-          const int key = ahead.kt * KT + row, block = key & ~15;
-          const int page = __shfl_sync(0xffffffffu, window, ((block >> a.page_shift) - window_first) & 31);
-          there = block < ahead.s.len && (unsigned)page < (unsigned)a.pages;
-          return there ? (((long long)page * a.Hkv + ahead.h) << a.page_shift) + (key & ((1 << a.page_shift) - 1)) : 0;
-        };
-        bool there;
-#pragma unroll
-        for (int i = 0; i < N_CHUNK; ++i) {
-          const long long at = place_of(i * RPI + row_l, there) * WIDTH + 16 * piece;
-          copy16(raw + slot + i * 2048, a.kc + at, there);
-          copy16(raw + slot + (N_CHUNK + i) * 2048, a.vc + at, there);
-        }
-        const long long at = place_of(ct & (KT - 1), there);
-        if (ct < KT) {
-          if (there) {
-            copy4(raw_scales + slot, a.ks + at);
-            copy4(raw_scales + slot + KT * 4, a.vs + at);
-          } else {                                   // no such key: a scale below zero says so
-            sts_f32(raw_scales + slot, -1.f);
-            sts_f32(raw_scales + slot + KT * 4, 0.f);
-          }
-        }
-        ++issued;
-        next_step(a, ahead, ROWS, KT);
-      }
-      copy_commit();
-    };
-    auto convert = [&](uint32_t from, uint32_t stage, bool as_int8) {
-      uint4 codes[N_CHUNK];
-#pragma unroll
-      for (int i = 0; i < N_CHUNK; ++i) codes[i] = lds16(from + i * 2048);
+    // This thread's pieces of a tile, turned into fp16, to the operand at `stage`.
+    auto store_codes = [&](const uint4 (&codes)[N_CHUNK], uint32_t stage, bool as_int8) {
 #pragma unroll
       for (int i = 0; i < N_CHUNK; ++i) {
         const int row = i * RPI + row_l;
@@ -552,40 +516,142 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       fence_async_smem();
       __syncwarp();
     };
+    auto stage_free = [&](int b, int n) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar(b + n % L::STAGES), ((uint32_t)(n / L::STAGES) & 1u) ^ 1u, watch, CODE_LOAD));
+    };
+    if constexpr (L::RAW_STAGES > 0) {
+      // Page ids: every warp keeps 32 of the sequence's, one per lane, and the 32 behind them, asked for long before
+      // they are needed.
+      int window = -1, window_next = -1, window_first = 0, window_b = -1;
+      auto ids_from = [&](int first) -> int {
+        return first + lane < a.table_width ? __ldg(a.table + ahead.b * a.table_st + first + lane) : -1;
+      };
+      auto find_window = [&]() {
+        const int first = (ahead.kt * KT) >> a.page_shift;                              // (a tile's pages never lie in two windows)
+        if (ahead.b == window_b && first >= window_first && first < window_first + 32) return;
+        if (ahead.b == window_b && first == window_first + 32) {
+          window = window_next;
+          window_first += 32;
+        } else {
+          window_b = ahead.b;
+          window_first = first & ~31;
+          window = ids_from(window_first);
+        }
+        window_next = ids_from(window_first + 32);
+      };
+      // The next tile's codes and scales into the ring: this thread's 16-byte pieces of K, of V, and the scales of key ct.
+      const uint32_t raw = base + L::OFF_RAW + 16 * ct, raw_scales = base + L::OFF_RAW + 2 * KT * WIDTH + 4 * ct;
+      int issued = 0;
+      auto issue_next = [&]() {
+        if (ahead.left > 0) {
+          find_window();
+          const uint32_t slot = (uint32_t)(issued % L::RAW_STAGES) * L::RAW_TILE;
+          auto place_of = [&](int row, bool& there) -> long long {
+            const int key = ahead.kt * KT + row, block = key & ~15;
+            const int page = __shfl_sync(0xffffffffu, window, ((block >> a.page_shift) - window_first) & 31);
+            there = block < ahead.s.len && (unsigned)page < (unsigned)a.pages;
+            return there ? row_of(page, key) : 0;
+          };
+          bool there;
+#pragma unroll
+          for (int i = 0; i < N_CHUNK; ++i) {
+            const long long at = place_of(i * RPI + row_l, there) * WIDTH + 16 * piece;
+            copy16(raw + slot + i * 2048, a.kc + at, there);
+            copy16(raw + slot + (N_CHUNK + i) * 2048, a.vc + at, there);
+          }
+          const long long at = place_of(ct & (KT - 1), there);
+          if (ct < KT) {
+            if (there) {
+              copy4(raw_scales + slot, a.ks + at);
+              copy4(raw_scales + slot + KT * 4, a.vs + at);
+            } else {                                   // no such key: a scale below zero says so
+              sts_f32(raw_scales + slot, -1.f);
+              sts_f32(raw_scales + slot + KT * 4, 0.f);
+            }
+          }
+          ++issued;
+          next_step(a, ahead, ROWS, KT);
+        }
+        copy_commit();
+      };
+      auto convert = [&](uint32_t from, uint32_t stage, bool as_int8) {
+        uint4 codes[N_CHUNK];
+#pragma unroll
+        for (int i = 0; i < N_CHUNK; ++i) codes[i] = lds16(from + i * 2048);
+        store_codes(codes, stage, as_int8);
+      };
 #pragma unroll 1
-    for (int i = 0; i < L::RAW_STAGES; ++i) issue_next();
-    bool ok = true;
-    for (int n = 0; n < issued; ++n) {
-      const int st = n % L::STAGES;
-      const uint32_t free_parity = ((uint32_t)(n / L::STAGES) & 1u) ^ 1u, slot = (uint32_t)(n % L::RAW_STAGES) * L::RAW_TILE;
-      copy_wait<L::RAW_STAGES - 1>();
-      // K, the scales, and the flags of keys that do not exist
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_KE + st), free_parity, watch, CODE_LOAD));
-      if (!ok) break;
-      if (ct < KT) {
-        const uint32_t sc = base + L::OFF_SC + (n % L::SLOTS) * L::SLOT;
-        const float sk = lds_f32(raw_scales + slot), sv = lds_f32(raw_scales + slot + KT * 4);
-        const bool none = sk < 0.f, nan = isnan(sk) || isnan(sv);
-        const float v = none || nan ? 1.f : fmaxf(sv, 1e-30f);       // (0: a row that nothing wrote, all codes 0; a part of the sum)
-        sts_f32(sc + 4 * ct, none || nan ? 1.f : fmaxf(sk, 1e-30f));
-        sts_f32(sc + L::SLOT_LV + 4 * ct, __log2f(v));
-        sts_f32(sc + L::SLOT_RV + 4 * ct, __fdividef(1.f, v));
-        const uint32_t none32 = __ballot_sync(0xffffffffu, none), nan32 = __ballot_sync(0xffffffffu, nan);
-        // (positive floats are ordered as their bits are)
-        const float big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))), small = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(v)));
-        if (lane == 0) sts16(sc + L::SLOT_SUM + 16 * (ct >> 5), none32, nan32, __float_as_uint(__log2f(big)), __float_as_uint(__log2f(small)));
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(L::B_SC + n % L::SLOTS));
+      for (int i = 0; i < L::RAW_STAGES; ++i) issue_next();
+      for (int n = 0; n < issued; ++n) {
+        const int st = n % L::STAGES;
+        const uint32_t slot = (uint32_t)(n % L::RAW_STAGES) * L::RAW_TILE;
+        copy_wait<L::RAW_STAGES - 1>();
+        if (!stage_free(L::B_KE, n)) break;
+        if (ct < KT) store_scales(n, lds_f32(raw_scales + slot), lds_f32(raw_scales + slot + KT * 4));
+        convert(raw + slot, base + L::OFF_K + st * L::KV_TILE, INT8);
+        if (lane == 0) mbar_arrive(bar(L::B_KF + st));
+        if (!stage_free(L::B_VE, n)) break;
+        convert(raw + slot + N_CHUNK * 2048, base + L::OFF_V + st * L::KV_TILE, false);
+        if (lane == 0) mbar_arrive(bar(L::B_VF + st));
+        issue_next();
       }
-      convert(raw + slot, base + L::OFF_K + st * L::KV_TILE, INT8);
-      if (lane == 0) mbar_arrive(bar(L::B_KF + st));
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_VE + st), free_parity, watch, CODE_LOAD));
-      if (!ok) break;
-      convert(raw + slot + N_CHUNK * 2048, base + L::OFF_V + st * L::KV_TILE, false);
-      if (lane == 0) mbar_arrive(bar(L::B_VF + st));
-      issue_next();
+      copy_wait<0>();                                // (a wait that gave up leaves none of its own copies in flight)
+    } else {
+      int pages[N_CHUNK], s_page = -1;               // of tile `ahead`: the page of each chunk's row, and of the key whose scales this thread fetches
+      auto page_of = [&](int key) -> int { return key < ahead.s.len ? __ldg(a.table + ahead.b * a.table_st + (key >> a.page_shift)) : -1; };
+      auto fetch_pages = [&]() {
+#pragma unroll
+        for (int i = 0; i < N_CHUNK; ++i) pages[i] = page_of(ahead.kt * KT + ((i * RPI + row_l) & ~15));
+        if (ct < KT) s_page = page_of(ahead.kt * KT + (ct & ~15));
+      };
+      uint4 kr[N_CHUNK], vr[N_CHUNK];
+      float sk = 0.f, sv = 0.f;
+      auto fetch = [&](const uint8_t* codes, uint4 (&to)[N_CHUNK]) {
+#pragma unroll
+        for (int i = 0; i < N_CHUNK; ++i) {
+          to[i] = make_uint4(0u, 0u, 0u, 0u);
+          if ((unsigned)pages[i] < (unsigned)a.pages)
+            to[i] = __ldcs(reinterpret_cast<const uint4*>(codes + row_of(pages[i], ahead.kt * KT + i * RPI + row_l) * WIDTH + 16 * piece));
+        }
+      };
+      auto fetch_scales = [&]() {
+        if (ct < KT) {
+          const bool there = (unsigned)s_page < (unsigned)a.pages;
+          const long long at = there ? row_of(s_page, ahead.kt * KT + ct) : 0;
+          sk = there ? __ldg(a.ks + at) : -1.f;
+          sv = there ? __ldg(a.vs + at) : 0.f;
+        }
+      };
+      auto advance = [&]() {                         // on to the next tile, whose pages are asked for at once
+        next_step(a, ahead, ROWS, KT);
+        if (ahead.left > 0) fetch_pages();
+      };
+      fetch_pages();
+      fetch(a.kc, kr);
+      fetch_scales();
+      fetch(a.vc, vr);
+      advance();
+      bool more = true;
+      for (int n = 0; more; ++n) {
+        const int st = n % L::STAGES;
+        more = ahead.left > 0;                       // `ahead` is tile n + 1
+        if (!stage_free(L::B_KE, n)) break;
+        store_scales(n, sk, sv);
+        store_codes(kr, base + L::OFF_K + st * L::KV_TILE, INT8);
+        if (lane == 0) mbar_arrive(bar(L::B_KF + st));
+        if (more) {
+          fetch(a.kc, kr);
+          fetch_scales();
+        }
+        if (!stage_free(L::B_VE, n)) break;
+        store_codes(vr, base + L::OFF_V + st * L::KV_TILE, false);
+        if (lane == 0) mbar_arrive(bar(L::B_VF + st));
+        if (more) {
+          fetch(a.vc, vr);
+          advance();
+        }
+      }
     }
-    copy_wait<0>();                                  // (a wait that gave up leaves none of its own copies in flight)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::REGS_ISSUER));
     const int g = warp - ISSUER;
