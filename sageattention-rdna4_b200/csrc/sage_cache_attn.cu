@@ -450,12 +450,12 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   }
 }
 
-// Joins the parts of the units that lie in several stretches, in a fixed order.  A CTA has 8 / WARPS_PER_ROW rows of a
-// unit: with all eight warps on a row the parts are spread over them (few rows, many parts: a step of one token), with
-// one each (hundreds of rows, two or three parts) a warp adds a row's by itself.
+// Joins the parts of the units that lie in several stretches, in a fixed order.  With all eight warps of a CTA on a row
+// the parts are spread over them (few rows, many parts: a step of one token); with one each (hundreds of rows, two or
+// three parts) a warp adds a row's by itself, and takes rows_per_warp of them.
 constexpr int CC_WARPS = 8, CC_THREADS = 32 * CC_WARPS;
 template <typename T, int WARPS_PER_ROW>
-__global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int keys, int width, int max_rt) {
+__global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int keys, int width, int max_rt, int rows_per_warp) {
   __shared__ unsigned total_s[CC_WARPS], before_s[CC_WARPS];
   __shared__ float acc_s[CC_WARPS][HD];
   __shared__ float2 ml_s[CC_WARPS];
@@ -464,7 +464,6 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
   const unsigned bh = blockIdx.x / (unsigned)max_rt;
   const int rt = (int)(blockIdx.x - bh * max_rt), b = (int)(bh / (unsigned)a.Hkv), h = (int)(bh - (unsigned)b * a.Hkv);
   const Seq s = seq_of(a, b);                        // (the lengths are older than the attention kernel)
-  const int r = blockIdx.y * (CC_WARPS / WARPS_PER_ROW) + warp / WARPS_PER_ROW, rr = rt * rows + r;
   // places before this sequence, and in all
   unsigned before = 0, total = 0;
   for (int i = tid; i < a.n_seq; i += CC_THREADS) {
@@ -486,72 +485,75 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
   wait_for_predecessor();
   // no such row, or written by the one that had all of its unit  (the whole CTA leaves, or whole warps of rows)
   if (rt >= row_tiles(a, s, rows) || c0 == c1) return;
-  const bool live = r < rows && rr < s.q_len * a.group;
-  if (WARPS_PER_ROW == 1 && !live) return;
-  if (WARPS_PER_ROW == CC_WARPS && !live) return;
-  auto at_of = [&](int x) { return (2LL * x + (u0 > line.begin(x) ? 1 : 0)) * a.part_rows + r; };
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f, top = NO_MAX;
-  const bool mine = 4 * lane < width;
-  constexpr int AT_ONCE = 8;
-  for (int i0 = c0 + share; i0 <= c1; i0 += WARPS_PER_ROW * AT_ONCE) {
-    float2 ml[AT_ONCE];
-    float4 v[AT_ONCE];
+  constexpr int STRIDE = CC_WARPS / WARPS_PER_ROW;
+#pragma unroll 1
+  for (int k = 0; k < rows_per_warp; ++k) {
+    const int r = (blockIdx.y * rows_per_warp + k) * STRIDE + warp / WARPS_PER_ROW;
+    const int rr = rt * rows + r;
+    if (r >= rows || rr >= s.q_len * a.group) return;                  // (nor any behind it)
+    auto at_of = [&](int x) { return (2LL * x + (u0 > line.begin(x) ? 1 : 0)) * a.part_rows + r; };
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f, top = NO_MAX;
+    const bool mine = 4 * lane < width;
+    constexpr int AT_ONCE = 8;
+    for (int i0 = c0 + share; i0 <= c1; i0 += WARPS_PER_ROW * AT_ONCE) {
+      float2 ml[AT_ONCE];
+      float4 v[AT_ONCE];
 #pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) {
-      const int i = i0 + j * WARPS_PER_ROW;
-      ml[j] = make_float2(NO_MAX, 0.f);
-      v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i <= c1) {
-        const long long at = at_of(i);
-        ml[j] = a.part_ml[at];
-        if (mine) v[j] = *reinterpret_cast<const float4*>(a.part_o + at * width + 4 * lane);
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const int i = i0 + j * WARPS_PER_ROW;
+        ml[j] = make_float2(NO_MAX, 0.f);
+        v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i <= c1) {
+          const long long at = at_of(i);
+          ml[j] = a.part_ml[at];
+          if (mine) v[j] = *reinterpret_cast<const float4*>(a.part_o + at * width + 4 * lane);
+        }
+      }
+      float up = top;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) up = fmaxf(up, ml[j].x);
+      const float fade = fast_ex2(top - up);
+      acc.x *= fade; acc.y *= fade; acc.z *= fade; acc.w *= fade; sum *= fade;
+      top = up;
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const float weight = fast_ex2(ml[j].x - top);
+        sum = fmaf(ml[j].y, weight, sum);
+        acc.x = fmaf(v[j].x, weight, acc.x); acc.y = fmaf(v[j].y, weight, acc.y); acc.z = fmaf(v[j].z, weight, acc.z); acc.w = fmaf(v[j].w, weight, acc.w);
       }
     }
-    float up = top;
+    const int tok = rr / a.group, head = h * a.group + rr - tok * a.group;
+    T* dst = reinterpret_cast<T*>(a.out) + (long long)(s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
+    if (WARPS_PER_ROW == 1) {
+      const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+      // (the many-row kernel leaves the columns of wide heads in the order of its accumulator)
+      const int n = 4 * lane, col = width == 128 ? 16 * ((n >> 3) & 7) + 8 * (n >> 6) + (n & 7) : n;
+      if (mine && col < a.D) *reinterpret_cast<uint2*>(dst + col) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
+    } else {
+      if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
+      if (lane == 0) ml_s[warp] = make_float2(top, sum);
+      __syncthreads();
+      top = NO_MAX; sum = 0.f;
+      float weight[CC_WARPS];
 #pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) up = fmaxf(up, ml[j].x);
-    const float fade = fast_ex2(top - up);
-    acc.x *= fade; acc.y *= fade; acc.z *= fade; acc.w *= fade; sum *= fade;
-    top = up;
+      for (int w = 0; w < CC_WARPS; ++w) top = fmaxf(top, ml_s[w].x);
 #pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) {
-      const float weight = fast_ex2(ml[j].x - top);
-      sum = fmaf(ml[j].y, weight, sum);
-      acc.x = fmaf(v[j].x, weight, acc.x); acc.y = fmaf(v[j].y, weight, acc.y); acc.z = fmaf(v[j].z, weight, acc.z); acc.w = fmaf(v[j].w, weight, acc.w);
+      for (int w = 0; w < CC_WARPS; ++w) { weight[w] = fast_ex2(ml_s[w].x - top); sum = fmaf(ml_s[w].y, weight[w], sum); }
+      const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+      if (tid < a.D) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < CC_WARPS; ++w) v = fmaf(acc_s[w][tid], weight[w], v);
+        dst[tid] = from_float<T>(v * inv);
+      }
     }
-  }
-  const int tok = rr / a.group, head = h * a.group + rr - tok * a.group;
-  T* dst = reinterpret_cast<T*>(a.out) + (long long)(s.q0 + tok) * a.o_st + (long long)head * a.o_sh;
-  if (WARPS_PER_ROW == 1) {
-    const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-    // (the many-row kernel leaves the columns of wide heads in the order of its accumulator)
-    const int n = 4 * lane, col = width == 128 ? 16 * ((n >> 3) & 7) + 8 * (n >> 6) + (n & 7) : n;
-    if (mine && col < a.D) *reinterpret_cast<uint2*>(dst + col) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
-  } else {
-    if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
-    if (lane == 0) ml_s[warp] = make_float2(top, sum);
-    __syncthreads();
-    top = NO_MAX; sum = 0.f;
-    float weight[CC_WARPS];
-#pragma unroll
-    for (int w = 0; w < CC_WARPS; ++w) top = fmaxf(top, ml_s[w].x);
-#pragma unroll
-    for (int w = 0; w < CC_WARPS; ++w) { weight[w] = fast_ex2(ml_s[w].x - top); sum = fmaf(ml_s[w].y, weight[w], sum); }
-    const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-    if (tid < a.D) {
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < CC_WARPS; ++w) v = fmaf(acc_s[w][tid], weight[w], v);
-      dst[tid] = from_float<T>(v * inv);
-    }
-  }
-  if (a.lse != nullptr && share == WARPS_PER_ROW - 1) {
-    float v = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * LN2_F;
-    if (a.shift != nullptr)
-      v += shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(s.q0 + tok) * a.q_st + (long long)head * a.q_sh, h, width, lane);
-    if (lane == 0) a.lse[(long long)(s.q0 + tok) * a.Hq + head] = v;
-  }
+    if (a.lse != nullptr && share == WARPS_PER_ROW - 1) {
+      float v = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * LN2_F;
+      if (a.shift != nullptr)
+        v += shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(s.q0 + tok) * a.q_st + (long long)head * a.q_sh, h, width, lane);
+      if (lane == 0) a.lse[(long long)(s.q0 + tok) * a.Hq + head] = v;
+    }  }
 }
 
 constexpr int CTAS_PER_SM = 2;
@@ -586,9 +588,14 @@ template <typename T>
 cudaError_t launch_combine_t(const CacheAttnKArgs& a, int rows, int keys, int width, int max_rt, cudaStream_t st) {
   const unsigned units = (unsigned)((long long)a.n_seq * a.Hkv * max_rt);
   if (rows <= 16)
-    return launch_after_predecessor(cache_combine_kernel<T, CC_WARPS>, dim3(units, (unsigned)a.part_rows), dim3(CC_THREADS), 0, st, a, rows, keys, width, max_rt);
-  return launch_after_predecessor(cache_combine_kernel<T, 1>, dim3(units, (unsigned)((a.part_rows + CC_WARPS - 1) / CC_WARPS)), dim3(CC_THREADS), 0, st,
-                                  a, rows, keys, width, max_rt);
+    return launch_after_predecessor(cache_combine_kernel<T, CC_WARPS>, dim3(units, (unsigned)a.part_rows), dim3(CC_THREADS), 0, st, a, rows, keys, width, max_rt, 1);
+  // One row per warp where all CTAs find room at once, eight to an SM; more rows at a time beyond that, since what a CTA
+  // does before its first row (it finds the unit's place in the line, for which it reads every sequence's length) would be
+  // most of its time.  With the attention before it: 32 units of 84 rows 36.0 us with one row per warp, 47.5 with four; 296
+  // units of 256 rows 70.1 and 43.9.
+  const unsigned ctas = (unsigned)((a.part_rows + CC_WARPS - 1) / CC_WARPS), per_warp = (unsigned long long)units * ctas <= 8 * SIZING_SMS ? 1 : 4;
+  return launch_after_predecessor(cache_combine_kernel<T, 1>, dim3(units, (ctas + per_warp - 1) / per_warp), dim3(CC_THREADS), 0, st, a, rows, keys, width,
+                                  max_rt, (int)per_warp);
 }
 
 }  // namespace

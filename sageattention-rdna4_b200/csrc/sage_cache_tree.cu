@@ -165,8 +165,8 @@ template <int WIDTH, int NQ> struct TreeShape {
   // of a tile: scales of K, log2 and reciprocal of the scales of V, and for every 32 keys {a bit for each that does not
   // exist, a bit for each that holds a NaN, the largest and the smallest log2 of a scale of V}
   static constexpr uint32_t SLOT_LV = KT * 4, SLOT_RV = KT * 8, SLOT_SUM = KT * 12, SLOT = SLOT_SUM + KT / 2;
-  static constexpr uint32_t OFF_ROW = OFF_SC + SLOTS * SLOT;                          // a float per row
-  static constexpr uint32_t OFF_BAR = OFF_ROW + SOFTMAX * 4;
+  static constexpr uint32_t OFF_ROW = OFF_SC + SLOTS * SLOT;                          // two floats per row
+  static constexpr uint32_t OFF_BAR = OFF_ROW + SOFTMAX * 8;
   // Barriers: per half of the rows (QF) and score buffer (SF, PF, PV), per stage (KF, KE, VF, VE), per slot (SC).  What is
   // waited for is never more than one phase away from where its barrier stands: the scores of a tile are issued after P V of
   // the tile two before, which waited for that tile's weights.
@@ -233,7 +233,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     const int g = warp >> 2, r = tid & 127;
     const uint32_t lane_sel = (uint32_t)(warp & 3) << 21;                             // 32 lanes of TMEM per warp
     const uint32_t o_addr = tmem_o(g) + lane_sel;
-    float* row_at = reinterpret_cast<float*>(gbase + L::OFF_ROW) + 128 * g;
+    float* row_at = reinterpret_cast<float*>(gbase + L::OFF_ROW) + 256 * g;           // of row r: [r] what undoes its power of two, [128 + r] its product with the shift
     // Rows of 2 * WIDTH bytes in this half's Q tile: piece c of row r, where Q goes and outputs pass through.
     uint8_t* q_tile = gbase + L::OFF_Q + g * L::Q_TILE;
     auto staged = [&](int row, int c) { return reinterpret_cast<uint4*>(q_tile + (c >> 3) * L::Q_HALF + row * 128 + 16 * ((c & 7) ^ (row & 7))); };
@@ -253,11 +253,26 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         return (long long)(cur.s.q0 + token) * st + (long long)(cur.h * a.group + x - token * a.group) * sh;
       };
       if (g < halves_of(cur)) {
-#pragma unroll 4
+        const bool whole = kt0 == 0 && count == cur.n_kt, dots = whole && a.lse != nullptr && a.shift != nullptr;
+        float shift[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};                    // of this lane's columns
+        if (dots) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) shift[e] = __ldg(a.shift + (long long)cur.h * WIDTH + 8 * c_l + e);
+        }
+#pragma unroll 8
         for (int i = 0; i < 32 / RPI; ++i) {
           const int row = row_l + i * RPI;
           uint4 u = make_uint4(0u, 0u, 0u, 0u);
           if (row < live && 8 * c_l < a.D) u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + row_of(row, a.q_st, a.q_sh) + 8 * c_l));
+          if (dots) {
+            float x[8], d = 0.f;
+            unpack8<T>(u, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d = fmaf(x[e], shift[e], d);
+#pragma unroll
+            for (int o = PIECES / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+            if (c_l == 0) row_at[128 + row] = d * a.sm_scale;
+          }
           float back = 1.f;                          // what undoes the row's power of two
           if (!__is_same(T, __half)) {               // bf16: the row's largest element to [2^14, 2^15)
             float x[8], amax = 0.f;
@@ -319,9 +334,16 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
               uint32_t b = upto >= 32 ? 0xffffffffu : upto <= 0 ? 0u : (1u << upto) - 1u;
               b &= ~(ch ? sum1.x : sum0.x);
               if (tree_row != nullptr && b != 0u && k0 + 32 > ctx) {
-#pragma unroll 4
-                for (int i = 0; i < 32; ++i)
-                  if (k0 + i >= ctx && (b >> i & 1u) && tree_row[k0 + i - ctx] == 0) b &= ~(1u << i);
+                uint32_t hidden = 0u;                // (sixteen bytes in flight at a time)
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32; i0 += 16)
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    const int at = k0 + i0 + i - ctx;
+                    const uint32_t seen = at >= 0 && (b >> (i0 + i) & 1u) ? __ldg(tree_row + at) : 1u;
+                    hidden |= (seen == 0u ? 1u : 0u) << (i0 + i);
+                  }
+                b &= ~hidden;
               }
               bits[ch] = b;
             }
@@ -407,7 +429,6 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_PV + 2 * g + ((done - 1) & 1)), (uint32_t)((done - 1) >> 1) & 1u, watch, CODE_SOFTMAX));
         if (!ok) break;
         tc_fence_after();
-        const bool whole = kt0 == 0 && count == cur.n_kt;
         // a unit that began before this stretch, or with it: its part is the stretch's first, else its last
         const long long part_row = (2LL * blockIdx.x + (cur.into > 0 ? 1 : 0)) * a.part_rows + 128 * g;
         if (whole) {
@@ -456,12 +477,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         tc_fence_before();
         if (exists && whole && a.lse != nullptr) {
           float v = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2_F;
-          if (a.shift != nullptr) {                  // the keys as they were before the shift was taken off
-            const T* q_row = reinterpret_cast<const T*>(a.q) + row_of(r, a.q_st, a.q_sh);
-            float d = 0.f;
-            for (int i = 0; i < a.D; ++i) d = fmaf((float)q_row[i], __ldg(a.shift + (long long)cur.h * WIDTH + i), d);
-            v += d * a.sm_scale;
-          }
+          if (dots) v += row_at[128 + r];            // the keys as they were before the shift was taken off
           a.lse[(long long)(cur.s.q0 + tok) * a.Hq + cur.h * a.group + rr - tok * a.group] = v;
         }
         __syncwarp();                                // (the rows that passed through are read before the next Q is written)
