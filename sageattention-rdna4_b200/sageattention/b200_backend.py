@@ -301,7 +301,8 @@ class _StreamState:
     live only until its attention kernel has run, and calls on one stream are ordered) and the
     pinned host word that receives the status word of a call that failed."""
 
-    __slots__ = ("ws", "host", "host_word", "status_off", "shape", "adaptive", "probe_host", "last_share")
+    __slots__ = ("ws", "host", "host_word", "status_off", "shape", "adaptive", "probe_host", "last_share", "cache_ws",
+                 "cache_lock")
 
     def __init__(self, host_word=None):
         self.adaptive = _Adaptive()
@@ -312,6 +313,8 @@ class _StreamState:
         self.host_word = host_word          # ctypes.c_int32 view of it (tests pass a plain c_int32)
         self.status_off = None
         self.shape = None
+        self.cache_ws = None                # of `sageattn_cached`, whose calls take the lock from choosing it to their last launch
+        self.cache_lock = threading.Lock()
 
     def pending(self) -> int:
         return 0 if self.host_word is None else int(self.host_word.value)

@@ -16,15 +16,15 @@ synchronises, and every call can be captured into a CUDA graph.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import operator
 from typing import Optional, Tuple
 
 import torch
 
 from . import _native
 from . import b200_backend as _be
-from .b200_backend import HEAD_DIM, _counters, _dtype_code, _grow, _report_to, _state, packed_view_reason, strided_view_reason
+from .b200_backend import HEAD_DIM, _WS_GRANULE, _counters, _dtype_code, _report_to, _state, packed_view_reason, strided_view_reason
 
 _E4M3 = torch.float8_e4m3fn
 
@@ -63,6 +63,20 @@ def _sig(t: torch.Tensor):
     return t.shape, t.stride(), t.dtype, t.device, t.data_ptr() & 15
 
 
+def _fixed(self, name, value):
+    """`__setattr__` of objects whose buffers' addresses are worked out once."""
+    if hasattr(self, "_plans"):
+        raise AttributeError("%s.%s is fixed when the object is made" % (type(self).__name__, name))
+    object.__setattr__(self, name, value)
+
+
+def _written(tensors):
+    """Tell autograd that these were written over, as it is told of torch's own writes."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _remember(plans: dict, key, plan):
     if len(plans) >= _PLANS:
         plans.clear()
@@ -79,12 +93,14 @@ class SageCache:
     k_shift : optional ``(Hkv, head_dim)`` float32 that is subtracted from K before it is quantised (the mean
         that `smooth_k` takes off, taken once over a prompt and kept).  Attention does not change by it: all
         keys of a head move alike.
+    The buffers stay the cache's for good (what they hold may change).
     page_size is a power of two, 16 .. 256.  The code buffers must start as zeros (`empty` does that): codes that
     no write has set may be read behind a mask, and must not be the e4m3 NaN.
     """
 
     __slots__ = ("k_codes", "k_scale", "v_codes", "v_scale", "k_shift", "head_dim", "num_pages", "page_size",
                  "num_kv_heads", "device", "_mode", "_args", "_sizes", "_plans")
+    __setattr__ = _fixed
 
     def __init__(self, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
                  head_dim: int, k_shift: Optional[torch.Tensor] = None):
@@ -210,6 +226,8 @@ def sage_cache_read(cache: SageCache, page_table: torch.Tensor, cu_seqlens: torc
     """
     _counters["calls"] += 1
     dev, heads, d = cache.device, cache.num_kv_heads, cache.head_dim
+    if total.__class__ is not int:
+        _refuse("total must be an int, not negative")
     key = ("read", _sig(page_table), _sig(cu_seqlens), total, dtype, None if out is None else tuple(_sig(t) for t in out))
     plan = cache._plans.get(key)
     if plan is None:
@@ -219,6 +237,9 @@ def sage_cache_read(cache: SageCache, page_table: torch.Tensor, cu_seqlens: torc
         v = torch.empty((total, heads, d), dtype=dtype, device=dev)
     else:
         k, v = out
+        if plan and _overlap(k, v):
+            _refuse("the two outputs must not overlap")
+        _written(out)
     if plan:
         rc = _call(_native.load().sage_cache_read, dev, (
             *cache._args, page_table.data_ptr(), plan[0], plan[1], cu_seqlens.data_ptr(), k.data_ptr(), v.data_ptr(), *plan[2:],
@@ -235,7 +256,7 @@ def _plan_read(cache, page_table, cu_seqlens, total, dtype, out):
     _check_index("cu_seqlens", cu_seqlens, dev, 1)
     if page_table.shape[0] < 1 or page_table.shape[1] < 1 or cu_seqlens.shape[0] != page_table.shape[0] + 1:
         _refuse("page_table and cu_seqlens must describe the same sequences, at least one")
-    if not isinstance(total, int) or total < 0:
+    if total < 0:
         _refuse("total must be an int, not negative")
     strides = [_native.strides2(heads * d, d)] * 2
     if out is not None:
@@ -268,12 +289,21 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
         ancestors and itself.
     sm_scale : default ``head_dim ** -0.5``.
     return_lse : also return the fp32 log-sum-exp ``(tokens, Hq)`` of ``sm_scale * q.k``.
-    out : optional output of q's shape and dtype.
-    A token that sees no key gets zeros and an LSE of -infinity.  The lengths stay on the GPU; the last bits of a
-    result depend on the lengths of the other sequences of the call (fp32 sums in another order).
+    out : optional output of q's shape and dtype, which shares no memory with q.
+    A token that sees no key gets zeros and an LSE of -infinity; one that sees a key whose row of K or V held a NaN or an
+    infinity gets NaN (its LSE: NaN, or for V alone that of the keys' scores).  The lengths stay on the GPU; the last bits
+    of a result depend on the lengths of the other sequences of the call (fp32 sums in another order).  Forward only: the
+    result carries no gradient, as that of `sageattn`.
     """
-    _counters["calls"] += 1
     dev = cache.device
+    if torch.cuda.current_device() != dev.index:     # (its current stream, and whether that is being captured)
+        with torch.cuda.device(dev):
+            return sageattn_cached(q, cache, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tree_mask, sm_scale, return_lse, out)
+    _counters["calls"] += 1
+    if max_seqlen_q is not None:
+        max_seqlen_q = operator.index(max_seqlen_q)
+    if sm_scale is not None:
+        sm_scale = float(sm_scale)
     key = ("attend", _sig(q), _sig(page_table), _sig(seqlens_k), None if cu_seqlens_q is None else _sig(cu_seqlens_q), max_seqlen_q,
            None if tree_mask is None else _sig(tree_mask), sm_scale, None if out is None else _sig(out))
     plan = cache._plans.get(key)
@@ -281,22 +311,31 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
         plan = _remember(cache._plans, key, _plan_attend(cache, q, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tree_mask, sm_scale, out))
     if out is None:
         out = q.new_empty(q.shape)
+    else:
+        if plan and _overlap(q, out):
+            _refuse("out must not overlap q")
+        _written((out,))
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
     if plan:
         ws_bytes, table_stride, width, tree_stride, rest = plan
         stream = _raw_stream(dev.index)
         capturing = torch.cuda.is_current_stream_capturing()
-        st = _state(dev, stream)                     # workspace and host word of the stream, as for `sageattn`
+        st = _state(dev, stream)                     # host word of the stream, as for `sageattn`
         if st.host_word is not None and st.host_word.value:
             st.raise_if_failed("the next call on the stream")
-        if capturing:                                # a captured call has memory of its graph's own: two graphs may run at once
-            ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
-        else:
-            ws = st.ws if st.ws is not None and st.ws.numel() >= ws_bytes else _grow(st, dev, ws_bytes)
-        rc = _call(_native.load().sage_cache_attention, dev, (
-            q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *cache._args, page_table.data_ptr(), table_stride, width,
-            seqlens_k.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(),
-            tree_stride, ws.data_ptr(), ws_bytes, *rest, _report_to(st, capturing), stream))
+        args = (seqlens_k.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(),
+                tree_stride)
+        with st.cache_lock:                          # the call's two kernels share a workspace: another thread's do not come between them
+            if capturing:                            # a captured call has memory of its graph's own: two graphs may run at once
+                ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+            else:
+                ws = st.cache_ws
+                if ws is None or ws.numel() < ws_bytes:
+                    st.cache_ws = None               # release first: the two need not be resident together
+                    ws = st.cache_ws = torch.empty(((ws_bytes + _WS_GRANULE - 1) // _WS_GRANULE * _WS_GRANULE,), dtype=torch.uint8, device=dev)
+            rc = _native.load().sage_cache_attention(
+                q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *cache._args, page_table.data_ptr(), table_stride, width,
+                *args, ws.data_ptr(), ws_bytes, *rest, _report_to(st, capturing), stream)
         if rc:
             _native.check(rc, "sage_cache_attention")
         if _be._STRICT and not capturing:
@@ -317,21 +356,21 @@ def _plan_attend(cache, q, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tr
     if batch < 1 or width < 1 or seqlens_k.shape[0] != batch:
         _refuse("page_table and seqlens_k must describe the same sequences, at least one")
     if cu_seqlens_q is None:
-        if tokens % batch or (max_seqlen_q is not None and int(max_seqlen_q) * batch != tokens):
+        if tokens % batch or (max_seqlen_q is not None and max_seqlen_q * batch != tokens):
             _refuse("without cu_seqlens_q every sequence needs the same number of new tokens")
         max_q = tokens // batch
     else:
         _check_index("cu_seqlens_q", cu_seqlens_q, dev, 1)
         if cu_seqlens_q.shape[0] != batch + 1:
             _refuse("cu_seqlens_q must have batch + 1 entries")
-        if max_seqlen_q is None or int(max_seqlen_q) < 1:
+        if max_seqlen_q is None or max_seqlen_q < 1:
             _refuse("cu_seqlens_q needs max_seqlen_q, at least 1")
-        max_q = min(int(max_seqlen_q), tokens)
+        max_q = min(max_seqlen_q, tokens)
     if tree_mask is not None:
         _check_index("tree_mask", tree_mask, dev, 2, (torch.bool, torch.uint8))
         if tree_mask.shape[0] != tokens or tree_mask.shape[1] < max_q:
             _refuse("tree_mask must be (tokens, >= max_seqlen_q)")
-    scale = d ** -0.5 if sm_scale is None else float(sm_scale)
+    scale = d ** -0.5 if sm_scale is None else sm_scale
     if not (0.0 < scale < float("inf")):
         _refuse("sm_scale must be finite and positive, got %r" % (sm_scale,))
     if out is not None:
@@ -360,6 +399,7 @@ class SageRotary:
     """
 
     __slots__ = ("head_dim", "rotary_dim", "interleaved", "inv_freq", "magnitude", "device", "_plans")
+    __setattr__ = _fixed
 
     def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0, interleaved: bool = False,
                  scaling: str = "none", factor: float = 1.0, original_length: int = 4096, fast: float = 32.0, slow: float = 1.0,
@@ -378,13 +418,14 @@ class SageRotary:
         if scaling == "ntk":
             base = base * factor ** (rot / (rot - 2))
         freq = [base ** (-i / rot) for i in range(0, rot, 2)]
-        self.magnitude = 1.0
+        magnitude = 1.0
         if scaling == "linear":
             freq = [f / factor for f in freq]
         elif scaling == "parts":
             keep = [min(1.0, max(0.0, (original_length * f / (2 * math.pi) - slow) / (fast - slow))) for f in freq]
             freq = [f * (k + (1 - k) / factor) for f, k in zip(freq, keep)]
-            self.magnitude = 0.1 * math.log(factor) + 1.0
+            magnitude = 0.1 * math.log(factor) + 1.0
+        self.magnitude = magnitude
         self.head_dim, self.rotary_dim, self.interleaved = head_dim, rot, bool(interleaved)
         self.inv_freq = torch.tensor(freq, dtype=torch.float64).to(device)
         self.device = self.inv_freq.device
@@ -438,6 +479,7 @@ def _rotate(q, k, positions, rotary, layout, backward, out):
         outs = (q.new_empty(q.shape),) if k is None else (q.new_empty(q.shape), k.new_empty(k.shape))
     else:
         outs = (out,) if isinstance(out, torch.Tensor) else tuple(out)
+        _written(outs)
     if plan:
         k_ptrs = (0, 0) if k is None else (k.data_ptr(), outs[1].data_ptr())
         rc = _call(_native.load().sage_rotary, dev, (

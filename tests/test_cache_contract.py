@@ -193,3 +193,11 @@ def test_shared_elements_of_views():
         seen.add(want)
     assert seen == {True, False}
     assert C._overlap(store[:64].view(8, 8), store[32:96].view(8, 8).T) and not C._overlap(store[:64].view(8, 8), store[64:128].view(4, 16))
+
+
+def test_buffers_and_frequencies_are_fixed():
+    rotary = S.SageRotary(64, device="cpu")
+    for name, value in (("inv_freq", torch.zeros(4, dtype=torch.float64)), ("magnitude", 2.0), ("rotary_dim", 128)):
+        with pytest.raises(AttributeError):
+            setattr(rotary, name, value)
+    assert rotary.magnitude == 1.0 and rotary.rotary_dim == 64

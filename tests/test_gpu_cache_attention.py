@@ -307,3 +307,41 @@ def test_page_of_a_cache_beyond_32_bits():
     # half a code's step of the row's largest / 127, then half a step of fp16 on the value that is read back
     top = k.float().abs().max()
     assert (k16.float() - k.float()).abs().max() <= top / 127 * 0.5 * (1 + 2.0 ** -20) + top * 2.0 ** -11
+
+
+def test_sizes_given_as_tensors_are_read_each_time():
+    cache, table, q, cu, _, _ = _make([40, 33], [4, 4], 8, 2, 64, 16, torch.float16, True)
+    lens, cu = torch.tensor([40, 33], dtype=torch.int32, device="cuda"), torch.tensor(cu, dtype=torch.int32, device="cuda")
+    count = torch.tensor(4)
+    whole = S.sageattn_cached(q, cache, table, lens, cu, count, out=torch.full_like(q, 7.0))
+    count.fill_(2)                                   # cut off behind the second new token of a sequence
+    out = S.sageattn_cached(q, cache, table, lens, cu, count, out=torch.full_like(q, 7.0))
+    assert torch.equal(out, S.sageattn_cached(q, cache, table, lens, cu, 2, out=torch.full_like(q, 7.0)))
+    assert not torch.equal(out, whole)
+
+
+def test_two_threads_on_one_stream():
+    """Calls of both threads are cut into parts that a second kernel joins: neither may join the other's."""
+    import threading
+    cases = []
+    for i in range(4):
+        n = 9000 + 700 * i
+        cache, table, q, _, _, _ = _make([n], [1 + 6 * (i % 2)], 8, 2, 128, 64, torch.float16, True, seed=i)
+        cases.append((q, cache, table, torch.tensor([n], dtype=torch.int32, device="cuda")))
+    call = lambda c: S.sageattn_cached(*c)
+    want = [call(c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(mine):
+        for n in range(150):
+            i = mine[n % len(mine)]
+            out = call(cases[i])
+            if not torch.equal(out, want[i]):
+                wrong.append(i)
+    threads = [threading.Thread(target=work, args=(m,)) for m in ((0, 1), (2, 3), (1, 2))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

@@ -69,3 +69,35 @@ def test_rotary(setup):
                      ((q, k, pos, S.SageRotary(64, device="cpu")), {}), ((q, k, pos[None], rotary), {})):
         with pytest.raises(ValueError):
             S.sage_rotary(*args, **kw)
+
+
+def test_outputs_that_share_memory(setup):
+    cache, x, q, table, lens = setup
+    cu = torch.arange(4, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        S.sageattn_cached(q, cache, table, lens, out=q)
+    both = torch.zeros((6, 4, 64), dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError):
+        S.sageattn_cached(both[:3], cache, table, lens, out=both[2:5])
+    S.sageattn_cached(both[:3], cache, table, lens, out=both[3:])
+    with pytest.raises(ValueError):
+        S.sage_cache_read(cache, table, cu, 3, out=(x, x))
+    fused = torch.zeros((3, 4, 64), dtype=torch.float16, device="cuda")
+    S.sage_cache_read(cache, table, cu, 3, out=(fused[:, :2], fused[:, 2:]))
+
+
+def test_buffers_are_fixed(setup):
+    cache = setup[0]
+    for name in ("k_codes", "v_codes", "k_scale", "v_scale", "k_shift", "num_pages"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name))
+
+
+def test_autograd_learns_of_outputs(setup):
+    cache, _, q, table, lens = setup
+    w = q.clone().requires_grad_()
+    held = q.clone()
+    y = (w * held).sum()                             # keeps `held` for its backward pass
+    S.sage_rotary(held, None, torch.arange(3, device="cuda"), S.SageRotary(64), out=held)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
