@@ -371,7 +371,7 @@ int sage_workspace_layout(int64_t B, int64_t H, int64_t N, size_t offsets[11]);
  * last page: the token is left out (padding).  Slots of one call are distinct; where two tokens name the same
  * one, each half of its row comes from either.  A row that holds a NaN or an infinity is stored with codes 0 and
  * scale NaN: it reads back as NaN throughout, and no code is ever a NaN, so that a key behind a mask reaches
- * nothing. */
+ * nothing.  tokens * Hkv is below 2^31, else SAGE_E_UNSUPPORTED. */
 int sage_cache_write(const void* k, const void* v, const void* slots, int slots_64,
                      void* k_codes, float* k_scale, void* v_codes, float* v_scale, const float* k_shift,
                      int64_t tokens, int64_t Hkv, int64_t head_dim, int64_t pages, int64_t page_size,
@@ -398,10 +398,13 @@ int sage_cache_read(const void* k_codes, const float* k_scale, const void* v_cod
  *   tree_mask   optional (total_q, max_q) bytes, rows tree_stride apart: row t sees new token j of its sequence
  *               where tree_mask[t, j] is not 0, and all keys before the new tokens.  Null: a chain, row t sees
  *               the keys up to its own token's
- * A row that sees no key is 0, its LSE -infinity.  Keys on a page that does not exist are not seen.  Scores and
- * sums in fp32; the weights of V are rounded to fp16.  What a result depends on: the keys are walked in
+ * A row that sees no key is 0, its LSE -infinity.  Keys on a page that does not exist are not seen.  A row that sees a
+ * key whose K or V scale is NaN is NaN (its LSE: NaN, or for V alone that of the scores); rows that do not see it keep
+ * their bits.  out shares no memory with q.  Scores and sums in fp32; the weights of V are rounded to fp16.  What a result depends on: the keys are walked in
  * stretches whose ends follow from the lengths of all sequences, so that the same sequence in another batch
  * may differ in the order of fp32 sums; the same call gives the same bits.
+ * Limits: n_seq * Hkv * (groups of eight of the max_q * Hq / Hkv rows) * (runs of 32 keys of a page table row, and 4)
+ * below 2^31, else SAGE_E_UNSUPPORTED.
  *   workspace   sage_cache_attention_workspace_bytes() bytes, 256-byte aligned; calls that may run at the same
  *               time (on two streams, in two captured graphs) each need their own
  *   status_host optional, as for sage_attention_reported: a pinned host word that receives a non-zero code when a

@@ -22,7 +22,15 @@
 // over the scale, so that one maximum serves both the softmax and fp16's range.
 //
 // NQ = 2 (rows beyond 128): one CTA per SM with all 512 TMEM columns.  NQ = 1: two CTAs per SM.  (Rows are added to a
-// CTA before CTAs are: a tile's codes are fetched and converted once per CTA.)
+// CTA before CTAs are: a tile's codes are fetched and converted once per CTA.  Figures of both: cache_form.)
+//
+// What bounds it.  8 x 16 384 keys x 8 heads, 256 rows: 213 us = 644 TFLOP/s, 0.39 of the rate of a large 16-bit product;
+// a tile of 64 keys takes about 3000 cycles of an SM, and no part of it alone decides: the tensor pipe is busy a third
+// of them, MUFU a third, half of the issue slots are used, and shared memory serves threads in 43 % and the tensor pipe in 39 %.
+// Without the softmax's arithmetic it would be 173 us, without fetching and converting the codes 195, without either's
+// work and one product per tile 108.  Twice the softmax warps (half the keys of a row each), or separate warps for K and V,
+// or separate threads for the two products, or a row's scores spread over four lanes (fewer reads of scales): 211 to 231.
+// 4 x 8771 keys, 84 rows: 36 us for 3.9 us of bytes; the same cycles for tiles that are two thirds full.
 //
 // Every wait is bounded (about two seconds): it then leaves a code in the caller's pinned host word, the CTA drains
 // its products, frees its TMEM and returns.
@@ -152,8 +160,10 @@ template <int WIDTH, int NQ> struct TreeShape {
   static constexpr int REGS_LAUNCH = NQ == 1 ? 80 : 128, REGS_SOFTMAX = NQ == 1 ? 120 : 168, REGS_LOADER = NQ == 1 ? 72 : 112,
                        REGS_ISSUER = NQ == 1 ? 48 : 64;
   static_assert(NQ * REGS_SOFTMAX + REGS_LOADER + REGS_ISSUER <= (NQ + 2) * REGS_LAUNCH, "setmaxnreg would wait forever");
-  // Stages of K and V; slots of scales.  A slot is written once the scores STAGES tiles back are complete, which means that
-  // the softmax is done with the tile two before that.
+  // Stages of K and V as operands, and of codes as they come: a ring of four for NQ = 2 (213 us; codes held in registers a
+  // tile ahead 243), none for NQ = 1, whose two CTAs share the memory: codes come through registers and leave room for two
+  // stages of operands (8 x 16 384 keys, 128 rows: 150 us; with a ring and one stage 181).  Slots of scales: one is written
+  // once the scores STAGES tiles back are complete, which means that the softmax is done with the tile two before that.
   static constexpr int STAGES = 2, SLOTS = 4, RAW_STAGES = NQ == 1 ? 0 : 4;
   static_assert(SLOTS >= STAGES + 2, "");
   static constexpr uint32_t HALVES = WIDTH / 64;
