@@ -458,9 +458,10 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
 
 // Joins the parts of the units that lie in several stretches, in a fixed order.  With all eight warps of a CTA on a row
 // the parts are spread over them (few rows, many parts: a step of one token); with one each (many rows, two or three
-// parts) a warp adds a row's by itself, and takes rows_per_warp of them.  (launch_combine_t chooses)
+// parts) a warp adds a row's by itself, and takes rows_per_warp of them.  A warp has AT_ONCE parts in flight.
+// (launch_combine_t chooses)
 constexpr int CC_WARPS = 8, CC_THREADS = 32 * CC_WARPS;
-template <typename T, int WARPS_PER_ROW>
+template <typename T, int WARPS_PER_ROW, int AT_ONCE>
 __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAttnKArgs a, int rows, int keys, int width, int max_rt, int rows_per_warp, bool permuted) {
   __shared__ unsigned total_s[CC_WARPS], before_s[CC_WARPS];
   __shared__ float acc_s[CC_WARPS][HD];
@@ -501,7 +502,6 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f, top = NO_MAX;
     const bool mine = 4 * lane < width;
-    constexpr int AT_ONCE = 8;
     for (int i0 = c0 + share; i0 <= c1; i0 += WARPS_PER_ROW * AT_ONCE) {
       float2 ml[AT_ONCE];
       float4 v[AT_ONCE];
@@ -595,18 +595,21 @@ template <typename T>
 cudaError_t launch_combine_t(const CacheAttnKArgs& a, int rows, int keys, int width, int max_rt, cudaStream_t st) {
   const unsigned units = (unsigned)((long long)a.n_seq * a.Hkv * max_rt);
   const bool permuted = cache_form((int64_t)a.max_q * a.group).tree;
-  // All of a CTA on a row where all rows find room at once, eight CTAs to an SM (few rows mean many parts each); a row per
-  // warp beyond that, and four where even those have no room: what a CTA does before its first row (it finds the unit's
-  // place in the line, for which it reads every sequence's length) would be most of its time.  With the attention before it:
-  // 2048 units of 4 rows over 300 keys 62.7 us with a CTA per row, 33.7 with a warp; 32 units of 84 rows 36.0 us with one row per warp, 47.5
-  // with four; 296 units of 256 rows 70.1 and 43.9.
+  // All of a CTA on a row while the rows make eight CTAs an SM at most (few rows mean many parts each); a row per warp
+  // beyond that, and four where even those are more: what a CTA does before its first row (it finds the unit's place in the
+  // line, for which it reads every sequence's length) would be most of its time.  With the attention before it: 2048 units
+  // of 4 rows over 300 keys 62.7 us with a CTA per row, 33.7 with a warp; 32 units of 84 rows 36.0 us with one row per
+  // warp, 47.5 with four; 296 units of 256 rows 70.1 and 43.9.  Parts in flight: registers decide how many CTAs are on an SM
+  // (80 with eight, 56 with four): 32 ragged sequences 45.1 us with eight, 43.0 with four; 64 units of 256 rows 214.7
+  // and 210.1; but 32 units of 84 rows, ten parts each, 36.0 and 38.0.
   constexpr unsigned long long ROOM = 8 * SIZING_SMS;
   if (!permuted && (unsigned long long)units * a.part_rows <= ROOM)
-    return launch_after_predecessor(cache_combine_kernel<T, CC_WARPS>, dim3(units, (unsigned)a.part_rows), dim3(CC_THREADS), 0, st, a, rows, keys, width, max_rt,
-                                    1, false);
-  const unsigned ctas = (unsigned)((a.part_rows + CC_WARPS - 1) / CC_WARPS), per_warp = (unsigned long long)units * ctas <= ROOM ? 1 : 4;
-  return launch_after_predecessor(cache_combine_kernel<T, 1>, dim3(units, (ctas + per_warp - 1) / per_warp), dim3(CC_THREADS), 0, st, a, rows, keys, width,
-                                  max_rt, (int)per_warp, permuted);
+    return launch_after_predecessor(cache_combine_kernel<T, CC_WARPS, 4>, dim3(units, (unsigned)a.part_rows), dim3(CC_THREADS), 0, st, a, rows, keys, width,
+                                    max_rt, 1, false);
+  const unsigned ctas = (unsigned)((a.part_rows + CC_WARPS - 1) / CC_WARPS);
+  if ((unsigned long long)units * ctas <= ROOM)
+    return launch_after_predecessor(cache_combine_kernel<T, 1, 8>, dim3(units, ctas), dim3(CC_THREADS), 0, st, a, rows, keys, width, max_rt, 1, permuted);
+  return launch_after_predecessor(cache_combine_kernel<T, 1, 4>, dim3(units, (ctas + 3) / 4), dim3(CC_THREADS), 0, st, a, rows, keys, width, max_rt, 4, permuted);
 }
 
 }  // namespace
