@@ -571,7 +571,8 @@ def sage_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     positions : int32 or int64 on the GPU, ``(tokens,)``, for 4-D tensors also ``(B, N)``; any value (angles are
         worked out in 64 bits).
     backward : the transposed map, which takes the gradient of the outputs to that of the inputs (for a magnitude
-        of 1, the inverse).  Inputs that require gradients get them by it.
+        of 1, the inverse).  Inputs that require gradients get them by it; a backward pass that is captured
+        into a graph is warmed up on the capture stream, with no eager graph of the same leaves left alive.
     out : optional output (for two inputs a pair), each its input itself or memory of its own; not differentiable.
     """
     _counters["calls"] += 1
