@@ -433,6 +433,25 @@ int sage_rotary(const void* q, void* q_out, const void* k, void* k_out, const vo
                 const int64_t q_strides[3], const int64_t qo_strides[3], const int64_t k_strides[3],
                 const int64_t ko_strides[3], const int64_t pos_strides[2], int dtype, void* stream);
 
+/* The four calls above with their arguments in an array of 64-bit words, for hosts whose calls into C cost by the
+ * argument (a step of generation is a handful of calls of a few microseconds): what changes from call to call
+ * first, then what a program keeps.  Pointers and integers as they are, strides word by word, floats as the bits of a
+ * double.  `count` is the number of words; a wrong one, or an unknown `call`, is SAGE_E_ARG.
+ *   SAGE_WORDS_CACHE_WRITE (21)      k v slots stream | slots_64 k_codes k_scale v_codes v_scale k_shift tokens Hkv
+ *       head_dim pages page_size k_strides[2] v_strides[2] dtype qk_mode
+ *   SAGE_WORDS_CACHE_READ (24)       page_table cu_seqlens k_out v_out stream | k_codes k_scale v_codes v_scale k_shift
+ *       page_table_stride page_table_width n_seq total Hkv head_dim pages page_size k_strides[2] v_strides[2] dtype qk_mode
+ *   SAGE_WORDS_CACHE_ATTENTION (34)  q out lse page_table seqlens_k cu_seqlens_q tree_mask workspace workspace_bytes
+ *       status_host stream | k_codes k_scale v_codes v_scale k_shift page_table_stride page_table_width tree_stride n_seq
+ *       Hq Hkv total_q max_q head_dim pages page_size q_strides[2] o_strides[2] dtype qk_mode sm_scale
+ *   SAGE_WORDS_ROTARY (32)           q q_out k k_out positions backward stream | inv_freq positions_64 magnitude B Hq Hk N
+ *       head_dim rotary_dim interleaved q_strides[3] qo_strides[3] k_strides[3] ko_strides[3] pos_strides[2] dtype */
+#define SAGE_WORDS_CACHE_WRITE 0
+#define SAGE_WORDS_CACHE_READ 1
+#define SAGE_WORDS_CACHE_ATTENTION 2
+#define SAGE_WORDS_ROTARY 3
+int sage_call_words(int call, const int64_t* words, int64_t count);
+
 #ifdef __cplusplus
 }
 #endif

@@ -697,4 +697,32 @@ int sage_rotary(const void* q, void* q_out, const void* k, void* k_out, const vo
   return SAGE_OK;
 }
 
+int sage_call_words(int call, const int64_t* words, int64_t count) {
+  const int64_t* w = words;
+  auto ptr = [&](int i) { return reinterpret_cast<void*>(static_cast<uintptr_t>(w[i])); };
+  auto bytes = [&](int i) { return static_cast<uint8_t*>(ptr(i)); };
+  auto f32 = [&](int i) { return static_cast<float*>(ptr(i)); };
+  auto i32 = [&](int i) { return static_cast<int32_t*>(ptr(i)); };
+  auto real = [&](int i) { double d; memcpy(&d, w + i, sizeof d); return static_cast<float>(d); };
+  auto num = [&](int i) { return static_cast<int>(w[i]); };
+  static const int64_t COUNT[4] = {21, 24, 34, 32};
+  if (call < 0 || call > 3 || !words || count != COUNT[call])
+    return fail(SAGE_E_ARG, "sage_call_words: unknown call, or not its number of words (%d, %lld)", call, (long long)count);
+  switch (call) {
+    case SAGE_WORDS_CACHE_WRITE:
+      return sage_cache_write(ptr(0), ptr(1), ptr(2), num(4), bytes(5), f32(6), bytes(7), f32(8), f32(9), w[10], w[11], w[12], w[13], w[14],
+                              w + 15, w + 17, num(19), num(20), ptr(3));
+    case SAGE_WORDS_CACHE_READ:
+      return sage_cache_read(bytes(5), f32(6), bytes(7), f32(8), f32(9), i32(0), w[10], w[11], i32(1), ptr(2), ptr(3), w[12], w[13], w[14], w[15],
+                             w[16], w[17], w + 18, w + 20, num(22), num(23), ptr(4));
+    case SAGE_WORDS_CACHE_ATTENTION:
+      return sage_cache_attention(ptr(0), ptr(1), f32(2), bytes(11), f32(12), bytes(13), f32(14), f32(15), i32(3), w[16], w[17], i32(4), i32(5), ptr(6),
+                                  w[18], ptr(7), static_cast<size_t>(w[8]), w[19], w[20], w[21], w[22], w[23], w[24], w[25], w[26], w + 27, w + 29, num(31),
+                                  num(32), real(33), i32(9), ptr(10));
+    default:
+      return sage_rotary(ptr(0), ptr(1), ptr(2), ptr(3), ptr(4), num(8), static_cast<double*>(ptr(7)), real(9), w[10], w[11], w[12], w[13], w[14], w[15],
+                         num(16), num(5), w + 17, w + 20, w + 23, w + 26, w + 29, num(31), ptr(6));
+  }
+}
+
 }  // extern "C"

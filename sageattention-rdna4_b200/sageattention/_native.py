@@ -84,6 +84,7 @@ SIGNATURES = {
     "sage_cache_attention": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _I64,
                                             _P, ctypes.c_size_t, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64,
                                             _S3, _S3, ctypes.c_int, ctypes.c_int, ctypes.c_float, _P, _P]),
+    "sage_call_words": (ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, _I64]),
     "sage_rotary": (ctypes.c_int, [_P, _P, _P, _P, _P, ctypes.c_int, _P, ctypes.c_float, _I64, _I64, _I64, _I64, _I64, _I64,
                                    ctypes.c_int, ctypes.c_int, _S3, _S3, _S3, _S3, _S3, ctypes.c_int, _P]),
 }

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import math
 import operator
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -39,16 +40,35 @@ def _check_head_dim(d: int):
         _refuse("head_dim must be a multiple of 8 in 8..128, got %d" % d, NotImplementedError)
 
 
-def _call(fn, dev, args):
+# The C calls take their arguments as 64-bit words: those that change from call to call, then those of the plan, kept as bytes
+# (27 arguments that are converted one by one take 6 us, the words one).
+_WRITE, _READ, _ATTEND, _ROTATE = range(4)           # SAGE_WORDS_* in sage_b200.h
+_COUNT = (21, 24, 34, 32)
+_FIRST = tuple(struct.Struct("%dQ" % n).pack for n in (4, 5, 11, 7))
+
+
+def _kept(*words) -> bytes:
+    return struct.pack("".join("d" if isinstance(x, float) else "q" for x in words), *words)
+
+
+def _call(what, dev, words):
     """The C call, on `dev` as the current device."""
     prev = torch.cuda.current_device()
     if prev == dev.index:
-        return fn(*args)
+        return _native.load().sage_call_words(what, words, _COUNT[what])
     torch.cuda.set_device(dev)
     try:
-        return fn(*args)
+        return _native.load().sage_call_words(what, words, _COUNT[what])
     finally:
         torch.cuda.set_device(prev)
+
+
+_PACKED = torch.contiguous_format
+
+
+def _like(shape, dtype, dev):
+    """A tensor of one element in that shape, for `empty_like`, which is twice as fast as `empty`."""
+    return torch.empty((1,) * len(shape), dtype=dtype, device=dev).expand(shape)
 
 
 # A step of generation is a handful of calls whose GPU work takes a few microseconds each, so that the host path must
@@ -194,8 +214,7 @@ def sage_cache_write(cache: SageCache, k: torch.Tensor, v: torch.Tensor, slots: 
         plan = _remember(cache._plans, key, _plan_write(cache, k, v, slots))
     if plan:
         dev = cache.device
-        rc = _call(_native.load().sage_cache_write, dev, (
-            k.data_ptr(), v.data_ptr(), slots.data_ptr(), plan[0], *cache._args, *plan[1:], _raw_stream(dev.index)))
+        rc = _call(_WRITE, dev, _FIRST[_WRITE](k.data_ptr(), v.data_ptr(), slots.data_ptr(), _raw_stream(dev.index)) + plan)
         if rc:
             _native.check(rc, "sage_cache_write")
 
@@ -210,9 +229,9 @@ def _plan_write(cache, k, v, slots):
     if slots.shape[0] != k.shape[0]:
         _refuse("slots must hold one entry per token")
     if k.shape[0] == 0:
-        return ()
-    return (slots.dtype == torch.int64, k.shape[0], heads, d, *cache._sizes, _native.strides2(k.stride(0), k.stride(1)),
-            _native.strides2(v.stride(0), v.stride(1)), _dtype_code(k.dtype), cache._mode)
+        return b""
+    return _kept(slots.dtype == torch.int64, *cache._args, k.shape[0], heads, d, *cache._sizes, k.stride(0), k.stride(1), v.stride(0),
+                 v.stride(1), _dtype_code(k.dtype), cache._mode)
 
 
 def sage_cache_read(cache: SageCache, page_table: torch.Tensor, cu_seqlens: torch.Tensor, total: int,
@@ -225,25 +244,23 @@ def sage_cache_read(cache: SageCache, page_table: torch.Tensor, cu_seqlens: torc
     (in fresh outputs: undefined); tokens on a page that does not exist read as zeros.
     """
     _counters["calls"] += 1
-    dev, heads, d = cache.device, cache.num_kv_heads, cache.head_dim
+    dev = cache.device
     if total.__class__ is not int:
         _refuse("total must be an int, not negative")
     key = ("read", _sig(page_table), _sig(cu_seqlens), total, dtype, None if out is None else tuple(_sig(t) for t in out))
     plan = cache._plans.get(key)
     if plan is None:
         plan = _remember(cache._plans, key, _plan_read(cache, page_table, cu_seqlens, total, dtype, out))
+    words, like = plan
     if out is None:
-        k = torch.empty((total, heads, d), dtype=dtype, device=dev)
-        v = torch.empty((total, heads, d), dtype=dtype, device=dev)
+        k, v = torch.empty_like(like, memory_format=_PACKED), torch.empty_like(like, memory_format=_PACKED)
     else:
         k, v = out
-        if plan and _overlap(k, v):
+        if words and _overlap(k, v):
             _refuse("the two outputs must not overlap")
         _written(out)
-    if plan:
-        rc = _call(_native.load().sage_cache_read, dev, (
-            *cache._args, page_table.data_ptr(), plan[0], plan[1], cu_seqlens.data_ptr(), k.data_ptr(), v.data_ptr(), *plan[2:],
-            _raw_stream(dev.index)))
+    if words:
+        rc = _call(_READ, dev, _FIRST[_READ](page_table.data_ptr(), cu_seqlens.data_ptr(), k.data_ptr(), v.data_ptr(), _raw_stream(dev.index)) + words)
         if rc:
             _native.check(rc, "sage_cache_read")
     return k, v
@@ -258,7 +275,7 @@ def _plan_read(cache, page_table, cu_seqlens, total, dtype, out):
         _refuse("page_table and cu_seqlens must describe the same sequences, at least one")
     if total < 0:
         _refuse("total must be an int, not negative")
-    strides = [_native.strides2(heads * d, d)] * 2
+    strides = (heads * d, d) * 2
     if out is not None:
         if len(out) != 2:
             _refuse("out must be a pair")
@@ -266,10 +283,12 @@ def _plan_read(cache, page_table, cu_seqlens, total, dtype, out):
             _check_rows(name, t, heads, d, dev)
             if t.shape[0] != total or t.dtype != dtype:
                 _refuse("%s must hold total rows of dtype" % name)
-        strides = [_native.strides2(t.stride(0), t.stride(1)) for t in out]
+        strides = [n for t in out for n in t.stride()[:2]]
+    like = _like((total, heads, d), dtype, dev)
     if total == 0:
-        return ()
-    return (page_table.stride(0), page_table.shape[1], page_table.shape[0], total, heads, d, *cache._sizes, *strides, code, cache._mode)
+        return b"", like
+    return _kept(*cache._args, page_table.stride(0), page_table.shape[1], page_table.shape[0], total, heads, d, *cache._sizes, *strides, code,
+                 cache._mode), like
 
 
 def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor, seqlens_k: torch.Tensor,
@@ -309,22 +328,20 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
     plan = cache._plans.get(key)
     if plan is None:
         plan = _remember(cache._plans, key, _plan_attend(cache, q, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tree_mask, sm_scale, out))
+    words, ws_bytes, like_lse = plan
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=_PACKED)
     else:
-        if plan and _overlap(q, out):
+        if words and _overlap(q, out):
             _refuse("out must not overlap q")
         _written((out,))
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
-    if plan:
-        ws_bytes, table_stride, width, tree_stride, rest = plan
+    lse = torch.empty_like(like_lse, memory_format=_PACKED) if return_lse else None
+    if words:
         stream = _raw_stream(dev.index)
         capturing = torch.cuda.is_current_stream_capturing()
         st = _state(dev, stream)                     # host word of the stream, as for `sageattn`
         if st.host_word is not None and st.host_word.value:
             st.raise_if_failed("the next call on the stream")
-        args = (seqlens_k.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(),
-                tree_stride)
         with st.cache_lock:                          # the call's two kernels share a workspace: another thread's do not come between them
             if capturing:                            # a captured call has memory of its graph's own: two graphs may run at once
                 ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
@@ -333,9 +350,10 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
                 if ws is None or ws.numel() < ws_bytes:
                     st.cache_ws = None               # release first: the two need not be resident together
                     ws = st.cache_ws = torch.empty(((ws_bytes + _WS_GRANULE - 1) // _WS_GRANULE * _WS_GRANULE,), dtype=torch.uint8, device=dev)
-            rc = _native.load().sage_cache_attention(
-                q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *cache._args, page_table.data_ptr(), table_stride, width,
-                *args, ws.data_ptr(), ws_bytes, *rest, _report_to(st, capturing), stream)
+            rc = _native.load().sage_call_words(_ATTEND, _FIRST[_ATTEND](
+                q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), page_table.data_ptr(), seqlens_k.data_ptr(),
+                0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), 0 if tree_mask is None else tree_mask.data_ptr(), ws.data_ptr(), ws_bytes,
+                _report_to(st, capturing), stream) + words, _COUNT[_ATTEND])
         if rc:
             _native.check(rc, "sage_cache_attention")
         if _be._STRICT and not capturing:
@@ -377,12 +395,12 @@ def _plan_attend(cache, q, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tr
         _check_rows("out", out, hq, d, dev)
         if out.shape != q.shape or out.dtype != q.dtype:
             _refuse("out must have q's shape and dtype")
+    like_lse = _like((tokens, hq), torch.float32, dev)
     if tokens == 0:
-        return ()
-    o2 = _native.strides2(hq * d, d) if out is None else _native.strides2(out.stride(0), out.stride(1))
-    rest = (batch, hq, hkv, tokens, max_q, d, *cache._sizes, _native.strides2(q.stride(0), q.stride(1)), o2, _dtype_code(q.dtype), cache._mode, scale)
-    return (int(_native.load().sage_cache_attention_workspace_bytes(batch, hq, hkv, max_q)), page_table.stride(0), width,
-            0 if tree_mask is None else tree_mask.stride(0), rest)
+        return b"", 0, like_lse
+    words = _kept(*cache._args, page_table.stride(0), width, 0 if tree_mask is None else tree_mask.stride(0), batch, hq, hkv, tokens, max_q, d,
+                  *cache._sizes, q.stride(0), q.stride(1), *((hq * d, d) if out is None else out.stride()[:2]), _dtype_code(q.dtype), cache._mode, scale)
+    return words, int(_native.load().sage_cache_attention_workspace_bytes(batch, hq, hkv, max_q)), like_lse
 
 
 # ---- rotary positions --------------------------------------------------------------------------------------------
@@ -476,15 +494,15 @@ def _rotate(q, k, positions, rotary, layout, backward, out):
             _remember(rotary._plans, key, plan)
     dev = rotary.device
     if out is None:
-        outs = (q.new_empty(q.shape),) if k is None else (q.new_empty(q.shape), k.new_empty(k.shape))
+        outs = (torch.empty_like(q, memory_format=_PACKED),) if k is None else \
+            (torch.empty_like(q, memory_format=_PACKED), torch.empty_like(k, memory_format=_PACKED))
     else:
         outs = (out,) if isinstance(out, torch.Tensor) else tuple(out)
         _written(outs)
     if plan:
-        k_ptrs = (0, 0) if k is None else (k.data_ptr(), outs[1].data_ptr())
-        rc = _call(_native.load().sage_rotary, dev, (
-            q.data_ptr(), outs[0].data_ptr(), *k_ptrs, positions.data_ptr(), positions.dtype == torch.int64, rotary.inv_freq.data_ptr(),
-            rotary.magnitude, *plan[0], rotary.rotary_dim, rotary.interleaved, backward, *plan[1], _raw_stream(dev.index)))
+        rc = _call(_ROTATE, dev, _FIRST[_ROTATE](
+            q.data_ptr(), outs[0].data_ptr(), 0 if k is None else k.data_ptr(), 0 if k is None else outs[1].data_ptr(), positions.data_ptr(),
+            backward, _raw_stream(dev.index)) + plan)
         if rc:
             _native.check(rc, "sage_rotary")
     return outs
@@ -529,18 +547,19 @@ def _plan_rotary(q, k, positions, rotary, layout, out):
     else:
         _refuse("positions must be (N,) or (B, N)")
     if not b * n:
-        return ()
+        return b""
 
     def triple(v):
-        return _native.strides3(v.stride(0), v.stride(1), v.stride(2))
+        return v.stride()[:3]
 
     def fresh(v):                                    # of a contiguous tensor in the inputs' layout
         h = v.shape[1]
-        return _native.strides3(n * h * d, d, h * d) if q.dim() == 3 or layout == "NHD" else _native.strides3(h * n * d, n * d, d)
+        return (n * h * d, d, h * d) if q.dim() == 3 or layout == "NHD" else (h * n * d, n * d, d)
     s3 = []
     for i in (0, len(ins) - 1):
-        s3 += [triple(views[i]), triple(o_views[i]) if o_views else fresh(views[i])]
-    return ((b, views[0].shape[1], views[1].shape[1] if k is not None else 0, n, d), (*s3, _native.strides2(*p2), _dtype_code(q.dtype)))
+        s3 += [*triple(views[i]), *(triple(o_views[i]) if o_views else fresh(views[i]))]
+    return _kept(rotary.inv_freq.data_ptr(), positions.dtype == torch.int64, rotary.magnitude, b, views[0].shape[1],
+                 views[1].shape[1] if k is not None else 0, n, d, rotary.rotary_dim, rotary.interleaved, *s3, *p2, _dtype_code(q.dtype))
 
 
 class _Rotary(torch.autograd.Function):

@@ -201,3 +201,45 @@ def test_buffers_and_frequencies_are_fixed():
         with pytest.raises(AttributeError):
             setattr(rotary, name, value)
     assert rotary.magnitude == 1.0 and rotary.rotary_dim == 64
+
+
+def test_calls_in_words():
+    """Argument by argument, the words reach the same checks."""
+    import struct
+    lib = _native.load()
+    code = (ctypes.addressof(buf) + 255) // 256 * 256
+    two = (1024, 128)
+    write = [code] * 3 + [0] + [1] + [code] * 5 + [4, 8, 128, 4, 64, *two, *two, 0, 0]
+    read = [code] * 4 + [0] + [code] * 5 + [4, 4, 1, 4, 8, 128, 4, 64, *two, *two, 0, 0]
+    attend = [code] * 8 + [1 << 40, 0, 0] + [code] * 5 + [4, 4, 4, 1, 8, 8, 4, 4, 128, 4, 64, *two, *two, 0, 0, 0.1]
+    rotary = [code] * 5 + [0, 0] + [code, 1, 1.0, 1, 8, 8, 4, 128, 128, 0] + [8192, 1024, 128] * 4 + [0, 1, 0]
+
+    def call(what, words, change=(), count=None):
+        words = list(words)
+        for i, x in change:
+            words[i] = x
+        data = struct.pack("".join("d" if isinstance(x, float) else "q" for x in words), *words)
+        return lib.sage_call_words(what, data, len(words) if count is None else count)
+
+    for what, words in enumerate((write, read, attend, rotary)):
+        assert len(words) == C._COUNT[what]
+        _refused(call(what, words[:-1]), ARG, "words")
+        _refused(call(what, words + [0]), ARG, "words")
+        _refused(call(what, words, [(0, code + 2)]), ARG, "aligned")
+    _refused(call(4, write), ARG, "words")
+    _refused(call(-1, write), ARG, "words")
+    _refused(lib.sage_call_words(0, None, 21), ARG, "words")
+    for at, value, rc, word in ((12, 136, UNSUPPORTED, "head_dim"), (13, 0, ARG, "pages"), (14, 24, UNSUPPORTED, "page_size"), (19, 2, ARG, "dtype"),
+                                (20, 2, ARG, "qk_mode"), (15, 4, ARG, "stride"), (18, 4, ARG, "stride"), (10, -1, ARG, "token")):
+        _refused(call(0, write, [(at, value)]), rc, word)
+    for at, value, rc, word in ((15, 136, UNSUPPORTED, "head_dim"), (16, 0, ARG, "pages"), (17, 24, UNSUPPORTED, "page_size"), (22, 2, ARG, "dtype"),
+                                (23, 2, ARG, "qk_mode"), (18, 4, ARG, "stride"), (21, 4, ARG, "stride"), (13, -1, ARG, "row"), (11, 0, ARG, "table")):
+        _refused(call(1, read, [(at, value)]), rc, word)
+    for at, value, rc, word in ((24, 136, UNSUPPORTED, "head_dim"), (25, 0, ARG, "pages"), (26, 24, UNSUPPORTED, "page_size"), (31, 2, ARG, "dtype"),
+                                (32, 2, ARG, "qk_mode"), (27, 4, ARG, "stride"), (30, 4, ARG, "stride"), (22, -1, ARG, "token"), (17, 0, ARG, "table"),
+                                (33, -1.0, ARG, "sm_scale"), (8, 16, WORKSPACE, "workspace"), (18, -1, ARG, "tree"), (20, 9, ARG, "heads"),
+                                (23, 5, ARG, "max_q"), (9, code + 2, ARG, "status_host"), (4, 0, ARG, "null")):
+        _refused(call(2, attend, [(at, value)]), rc, word)
+    for at, value, rc, word in ((14, 136, UNSUPPORTED, "head_dim"), (15, 4, UNSUPPORTED, "rotary_dim"), (31, 2, ARG, "dtype"), (17, 4, ARG, "stride"),
+                                (28, 4, ARG, "stride"), (29, -1, ARG, "position"), (10, -1, ARG, "sizes"), (7, code + 4, ARG, "misaligned")):
+        _refused(call(3, rotary, [(at, value)]), rc, word)
