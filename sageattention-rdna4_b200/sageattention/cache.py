@@ -66,6 +66,11 @@ def _call(what, dev, words):
 _PACKED = torch.contiguous_format
 
 
+def _fresh(t):
+    """Packed memory for an output like t."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=_PACKED)
+
+
 def _like(shape, dtype, dev):
     """A tensor of one element in that shape, for `empty_like`, which is twice as fast as `empty`."""
     return torch.empty((1,) * len(shape), dtype=dtype, device=dev).expand(shape)
@@ -330,7 +335,7 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
         plan = _remember(cache._plans, key, _plan_attend(cache, q, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tree_mask, sm_scale, out))
     words, ws_bytes, like_lse = plan
     if out is None:
-        out = torch.empty_like(q, memory_format=_PACKED)
+        out = _fresh(q)
     else:
         if words and _overlap(q, out):
             _refuse("out must not overlap q")
@@ -494,8 +499,7 @@ def _rotate(q, k, positions, rotary, layout, backward, out):
             _remember(rotary._plans, key, plan)
     dev = rotary.device
     if out is None:
-        outs = (torch.empty_like(q, memory_format=_PACKED),) if k is None else \
-            (torch.empty_like(q, memory_format=_PACKED), torch.empty_like(k, memory_format=_PACKED))
+        outs = (_fresh(q),) if k is None else (_fresh(q), _fresh(k))
     else:
         outs = (out,) if isinstance(out, torch.Tensor) else tuple(out)
         _written(outs)
@@ -552,12 +556,12 @@ def _plan_rotary(q, k, positions, rotary, layout, out):
     def triple(v):
         return v.stride()[:3]
 
-    def fresh(v):                                    # of a contiguous tensor in the inputs' layout
+    def packed(v):                                   # strides of a contiguous tensor in the inputs' layout
         h = v.shape[1]
         return (n * h * d, d, h * d) if q.dim() == 3 or layout == "NHD" else (h * n * d, n * d, d)
     s3 = []
     for i in (0, len(ins) - 1):
-        s3 += [*triple(views[i]), *(triple(o_views[i]) if o_views else fresh(views[i]))]
+        s3 += [*triple(views[i]), *(triple(o_views[i]) if o_views else packed(views[i]))]
     return _kept(rotary.inv_freq.data_ptr(), positions.dtype == torch.int64, rotary.magnitude, b, views[0].shape[1],
                  views[1].shape[1] if k is not None else 0, n, d, rotary.rotary_dim, rotary.interleaved, *s3, *p2, _dtype_code(q.dtype))
 
