@@ -24,10 +24,10 @@
 // NQ = 2 (rows beyond 128): one CTA per SM with all 512 TMEM columns.  NQ = 1: two CTAs per SM.  (Rows are added to a
 // CTA before CTAs are: a tile's codes are fetched and converted once per CTA.  Figures of both: cache_form.)
 //
-// What bounds it.  8 x 16 384 keys x 8 heads, 256 rows: 213 us = 644 TFLOP/s, 0.39 of the rate of a large 16-bit product;
+// What bounds it.  8 x 16 384 keys x 8 heads, 256 rows: 208 us = 660 TFLOP/s, 0.40 of the rate of a large 16-bit product;
 // a tile of 64 keys takes about 3000 cycles of an SM, and no part of it alone decides: the tensor pipe is busy a third
 // of them, MUFU a third, half of the issue slots are used, and shared memory serves threads in 43 % and the tensor pipe in 39 %.
-// Without the softmax's arithmetic it would be 173 us, without fetching and converting the codes 195, without either's
+// Without the softmax's arithmetic it would have been 173 us of 213, without fetching and converting the codes 195, without either's
 // work and one product per tile 108.  Twice the softmax warps (half the keys of a row each), or separate warps for K and V,
 // or separate threads for the two products, or a row's scores spread over four lanes (fewer reads of scales): 211 to 231.
 // 4 x 8771 keys, 84 rows: 36 us for 3.9 us of bytes; the same cycles for tiles that are two thirds full.
@@ -83,13 +83,18 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+// Descriptors of operands in shared memory have the same upper word throughout (rows of 128 bytes, swizzled, eight of
+// them 1024 bytes apart); of the lower one the address moves, by constants within a tile.
+constexpr uint32_t DESC_HIGH = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_desc, uint32_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+               ::"r"(d), "r"(a_desc), "r"(b_desc), "r"(idesc), "r"(accumulate), "n"(DESC_HIGH) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-               ::"r"(d), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+               ::"r"(d), "r"(a_tmem), "r"(b_desc), "r"(idesc), "r"(accumulate), "n"(DESC_HIGH) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
   asm volatile(
@@ -123,12 +128,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // Descriptors of 128-byte rows in the 128-byte swizzle, 8-row groups 1024 bytes apart: as a K-major operand, and as
 // an MN-major one whose next 64 columns lie `lead` bytes further.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t lead) {
-  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr & 0x3FFFFu) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr, uint32_t lead) { return ((addr & 0x3FFFFu) >> 4) | ((lead >> 4) << 16); }
 
 // 16 codes -> 16 fp16 in eight registers, exact.
 template <bool INT8>
@@ -690,10 +691,10 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         const int st = n % L::STAGES;
         if (!mbar_wait(bar(L::B_KF + st), (uint32_t)(n / L::STAGES) & 1u, watch, CODE_MMA)) return false;
         tc_fence_after();
+        const uint32_t q_at = desc_k(base + L::OFF_Q + g * L::Q_TILE), k_at = desc_k(base + L::OFF_K + st * L::KV_TILE);
 #pragma unroll
         for (int i = 0; i < WIDTH / 16; ++i)
-          mma_ss(tmem_s(g, to), desc_k(base + L::OFF_Q + g * L::Q_TILE + (i >> 2) * L::Q_HALF + 32 * (i & 3)),
-                 desc_k(base + L::OFF_K + st * L::KV_TILE + (i >> 2) * L::KV_HALF + 32 * (i & 3)), IDESC_QK, i > 0);
+          mma_ss(tmem_s(g, to), q_at + (((i >> 2) * L::Q_HALF + 32 * (i & 3)) >> 4), k_at + (((i >> 2) * L::KV_HALF + 32 * (i & 3)) >> 4), IDESC_QK, i > 0);
         tc_commit(bar(L::B_SF + 2 * g + to));
         tc_commit(bar(L::B_KE + st));
         ++n;
@@ -713,9 +714,10 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
                  mbar_wait(bar(L::B_PF + 2 * g + (k & 1)), (uint32_t)(k >> 1) & 1u, watch, CODE_MMA);
             if (!ok) break;
             tc_fence_after();
+            const uint32_t v_at = desc_mn(base + L::OFF_V + st * L::KV_TILE, L::KV_HALF);
 #pragma unroll
             for (int i = 0; i < KT / 16; ++i)
-              mma_ts(tmem_o(g), tmem_s(g, k & 1) + 8 * i, desc_mn(base + L::OFF_V + st * L::KV_TILE + 2048 * i, L::KV_HALF), IDESC_PV, t > 0 || i > 0);
+              mma_ts(tmem_o(g), tmem_s(g, k & 1) + 8 * i, v_at + (2048 * i >> 4), IDESC_PV, t > 0 || i > 0);
             tc_commit(bar(L::B_PV + 2 * g + (k & 1)));
             tc_commit(bar(L::B_VE + st));
           }
