@@ -433,3 +433,31 @@ def test_views_and_rows_behind_at_any_number_of_rows(t):
 def test_many_sequences_of_many_rows(batch, t):
     lens = [(37 * i) % 90 + (t if i % 5 else 0) for i in range(batch)]
     _check(lens, [t if i % 4 else max(1, t // 2) for i in range(batch)], 16, 4, 64, 16, torch.float16, True, tree=t % 2 == 0)
+
+
+def test_first_call_of_a_signature_is_captured_and_replayed():
+    """Nothing of a call needs an earlier eager one; replays read what the tensors hold by then."""
+    cache, table, q, cu, _, gen = _make([300, 77], [2, 2], 8, 2, 128, 16, torch.float16, True)
+    lens = torch.tensor([300, 77], dtype=torch.int32).cuda()
+    rotary = S.SageRotary(128)
+    pos = torch.tensor([298, 299, 75, 76]).cuda()
+    k, v = (torch.randn((4, 2, 128), generator=gen).half().cuda() for _ in range(2))
+    slots = torch.tensor([int(table[i, n // 16]) * 16 + n % 16 for i, n in ((0, 298), (0, 299), (1, 75), (1, 76))]).cuda()
+    cu_k = torch.tensor([0, 300, 377], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        qr, kr = S.sage_rotary(q, k, pos, rotary)
+        S.sage_cache_write(cache, kr, v, slots)
+        out, lse = S.sageattn_cached(qr, cache, table, lens, return_lse=True)
+        back = S.sage_cache_read(cache, table, cu_k, 377)
+    for _ in range(2):
+        q.copy_(torch.randn(q.shape, generator=gen)); k.copy_(torch.randn(k.shape, generator=gen)); v.copy_(torch.randn(v.shape, generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        qe, ke = S.sage_rotary(q, k, pos, rotary)
+        S.sage_cache_write(cache, ke, v, slots)
+        want, want_lse = S.sageattn_cached(qe, cache, table, lens, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        whole = S.sage_cache_read(cache, table, cu_k, 377)
+        assert torch.equal(back[0], whole[0]) and torch.equal(back[1], whole[1])

@@ -101,3 +101,13 @@ def test_autograd_learns_of_outputs(setup):
     S.sage_rotary(held, None, torch.arange(3, device="cuda"), S.SageRotary(64), out=held)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_nothing_to_do(setup):
+    cache, x, q, table, lens = setup
+    k, v = S.sage_cache_read(cache, table, torch.zeros(4, dtype=torch.int32, device="cuda"), 0)
+    assert k.shape == v.shape == (0, 2, 64) and k.dtype == torch.float16
+    out, lse = S.sageattn_cached(q[:0], cache, table, lens, return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4) and lse.dtype == torch.float32
+    S.sage_cache_write(cache, x[:0], x[:0], torch.zeros(0, dtype=torch.int64, device="cuda"))
+    assert S.sage_rotary(q[:0], None, torch.zeros(0, dtype=torch.int64, device="cuda"), S.SageRotary(64)).shape == (0, 4, 64)
