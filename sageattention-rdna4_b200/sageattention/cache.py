@@ -165,6 +165,10 @@ class SageCache:
         self._sizes = (pages, page)
         self._plans = {}                             # call signature -> what the C call is given for it
 
+    def __reduce__(self):                            # a copy has buffers, and addresses, of its own
+        shift = None if self.k_shift is None else self.k_shift[:, :self.head_dim]
+        return type(self), (self.k_codes, self.k_scale, self.v_codes, self.v_scale, self.head_dim, shift)
+
     @classmethod
     def empty(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16,
               int8: Optional[bool] = None, device="cuda", k_shift: Optional[torch.Tensor] = None) -> "SageCache":
@@ -448,11 +452,21 @@ class SageRotary:
             keep = [min(1.0, max(0.0, (original_length * f / (2 * math.pi) - slow) / (fast - slow))) for f in freq]
             freq = [f * (k + (1 - k) / factor) for f, k in zip(freq, keep)]
             magnitude = 0.1 * math.log(factor) + 1.0
-        self.magnitude = magnitude
-        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rot, bool(interleaved)
-        self.inv_freq = torch.tensor(freq, dtype=torch.float64).to(device)
-        self.device = self.inv_freq.device
+        self._set(head_dim, rot, bool(interleaved), torch.tensor(freq, dtype=torch.float64).to(device), magnitude)
+
+    def _set(self, head_dim, rotary_dim, interleaved, inv_freq, magnitude):
+        self.head_dim, self.rotary_dim, self.interleaved, self.inv_freq, self.magnitude = head_dim, rotary_dim, interleaved, inv_freq, magnitude
+        self.device = inv_freq.device
         self._plans = {}
+
+    def __reduce__(self):                            # a copy has frequencies, and their address, of its own
+        return _rotary_of, (self.head_dim, self.rotary_dim, self.interleaved, self.inv_freq, self.magnitude)
+
+
+def _rotary_of(*parts):
+    rotary = object.__new__(SageRotary)
+    rotary._set(*parts)
+    return rotary
 
 
 def _rotary_views(x, layout):

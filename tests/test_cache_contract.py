@@ -243,3 +243,14 @@ def test_calls_in_words():
     for at, value, rc, word in ((14, 136, UNSUPPORTED, "head_dim"), (15, 4, UNSUPPORTED, "rotary_dim"), (31, 2, ARG, "dtype"), (17, 4, ARG, "stride"),
                                 (28, 4, ARG, "stride"), (29, -1, ARG, "position"), (10, -1, ARG, "sizes"), (7, code + 4, ARG, "misaligned")):
         _refused(call(3, rotary, [(at, value)]), rc, word)
+
+
+def test_copies_have_frequencies_of_their_own():
+    import copy
+    import pickle
+    rotary = S.SageRotary(96, rotary_dim=64, interleaved=True, scaling="parts", factor=4.0, device="cpu")
+    rotary._plans["call"] = b"addresses"
+    for twin in (copy.deepcopy(rotary), pickle.loads(pickle.dumps(rotary)), copy.copy(rotary)):
+        assert not twin._plans and twin.inv_freq.device == rotary.inv_freq.device and torch.equal(twin.inv_freq, rotary.inv_freq)
+        assert (twin.head_dim, twin.rotary_dim, twin.interleaved, twin.magnitude) == (96, 64, True, rotary.magnitude)
+    assert copy.deepcopy(rotary).inv_freq.data_ptr() != rotary.inv_freq.data_ptr()

@@ -461,3 +461,20 @@ def test_first_call_of_a_signature_is_captured_and_replayed():
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
         whole = S.sage_cache_read(cache, table, cu_k, 377)
         assert torch.equal(back[0], whole[0]) and torch.equal(back[1], whole[1])
+
+
+def test_a_copy_of_a_cache_is_its_own():
+    import copy
+    cache, table, q, _, _, gen = _make([90], [1], 8, 2, 72, 16, torch.float16, True, shift=True)
+    lens = torch.tensor([90], dtype=torch.int32).cuda()
+    rotary, pos = S.SageRotary(72), torch.tensor([89]).cuda()
+    want, turned = S.sageattn_cached(q, cache, table, lens), S.sage_rotary(q, None, pos, rotary)
+    twin, turn = copy.deepcopy(cache), copy.deepcopy(rotary)
+    assert torch.equal(twin.k_shift, cache.k_shift) and torch.equal(S.sageattn_cached(q, twin, table, lens), want)
+    x = torch.randn((90, 2, 72), generator=gen).half().cuda()
+    at = torch.arange(90).cuda()
+    S.sage_cache_write(twin, x, x, table[0, at // 16].long() * 16 + at % 16)
+    assert not torch.equal(S.sageattn_cached(q, twin, table, lens), want)
+    assert torch.equal(S.sageattn_cached(q, cache, table, lens), want)
+    rotary.inv_freq.zero_()
+    assert torch.equal(S.sage_rotary(q, None, pos, turn), turned) and torch.equal(S.sage_rotary(q, None, pos, rotary), q)
