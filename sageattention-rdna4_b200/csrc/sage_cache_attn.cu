@@ -30,10 +30,10 @@
 // that lies in several stretches leaves partial rows in the workspace, which cache_combine_kernel joins in the
 // order of the keys.
 //
-// What bounds it.  The cache's bytes: 4 x 47 520 keys x 48 heads, 365 us = 6.6 TB/s, the rate of a plain copy.  32 ragged
-// sequences of up to 8192 keys x 8 heads: 45 us = 4.4 TB/s; joining the parts, the launches and the two to three units
-// that a warp begins take the difference.  One sequence of 16 384 keys: 15.5 us, of which 6 are the cache's bytes and the
-// rest the chain launch, lengths, pages, codes, parts, join.  16 rows instead of 8 cost instructions (codes are unpacked
+// What bounds it.  The cache's bytes: 4 x 47 520 keys x 48 heads, 356 to 370 us = 6.6 TB/s, the rate of a plain copy.  32
+// ragged sequences of up to 8192 keys x 8 heads: 43 us = 4.5 TB/s; joining the parts, the launches and the two to three
+// units that a warp begins take the difference.  One sequence of 16 384 keys: 15 us, of which 6 are the cache's bytes and
+// the rest the chain launch, lengths, pages, codes, parts, join.  16 rows instead of 8 cost instructions (codes are unpacked
 // once for all rows of a tile): 8 x 16 384 keys x 8 heads 56 us with 8 rows, 63 with 16.
 #include "sage_cache_attn.cuh"
 
