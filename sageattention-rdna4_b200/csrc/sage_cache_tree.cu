@@ -24,7 +24,7 @@
 // NQ = 2 (rows beyond 128): one CTA per SM with all 512 TMEM columns.  NQ = 1: two CTAs per SM.  (Rows are added to a
 // CTA before CTAs are: a tile's codes are fetched and converted once per CTA.  Figures of both: cache_form.)
 //
-// What bounds it.  8 x 16 384 keys x 8 heads, 256 rows: 208 us = 660 TFLOP/s, 0.40 of the rate of a large 16-bit product;
+// What bounds it.  8 x 16 384 keys x 8 heads, 256 rows: 206 us = 665 TFLOP/s, 0.40 of the rate of a large 16-bit product;
 // a tile of 64 keys takes about 3000 cycles of an SM, and no part of it alone decides: the tensor pipe is busy a third
 // of them, MUFU a third, half of the issue slots are used, and shared memory serves threads in 43 % and the tensor pipe in 39 %.
 // Without the softmax's arithmetic it would have been 173 us of 213, without fetching and converting the codes 195, without either's
@@ -32,7 +32,7 @@
 // or separate threads for the two products, or a row's scores spread over four lanes (fewer reads of scales): 211 to 231.
 // 4 x 8771 keys, 84 rows: 36 us for 3.9 us of bytes; the same cycles for tiles that are two thirds full.
 //
-// Every wait is bounded (about two seconds): it then leaves a code in the caller's pinned host word, the CTA drains
+// Every wait is bounded (about a second): it then leaves a code in the caller's pinned host word, the CTA drains
 // its products, frees its TMEM and returns.
 #include "sage_cache_attn.cuh"
 
@@ -46,34 +46,35 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-constexpr long long WAIT_CYCLES = 4000000000LL;      // about two seconds of SM clock
+constexpr uint32_t WAIT_CYCLES = 2000000000u;        // about a second of SM clock
 struct Watch {
   volatile uint32_t* abort;                          // in shared memory: someone of this CTA gave up
   int32_t* host;                                     // optional pinned word
 };
-__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, const Watch& w, int code) {
-  const long long t0 = clock64();
-  for (uint32_t it = 1;; ++it) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    if (ok) return true;
-    if ((it & 255u) == 0u) {
-      if (*w.abort) return false;
-      if (clock64() - t0 > WAIT_CYCLES) {
-        *w.abort = 1u;
-        if (w.host != nullptr) *reinterpret_cast<volatile int32_t*>(w.host) = code;
-        return false;
-      }
-    }
-  }
+__device__ __forceinline__ uint32_t clock32() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%clock;" : "=r"(t));
+  return t;
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Watch& w, int code) {
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {             // (sleeps up to 20 us for it)
   uint32_t ok;
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
-  if (__builtin_expect(ok != 0u, 1)) return true;
-  return mbar_wait_slow(bar, parity, w, code);
+  return ok != 0u;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Watch& w, int code) {
+  if (__builtin_expect(mbar_try(bar, parity), 1)) return true;
+  const uint32_t t0 = clock32();
+#pragma unroll 1
+  while (!mbar_try(bar, parity)) {
+    if (*w.abort) return false;
+    if (clock32() - t0 > WAIT_CYCLES) {
+      *w.abort = 1u;
+      if (w.host != nullptr) *reinterpret_cast<volatile int32_t*>(w.host) = code;
+      return false;
+    }
+  }
+  return true;
 }
 enum { CODE_LOAD = 1, CODE_MMA = 2, CODE_SOFTMAX = 4 };   // the bits of the framework's status words
 
