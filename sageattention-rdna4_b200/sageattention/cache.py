@@ -502,10 +502,12 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _rotate(q, k, positions, rotary, layout, backward, out):
-    # (an output that is its input needs no more of a plan than that the two inputs share nothing: their distance)
+    # (an output that is its input needs no more of a plan than that the two inputs share nothing: their distance; a plan
+    # holds the outputs' strides, so that fresh outputs, marked by None, have plans of their own)
     in_place = out is not None and (out is q if k is None else len(out) == 2 and out[0] is q and out[1] is k)
-    key = (_sig(q), None if k is None else _sig(k), _sig(positions), layout, in_place and (0 if k is None else k.data_ptr() - q.data_ptr()))
     kept = out is None or in_place
+    distance = None if not in_place else 0 if k is None else k.data_ptr() - q.data_ptr()
+    key = (_sig(q), None if k is None else _sig(k), _sig(positions), layout, distance)
     plan = rotary._plans.get(key) if kept else None
     if plan is None:
         plan = _plan_rotary(q, k, positions, rotary, layout, out)

@@ -254,3 +254,27 @@ def test_copies_have_frequencies_of_their_own():
         assert not twin._plans and twin.inv_freq.device == rotary.inv_freq.device and torch.equal(twin.inv_freq, rotary.inv_freq)
         assert (twin.head_dim, twin.rotary_dim, twin.interleaved, twin.magnitude) == (96, 64, True, rotary.magnitude)
     assert copy.deepcopy(rotary).inv_freq.data_ptr() != rotary.inv_freq.data_ptr()
+
+
+def _recorded(monkeypatch):
+    """The Python layer on CPU tensors: a plan is its output's strides in words, a C call is recorded instead of made."""
+    calls = []
+    monkeypatch.setattr(C, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(C, "_call", lambda what, dev, words: calls.append(words) or 0)
+    monkeypatch.setattr(C, "_plan_rotary", lambda q, k, positions, rotary, layout, out: b"fresh" if out is None else b"given")
+    return calls
+
+
+@pytest.mark.parametrize("fresh_first", [True, False])
+def test_fresh_and_in_place_rotations_have_plans_of_their_own(monkeypatch, fresh_first):
+    calls = _recorded(monkeypatch)
+    rotary, pos = S.SageRotary(64, device="cpu"), torch.arange(5)
+    q = torch.zeros((5, 6, 64), dtype=torch.float16)[:, :2]          # strided, as a part of a fused projection
+    for _ in range(2):
+        for fresh in (fresh_first, not fresh_first):
+            C._rotate(q, None, pos, rotary, "HND", False, None if fresh else q)
+            assert calls.pop().endswith(b"fresh" if fresh else b"given")
+    # one tensor as both inputs: the outputs of a call in place would overlap, which only its own checks can see
+    for fresh in (fresh_first, not fresh_first):
+        C._rotate(q, q, pos, rotary, "HND", False, None if fresh else (q, q))
+        assert calls.pop().endswith(b"fresh" if fresh else b"given")

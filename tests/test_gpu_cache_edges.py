@@ -1,0 +1,59 @@
+"""Calls of the cache operators at the edges of what they allow, on the GPU, against the formula in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import cache_reference as R
+import sageattention as S
+from sageattention import cache as C
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _seed():
+    torch.manual_seed(0)
+
+
+# ---- rotary ------------------------------------------------------------------------------------------------------
+
+def _turned(x, pos, rotary, backward=False):
+    return R.rotate(x.transpose(0, 1), pos, rotary.inv_freq, rotary.magnitude, rotary.interleaved, backward).transpose(0, 1)
+
+
+def _rot_close(got, want, x):
+    """Angles to 2^-24 of pi, products and sums in fp32: 2^-21 of the pair's length at most; half a step of the output."""
+    eps = torch.finfo(got.dtype).eps / 2
+    size = x.double().abs().amax(-1, keepdim=True) * 1.5 * 1.42
+    assert ((got.double() - want).abs() <= eps * want.abs() + 2.0 ** -21 * size + torch.finfo(got.dtype).tiny * eps).all()
+
+
+@pytest.mark.parametrize("fresh_first", [True, False])
+def test_a_part_of_a_fused_projection_turned_fresh_and_in_place(fresh_first):
+    """One SageRotary, one strided q alone: fresh outputs are packed, those in place have the projection's strides."""
+    rotary, pos = S.SageRotary(64), torch.arange(100, 137, device="cuda")
+    qkv = torch.randn((37, 8, 64), device="cuda").half()
+    for fresh in (fresh_first, not fresh_first, fresh_first):
+        before = qkv.clone()
+        q = qkv[:, 2:6]
+        # on the host first: a plan of the other form would write with the other form's strides
+        key_out = None if fresh else q
+        words = C._plan_rotary(q, None, pos, rotary, "HND", key_out)
+        kept = [p for k, p in rotary._plans.items() if (k[-1] is None) == fresh]
+        assert all(p == words for p in kept) and C._plan_rotary(q, None, pos, rotary, "HND", None) != C._plan_rotary(q, None, pos, rotary, "HND", q)
+        got = S.sage_rotary(q, None, pos, rotary, out=key_out)
+        _rot_close(got, _turned(before[:, 2:6], pos, rotary), before)
+        assert torch.equal(qkv[:, :2], before[:, :2]) and torch.equal(qkv[:, 6:], before[:, 6:])
+        assert got.is_contiguous() if fresh else got is q
+        if fresh:
+            assert torch.equal(qkv, before)
+
+
+def test_one_tensor_as_both_inputs_is_not_turned_in_place_twice():
+    rotary, pos = S.SageRotary(64), torch.arange(9, device="cuda")
+    q = torch.randn((9, 2, 64), device="cuda").half()
+    a, b = S.sage_rotary(q, q, pos, rotary)
+    assert torch.equal(a, b)
+    with pytest.raises(ValueError, match="overlaps"):
+        S.sage_rotary(q, q, pos, rotary, out=(q, q))
