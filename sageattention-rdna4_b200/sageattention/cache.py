@@ -530,6 +530,8 @@ def _rotate(q, k, positions, rotary, layout, backward, out):
 
 def _plan_rotary(q, k, positions, rotary, layout, out):
     ins = [x for x in (q, k) if x is not None]
+    if ins[-1].dim() != q.dim():
+        _refuse("q and k must both be packed or both be 4-D")
     views = [_rotary_views(x, layout) for x in ins]
     dev = q.device
     o_views = []

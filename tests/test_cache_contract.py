@@ -278,3 +278,13 @@ def test_fresh_and_in_place_rotations_have_plans_of_their_own(monkeypatch, fresh
     for fresh in (fresh_first, not fresh_first):
         C._rotate(q, q, pos, rotary, "HND", False, None if fresh else (q, q))
         assert calls.pop().endswith(b"fresh" if fresh else b"given")
+
+
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+def test_rotary_refuses_a_packed_tensor_next_to_a_batched_one(layout):
+    rotary, pos = S.SageRotary(64, device="cpu"), torch.arange(5)
+    packed = torch.zeros((5, 2, 64), dtype=torch.float16)
+    batched = torch.zeros((1, 5, 2, 64) if layout == "NHD" else (1, 2, 5, 64), dtype=torch.float16)
+    for q, k in ((packed, batched), (batched, packed)):
+        with pytest.raises(ValueError, match="both"):
+            S.sage_rotary(q, k, pos, rotary, tensor_layout=layout)

@@ -57,3 +57,17 @@ def test_one_tensor_as_both_inputs_is_not_turned_in_place_twice():
     assert torch.equal(a, b)
     with pytest.raises(ValueError, match="overlaps"):
         S.sage_rotary(q, q, pos, rotary, out=(q, q))
+
+
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+def test_packed_and_batched_tensors_do_not_mix(layout):
+    rotary, pos = S.SageRotary(64), torch.arange(5, device="cuda")
+    packed = torch.randn((5, 2, 64), device="cuda").half()
+    batched = packed[None] if layout == "NHD" else packed.transpose(0, 1)[None]
+    for q, k in ((packed, batched), (batched, packed)):
+        with pytest.raises(ValueError, match="both"):
+            S.sage_rotary(q, k, pos, rotary, tensor_layout=layout)
+    want = S.sage_rotary(packed, None, pos, rotary)
+    got = S.sage_rotary(batched, batched, pos, rotary, tensor_layout=layout)
+    for x in got:
+        assert torch.equal(x[0] if layout == "NHD" else x[0].transpose(0, 1), want)
