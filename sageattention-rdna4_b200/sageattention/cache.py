@@ -479,8 +479,9 @@ def _rotary_views(x, layout):
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two servable views share an element.  Views of one buffer with the same strides (the parts of a fused
-    projection) are told apart exactly; others that reach into one another count as sharing."""
+    """Whether two views share an element.  Views of one buffer with the same strides (the parts of a fused projection)
+    are told apart exactly where each stride steps over all that the smaller ones reach, as those of servable views do;
+    others that reach into one another count as sharing."""
     def span(t):
         return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
     (a0, a1), (b0, b1) = span(a), span(b)
@@ -488,10 +489,16 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
         return False
     if a.stride() != b.stride():
         return True
-    axes = sorted(zip(a.stride(), a.shape, b.shape), reverse=True)
+    # (an axis of one element has no say, whatever its stride)
+    axes = sorted(((s, na, nb) for s, na, nb in zip(a.stride(), a.shape, b.shape) if na > 1 or nb > 1), reverse=True)
+    reach = 0
+    for stride, na, nb in reversed(axes):
+        if stride <= reach:
+            return True
+        reach += stride * (max(na, nb) - 1)
 
     def reachable(rest, k):
-        # is rest = sum over the axes of (index in b - index in a) * stride?  Each stride steps over all the smaller reach.
+        # is rest = sum over the axes of (index in b - index in a) * stride?
         if k == len(axes):
             return rest == 0
         stride, na, nb = axes[k]

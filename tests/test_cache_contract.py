@@ -288,3 +288,35 @@ def test_rotary_refuses_a_packed_tensor_next_to_a_batched_one(layout):
     for q, k in ((packed, batched), (batched, packed)):
         with pytest.raises(ValueError, match="both"):
             S.sage_rotary(q, k, pos, rotary, tensor_layout=layout)
+
+
+def test_shared_elements_of_views_with_axes_of_one():
+    """As above with axes of one element at any stride, 0 among them, and with axes that lie over each other."""
+    gen = torch.Generator().manual_seed(1)
+    store = torch.zeros(4096, dtype=torch.float16)
+    pick = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=gen))
+
+    def elements(t):
+        at = [t.data_ptr() // 2]
+        for n, s in zip(t.shape, t.stride()):
+            at = [x + i * s for x in at for i in range(n)]
+        return set(at)
+
+    seen = set()
+    for _ in range(600):
+        ones = [pick(0, 2) for _ in range(3)]
+        full = [1 if one else pick(2, 5) for one in ones] + [pick(1, 9)]
+        strides, step = [0, 0, 0, 1], full[3]
+        for i in (2, 1, 0):
+            strides[i] = pick(0, 60) if ones[i] else step
+            step *= full[i]
+        a, b = (store.as_strided([n if one else pick(1, n + 1) for n, one in zip(full, ones + [0])], strides, pick(0, 100)) for _ in range(2))
+        want = bool(elements(a) & elements(b))
+        assert C._overlap(a, b) == want, (a.shape, b.shape, strides)
+        seen.add(want)
+    assert seen == {True, False}
+    # what cannot be told apart exactly counts as sharing: never a miss
+    for _ in range(300):
+        strides = [pick(0, 9) for _ in range(3)]
+        a, b = (store.as_strided([pick(1, 4) for _ in range(3)], strides, pick(0, 20)) for _ in range(2))
+        assert C._overlap(a, b) or not elements(a) & elements(b), (a.shape, b.shape, strides)
