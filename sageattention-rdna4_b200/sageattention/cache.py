@@ -185,8 +185,8 @@ class SageCache:
         return cls(codes[0].view(torch.int8 if int8 else _E4M3), scales[0], codes[1].view(_E4M3), scales[1], head_dim, k_shift)
 
 
-def _check_rows(name: str, t: torch.Tensor, heads: int, d: int, dev):
-    """A packed (tokens, heads, head_dim) tensor next to a cache."""
+def _check_rows(name: str, t: torch.Tensor, heads: int, d: int, dev, output: bool = False):
+    """A packed (tokens, heads, head_dim) tensor next to a cache; in an output every row has memory of its own."""
     if t.device != dev:
         _refuse("%s must be on the cache's device" % name)
     if t.dtype not in (torch.float16, torch.bfloat16):
@@ -197,6 +197,12 @@ def _check_rows(name: str, t: torch.Tensor, heads: int, d: int, dev):
         reason = packed_view_reason(t)
         if reason is not None:
             _refuse("cannot serve %s: %s" % (name, reason))
+    reach = d
+    for stride, n in sorted(zip(t.stride()[:2], t.shape[:2])) if output else ():
+        if n > 1:
+            if stride < reach:
+                _refuse("the rows of %s must not overlap" % name)
+            reach += stride * (n - 1)
 
 
 def _check_index(name: str, t: torch.Tensor, dev, dims: int, dtypes=(torch.int32,)):
@@ -289,7 +295,7 @@ def _plan_read(cache, page_table, cu_seqlens, total, dtype, out):
         if len(out) != 2:
             _refuse("out must be a pair")
         for name, t in (("out[0]", out[0]), ("out[1]", out[1])):
-            _check_rows(name, t, heads, d, dev)
+            _check_rows(name, t, heads, d, dev, output=True)
             if t.shape[0] != total or t.dtype != dtype:
                 _refuse("%s must hold total rows of dtype" % name)
         strides = [n for t in out for n in t.stride()[:2]]
@@ -401,7 +407,7 @@ def _plan_attend(cache, q, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tr
     if not (0.0 < scale < float("inf")):
         _refuse("sm_scale must be finite and positive, got %r" % (sm_scale,))
     if out is not None:
-        _check_rows("out", out, hq, d, dev)
+        _check_rows("out", out, hq, d, dev, output=True)
         if out.shape != q.shape or out.dtype != q.dtype:
             _refuse("out must have q's shape and dtype")
     like_lse = _like((tokens, hq), torch.float32, dev)

@@ -320,3 +320,30 @@ def test_shared_elements_of_views_with_axes_of_one():
         strides = [pick(0, 9) for _ in range(3)]
         a, b = (store.as_strided([pick(1, 4) for _ in range(3)], strides, pick(0, 20)) for _ in range(2))
         assert C._overlap(a, b) or not elements(a) & elements(b), (a.shape, b.shape, strides)
+
+
+def _host_cache(pages=4, page=16, heads=2, d=64):
+    """What the checks of a call read of a cache, on the CPU."""
+    from types import SimpleNamespace
+    return SimpleNamespace(device=torch.device("cpu"), num_kv_heads=heads, head_dim=d, _sizes=(pages, page), _args=(0,) * 5, _mode=0, num_pages=pages,
+                           page_size=page, _plans={})
+
+
+def test_rows_of_an_output_have_memory_of_their_own():
+    cache, store = _host_cache(), torch.zeros(4096, dtype=torch.float16)
+    table, lens, cu = torch.zeros((3, 2), dtype=torch.int32), torch.ones(3, dtype=torch.int32), torch.arange(4, dtype=torch.int32)
+    q, x = torch.zeros((3, 4, 64), dtype=torch.float16), torch.zeros((3, 2, 64), dtype=torch.float16)
+    view = lambda shape, *strides: store.as_strided(shape, (*strides, 1))
+    for strides in ((256, 64), (64, 192), (512, 72), (72, 512)):     # rows side by side, tokens or heads first
+        C._plan_attend(cache, q, table, lens, None, None, None, None, view((3, 4, 64), *strides))
+        C._plan_read(cache, table, cu, 3, torch.float16, (view((3, 2, 64), *strides), x))
+    for strides in ((64, 64), (8, 64), (256, 8), (128, 64), (64, 128)):
+        with pytest.raises(ValueError, match="overlap"):
+            C._plan_attend(cache, q, table, lens, None, None, None, None, view((3, 4, 64), *strides))
+    for strides in ((64, 64), (8, 128), (128, 8), (64, 128)):
+        with pytest.raises(ValueError, match="overlap"):
+            C._plan_read(cache, table, cu, 3, torch.float16, (view((3, 2, 64), *strides), x))
+    one = C._plan_attend(cache, q[:1], table[:1], lens[:1], None, None, None, None, view((1, 4, 64), 8, 64))     # a single token has no next one
+    assert one[0]
+    same = C._plan_attend(cache, view((3, 4, 64), 8, 8), table, lens, None, None, None, None, None)             # inputs may
+    assert same[0]
