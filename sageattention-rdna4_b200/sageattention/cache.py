@@ -22,6 +22,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from . import b200_backend as _be
@@ -597,6 +598,12 @@ def _plan_rotary(q, k, positions, rotary, layout, out):
                  views[1].shape[1] if k is not None else 0, n, d, rotary.rotary_dim, rotary.interleaved, *s3, *p2, _dtype_code(q.dtype))
 
 
+def _tangent(t: torch.Tensor) -> bool:
+    """Whether t carries a forward-mode derivative.  (Outside of every dual level, which is where calls are made that take
+    a few microseconds, none does: asking the tensor takes 0.4.)"""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 class _Rotary(torch.autograd.Function):
     """The map is linear: its gradient is the transposed map of the outputs' gradients."""
 
@@ -626,12 +633,15 @@ def sage_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
         worked out in 64 bits).
     backward : the transposed map, which takes the gradient of the outputs to that of the inputs (for a magnitude
         of 1, the inverse).  Inputs that require gradients get them by it; a backward pass that is captured
-        into a graph is warmed up on the capture stream, with no eager graph of the same leaves left alive.
+        into a graph is warmed up on the capture stream, with no eager graph of the same leaves left alive.  Forward-mode
+        derivatives are refused.
     out : optional output (for two inputs a pair), each its input itself or memory of its own; not differentiable.
     """
     _counters["calls"] += 1
     if tensor_layout not in ("HND", "NHD"):
         _refuse("tensor_layout must be 'HND' or 'NHD'")
+    if _tangent(q) or (k is not None and _tangent(k)):
+        _refuse("forward-mode derivatives are not carried", NotImplementedError)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out is not None:
             _refuse("out cannot be given for inputs that require gradients")

@@ -347,3 +347,21 @@ def test_rows_of_an_output_have_memory_of_their_own():
     assert one[0]
     same = C._plan_attend(cache, view((3, 4, 64), 8, 8), table, lens, None, None, None, None, None)             # inputs may
     assert same[0]
+
+
+def test_rotary_refuses_forward_mode_derivatives(monkeypatch):
+    import torch.autograd.forward_ad as fw
+    calls = _recorded(monkeypatch)
+    rotary, pos, x = S.SageRotary(64, device="cpu"), torch.arange(5), torch.zeros((5, 2, 64), dtype=torch.float16)
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for args in ((dual, None), (dual, x), (x, dual)):
+            with pytest.raises(NotImplementedError):
+                S.sage_rotary(*args, pos, rotary)
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            S.sage_rotary(dual, None, pos, rotary)
+        with pytest.raises(NotImplementedError):
+            S.sage_rotary(fw.make_dual(x.clone().requires_grad_(), torch.ones_like(x)), None, pos, rotary)
+        assert not calls
+        S.sage_rotary(x, x, pos, rotary)             # the level alone changes nothing
+    assert len(calls) == 1
