@@ -99,6 +99,8 @@ def _fixed(self, name, value):
 def _written(tensors):
     """Tell autograd that these were written over, as it is told of torch's own writes."""
     for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            _refuse("an output must not require gradients")
         if not t.is_inference():
             torch.autograd.graph.increment_version(t)
 

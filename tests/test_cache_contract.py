@@ -365,3 +365,22 @@ def test_rotary_refuses_forward_mode_derivatives(monkeypatch):
         assert not calls
         S.sage_rotary(x, x, pos, rotary)             # the level alone changes nothing
     assert len(calls) == 1
+
+
+def test_outputs_that_require_gradients_are_refused(monkeypatch):
+    calls = _recorded(monkeypatch)
+    rotary, pos = S.SageRotary(64, device="cpu"), torch.arange(5)
+    x, leaf = torch.zeros((5, 2, 64), dtype=torch.float16), torch.zeros((5, 2, 64), dtype=torch.float16, requires_grad=True)
+    later = leaf * 2
+    for out in (leaf, later):
+        with pytest.raises(ValueError, match="gradients"):
+            S.sage_rotary(x, None, pos, rotary, out=out)
+        with pytest.raises(ValueError, match="gradients"):
+            S.sage_rotary(x, x.clone(), pos, rotary, out=(torch.zeros_like(x), out))
+    table, cu = torch.zeros((1, 1), dtype=torch.int32), torch.tensor([0, 5], dtype=torch.int32)
+    with pytest.raises(ValueError, match="gradients"):
+        S.sage_cache_read(_host_cache(), table, cu, 5, out=(x, leaf))
+    assert not calls
+    with torch.no_grad():                            # a parameter may be turned in place, as it may be written to
+        S.sage_rotary(leaf, None, pos, rotary, out=leaf)
+    assert len(calls) == 1
