@@ -127,7 +127,7 @@ class SageCache:
     """
 
     __slots__ = ("k_codes", "k_scale", "v_codes", "v_scale", "k_shift", "head_dim", "num_pages", "page_size",
-                 "num_kv_heads", "device", "_mode", "_args", "_sizes", "_plans")
+                 "num_kv_heads", "device", "_mode", "_args", "_sizes", "_tracked", "_plans")
     __setattr__ = _fixed
 
     def __init__(self, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
@@ -166,6 +166,7 @@ class SageCache:
         self._args = (k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
                       0 if k_shift is None else k_shift.data_ptr())
         self._sizes = (pages, page)
+        self._tracked = [t for t in (k_codes, k_scale, v_codes, v_scale) if not t.is_inference()]
         self._plans = {}                             # call signature -> what the C call is given for it
 
     def __reduce__(self):                            # a copy has buffers, and addresses, of its own
@@ -231,6 +232,7 @@ def sage_cache_write(cache: SageCache, k: torch.Tensor, v: torch.Tensor, slots: 
     if plan is None:
         plan = _remember(cache._plans, key, _plan_write(cache, k, v, slots))
     if plan:
+        torch.autograd.graph.increment_version(cache._tracked)       # as for torch's own writes
         dev = cache.device
         rc = _call(_WRITE, dev, _FIRST[_WRITE](k.data_ptr(), v.data_ptr(), slots.data_ptr(), _raw_stream(dev.index)) + plan)
         if rc:

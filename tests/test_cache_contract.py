@@ -384,3 +384,16 @@ def test_outputs_that_require_gradients_are_refused(monkeypatch):
     with torch.no_grad():                            # a parameter may be turned in place, as it may be written to
         S.sage_rotary(leaf, None, pos, rotary, out=leaf)
     assert len(calls) == 1
+
+
+def test_autograd_learns_of_writes_to_the_cache(monkeypatch):
+    calls = _recorded(monkeypatch)
+    cache = _host_cache()
+    cache._tracked = [torch.ones(4), torch.ones(4)]
+    w = torch.ones(4, requires_grad=True)
+    y = (w * cache._tracked[1]).sum()                # keeps the scales for its backward pass
+    x = torch.zeros((3, 2, 64), dtype=torch.float16)
+    S.sage_cache_write(cache, x, x, torch.arange(3))
+    assert len(calls) == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

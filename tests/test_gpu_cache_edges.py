@@ -71,3 +71,19 @@ def test_packed_and_batched_tensors_do_not_mix(layout):
     got = S.sage_rotary(batched, batched, pos, rotary, tensor_layout=layout)
     for x in got:
         assert torch.equal(x[0] if layout == "NHD" else x[0].transpose(0, 1), want)
+
+
+# ---- writing -----------------------------------------------------------------------------------------------------
+
+def test_autograd_learns_of_writes_to_the_cache():
+    cache = S.SageCache.empty(2, 16, 2, 64)
+    x, slots = torch.randn((3, 2, 64), device="cuda").half(), torch.arange(3, device="cuda")
+    w = torch.ones_like(cache.v_scale, requires_grad=True)
+    y = (w * cache.v_scale).sum()
+    S.sage_cache_write(cache, x, x, slots)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        served = S.SageCache.empty(2, 16, 2, 64)
+    S.sage_cache_write(served, x, x, slots)          # tensors of inference mode have no versions
+    assert torch.equal(served.k_scale, cache.k_scale) and torch.equal(served.v_scale, cache.v_scale)
