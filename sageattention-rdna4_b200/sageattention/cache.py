@@ -608,6 +608,15 @@ def _tangent(t: torch.Tensor) -> bool:
     return getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None
 
 
+def _servable(grad: torch.Tensor) -> torch.Tensor:
+    """A gradient as the kernel takes it: autograd hands over whatever the next operation left, broadcast or cut out of
+    something larger at any offset."""
+    grad = grad.contiguous()
+    if grad.data_ptr() & 15 or any(s <= 0 or s % 8 for s in grad.stride()[:-1]):     # (the stride of an axis of one may be anything)
+        grad = grad.clone(memory_format=_PACKED)
+    return grad
+
+
 class _Rotary(torch.autograd.Function):
     """The map is linear: its gradient is the transposed map of the outputs' gradients."""
 
@@ -622,7 +631,7 @@ class _Rotary(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
         rotary, layout, backward = ctx.rest
-        res = _rotate(grads[0].contiguous(), grads[1].contiguous() if len(grads) > 1 else None, ctx.saved_tensors[0], rotary, layout,
+        res = _rotate(_servable(grads[0]), _servable(grads[1]) if len(grads) > 1 else None, ctx.saved_tensors[0], rotary, layout,
                       not backward, None)
         return res[0], res[1] if len(grads) > 1 else None, None, None, None, None
 

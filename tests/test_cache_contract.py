@@ -397,3 +397,26 @@ def test_autograd_learns_of_writes_to_the_cache(monkeypatch):
     assert len(calls) == 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_gradients_arrive_as_the_kernel_takes_them(monkeypatch):
+    """Broadcast, at an odd offset of a larger gradient, with an axis of one of any stride."""
+    _recorded(monkeypatch)
+    taken = []
+
+    def plan(q, k, positions, rotary, layout, out):
+        taken.extend(C.strided_view_reason(C._rotary_views(x, layout)) for x in (q, k) if x is not None)
+        return b""
+    monkeypatch.setattr(C, "_plan_rotary", plan)
+    monkeypatch.setattr(C, "_remember", lambda plans, key, words: words)
+    rotary = S.SageRotary(64, device="cpu")
+    for n in (1, 5):
+        pos = torch.arange(n)
+        q = torch.zeros((n, 2, 64), dtype=torch.float16, requires_grad=True)
+        odd = torch.zeros(3, dtype=torch.float16, requires_grad=True)
+        a, b = S.sage_rotary(q, q, pos, rotary)
+        torch.cat([odd, a.flatten(), b.flatten()]).pow(2).sum().backward()
+        S.sage_rotary(q, None, pos, rotary).sum().backward()
+        strange = torch.zeros(4096, dtype=torch.float16).as_strided((1, 2, 64), (3, 64, 1))
+        S.sage_rotary(q[:1], None, pos[:1], rotary).backward(strange)
+    assert len(taken) == 2 * (4 + 2 + 2) and not any(taken), taken

@@ -73,6 +73,18 @@ def test_packed_and_batched_tensors_do_not_mix(layout):
         assert torch.equal(x[0] if layout == "NHD" else x[0].transpose(0, 1), want)
 
 
+def test_gradients_at_any_offset():
+    """The gradient of a part of something larger, behind an odd number of elements: against the formula."""
+    rotary, pos = S.SageRotary(64, rotary_dim=32), torch.arange(7, 18, device="cuda")
+    q = torch.randn((11, 3, 64), device="cuda").half().requires_grad_()
+    odd = torch.randn(3, device="cuda").half().requires_grad_()
+    y = torch.cat([odd, S.sage_rotary(q, None, pos, rotary).flatten()])
+    g = torch.randn_like(y)
+    y.backward(g)
+    g = g[3:].view(11, 3, 64)
+    _rot_close(q.grad, _turned(g, pos, rotary, backward=True), g)
+
+
 # ---- writing -----------------------------------------------------------------------------------------------------
 
 def test_autograd_learns_of_writes_to_the_cache():
