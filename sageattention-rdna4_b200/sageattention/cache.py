@@ -120,7 +120,7 @@ class SageCache:
     k_scale, v_scale : ``(pages, Hkv, page_size)`` float32
     k_shift : optional ``(Hkv, head_dim)`` float32 that is subtracted from K before it is quantised (the mean
         that `smooth_k` takes off, taken once over a prompt and kept).  Attention does not change by it: all
-        keys of a head move alike.
+        keys of a head move alike.  The cache keeps a copy of it, which is what the attribute of that name shows.
     The buffers stay the cache's for good (what they hold may change).
     page_size is a power of two, 16 .. 256.  The code buffers must start as zeros (`empty` does that): codes that
     no write has set may be read behind a mask, and must not be the e4m3 NaN.
@@ -157,8 +157,8 @@ class SageCache:
             if tuple(k_shift.shape) != (heads, head_dim) or k_shift.device != k_codes.device:
                 _refuse("k_shift must be (heads, head_dim) on the cache's device")
             padded = torch.zeros((heads, width), dtype=torch.float32, device=k_codes.device)
-            padded[:, :head_dim] = k_shift
-            k_shift = padded
+            padded[:, :head_dim] = k_shift.detach()
+            k_shift = padded[:, :head_dim]
         self.k_codes, self.k_scale, self.v_codes, self.v_scale, self.k_shift = k_codes, k_scale, v_codes, v_scale, k_shift
         self.head_dim, self.num_pages, self.page_size, self.num_kv_heads = head_dim, pages, page, heads
         self.device = k_codes.device
@@ -170,8 +170,7 @@ class SageCache:
         self._plans = {}                             # call signature -> what the C call is given for it
 
     def __reduce__(self):                            # a copy has buffers, and addresses, of its own
-        shift = None if self.k_shift is None else self.k_shift[:, :self.head_dim]
-        return type(self), (self.k_codes, self.k_scale, self.v_codes, self.v_scale, self.head_dim, shift)
+        return type(self), (self.k_codes, self.k_scale, self.v_codes, self.v_scale, self.head_dim, self.k_shift)
 
     @classmethod
     def empty(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype = torch.float16,

@@ -99,3 +99,22 @@ def test_autograd_learns_of_writes_to_the_cache():
         served = S.SageCache.empty(2, 16, 2, 64)
     S.sage_cache_write(served, x, x, slots)          # tensors of inference mode have no versions
     assert torch.equal(served.k_scale, cache.k_scale) and torch.equal(served.v_scale, cache.v_scale)
+
+
+@pytest.mark.parametrize("d", [40, 72, 128])
+def test_the_shift_of_a_cache_is_a_copy_in_the_shape_it_was_given(d):
+    import copy
+    shift = torch.randn((2, d), device="cuda", requires_grad=True)
+    cache = S.SageCache.empty(2, 16, 2, d, k_shift=shift)
+    assert cache.k_shift.shape == (2, d) and torch.equal(cache.k_shift, shift) and not cache.k_shift.requires_grad
+    k, slots = torch.randn((20, 2, d), device="cuda").half(), torch.arange(20, device="cuda")
+    twin = S.SageCache(*(torch.zeros_like(t) for t in (cache.k_codes, cache.k_scale, cache.v_codes, cache.v_scale)), d, cache.k_shift)
+    want = shift.detach().clone()
+    with torch.no_grad():
+        shift.zero_()
+    for c in (cache, twin, copy.deepcopy(cache)):
+        assert torch.equal(c.k_shift, want)
+        S.sage_cache_write(c, k, k, slots)
+        codes, scale = R.quantise(k.float() - want, True)
+        assert torch.equal(c.k_codes.transpose(1, 2).flatten(0, 1)[:20, :, :d].double(), codes) and (c.k_codes[..., d:] == 0).all()
+        assert torch.equal(c.k_scale.transpose(1, 2).flatten(0, 1)[:20], scale)
