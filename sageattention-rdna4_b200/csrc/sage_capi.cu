@@ -551,7 +551,7 @@ static int check_table(const char* who, const int32_t* table, int64_t stride, in
   if (!table) return fail(SAGE_E_ARG, "%s: page_table is null", who);
   if (reinterpret_cast<uintptr_t>(table) & 3u) return fail(SAGE_E_ARG, "%s: page_table must be 4-byte aligned", who);
   if (width < 1 || stride < 0) return fail(SAGE_E_ARG, "%s: bad page_table width or stride", who);
-  if (width * page_size > ((int64_t)1 << 30)) return fail(SAGE_E_UNSUPPORTED, "%s: sequence length exceeds 2^30", who);
+  if (width > ((int64_t)1 << 30) / page_size) return fail(SAGE_E_UNSUPPORTED, "%s: sequence length exceeds 2^30", who);
   return SAGE_OK;
 }
 
@@ -606,6 +606,7 @@ int sage_cache_read(const void* k_codes, const float* k_scale, const void* v_cod
 
 size_t sage_cache_attention_workspace_bytes(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q) {
   if (n_seq < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || max_q < 1) return 0;
+  if (max_q > ((int64_t)1 << 28) / (Hq / Hkv)) return 0;               // more rows than sage_cache_attention takes
   return align256(sage::cache_attention_scratch(n_seq, Hq, Hkv, max_q));
 }
 

@@ -420,3 +420,12 @@ def test_gradients_arrive_as_the_kernel_takes_them(monkeypatch):
         strange = torch.zeros(4096, dtype=torch.float16).as_strided((1, 2, 64), (3, 64, 1))
         S.sage_rotary(q[:1], None, pos[:1], rotary).backward(strange)
     assert len(taken) == 2 * (4 + 2 + 2) and not any(taken), taken
+
+
+def test_sizes_whose_products_pass_64_bits():
+    for width in (1 << 56, (1 << 55) + 1, 1 << 60, (1 << 63) - 1):
+        _refused(_read(width=width, page=256), UNSUPPORTED, "2^30")
+        _refused(_attend(width=width, page=256), UNSUPPORTED, "2^30")
+    _refused(_read(width=(1 << 26) + 1, page=16), UNSUPPORTED, "2^30")
+    size = _native.load().sage_cache_attention_workspace_bytes
+    assert size(1, 1 << 40, 1, 1 << 40) == size(1, 2, 1, (1 << 63) - 1) == size(1, 8, 2, (1 << 26) + 1) == 0 and size(1, 8, 2, 1 << 26) > 0
