@@ -76,6 +76,17 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
   }
   return true;
 }
+// Until this CTA's own products are complete, whoever has given up on anything: what they read and write stays theirs.
+__device__ __forceinline__ void drain_wait(uint32_t bar, const Watch& w, int code) {
+  const uint32_t t0 = clock32();
+#pragma unroll 1
+  while (!mbar_try(bar, 0)) {
+    if (clock32() - t0 > WAIT_CYCLES) {
+      if (w.host != nullptr) *reinterpret_cast<volatile int32_t*>(w.host) = code;
+      return;
+    }
+  }
+}
 enum { CODE_LOAD = 1, CODE_MMA = 2, CODE_SOFTMAX = 4 };   // the bits of the framework's status words
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -734,7 +745,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         next_unit(a, cur, cur.kt, ROWS, KT);
       }
       tc_commit(bar(L::B_DRAIN));                    // every product issued is complete before the TMEM is freed
-      mbar_wait(bar(L::B_DRAIN), 0, watch, CODE_MMA);
+      drain_wait(bar(L::B_DRAIN), watch, CODE_MMA);
     }
   }
   tc_fence_before();
