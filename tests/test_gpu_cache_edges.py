@@ -43,7 +43,7 @@ def test_a_part_of_a_fused_projection_turned_fresh_and_in_place(fresh_first):
         kept = [p for k, p in rotary._plans.items() if (k[-1] is None) == fresh]
         assert all(p == words for p in kept) and C._plan_rotary(q, None, pos, rotary, "HND", None) != C._plan_rotary(q, None, pos, rotary, "HND", q)
         got = S.sage_rotary(q, None, pos, rotary, out=key_out)
-        _rot_close(got, _turned(before[:, 2:6], pos, rotary), before)
+        _rot_close(got, _turned(before[:, 2:6], pos, rotary), before[:, 2:6])
         assert torch.equal(qkv[:, :2], before[:, :2]) and torch.equal(qkv[:, 6:], before[:, 6:])
         assert got.is_contiguous() if fresh else got is q
         if fresh:
@@ -118,3 +118,58 @@ def test_the_shift_of_a_cache_is_a_copy_in_the_shape_it_was_given(d):
         codes, scale = R.quantise(k.float() - want, True)
         assert torch.equal(c.k_codes.transpose(1, 2).flatten(0, 1)[:20, :, :d].double(), codes) and (c.k_codes[..., d:] == 0).all()
         assert torch.equal(c.k_scale.transpose(1, 2).flatten(0, 1)[:20], scale)
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------
+
+def _setup(lens, t, hq=8, hkv=2, d=128, page=16, dtype=torch.float16, int8=True, shift=False, seed=0):
+    """Sequences of those lengths in scattered pages, written; queries of t new tokens each."""
+    gen = torch.Generator().manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    k_shift = 0.5 * torch.randn((hkv, d), generator=gen).cuda() if shift else None
+    cache = S.SageCache.empty(sum(need) + 3, page, hkv, d, dtype=dtype, int8=int8, k_shift=k_shift)
+    table = torch.full((len(lens), max(need) + 1), -1, dtype=torch.int32)
+    order, at = torch.randperm(cache.num_pages, generator=gen).int(), 0
+    for i, m in enumerate(need):
+        table[i, :m] = order[at:at + m]
+        at += m
+    k, v = (torch.randn((sum(lens), hkv, d), generator=gen).to(dtype).cuda() for _ in range(2))
+    S.sage_cache_write(cache, k, v, torch.cat([_slots(cache, table, i, torch.arange(n)) for i, n in enumerate(lens)]).cuda())
+    q = torch.randn((len(lens) * t, hq, d), generator=gen).to(dtype).cuda()
+    return cache, table.cuda(), q, torch.tensor(lens, dtype=torch.int32).cuda(), gen
+
+
+def _slots(cache, table, i, at):
+    return table[i, at // cache.page_size].long() * cache.page_size + at % cache.page_size
+
+
+# New tokens x 4 query heads: one and two row tiles of the kernel for few rows, both forms of the kernel for many.
+ROWS = [1, 3, 6, 12, 40]
+
+
+@pytest.mark.parametrize("lens", [(230, 150), (9000, 40)])            # the longer ones are cut and joined
+@pytest.mark.parametrize("which", ["k", "v", "both"])
+@pytest.mark.parametrize("t", ROWS)
+def test_a_nan_in_one_of_key_and_value(t, which, lens):
+    """A row that sees it is NaN; its LSE is NaN for K, and for V alone that of the scores; no other row changes a bit."""
+    cache, table, q, lens_d, gen = _setup(lens, t, dtype=torch.bfloat16)
+    mask = torch.eye(t, dtype=torch.bool).repeat(2, 1).cuda()
+    call = lambda: S.sageattn_cached(q, cache, table, lens_d, tree_mask=mask, return_lse=True)
+    k, v = (torch.randn((1, 2, 128), generator=gen).cuda().bfloat16() for _ in range(2))
+    slot = _slots(cache, table.cpu(), 0, torch.tensor([lens[0] - 1])).cuda()          # the last draft of the first sequence, which that alone sees
+    S.sage_cache_write(cache, k, v, slot)
+    clean, clean_lse = call()
+    if which != "v":
+        k[0, 0, 3] = math.nan
+    if which != "k":
+        v[0, 0, 100] = -math.inf
+    S.sage_cache_write(cache, k, v, slot)
+    out, lse = call()
+    hit = torch.zeros((2 * t, 8), dtype=torch.bool, device="cuda")
+    hit[t - 1, :4] = True                            # (query heads 0-3 share K/V head 0)
+    assert torch.isnan(out[hit]).all()
+    assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+    if which == "v":                                 # the same scores; the fp32 sum over the scale of V takes other roundings
+        assert ((lse - clean_lse)[hit].abs() <= 2e-5 * clean_lse[hit].abs().clamp(min=1)).all()
+    else:
+        assert torch.isnan(lse[hit]).all()
