@@ -185,8 +185,9 @@ template <int WIDTH, int NQ> struct TreeShape {
   static constexpr uint32_t RAW_TILE = 2 * KT * WIDTH + 2 * KT * 4;                   // codes and scales of K and V as they come
   static constexpr uint32_t OFF_Q = 0, OFF_K = NQ * Q_TILE, OFF_V = OFF_K + STAGES * KV_TILE, OFF_RAW = OFF_V + STAGES * KV_TILE;
   static constexpr uint32_t OFF_SC = OFF_RAW + RAW_STAGES * RAW_TILE;
-  // of a tile: scales of K, log2 and reciprocal of the scales of V, and for every 32 keys {a bit for each that does not
-  // exist, a bit for each that holds a NaN, the largest and the smallest log2 of a scale of V}
+  // of a tile: scales of K, log2 and reciprocal of the scales of V, and for every 32 keys {two words with a bit for each: the
+  // first alone for a key that does not exist, the second alone for a NaN in K, both for one in V alone; the largest and
+  // the smallest log2 of a scale of V}
   static constexpr uint32_t SLOT_LV = KT * 4, SLOT_RV = KT * 8, SLOT_SUM = KT * 12, SLOT = SLOT_SUM + KT / 2;
   static constexpr uint32_t OFF_ROW = OFF_SC + SLOTS * SLOT;                          // two floats per row
   static constexpr uint32_t OFF_BAR = OFF_ROW + SOFTMAX * 8;
@@ -256,7 +257,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     const int g = warp >> 2, r = tid & 127;
     const uint32_t lane_sel = (uint32_t)(warp & 3) << 21;                             // 32 lanes of TMEM per warp
     const uint32_t o_addr = tmem_o(g) + lane_sel;
-    float* row_at = reinterpret_cast<float*>(gbase + L::OFF_ROW) + 256 * g;           // of row r: [r] what undoes its power of two, [128 + r] its product with the shift
+    float* row_at = reinterpret_cast<float*>(gbase + L::OFF_ROW) + 256 * g;           // of row r: [r] what undoes its power of two (read once; a NaN from then on: the row sees one in V alone), [128 + r] its product with the shift
     // Rows of 2 * WIDTH bytes in this half's Q tile: piece c of row r, where Q goes and outputs pass through.
     uint8_t* q_tile = gbase + L::OFF_Q + g * L::Q_TILE;
     auto staged = [&](int row, int c) { return reinterpret_cast<uint4*>(q_tile + (c >> 3) * L::Q_HALF + row * 128 + 16 * ((c & 7) ^ (row & 7))); };
@@ -355,7 +356,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
             for (int ch = 0; ch < 2; ++ch) {
               const int k0 = key0 + 32 * ch, upto = lim - k0;
               uint32_t b = upto >= 32 ? 0xffffffffu : upto <= 0 ? 0u : (1u << upto) - 1u;
-              b &= ~(ch ? sum1.x : sum0.x);
+              b &= ~(ch ? sum1.x & ~sum1.y : sum0.x & ~sum0.y);
               if (tree_row != nullptr && b != 0u && k0 + 32 > ctx) {
                 uint32_t hidden = 0u;                // (sixteen bytes in flight at a time)
 #pragma unroll 1
@@ -369,16 +370,18 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
                 b &= ~hidden;
               }
               bits[ch] = b;
+              if (b & (ch ? sum1.x & sum1.y : sum0.x & sum0.y)) row_at[r] = __int_as_float(0x7fffffff);
             }
             __syncwarp();
           }
           tmem_ld_wait();
           if (masked) {
             // What this row does not see becomes -infinity before anything is made of it, what it sees of a key that holds
-            // a NaN becomes one (such keys' scales stand at 1, so that they reach no other row).
+            // a NaN in K becomes one (such keys' scales stand at 1, so that they reach no other row).
+            const uint32_t nan0 = sum0.y & ~sum0.x, nan1 = sum1.y & ~sum1.x;
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
-              const uint32_t nan = i < 32 ? sum0.y : sum1.y;
+              const uint32_t nan = i < 32 ? nan0 : nan1;
               x[i] = !(bits[i / 32] >> (i & 31) & 1u) ? 0xff800000u : (nan >> (i & 31) & 1u) ? 0x7fffffffu : x[i];
             }
           }
@@ -452,10 +455,11 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_PV + 2 * g + ((done - 1) & 1)), (uint32_t)((done - 1) >> 1) & 1u, watch, CODE_SOFTMAX));
         if (!ok) break;
         tc_fence_after();
+        const bool poisoned = isnan(row_at[r]);      // the row sees a NaN in V alone: its output is one, its sum is not
         // a unit that began before this stretch, or with it: its part is the stretch's first, else its last
         const long long part_row = (2LL * blockIdx.x + (cur.into > 0 ? 1 : 0)) * a.part_rows + 128 * g;
         if (whole) {
-          const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
+          const float inv = poisoned ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : __fdividef(1.f, l);
 #pragma unroll 1
           for (int ch = 0; ch < WIDTH / 16; ++ch) {
             uint32_t o[16];
@@ -484,6 +488,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
               uint32_t o[16];
               tmem_ld16(o_addr + half * (WIDTH / 2) + 16 * ch, o);
               tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = poisoned ? 0x7fffffffu : o[i];
 #pragma unroll
               for (int i = 0; i < 4; ++i) *staged(r, 4 * ch + i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
             }
@@ -522,15 +528,15 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     auto store_scales = [&](int n, float sk, float sv) {
       if (ct < KT) {
         const uint32_t sc = base + L::OFF_SC + (n % L::SLOTS) * L::SLOT;
-        const bool none = sk < 0.f, nan = isnan(sk) || isnan(sv);
-        const float v = none || nan ? 1.f : fmaxf(sv, 1e-30f);       // (0: a row that nothing wrote, all codes 0; a part of the sum)
-        sts_f32(sc + 4 * ct, none || nan ? 1.f : fmaxf(sk, 1e-30f));
+        const bool none = sk < 0.f, nan_k = isnan(sk), nan_v = !nan_k && isnan(sv);
+        const float v = none || nan_k || nan_v ? 1.f : fmaxf(sv, 1e-30f);             // (0: a row that nothing wrote, all codes 0; a part of the sum)
+        sts_f32(sc + 4 * ct, none || nan_k ? 1.f : fmaxf(sk, 1e-30f));
         sts_f32(sc + L::SLOT_LV + 4 * ct, __log2f(v));
         sts_f32(sc + L::SLOT_RV + 4 * ct, __fdividef(1.f, v));
-        const uint32_t none32 = __ballot_sync(0xffffffffu, none), nan32 = __ballot_sync(0xffffffffu, nan);
+        const uint32_t first32 = __ballot_sync(0xffffffffu, none || nan_v), second32 = __ballot_sync(0xffffffffu, nan_k || nan_v);
         // (positive floats are ordered as their bits are)
         const float big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))), small = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(v)));
-        if (lane == 0) sts16(sc + L::SLOT_SUM + 16 * (ct >> 5), none32, nan32, __float_as_uint(__log2f(big)), __float_as_uint(__log2f(small)));
+        if (lane == 0) sts16(sc + L::SLOT_SUM + 16 * (ct >> 5), first32, second32, __float_as_uint(__log2f(big)), __float_as_uint(__log2f(small)));
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(L::B_SC + n % L::SLOTS));
       }
