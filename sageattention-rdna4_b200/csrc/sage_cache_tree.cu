@@ -191,9 +191,15 @@ template <int WIDTH, int NQ> struct TreeShape {
   static constexpr uint32_t SLOT_LV = KT * 4, SLOT_RV = KT * 8, SLOT_SUM = KT * 12, SLOT = SLOT_SUM + KT / 2;
   static constexpr uint32_t OFF_ROW = OFF_SC + SLOTS * SLOT;                          // two floats per row
   static constexpr uint32_t OFF_BAR = OFF_ROW + SOFTMAX * 8;
-  // Barriers: per half of the rows (QF) and score buffer (SF, PF, PV), per stage (KF, KE, VF, VE), per slot (SC).  What is
-  // waited for is never more than one phase away from where its barrier stands: the scores of a tile are issued after P V of
-  // the tile two before, which waited for that tile's weights.
+  // Barriers: per half of the rows (QF) and score buffer (SF, PF, PV), per stage (KF, KE, VF, VE), per slot (SC).  A wait by
+  // parity must find its barrier in the phase it waits for, or just past it.  Those of a half count its own tiles: the
+  // scores of a tile are issued after P V of the tile two before, which waited for that tile's weights.  Those of the
+  // stages are waited for by loaders and issuers, which go through every tile, whether or not a half has rows.  The slots'
+  // are the exception: the softmax of a half without rows passes over a unit's tiles, and its next tile may be many phases
+  // ahead of the slot's barrier, where a wait by parity means nothing.  It therefore waits for its scores first.  Their products
+  // were issued after KF of the tile, which every loader warp arrives on after SC, so that the slot's phase is complete
+  // by then; and it is the last one that is, for a slot is written again only after the scores two tiles on, which follow
+  // this tile's weights.
   static constexpr int B_QF = 0, B_PV = 2, B_SF = 6, B_PF = 10, B_DRAIN = 14, B_KF = 15, B_KE = B_KF + STAGES, B_VF = B_KE + STAGES,
                        B_VE = B_VF + STAGES, B_SC = B_VE + STAGES, B_COUNT = B_SC + SLOTS;
   static constexpr uint32_t OFF_MISC = OFF_BAR + (B_COUNT * 8 + 15) / 16 * 16, USED = OFF_MISC + 16;
@@ -332,8 +338,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
 
         for (int t = 0; t < count; ++t) {
           const int k = done + t, buf = k & 1;       // tiles of this half so far
-          ok = mbar_wait(bar(L::B_SC + (n + t) % L::SLOTS), (uint32_t)((n + t) / L::SLOTS) & 1u, watch, CODE_SOFTMAX) &&
-               mbar_wait(bar(L::B_SF + 2 * g + buf), (uint32_t)(k >> 1) & 1u, watch, CODE_SOFTMAX);
+          ok = mbar_wait(bar(L::B_SF + 2 * g + buf), (uint32_t)(k >> 1) & 1u, watch, CODE_SOFTMAX) &&
+               mbar_wait(bar(L::B_SC + (n + t) % L::SLOTS), (uint32_t)((n + t) / L::SLOTS) & 1u, watch, CODE_SOFTMAX);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();

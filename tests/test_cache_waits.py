@@ -64,3 +64,122 @@ def test_the_products_are_drained_before_their_memory_is_freed(source):
     drain, commit, free = (source.index(x) for x in ("drain_wait(bar(L::B_DRAIN)", "tc_commit(bar(L::B_DRAIN))", "tcgen05.dealloc"))
     assert commit < drain < free
     assert not re.search(r"mbar_wait\(bar\(L::B_DRAIN\)", source)
+
+
+# ---- the barriers of the two-half form, as processes in any order -----------------------------------------------------
+# Every wait of the kernel is by parity, which says what is meant only while the barrier stands in the phase that is waited
+# for or just past it.  The processes below make the kernel's arrivals and waits for random units of one and two halves;
+# a scheduler runs them in random order and notes each wait that passes at any other phase.
+
+STAGES, SLOTS = 2, 4
+
+
+class _Bar:
+    def __init__(self, count):
+        self.count, self.left, self.done = count, count, 0
+
+    def arrive(self):
+        self.left -= 1
+        if self.left == 0:
+            self.left, self.done = self.count, self.done + 1
+
+
+def _run_protocol(units, rng, scores_first):
+    bars = {}
+
+    def bar(name, *at):
+        count = 2 if name in ("KE", "VE") else 1
+        return bars.setdefault((name,) + at, _Bar(count))
+    wrong, pipe = [], [[], []]
+
+    def wait(phase, name, *at):
+        while (bar(name, *at).done - 1) & 1 != phase & 1:
+            yield
+        if bar(name, *at).done != phase + 1:
+            wrong.append((name, at, phase, bar(name, *at).done))
+
+    def loader():
+        for n in range(sum(count for count, _ in units)):
+            yield from wait(n // STAGES - 1, "KE", n % STAGES)
+            bar("SC", n % SLOTS).arrive()
+            yield
+            bar("KF", n % STAGES).arrive()
+            yield from wait(n // STAGES - 1, "VE", n % STAGES)
+            bar("VF", n % STAGES).arrive()
+            yield
+
+    def issuer(g):
+        n = k = segments = 0
+
+        def scores(n, to):
+            yield from wait(n // STAGES, "KF", n % STAGES)
+            pipe[g].append([("SF", g, to), ("KE", n % STAGES)])
+        for count, halves in units:
+            if g < halves:
+                yield from wait(segments, "QF", g)
+                segments += 1
+                yield from scores(n, k & 1)
+                for t in range(count):
+                    if t + 1 < count:
+                        yield from scores(n + t + 1, (k + 1) & 1)
+                    yield from wait((n + t) // STAGES, "VF", (n + t) % STAGES)
+                    yield from wait(k >> 1, "PF", g, k & 1)
+                    pipe[g].append([("PV", g, k & 1), ("VE", (n + t) % STAGES)])
+                    k += 1
+            else:
+                for t in range(count):
+                    yield from wait((n + t) // STAGES, "KF", (n + t) % STAGES)
+                    bar("KE", (n + t) % STAGES).arrive()
+                    yield from wait((n + t) // STAGES, "VF", (n + t) % STAGES)
+                    bar("VE", (n + t) % STAGES).arrive()
+            n += count
+
+    def tensor(g):
+        while True:
+            if pipe[g]:
+                for at in pipe[g].pop(0):
+                    bar(*at).arrive()
+            yield
+
+    def softmax(g):
+        n = done = 0
+        for count, halves in units:
+            if g < halves:
+                bar("QF", g).arrive()
+                for t in range(count):
+                    k = done + t
+                    waits = [("SF", k >> 1, (g, k & 1)), ("SC", (n + t) // SLOTS, ((n + t) % SLOTS,))]
+                    for name, phase, at in waits if scores_first else reversed(waits):
+                        yield from wait(phase, name, *at)
+                    if t and rng.random() < 0.5:
+                        yield from wait((k - 1) >> 1, "PV", g, (k & 1) ^ 1)
+                    bar("PF", g, k & 1).arrive()
+                    yield
+                done += count
+                yield from wait((done - 1) >> 1, "PV", g, (done - 1) & 1)
+            n += count
+
+    live = [loader(), issuer(0), issuer(1), softmax(0), softmax(1)]
+    unit, steps = [tensor(0), tensor(1)], 0
+    while live:
+        steps += 1
+        assert steps < 200000, "the processes wait for one another"
+        p = rng.choice(live + unit + [live[rng.randrange(len(live))]] * rng.randrange(20))   # (some run ahead for a while)
+        try:
+            next(p)
+        except StopIteration:
+            live.remove(p)
+    return wrong
+
+
+def test_every_wait_finds_its_barrier_where_it_expects_it(source):
+    import random
+    seen = set()
+    for seed in range(120):
+        rng = random.Random(seed)
+        units = [(rng.choice([1, 2, 3, 7, 12, 20]), rng.choice([1, 2])) for _ in range(rng.randrange(1, 8))]
+        assert _run_protocol(units, rng, True) == []
+        seen.update(w[0] for w in _run_protocol(units, rng, False))
+    assert seen == {"SC"}                            # what the order of a tile's two waits is for
+    scores, scales = (source.index("mbar_wait(bar(L::%s" % b) for b in ("B_SF", "B_SC"))
+    assert scores < scales
