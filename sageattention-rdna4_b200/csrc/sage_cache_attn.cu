@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   uint32_t qf[NB][KSTEPS][2];                        // Q^T: k-step s of query row 8 nb + g
   float row_c[NB][2];                                // score factor of rows 8 nb + 2c + {0, 1}
   int row_lim[NB][2], row_tok[NB][2];                // keys that a row may see; its token within the sequence
-  float m[NB][2], l[NB][2], nf[NB][2];               // running maximum, this lane's sum, factor N
+  float m[NB][2], l[NB][2], lc[NB][2], nf[NB][2];    // running maximum, this lane's sum and what its rounding carries, factor N
   float o[NB][KSTEPS][4];                            // O^T: columns 16g + 2j + {0, 1} of rows 8 nb + 2c + {0, 1}
   int plain_end = 0;                                 // keys below this need no mask
 
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           const int r2 = 8 * nb + 2 * c + e, tok2 = (cur.rt * ROWS + r2) / a.group;
           row_tok[nb][e] = tok2;
           row_lim[nb][e] = r2 < live ? (a.tree ? cur.s.len : min(cur.s.len, ctx + tok2 + 1)) : 0;
-          m[nb][e] = NO_MAX; l[nb][e] = 0.f; nf[nb][e] = 0.f;
+          m[nb][e] = NO_MAX; l[nb][e] = 0.f; lc[nb][e] = 0.f; nf[nb][e] = 0.f;
         }
 #pragma unroll
         for (int j = 0; j < KSTEPS; ++j)
@@ -347,6 +347,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           m[nb][x] = top;
           nf[nb][x] = n_new;
           l[nb][x] *= fade;
+          lc[nb][x] *= fade;
 #pragma unroll
           for (int j = 0; j < KSTEPS; ++j) { o[nb][j][x] *= scale; o[nb][j][2 + x] *= scale; }
 #pragma unroll
@@ -359,9 +360,9 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           if (s[i >> 2][nb][i & 3] == -INFINITY) w[i >> 2][i & 3] = 0.f;
       }
 #pragma unroll
+      for (int x = 0; x < 2; ++x) add_carrying(l[nb][x], lc[nb][x], (p[0][x] + p[0][2 + x]) + (p[1][x] + p[1][2 + x]));
+#pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
-        l[nb][0] += p[blk][0] + p[blk][2];
-        l[nb][1] += p[blk][1] + p[blk][3];
         const __half2 u = __floats2half2_rn(w[blk][0], w[blk][1]), v = __floats2half2_rn(w[blk][2], w[blk][3]);
         pf[blk][nb][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&u));
         pf[blk][nb][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&v));

@@ -178,6 +178,13 @@ __device__ __forceinline__ void enter_line(const CacheAttnKArgs& a, Cursor& c, u
   if (at >= c.n_kt) next_unit(a, c, at, rows, keys);
 }
 
+// sum += x with the rounding error carried along: a row may see 2^30 keys, and weights that are each below the last bit of
+// the sum so far still count.
+__device__ __forceinline__ void add_carrying(float& sum, float& carry, float x) {
+  const float y = x - carry, t = sum + y;
+  carry = (t - sum) - y;
+  sum = t;
+}
 __device__ __forceinline__ float fast_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -332,8 +332,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         const int plain_end = a.tree ? max(ctx, 0) : max(0, min(cur.s.len, ctx + first_row / a.group + 1));   // keys below need no mask
         const int lim = exists ? (a.tree ? cur.s.len : min(cur.s.len, ctx + tok + 1)) : 0;
         const uint8_t* tree_row = a.tree ? a.tree + (long long)(cur.s.q0 + tok) * a.tree_st : nullptr;
-        // m: running maximum of e; l: sum of the weights of V over their scales
-        float m = NO_MAX, l = 0.f;
+        // m: running maximum of e; l: sum of the weights of V over their scales, and what its rounding carries
+        float m = NO_MAX, l = 0.f, l_carry = 0.f;
         const float2 c2 = make_float2(row_c, row_c);
 
         for (int t = 0; t < count; ++t) {
@@ -415,6 +415,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
             const float fade = fast_ex2(m - top);
             m = top;
             l *= fade;
+            l_carry *= fade;
             if (t > 0) {                             // (the unit's first product overwrites the accumulator)
               ok = __all_sync(0xffffffffu, mbar_wait(bar(L::B_PV + 2 * g + (buf ^ 1)), (uint32_t)((k - 1) >> 1) & 1u, watch, CODE_SOFTMAX));
               if (!ok) break;
@@ -430,7 +431,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
               }
             }
           }
-          float2 l2 = make_float2(l, 0.f);
+          float2 l2 = make_float2(0.f, 0.f);
           const float2 nm2 = make_float2(-m, -m);
 #pragma unroll
           for (int ch = 0; ch < 2; ++ch) {
@@ -449,7 +450,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
             }
             tmem_st16(s_addr + 16 * ch, pw);         // over the scores, which are in registers
           }
-          l = l2.x + l2.y;
+          add_carrying(l, l_carry, l2.x + l2.y);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();

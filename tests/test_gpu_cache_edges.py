@@ -173,3 +173,34 @@ def test_a_nan_in_one_of_key_and_value(t, which, lens):
         assert ((lse - clean_lse)[hit].abs() <= 2e-5 * clean_lse[hit].abs().clamp(min=1)).all()
     else:
         assert torch.isnan(lse[hit]).all()
+
+
+# One key whose weight dwarfs that of each of the others, which together still count: 262 144 of them at 2^-25.2.  Units are
+# not cut (there are more than the GPU has places for, all of them over the same two pages), so that a row's maximum
+# is that key's throughout.
+def _dominated(t, n_seq, n=262144, d=128, hkv=8, page=256):
+    cache = S.SageCache.empty(2, page, hkv, d, int8=True)
+    k, v = torch.zeros((2 * page, hkv, d), dtype=torch.float16, device="cuda"), torch.ones((2 * page, hkv, d), dtype=torch.float16, device="cuda")
+    k[0] = 1.544                                     # times 1 / sqrt(128) and log2(e), over 128 columns: 25.2
+    S.sage_cache_write(cache, k, v, torch.arange(2 * page, device="cuda"))
+    table = torch.ones((1, n // page), dtype=torch.int32, device="cuda")
+    table[0, 0] = 0
+    q = torch.ones((n_seq * t, 4 * hkv, d), dtype=torch.float16, device="cuda")
+    lens = torch.full((n_seq,), n, dtype=torch.int32, device="cuda")
+    top = (cache.k_codes[0, 0, 0].double() * cache.k_scale[0, 0, 0].double()).sum() * d ** -0.5
+    row = torch.arange(t, device="cuda").repeat(n_seq)
+    others = (n - t + row).double()                  # keys of weight 1 that the row sees beside the first
+    lse = torch.logaddexp(top, others.log())
+    return cache, table.expand(n_seq, -1), q, lens, lse[:, None].expand(-1, 4 * hkv)
+
+
+DOMINATED = [(1, 160), (6, 160), (12, 40), (40, 40)]
+
+
+@pytest.mark.parametrize("t,n_seq", DOMINATED)
+def test_the_sum_of_small_weights_beside_a_dominant_one(t, n_seq):
+    """The LSE's bound is that of every other call: 2e-5 max(1, |lse|)."""
+    cache, table, q, lens, want = _dominated(t, n_seq)
+    _, lse = S.sageattn_cached(q, cache, table, lens, return_lse=True)
+    off = ((lse.double() - want).abs() / want.abs().clamp(min=1)).max().item()
+    assert off <= 2e-5, off
