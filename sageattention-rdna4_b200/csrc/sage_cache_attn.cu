@@ -19,10 +19,12 @@
 //
 // Numerics.  Q in fp16: bf16 rows are scaled by a power of two each, which is undone in the score's factor, so
 // that no bit is lost but in elements 2^-28 below their row's largest.  Scores, maxima, sums and outputs in
-// fp32.  A weight enters the second product as fp16(p * v_scale * N), where N is a factor per row that keeps the
-// largest one seen near 1 (fp16 has 11 bits there; its relative error, 2^-11, is that of the output format).
-// The running maximum moves only when a score passes it by 2^14, and N when a product does: the accumulator is
-// rarely touched, weights stay below fp16's 65504 and keep its 11 bits down to 2^-14, and fp32 sums lose nothing by it.
+// fp32.  A weight enters the second product as fp16(p * v_scale * N), where N is a factor per row that puts the
+// largest one seen between 2^4 and 2^15 (fp16 has 11 bits there; its relative error, 2^-11, is that of the output format).
+// The running maximum moves only when a score passes it by 2^15, and N when a weight does: the accumulator is
+// rarely touched.  Weights keep 11 bits down to 2^-18 of the row's largest, 2^-29 of it is what each may lose, and the fp32
+// accumulator loses up to 2^-23 of its sum with every 16 keys: what bounds a row of very many keys (2^20: 2^-7 at worst, where
+// all errors have one sign).
 //
 // Work.  The steps of 32 keys of all (sequence, K/V head, row tile) units are numbered in one line, and every
 // warp of the GPU takes an equal stretch of it, by itself: its own ring of cp.async stages, no barrier, no spinning
@@ -43,6 +45,7 @@ namespace {
 
 constexpr int CA_WARPS = 4, CA_THREADS = 32 * CA_WARPS;
 constexpr int CA_KEYS = 32;                    // keys of a step: two blocks of 16
+constexpr float LIMIT = (float)(1 << LIMIT_LOG2);
 
 __device__ __forceinline__ uint2 lds8(uint32_t addr) {
   uint2 v;
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           p_top = fmaxf(p_top, p[blk][e]);
           w_top = fmaxf(w_top, w[blk][e]);
         }
-      if (__any_sync(0xffffffffu, fmaxf(p_top, w_top) > 16384.f)) {
+      if (__any_sync(0xffffffffu, fmaxf(p_top, w_top) > LIMIT)) {
         // new maxima and factors; the sums and the accumulator follow
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -324,8 +327,8 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
             if (s[i >> 1][nb][2 * (i & 1) + x] != -INFINITY) big = fmaxf(big, w[i >> 1][2 * (i & 1) + x]);
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, sh));
-          if (!(top > m[nb][x] + 14.f || big > 16384.f)) top = m[nb][x];
-          const bool move = top != m[nb][x] || big > 16384.f;
+          if (!(top > m[nb][x] + LIMIT_LOG2 || big > LIMIT)) top = m[nb][x];
+          const bool move = top != m[nb][x] || big > LIMIT;
           const float fade = fast_ex2(m[nb][x] - top);
           big = 0.f;
 #pragma unroll
@@ -336,13 +339,13 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           }
 #pragma unroll
           for (int sh = 4; sh < 32; sh <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, sh));
+          // N for the largest weight of this step, or what leaves the accumulator as it is where that holds larger ones
+          // (nothing but values of 0 here, or fade 0: infinite, the other one counts; both: there is nothing to scale)
           float n_new = nf[nb][x], scale = fade;
-          if (move && big > 0.f) {
-            n_new = __fdividef(1.f, big);
-            if (nf[nb][x] > 0.f) {
-              n_new = fminf(n_new, __fdividef(nf[nb][x], fade));       // (fade 0: infinite, the new one counts)
-              scale = fade * __fdividef(n_new, nf[nb][x]);
-            }
+          const float n_least = fminf(__fdividef((float)(1 << TOP_LOG2), big), n_new > 0.f ? __fdividef(n_new, fade) : INFINITY);
+          if (move && n_least < INFINITY) {
+            if (n_new > 0.f) scale = fade * __fdividef(n_least, n_new);
+            n_new = n_least;
           }
           m[nb][x] = top;
           nf[nb][x] = n_new;

@@ -11,6 +11,13 @@ namespace sage {
 
 constexpr float LN2_F = 0.6931471805599453f;
 constexpr float NO_MAX = -3.0e38f;
+// Weights of V enter their product in fp16.  A row's largest one is put at 2^TOP_LOG2, and the row is scaled anew once one
+// passes 2^LIMIT_LOG2 (fp16 ends below 2^16): a weight keeps its 11 bits down to 2^-18 of the largest and is lost below 2^-29 of
+// it.  At 2^0 that was 2^-25: 262 144 keys at 2^-25.2 of a first one, 6.8e-3 of the output.  The room above keeps rows from being
+// scaled anew with every new maximum: 8 x 16 384 keys, some of them four times as large as the others, 256 rows: 204.8 us at
+// 2^0, 211.2 at 2^4, 214.5 at 2^6, 217 at 2^8; 32 rows 105.6, 108, 110.5, 109.6.  Beyond 2^4 nothing is to be had: the fp32
+// accumulators lose up to 2^-23 of the sum per 16 keys, more than this.
+constexpr int TOP_LOG2 = 4, LIMIT_LOG2 = 15;
 
 struct CacheAttnKArgs {
   const void* q;

@@ -19,7 +19,7 @@
 // free, and that of V's is undone where the output is written).
 //
 // The scale of V goes into the exponent: e = score + log2(scale), the weight is 2^(e - m) and the row's sum takes the weight
-// over the scale, so that one maximum serves both the softmax and fp16's range.
+// over the scale, so that one maximum serves both the softmax and fp16's range: m is 2^TOP_LOG2 below the largest e.
 //
 // NQ = 2 (rows beyond 128): one CTA per SM with all 512 TMEM columns.  NQ = 1: two CTAs per SM.  (Rows are added to a
 // CTA before CTAs are: a tile's codes are fetched and converted once per CTA.  Figures of both: cache_form.)
@@ -409,9 +409,9 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
 #pragma unroll
             for (int i = 0; i < 64; ++i) top = fmaxf(top, fmaf(__uint_as_float(x[i]), row_c, lv[i]));
           }
-          if (__any_sync(0xffffffffu, top > m + 14.f)) {
-            // the maximum moves; the sum and the accumulator follow (weights stay below 2^14: fp16 keeps 11 bits from there to 2^-14)
-            top = top > m + 14.f ? top : m;          // (each row by itself)
+          if (__any_sync(0xffffffffu, top > m + LIMIT_LOG2)) {
+            // the maximum moves; the sum and the accumulator follow
+            top = top > m + LIMIT_LOG2 ? top - TOP_LOG2 : m;           // (each row by itself)
             const float fade = fast_ex2(m - top);
             m = top;
             l *= fade;
@@ -536,7 +536,9 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       if (ct < KT) {
         const uint32_t sc = base + L::OFF_SC + (n % L::SLOTS) * L::SLOT;
         const bool none = sk < 0.f, nan_k = isnan(sk), nan_v = !nan_k && isnan(sv);
-        const float v = none || nan_k || nan_v ? 1.f : fmaxf(sv, 1e-30f);             // (0: a row that nothing wrote, all codes 0; a part of the sum)
+        // (0: a row that nothing wrote, all codes 0, a part of the sum; written ones are 1e-12 at least.  The sum takes weights of
+        // up to 2^LIMIT_LOG2 over this: 2^30 keys of them stay below fp32's largest.)
+        const float v = none || nan_k || nan_v ? 1.f : fmaxf(sv, 1e-20f);
         sts_f32(sc + 4 * ct, none || nan_k ? 1.f : fmaxf(sk, 1e-30f));
         sts_f32(sc + L::SLOT_LV + 4 * ct, __log2f(v));
         sts_f32(sc + L::SLOT_RV + 4 * ct, __fdividef(1.f, v));

@@ -198,9 +198,40 @@ DOMINATED = [(1, 160), (6, 160), (12, 40), (40, 40)]
 
 
 @pytest.mark.parametrize("t,n_seq", DOMINATED)
+def test_small_weights_beside_a_dominant_one(t, n_seq):
+    """Values of 1: every output is 1.  A weight is off by 2^-11 of itself, or by 2^-25 where fp16 is subnormal, and the row's
+    largest stands at 2^4 at least: 2^-29 of it per key.  The matrix instructions add 16 keys at a time to an fp32 accumulator: 2^-23
+    of the sum each time.  As above, 1.25 covers the fp32 parts beside these, and half a step is the output's."""
+    n = 262144
+    cache, table, q, lens, _ = _dominated(t, n_seq, n)
+    out = S.sageattn_cached(q, cache, table, lens)
+    off = (out.double() - 1).abs().max().item()
+    assert off <= 1.25 * 2.0 ** -11 + n * 2.0 ** -29 + n / 16 * 2.0 ** -23 + 2.0 ** -11, off
+
+
+@pytest.mark.parametrize("t,n_seq", DOMINATED)
 def test_the_sum_of_small_weights_beside_a_dominant_one(t, n_seq):
     """The LSE's bound is that of every other call: 2e-5 max(1, |lse|)."""
     cache, table, q, lens, want = _dominated(t, n_seq)
     _, lse = S.sageattn_cached(q, cache, table, lens, return_lse=True)
     off = ((lse.double() - want).abs() / want.abs().clamp(min=1)).max().item()
     assert off <= 2e-5, off
+
+
+@pytest.mark.parametrize("t", ROWS)
+def test_rows_that_nothing_wrote(t):
+    """Keys and values of zero: outputs of zero, an LSE of the keys' number, whatever is seen beside them."""
+    cache = S.SageCache.empty(4, 64, 2, 128)
+    q = torch.randn((t, 8, 128), device="cuda").half()
+    table = torch.arange(4, dtype=torch.int32, device="cuda").repeat(1, 256)           # 65 536 keys
+    for n in (t, 200, 65536):
+        out, lse = S.sageattn_cached(q, cache, table, torch.tensor([n], dtype=torch.int32, device="cuda"), return_lse=True)
+        want = (n - t + 1 + torch.arange(t, device="cuda")).double().log()[:, None]
+        assert (out == 0).all() and ((lse.double() - want).abs() <= 2e-5 * want.clamp(min=1)).all()
+    v = torch.full((1, 2, 128), 50000.0, dtype=torch.float16, device="cuda")
+    S.sage_cache_write(cache, torch.zeros_like(v), v, torch.zeros(1, dtype=torch.int64, device="cuda"))
+    out, lse = S.sageattn_cached(q, cache, table[:, :4], torch.tensor([256], dtype=torch.int32, device="cuda"), return_lse=True)
+    n = (256 - t + 1 + torch.arange(t, device="cuda")).double()[:, None]
+    assert ((lse.double() - n.log()).abs() <= 2e-5 * n.log()).all()
+    value = 448.0 * cache.v_scale[0, 0, 0].item()
+    assert ((out.double() - value / n[..., None]).abs() <= 1.25 * 2.0 ** -11 * value / n[..., None] + 2.0 ** -11 * value / n[..., None]).all()
