@@ -7,6 +7,7 @@ import torch
 import cache_reference as R
 import sageattention as S
 from sageattention import cache as C
+from test_gpu_cache_attention import _check            # a call against the formula, with that file's bound
 
 pytestmark = pytest.mark.gpu
 
@@ -235,3 +236,29 @@ def test_rows_that_nothing_wrote(t):
     assert ((lse.double() - n.log()).abs() <= 2e-5 * n.log()).all()
     value = 448.0 * cache.v_scale[0, 0, 0].item()
     assert ((out.double() - value / n[..., None]).abs() <= 1.25 * 2.0 ** -11 * value / n[..., None] + 2.0 ** -11 * value / n[..., None]).all()
+
+
+# ---- every form of attention by kind of codes, page and width ------------------------------------------------------------
+# e4m3 keys (the rule for bfloat16) and int8 ones, more than 32 and more than 128 rows per K/V head.
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("d", [8, 40, 64, 72, 96, 128])
+def test_many_rows_of_any_width_and_page(d, page):
+    _check([300, 12, 77], [12, 5, 12], 4, 1, d, page, torch.bfloat16, False, tree=True, shift=True)
+    _check([300, 41], [12, 12], 4, 1, d, page, torch.float16, True, shift=True)
+    _check([290, 40], [40, 33], 4, 1, d, page, torch.float16, False, shift=True)
+    _check([600], [40], 4, 1, d, page, torch.bfloat16, True, tree=True, shift=True)
+
+
+@pytest.mark.parametrize("int8", [True, False])
+@pytest.mark.parametrize("t", ROWS)
+def test_long_sequences_that_are_cut_and_joined(t, int8):
+    _check([7000, 90, 3001], [t, t, max(1, t // 3)], 8, 2, 128, 32, torch.bfloat16, int8, tree=True)
+    _check([5003], [t], 4, 1, 64, 128, torch.float16, int8, shift=True)
+
+
+@pytest.mark.parametrize("batch,t", [(160, 3), (120, 6), (90, 12), (40, 40)])
+def test_many_short_sequences_of_e4m3_keys(batch, t):
+    """More units than places: most of them whole, some cut."""
+    lens = [(37 * i) % 90 + (t if i % 5 else 0) for i in range(batch)]
+    _check(lens, [t if i % 4 else max(1, t // 2) for i in range(batch)], 16, 4, 64, 16, torch.bfloat16, False, tree=t % 2 == 1, shift=True)
