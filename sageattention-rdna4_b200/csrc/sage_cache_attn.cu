@@ -563,7 +563,8 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
       if (a.shift != nullptr)
         v += shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(s.q0 + tok) * a.q_st + (long long)head * a.q_sh, h, width, lane);
       if (lane == 0) a.lse[(long long)(s.q0 + tok) * a.Hq + head] = v;
-    }  }
+    }
+  }
 }
 
 constexpr int CTAS_PER_SM = 2;
@@ -634,8 +635,7 @@ CacheForm cache_form(int64_t rows) {
   return rows <= 128 ? CacheForm{true, 128, 64, 2 * SIZING_SMS} : CacheForm{true, 256, 64, SIZING_SMS};
 }
 
-size_t cache_attention_scratch(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q) {
-  (void)n_seq;
+size_t cache_attention_scratch(int64_t Hq, int64_t Hkv, int64_t max_q) {
   const int64_t rows = max_q * (Hq / Hkv);
   const CacheForm f = cache_form(rows);
   return (size_t)2 * f.max_stretches * std::min<int64_t>(rows, f.rows) * (HD * sizeof(float) + sizeof(float2));

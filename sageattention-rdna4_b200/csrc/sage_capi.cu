@@ -607,7 +607,7 @@ int sage_cache_read(const void* k_codes, const float* k_scale, const void* v_cod
 size_t sage_cache_attention_workspace_bytes(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q) {
   if (n_seq < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || max_q < 1) return 0;
   if (max_q > ((int64_t)1 << 28) / (Hq / Hkv)) return 0;               // more rows than sage_cache_attention takes
-  return align256(sage::cache_attention_scratch(n_seq, Hq, Hkv, max_q));
+  return align256(sage::cache_attention_scratch(Hq, Hkv, max_q));
 }
 
 int sage_cache_attention(const void* q, void* out, float* lse,

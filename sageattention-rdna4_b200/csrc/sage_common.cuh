@@ -97,16 +97,6 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
 }
 
-// Round-half-even to int8 with the [-128, 127] clamp, four codes per word (a in the low byte).
-__device__ __forceinline__ uint32_t i8_rne(float y) {
-  int q = __float2int_rn(y);
-  q = max(-128, min(127, q));
-  return (uint32_t)q & 0xFFu;
-}
-__device__ __forceinline__ uint32_t i8x4(float a, float b, float c, float d) {
-  return i8_rne(a) | (i8_rne(b) << 8) | (i8_rne(c) << 16) | (i8_rne(d) << 24);
-}
-
 // ---- quantising a row (one scale per token and head) -------------------------------------------------
 #ifdef __CUDACC__
 __device__ __forceinline__ float quarter_warp_max(float x) {

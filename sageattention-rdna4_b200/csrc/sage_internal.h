@@ -155,7 +155,7 @@ struct CacheAttnParams {
   void* scratch;                          // cache_attention_scratch() bytes
   int32_t* status_host;                   // optional, pinned host memory: receives a code when a bounded wait ran out
 };
-size_t cache_attention_scratch(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q);
+size_t cache_attention_scratch(int64_t Hq, int64_t Hkv, int64_t max_q);
 cudaError_t launch_cache_attention(const CacheView& c, const CacheAttnParams& p, cudaStream_t st);
 
 }  // namespace sage
