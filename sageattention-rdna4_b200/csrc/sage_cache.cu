@@ -37,16 +37,6 @@ template <bool WIDE> __device__ __forceinline__ void st_stream32(void* p, const 
   }
 }
 
-template <typename T> __device__ __forceinline__ uint32_t to_pair(float a, float b);
-template <> __device__ __forceinline__ uint32_t to_pair<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <> __device__ __forceinline__ uint32_t to_pair<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // The larger of two magnitudes, NaN if either is (fmaxf drops it).
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -136,7 +126,7 @@ __global__ void __launch_bounds__(CACHE_THREADS) rotary_kernel(const RotaryKArgs
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 t = cs[4 * item + e];
-          o[e] = to_pair<T>(x[2 * e] * t.x - x[2 * e + 1] * t.y, x[2 * e + 1] * t.x + x[2 * e] * t.y);
+          o[e] = pack2<T>(x[2 * e] * t.x - x[2 * e + 1] * t.y, x[2 * e + 1] * t.x + x[2 * e] * t.y);
         }
         st_stream(dst + at, make_uint4(o[0], o[1], o[2], o[3]));
       } else {
@@ -147,8 +137,8 @@ __global__ void __launch_bounds__(CACHE_THREADS) rotary_kernel(const RotaryKArgs
 #pragma unroll
         for (int e = 0; e < VEC / 2; ++e) {
           const float2 t0 = cs[VEC * item + 2 * e], t1 = cs[VEC * item + 2 * e + 1];
-          o[e] = to_pair<T>(x[2 * e] * t0.x - y[2 * e] * t0.y, x[2 * e + 1] * t1.x - y[2 * e + 1] * t1.y);
-          p[e] = to_pair<T>(y[2 * e] * t0.x + x[2 * e] * t0.y, y[2 * e + 1] * t1.x + x[2 * e + 1] * t1.y);
+          o[e] = pack2<T>(x[2 * e] * t0.x - y[2 * e] * t0.y, x[2 * e + 1] * t1.x - y[2 * e + 1] * t1.y);
+          p[e] = pack2<T>(y[2 * e] * t0.x + x[2 * e] * t0.y, y[2 * e + 1] * t1.x + x[2 * e + 1] * t1.y);
         }
         if (VEC == 8) {
           st_stream(dst + at, make_uint4(o[0], o[1], o[2], o[3]));
@@ -304,7 +294,7 @@ template <typename T, bool WIDE>
 __device__ __forceinline__ void store16(T* dst, const float2* x, bool lo, bool hi) {
   uint32_t w[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = to_pair<T>(x[i].x, x[i].y);
+  for (int i = 0; i < 8; ++i) w[i] = pack2<T>(x[i].x, x[i].y);
   st_stream32<WIDE>(dst, make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7]), lo, hi);
 }
 

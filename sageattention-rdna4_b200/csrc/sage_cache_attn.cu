@@ -63,27 +63,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// Four e4m3 codes -> two registers of two fp16 each.
-__device__ __forceinline__ void e4m3_quad(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
-      : "=r"(lo), "=r"(hi) : "r"(w));
-}
-// Four K codes -> two registers of two fp16 each.
-template <bool INT8>
-__device__ __forceinline__ void k_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if (INT8) {
-    const uint32_t t = w ^ 0x80808080u;                              // code + 128 in a byte; 0x6400 + it is 1024 + it
-    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));     // 1024 + 128
-    uint32_t u = __byte_perm(t, 0x64646464u, 0x4140), v = __byte_perm(t, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&u), bias), y = __hsub2(*reinterpret_cast<__half2*>(&v), bias);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  } else {
-    e4m3_quad(w, lo, hi);
-  }
-}
-
 // Shared memory of a CTA: a ring per warp.
 template <int WIDTH, int STAGES> struct CaSmem {
   static constexpr uint32_t CODES = CA_KEYS * WIDTH;
@@ -429,7 +408,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
               T* dst = reinterpret_cast<T*>(a.out) + (long long)(cur.s.q0 + tok) * a.o_st + (long long)head * a.o_sh + (WIDTH / 8) * g;
 #pragma unroll
               for (int j = 0; j < KSTEPS; ++j)
-                if ((WIDTH / 8) * g + 2 * j < a.D) *reinterpret_cast<uint32_t*>(dst + 2 * j) = pair16<T>(o[nb][j][x] * inv, o[nb][j][2 + x] * inv);
+                if ((WIDTH / 8) * g + 2 * j < a.D) *reinterpret_cast<uint32_t*>(dst + 2 * j) = pack2<T>(o[nb][j][x] * inv, o[nb][j][2 + x] * inv);
               if (a.lse != nullptr && g == 0) a.lse[(long long)(cur.s.q0 + tok) * a.Hq + head] = sum == 0.f ? -INFINITY : (m[nb][x] + __log2f(sum)) * LN2_F;
             } else {
               float* dst = a.part_o + (slot * a.part_rows + r) * WIDTH + (WIDTH / 8) * g;
@@ -539,7 +518,7 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
       const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
       // (the many-row kernel leaves the columns of wide heads in the order of its accumulator)
       const int n = 4 * lane, col = permuted && width == 128 ? 16 * ((n >> 3) & 7) + 8 * (n >> 6) + (n & 7) : n;
-      if (mine && col < a.D) *reinterpret_cast<uint2*>(dst + col) = make_uint2(pair16<T>(acc.x * inv, acc.y * inv), pair16<T>(acc.z * inv, acc.w * inv));
+      if (mine && col < a.D) *reinterpret_cast<uint2*>(dst + col) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
     } else {
       if (mine) *reinterpret_cast<float4*>(&acc_s[warp][4 * lane]) = acc;
       if (lane == 0) ml_s[warp] = make_float2(top, sum);

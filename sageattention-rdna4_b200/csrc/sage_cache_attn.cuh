@@ -226,14 +226,25 @@ __device__ __forceinline__ float shift_dot(const CacheAttnKArgs& a, const T* q, 
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   return d * a.sm_scale;
 }
-template <typename T> __device__ __forceinline__ uint32_t pair16(float a, float b);
-template <> __device__ __forceinline__ uint32_t pair16<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// Four e4m3 codes -> two registers of two fp16 each.
+__device__ __forceinline__ void e4m3_quad(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
 }
-template <> __device__ __forceinline__ uint32_t pair16<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
+// Four K codes -> two registers of two fp16 each.
+template <bool INT8>
+__device__ __forceinline__ void k_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (INT8) {
+    const uint32_t t = w ^ 0x80808080u;                              // code + 128 in a byte; 0x6400 + it is 1024 + it
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));     // 1024 + 128
+    uint32_t u = __byte_perm(t, 0x64646464u, 0x4140), v = __byte_perm(t, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&u), bias), y = __hsub2(*reinterpret_cast<__half2*>(&v), bias);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    e4m3_quad(w, lo, hi);
+  }
 }
 template <typename T> __device__ __forceinline__ T from_float(float x);
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }

@@ -147,19 +147,7 @@ template <bool INT8>
 __device__ __forceinline__ void codes_to_half(const uint4& u, uint32_t (&h)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (INT8) {
-      const uint32_t t = w[i] ^ 0x80808080u;         // code + 128 in a byte; 0x6400 + it is 1024 + it
-      const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-      const uint32_t a = __byte_perm(t, 0x64646464u, 0x4140), b = __byte_perm(t, 0x64646464u, 0x4342);
-      const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
-      h[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
-      h[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
-    } else {
-      asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
-          : "=r"(h[2 * i]), "=r"(h[2 * i + 1]) : "r"(w[i]));
-    }
-  }
+  for (int i = 0; i < 4; ++i) k_halves<INT8>(w[i], h[2 * i], h[2 * i + 1]);
 }
 
 constexpr int KT = 64;                               // keys of a tile
@@ -317,8 +305,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
               up = __uint_as_float((uint32_t)f << 23);
               back = f <= 253 ? __uint_as_float((uint32_t)(254 - f) << 23) : 5.877471754111438e-39f;
             }
-            u = make_uint4(pair16<__half>(x[0] * up, x[1] * up), pair16<__half>(x[2] * up, x[3] * up), pair16<__half>(x[4] * up, x[5] * up),
-                           pair16<__half>(x[6] * up, x[7] * up));
+            u = make_uint4(pack2<__half>(x[0] * up, x[1] * up), pack2<__half>(x[2] * up, x[3] * up), pack2<__half>(x[4] * up, x[5] * up),
+                           pack2<__half>(x[6] * up, x[7] * up));
           }
           *staged(row, WIDTH == 128 ? (c_l & 1) * 8 + (c_l >> 1) : c_l) = u;
           if (c_l == 0) row_at[row] = fmaxf(a.scale_log2 * back, 1.17549435e-38f);    // (a masked score stays -infinity)
@@ -444,8 +432,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
               const float2 w = make_float2(fast_ex2(u.x), fast_ex2(u.y)), z = make_float2(fast_ex2(v.x), fast_ex2(v.y));
               l2 = __ffma2_rn(w, make_float2(rv.x, rv.y), l2);
               l2 = __ffma2_rn(z, make_float2(rv.z, rv.w), l2);
-              pw[2 * i] = pair16<__half>(w.x, w.y);
-              pw[2 * i + 1] = pair16<__half>(z.x, z.y);
+              pw[2 * i] = pack2<__half>(w.x, w.y);
+              pw[2 * i + 1] = pack2<__half>(z.x, z.y);
             }
             tmem_st16(s_addr + 16 * ch, pw);         // over the scores, which are in registers
           }
@@ -473,7 +461,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
             tmem_ld_wait();
             uint32_t h[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = pair16<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            for (int i = 0; i < 8; ++i) h[i] = pack2<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
             *staged(r, 2 * ch) = make_uint4(h[0], h[1], h[2], h[3]);
             *staged(r, 2 * ch + 1) = make_uint4(h[4], h[5], h[6], h[7]);
           }
