@@ -424,7 +424,8 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
         for (int r = 0; r < live; ++r) {
           const int rr = cur.rt * ROWS + r, tok = rr / a.group, head = cur.h * a.group + rr - tok * a.group;
           const float d = shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(cur.s.q0 + tok) * a.q_st + (long long)head * a.q_sh, cur.h, WIDTH, lane);
-          if (lane == 0) a.lse[(long long)(cur.s.q0 + tok) * a.Hq + head] += d;
+          float* at = a.lse + (long long)(cur.s.q0 + tok) * a.Hq + head;
+          if (lane == 0 && *at != -INFINITY) *at += d;                  // (a row that sees no key stays, whatever its Q holds)
         }
         __syncwarp();
       }
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
     }
     if (a.lse != nullptr && share == WARPS_PER_ROW - 1) {
       float v = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * LN2_F;
-      if (a.shift != nullptr)
+      if (a.shift != nullptr && sum != 0.f)
         v += shift_dot(a, reinterpret_cast<const T*>(a.q) + (long long)(s.q0 + tok) * a.q_st + (long long)head * a.q_sh, h, width, lane);
       if (lane == 0) a.lse[(long long)(s.q0 + tok) * a.Hq + head] = v;
     }

@@ -500,7 +500,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
         tc_fence_before();
         if (exists && whole && a.lse != nullptr) {
           float v = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2_F;
-          if (dots) v += row_at[128 + r];            // the keys as they were before the shift was taken off
+          if (dots && l != 0.f) v += row_at[128 + r];                  // the keys as they were before the shift was taken off
           a.lse[(long long)(cur.s.q0 + tok) * a.Hq + cur.h * a.group + rr - tok * a.group] = v;
         }
         __syncwarp();                                // (the rows that passed through are read before the next Q is written)

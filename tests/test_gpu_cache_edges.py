@@ -262,3 +262,25 @@ def test_many_short_sequences_of_e4m3_keys(batch, t):
     """More units than places: most of them whole, some cut."""
     lens = [(37 * i) % 90 + (t if i % 5 else 0) for i in range(batch)]
     _check(lens, [t if i % 4 else max(1, t // 2) for i in range(batch)], 16, 4, 64, 16, torch.bfloat16, False, tree=t % 2 == 1, shift=True)
+
+
+@pytest.mark.parametrize("shift", [False, True])
+@pytest.mark.parametrize("t", ROWS)
+def test_padding_with_queries_of_anything(t, shift):
+    """A sequence without keys, one whose pages do not exist and a token that its mask leaves nothing, with queries that
+    are not finite: zeros and an LSE of -infinity."""
+    for bad in (math.nan, math.inf):
+        for n in (90, 3000):                         # whole units, and units that are cut
+            cache, table, q, lens, _ = _setup((n, n + 1, n + 2), t, dtype=torch.bfloat16, shift=shift)
+            mask = torch.ones((3 * t, t), dtype=torch.bool, device="cuda")
+            want, want_lse = S.sageattn_cached(q, cache, table, lens, tree_mask=mask, return_lse=True)
+            lens[1] = 0
+            table[2] = -1
+            q[t:] = bad
+            out, lse = S.sageattn_cached(q, cache, table, lens, tree_mask=mask, return_lse=True)
+            assert (out[t:] == 0).all() and (lse[t:] == -math.inf).all()
+            assert torch.isfinite(lse[:t]).all() and ((lse - want_lse)[:t].abs() <= 4e-5 * want_lse[:t].abs().clamp(min=1)).all()
+            lens[1] = t                              # only its own new tokens are cached, and masked
+            mask[t:2 * t] = False
+            out, lse = S.sageattn_cached(q, cache, table, lens, tree_mask=mask, return_lse=True)
+            assert (out[t:] == 0).all() and (lse[t:] == -math.inf).all()
