@@ -400,7 +400,7 @@ int sage_cache_read(const void* k_codes, const float* k_scale, const void* v_cod
  *               the keys up to its own token's
  * A row that sees no key is 0, its LSE -infinity.  Keys on a page that does not exist are not seen.  A row that sees a
  * key whose K or V scale is NaN is NaN (its LSE: NaN, or for V alone that of the scores); rows that do not see it keep
- * their bits.  out shares no memory with q.
+ * their bits.  A row of q that holds a NaN or an infinity is NaN if it sees a key.  out shares no memory with q.
  * Scores and sums in fp32; the weights of V are rounded to fp16: 2^-11 of each, or, where that is more, 2^-29 of the
  * row's largest times the largest |v|; the sum of weighted values takes up to 2^-23 of itself with every 16 keys.
  * What a result depends on: the keys are walked in

@@ -199,9 +199,8 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
         }
 #pragma unroll
         for (int s = 0; s < KSTEPS; ++s) {
-          const __half2 u = __floats2half2_rn(x[4 * s], x[4 * s + 1]), v = __floats2half2_rn(x[4 * s + 2], x[4 * s + 3]);
-          qf[nb][s][0] = *reinterpret_cast<const uint32_t*>(&u);
-          qf[nb][s][1] = *reinterpret_cast<const uint32_t*>(&v);
+          qf[nb][s][0] = inf_to_nan(pack2<__half>(x[4 * s], x[4 * s + 1]));
+          qf[nb][s][1] = inf_to_nan(pack2<__half>(x[4 * s + 2], x[4 * s + 3]));
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

@@ -226,6 +226,12 @@ __device__ __forceinline__ float shift_dot(const CacheAttnKArgs& a, const T* q, 
   for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
   return d * a.sm_scale;
 }
+// Two fp16 values of Q, an infinity as a NaN.  A row that holds one has no softmax; its scores may all be -infinity, which is what
+// a key that is not seen gets.
+__device__ __forceinline__ uint32_t inf_to_nan(uint32_t w) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&w), x = __hfma2(h, __half2half2(__ushort_as_half(0)), h);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
 // Four e4m3 codes -> two registers of two fp16 each.
 __device__ __forceinline__ void e4m3_quad(uint32_t w, uint32_t& lo, uint32_t& hi) {
   asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\t"

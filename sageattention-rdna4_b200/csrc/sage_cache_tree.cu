@@ -308,6 +308,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
             u = make_uint4(pack2<__half>(x[0] * up, x[1] * up), pack2<__half>(x[2] * up, x[3] * up), pack2<__half>(x[4] * up, x[5] * up),
                            pack2<__half>(x[6] * up, x[7] * up));
           }
+          u = make_uint4(inf_to_nan(u.x), inf_to_nan(u.y), inf_to_nan(u.z), inf_to_nan(u.w));
           *staged(row, WIDTH == 128 ? (c_l & 1) * 8 + (c_l >> 1) : c_l) = u;
           if (c_l == 0) row_at[row] = fmaxf(a.scale_log2 * back, 1.17549435e-38f);    // (a masked score stays -infinity)
         }

@@ -329,7 +329,9 @@ def sageattn_cached(q: torch.Tensor, cache: SageCache, page_table: torch.Tensor,
     return_lse : also return the fp32 log-sum-exp ``(tokens, Hq)`` of ``sm_scale * q.k``.
     out : optional output of q's shape and dtype, which shares no memory with q.
     A token that sees no key gets zeros and an LSE of -infinity; one that sees a key whose row of K or V held a NaN or an
-    infinity gets NaN (its LSE: NaN, or for V alone that of the keys' scores).  The lengths stay on the GPU; the last bits
+    infinity gets NaN (its LSE: NaN, or for V alone that of the keys' scores), and so does one that sees a key and whose query
+    holds one (its LSE too).  A key on a page that does not exist is not seen.  Rows of no sequence, and those past
+    `max_seqlen_q` of theirs, are left as they are (in fresh outputs: undefined).  The lengths stay on the GPU; the last bits
     of a result depend on the lengths of the other sequences of the call (fp32 sums in another order).  Forward only: the
     result carries no gradient, as that of `sageattn`.
     """

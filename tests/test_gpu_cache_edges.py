@@ -284,3 +284,20 @@ def test_padding_with_queries_of_anything(t, shift):
             mask[t:2 * t] = False
             out, lse = S.sageattn_cached(q, cache, table, lens, tree_mask=mask, return_lse=True)
             assert (out[t:] == 0).all() and (lse[t:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("t", ROWS)
+def test_queries_that_are_not_finite(t, dtype):
+    """NaN for the row, whatever the signs of its scores, and no bit of another row."""
+    for n in (t, 200, 3000):
+        cache, table, q, lens, _ = _setup((n, n + 5), t, dtype=dtype)
+        mask = torch.eye(t, dtype=torch.bool, device="cuda").repeat(2, 1)
+        want, want_lse = S.sageattn_cached(q, cache, table, lens, tree_mask=mask, return_lse=True)
+        for at, value in (((0, 1, 5), math.inf), ((0, 2, 64), -math.inf), ((2 * t - 1, 6, 127), -math.inf), ((2 * t - 1, 7, 0), math.nan)):
+            q[at] = value
+        hit = ~torch.isfinite(q).all(-1)
+        assert hit.sum() == 4
+        out, lse = S.sageattn_cached(q, cache, table, lens, tree_mask=mask, return_lse=True)
+        assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all()
+        assert torch.equal(out[~hit], want[~hit]) and torch.equal(lse[~hit], want_lse[~hit])
