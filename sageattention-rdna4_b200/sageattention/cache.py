@@ -6,7 +6,8 @@
     sage_cache_write(cache, k, v, slots)                        # quantised as it is written
     out = sageattn_cached(q, cache, page_table, seqlens_k)      # one new token per sequence
     out = sageattn_cached(q, cache, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q, tree_mask=mask)
-    k16, v16 = sage_cache_read(cache, page_table, cu_seqlens_k, total)      # e.g. for sageattn_varlen
+    out = sageattn_cached(q, cache, page_table, seqlens_k, cu_seqlens_q, max_seqlen_q)      # the next chunk of a prompt: a chain
+    k16, v16 = sage_cache_read(cache, page_table, cu_seqlens_k, total)      # e.g. for sageattn_varlen without a causal mask
 
 The reference keeps no cache: its callers hand over the whole K and V with every call, which are then
 quantised again (sageattention/core.py:1037-1252).  Codes and scales here are those of its quantiser

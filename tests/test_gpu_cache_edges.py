@@ -301,3 +301,10 @@ def test_queries_that_are_not_finite(t, dtype):
         out, lse = S.sageattn_cached(q, cache, table, lens, tree_mask=mask, return_lse=True)
         assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all()
         assert torch.equal(out[~hit], want[~hit]) and torch.equal(lse[~hit], want_lse[~hit])
+
+
+@pytest.mark.parametrize("dtype,int8", [(torch.float16, True), (torch.bfloat16, False)])
+def test_a_chunk_of_a_prompt_continues_a_cached_one(dtype, int8):
+    """Many row tiles per sequence, as a chain: the way to go on with a prompt whose first part is cached."""
+    _check([1600, 300, 257], [600, 1, 257], 2, 1, 128, 64, dtype, int8, shift=True)
+    _check([700, 690], [700, 333], 3, 3, 72, 16, dtype, int8)
