@@ -308,3 +308,35 @@ def test_a_chunk_of_a_prompt_continues_a_cached_one(dtype, int8):
     """Many row tiles per sequence, as a chain: the way to go on with a prompt whose first part is cached."""
     _check([1600, 300, 257], [600, 1, 257], 2, 1, 128, 64, dtype, int8, shift=True)
     _check([700, 690], [700, 333], 3, 3, 72, 16, dtype, int8)
+
+
+@pytest.mark.parametrize("t", ROWS)
+def test_graphs_and_eager_calls_at_once(t):
+    """Two graphs and eager calls on a third stream, all cut into parts, beside `sageattn` on a fourth: each its own bits."""
+    calls = []
+    for seed, lens in enumerate(((5000, 30), (3100, 2900), (9000, 17))):
+        lens = tuple(max(n, t) for n in lens)
+        cache, table, q, lens_d, _ = _setup(lens, t, seed=seed, shift=seed == 1)
+        calls.append(lambda q=q, cache=cache, table=table, lens_d=lens_d: S.sageattn_cached(q, cache, table, lens_d, return_lse=True))
+    x = [torch.randn((1, 8, 2048, 128), device="cuda").half() for _ in range(3)]
+    calls.append(lambda: (S.sageattn(*x),))
+    want = [[y.clone() for y in call()] for call in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for call, st in zip(calls[:2], streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            outs.append(call())
+        graphs.append(graph)
+    got = [[], []]
+    for _ in range(10):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        for i in (2, 3):
+            with torch.cuda.stream(streams[i]):
+                got[i - 2].append(calls[i]())
+    torch.cuda.synchronize()
+    for res, first in [(outs[0], want[0]), (outs[1], want[1])] + [(g, want[2]) for g in got[0]] + [(g, want[3]) for g in got[1]]:
+        assert all(torch.equal(a, b) for a, b in zip(res, first))
