@@ -86,6 +86,30 @@ def test_gradients_at_any_offset():
     _rot_close(q.grad, _turned(g, pos, rotary, backward=True), g)
 
 
+def test_a_training_step_is_captured_and_replayed():
+    """Forward and backward in one graph, warmed up on its stream; replays follow what the inputs and positions hold by then."""
+    rotary = S.SageRotary(64, rotary_dim=48, scaling="parts", factor=4.0)
+    q, k = (torch.randn((13, h, 64), device="cuda").bfloat16().requires_grad_() for h in (4, 2))
+    pos, g = torch.arange(13, device="cuda"), [torch.randn((13, h, 64), device="cuda").bfloat16() for h in (4, 2)]
+    step = lambda: torch.autograd.grad(S.sage_rotary(q, k, pos, rotary), (q, k), g)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        grads = step()
+    for _ in range(2):
+        pos.add_(1000)
+        for x in g:
+            x.copy_(torch.randn_like(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, x in zip(grads, g):
+            _rot_close(got, _turned(x, pos, rotary, backward=True), x)
+
+
 # ---- writing -----------------------------------------------------------------------------------------------------
 
 def test_autograd_learns_of_writes_to_the_cache():
