@@ -406,10 +406,10 @@ int sage_cache_read(const void* k_codes, const float* k_scale, const void* v_cod
  * What a result depends on: the keys are walked in
  * stretches whose ends follow from the lengths of all sequences, so that the same sequence in another batch
  * may differ in the order of fp32 sums; the same call gives the same bits.
- * Limits: n_seq * Hkv * (groups of eight of the max_q * Hq / Hkv rows) * (runs of 32 keys of a page table row, and 4)
+ * Limits: n_seq up to 65535; n_seq * Hkv * (groups of eight of the max_q * Hq / Hkv rows) * (runs of 32 keys of a page table row, and 4)
  * below 2^31, else SAGE_E_UNSUPPORTED.
- *   workspace   sage_cache_attention_workspace_bytes() bytes (0: not a call that is taken), 256-byte aligned; calls that may run at the same
- *               time (on two streams, in two captured graphs) each need their own
+ *   workspace   sage_cache_attention_workspace_bytes() bytes (0: not a call that is taken), 256-byte aligned; calls
+ *               that may run at the same time (on two streams, in two captured graphs) each need their own
  *   status_host optional, as for sage_attention_reported: a pinned host word that receives a non-zero code when a
  *               bounded wait of the kernel ran out (the output is then undefined); never written otherwise */
 size_t sage_cache_attention_workspace_bytes(int64_t n_seq, int64_t Hq, int64_t Hkv, int64_t max_q);

@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(CACHE_THREADS) rotary_kernel(const RotaryKArgs
 // NaN and codes of 0, so that no code is ever a NaN: a key that a mask hides cannot reach a product.
 // Bound by HBM: 27 280 tokens x 48 heads 178 us = 5.7 TB/s (0.87 of a copy); 8771 x 8 heads 13 us = 4.2 TB/s, of which a
 // launch and the first loads are 4.  32-byte loads, as when reading back, took 198 us for the former.
+
 // Largest magnitude of sixteen packed values, NaN if one is.
 template <typename T>
 __device__ __forceinline__ float absmax16_nan(const uint4& u, const uint4& v) {

@@ -32,11 +32,12 @@
 // that lies in several stretches leaves partial rows in the workspace, which cache_combine_kernel joins in the
 // order of the keys.
 //
-// What bounds it.  The cache's bytes: 4 x 47 520 keys x 48 heads, 356 to 370 us = 6.6 TB/s, the rate of a plain copy.  32
-// ragged sequences of up to 8192 keys x 8 heads: 43 us = 4.5 TB/s; joining the parts, the launches and the two to three
-// units that a warp begins take the difference.  One sequence of 16 384 keys: 15 us, of which 6 are the cache's bytes and
-// the rest the chain launch, lengths, pages, codes, parts, join.  16 rows instead of 8 cost instructions (codes are unpacked
-// once for all rows of a tile): 8 x 16 384 keys x 8 heads 56 us with 8 rows, 63 with 16.
+// What bounds it.  The cache's bytes: 4 x 47 520 keys x 48 heads, 357 to 371 us in a graph = 6.5 to 6.7 TB/s, the rate of a
+// plain copy (called one by one with other inputs each time, 372 to 410 from GPU to GPU).  32 ragged sequences of up to 8192
+// keys x 8 heads: 43 us = 4.5 TB/s; joining the parts, the launches and the two to three units that a warp begins take the
+// difference.  One sequence of 16 384 keys: 15.5 us, of which 6 are the cache's bytes and the rest the chain launch, lengths,
+// pages, codes, parts, join.  16 rows instead of 8 cost instructions (codes are unpacked once for all rows of a tile): 8 x
+// 16 384 keys x 8 heads 54 us with 8 rows, 63 with 16.
 #include "sage_cache_attn.cuh"
 
 namespace sage {
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
 }
 
 constexpr int CTAS_PER_SM = 2;
-constexpr int SIZING_SMS = 160;                      // the workspace is sized without a device at hand, for the largest SM count an sm_100 part has
+constexpr int SIZING_SMS = 160;                      // largest SM count of an sm_100 part: the workspace is sized without a device at hand
 
 template <typename T, bool INT8, int WIDTH, int NB>
 cudaError_t launch_attn(CacheAttnKArgs& a, int sms, cudaStream_t st) {
@@ -582,10 +583,10 @@ cudaError_t launch_combine_t(const CacheAttnKArgs& a, int rows, int keys, int wi
   // All of a CTA on a row while the rows make eight CTAs an SM at most (few rows mean many parts each); a row per warp
   // beyond that, and four where even those are more: what a CTA does before its first row (it finds the unit's place in the
   // line, for which it reads every sequence's length) would be most of its time.  With the attention before it: 2048 units
-  // of 4 rows over 300 keys 62.7 us with a CTA per row, 33.7 with a warp; 32 units of 84 rows 36.0 us with one row per
-  // warp, 47.5 with four; 296 units of 256 rows 70.1 and 43.9.  Parts in flight: registers decide how many CTAs are on an SM
-  // (80 with eight, 56 with four): 32 ragged sequences 45.1 us with eight, 43.0 with four; 64 units of 256 rows 214.7
-  // and 210.1; but 32 units of 84 rows, ten parts each, 36.0 and 38.0.
+  // of 4 rows over 300 keys 74.0 us with a CTA per row, 48.5 with a row per warp, 46.7 with four; one unit of 4 rows over 16 384
+  // keys 15.5, 28.4 and 35.6; 32 units of 84 rows 37.0 us with a row per warp, 52.8 with four; 296 units of 256 rows 99.4 and
+  // 72.1.  Parts in flight: registers decide how many CTAs are on an SM (80 with eight, 56 with four): 32 ragged sequences 45.1 us
+  // with eight, 43.0 with four; 64 units of 256 rows 217.4 and 212.4; but 32 units of 84 rows, ten parts each, 37.0 and 38.9.
   constexpr unsigned long long ROOM = 8 * SIZING_SMS;
   if (!permuted && (unsigned long long)units * a.part_rows <= ROOM)
     return launch_after_predecessor(cache_combine_kernel<T, CC_WARPS, 4>, dim3(units, (unsigned)a.part_rows), dim3(CC_THREADS), 0, st, a, rows, keys, width,
@@ -602,13 +603,14 @@ cudaError_t launch_cache_combine(const CacheAttnKArgs& a, int dtype, int rows, i
   return dtype == 0 ? launch_combine_t<__half>(a, rows, keys, width, max_rt, st) : launch_combine_t<__nv_bfloat16>(a, rows, keys, width, max_rt, st);
 }
 
-// Which kernel, and rows of its row tiles.  All figures for 8 K/V heads; the first is with the form that is taken.
-//   8-row tiles up to 8 rows: a token of 4 query heads, 32 ragged sequences of up to 8192 keys, 45 us; with 16-row tiles 49.
+// Which kernel, and rows of its row tiles.  All figures for 8 K/V heads, in a graph; the first is with the form that is taken.
+//   8-row tiles up to 8 rows: a token of 4 query heads, 32 ragged sequences of up to 8192 keys, 42.5 us; with 16-row tiles
+//   47.5 (8 x 16384 keys, 8 rows: 53.5 and 57.4).
 //   16-row tiles of mma.sync up to 32 rows, whose keys are then read twice, but mostly from L2: 8 x 16384 keys, 32 rows,
-//   102 us, with tcgen05 141; 16 rows 63 and 139.  48 rows: 142 with tcgen05, 164 with three such tiles (4 x 8771 keys: 40
-//   and 30; long contexts, where more is at stake, decide).
-//   tcgen05, 128 rows and two CTAs an SM up to 128 rows: 8 x 16384 keys, 128 rows, 150 us, with the 256-row form 180; 84
-//   rows of 4 x 8771 keys 36 and 41.  256 rows and one CTA beyond: 160 rows 209 us, with 128-row tiles 274; 256 rows 214 and 282.
+//   107 us, with tcgen05 143; 16 rows 63 and 139.  48 rows: 144 with tcgen05, 151 with three such tiles (4 x 8771 keys: 41
+//   and 31; long contexts, where more is at stake, decide).
+//   tcgen05, 128 rows and two CTAs an SM up to 128 rows: 8 x 16384 keys, 128 rows, 153 us, with the 256-row form 179; 84
+//   rows of 4 x 8771 keys 37 and 43.  256 rows and one CTA beyond: 160 rows 210 us, with 128-row tiles 278; 256 rows 212 and 284.
 CacheForm cache_form(int64_t rows) {
   if (rows <= 32) return {false, rows <= 8 ? 8 : 16, CA_KEYS, SIZING_SMS * CTAS_PER_SM * CA_WARPS};
   return rows <= 128 ? CacheForm{true, 128, 64, 2 * SIZING_SMS} : CacheForm{true, 256, 64, SIZING_SMS};

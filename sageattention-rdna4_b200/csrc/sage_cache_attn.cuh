@@ -15,7 +15,7 @@ constexpr float NO_MAX = -3.0e38f;
 // passes 2^LIMIT_LOG2 (fp16 ends below 2^16): a weight keeps its 11 bits down to 2^-18 of the largest and is lost below 2^-29 of
 // it.  At 2^0 that was 2^-25: 262 144 keys at 2^-25.2 of a first one, 6.8e-3 of the output.  The room above keeps rows from being
 // scaled anew with every new maximum: 8 x 16 384 keys, some of them four times as large as the others, 256 rows: 204.8 us at
-// 2^0, 211.2 at 2^4, 214.5 at 2^6, 217 at 2^8; 32 rows 105.6, 108, 110.5, 109.6.  Beyond 2^4 nothing is to be had: the fp32
+// 2^0, 211.2 at 2^4, 214.5 at 2^6, 217 at 2^8; 32 rows 105, 107, 110.5, 109.6.  Beyond 2^4 nothing is to be had: the fp32
 // accumulators lose up to 2^-23 of the sum per 16 keys, more than this.
 constexpr int TOP_LOG2 = 4, LIMIT_LOG2 = 15;
 
@@ -55,13 +55,15 @@ __device__ __forceinline__ Seq seq_of(const CacheAttnKArgs& a, int b) {
   return s;
 }
 __device__ __forceinline__ int row_tiles(const CacheAttnKArgs& a, const Seq& s, int rows) { return (s.q_len * a.group + rows - 1) / rows; }
-__device__ __forceinline__ int key_steps(const Seq& s, int keys) { return max(1, (s.len + keys - 1) / keys); }   // an empty sequence's rows are written too
+// (an empty sequence's rows are written too)
+__device__ __forceinline__ int key_steps(const Seq& s, int keys) { return max(1, (s.len + keys - 1) / keys); }
 
 // The line of steps (of so many keys each): sequence by sequence, K/V head by K/V head, row tile by row tile (of so many
 // rows each), step by step, and behind every unit UNIT_STEPS more places that stand for what a unit costs beyond its keys
 // (fetching Q, writing the rows): without them a stretch through many short sequences takes several times as long as one
-// through a long one (32 ragged sequences of up to 8192 keys, a token each: 56 us without them, 45 with).  Fewer than 2^31 places, the host sees to that.  Its stretches differ by one place at most; a line
-// of fewer places than stretches wanted leaves the last ones out.
+// through a long one (32 ragged sequences of up to 8192 keys, a token each: 56 us without them, 45 with them at the time).
+// There are fewer than 2^31 places, the host sees to that.  The line's stretches differ by one place at most; a line of
+// fewer places than stretches wanted leaves the last ones out.
 constexpr int UNIT_STEPS = 4;
 struct Line {
   unsigned total, n, per, longer;                    // places, stretches, places of a stretch, stretches that have one more

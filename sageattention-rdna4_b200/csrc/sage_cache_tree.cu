@@ -24,13 +24,15 @@
 // NQ = 2 (rows beyond 128): one CTA per SM with all 512 TMEM columns.  NQ = 1: two CTAs per SM.  (Rows are added to a
 // CTA before CTAs are: a tile's codes are fetched and converted once per CTA.  Figures of both: cache_form.)
 //
-// What bounds it.  8 x 16 384 keys x 8 heads, 256 rows: 206 us = 665 TFLOP/s, 0.40 of the rate of a large 16-bit product;
-// a tile of 64 keys takes about 3000 cycles of an SM, and no part of it alone decides: the tensor pipe is busy a third
-// of them, MUFU a third, half of the issue slots are used, and shared memory serves threads in 43 % and the tensor pipe in 39 %.
-// Without the softmax's arithmetic it would have been 173 us of 213, without fetching and converting the codes 195, without either's
-// work and one product per tile 108.  Twice the softmax warps (half the keys of a row each), or separate warps for K and V,
-// or separate threads for the two products, or a row's scores spread over four lanes (fewer reads of scales): 211 to 231.
-// 4 x 8771 keys, 84 rows: 36 us for 3.9 us of bytes; the same cycles for tiles that are two thirds full.
+// What bounds it.  8 x 16 384 keys x 8 heads, 256 rows: 212 us in a graph = 646 TFLOP/s, 0.39 of the rate of a large 16-bit
+// product; a chain of 512 new tokens, 2048 rows: 1512 us = 716.  A tile of 64 keys takes about 3000 cycles of an SM, and no part
+// of it alone decides: the tensor pipe is busy a third of them, MUFU a third, half of the issue slots are used, and shared
+// memory serves threads in 43 % and the tensor pipe in 39 %.  When it took 213 us, it would have been 173 without the softmax's
+// arithmetic, 195 without fetching and converting the codes, 108 without either's work and one product per tile; twice the
+// softmax warps (half the keys of a row each), separate warps for K and V, separate threads for the two products, or
+// a row's scores spread over four lanes (fewer reads of scales) took 211 to 231.  The issuing warps spill: 372 bytes of stores
+// and 224 of loads per thread at width 128 (472 and 284 at 64), the 128-row form 428 to 440 and 312 to 372.
+// 4 x 8771 keys, 84 rows: 37 us for 3.9 us of bytes; the same cycles for tiles that are two thirds full.
 //
 // Every wait is bounded (about a second): it then leaves a code in the caller's pinned host word, the CTA drains
 // its products, frees its TMEM and returns.
@@ -160,7 +162,7 @@ template <int WIDTH, int NQ> struct TreeShape {
   static constexpr int REGS_LAUNCH = NQ == 1 ? 80 : 128, REGS_SOFTMAX = NQ == 1 ? 120 : 168, REGS_LOADER = NQ == 1 ? 72 : 112,
                        REGS_ISSUER = NQ == 1 ? 48 : 64;
   static_assert(NQ * REGS_SOFTMAX + REGS_LOADER + REGS_ISSUER <= (NQ + 2) * REGS_LAUNCH, "setmaxnreg would wait forever");
-  // Stages of K and V as operands, and of codes as they come: a ring of four for NQ = 2 (213 us; codes held in registers a
+  // Stages of K and V as operands, and of codes as they come: a ring of four for NQ = 2 (213 us at the time; codes held in registers a
   // tile ahead 243), none for NQ = 1, whose two CTAs share the memory: codes come through registers and leave room for two
   // stages of operands (8 x 16 384 keys, 128 rows: 150 us; with a ring and one stage 181).  Slots of scales: one is written
   // once the scores STAGES tiles back are complete, which means that the softmax is done with the tile two before that.
@@ -250,7 +252,9 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
     const int g = warp >> 2, r = tid & 127;
     const uint32_t lane_sel = (uint32_t)(warp & 3) << 21;                             // 32 lanes of TMEM per warp
     const uint32_t o_addr = tmem_o(g) + lane_sel;
-    float* row_at = reinterpret_cast<float*>(gbase + L::OFF_ROW) + 256 * g;           // of row r: [r] what undoes its power of two (read once; a NaN from then on: the row sees one in V alone), [128 + r] its product with the shift
+    // Of row r: [r] what undoes its power of two (read once; a NaN from then on: the row sees one in V alone), [128 + r] its
+    // product with the shift.
+    float* row_at = reinterpret_cast<float*>(gbase + L::OFF_ROW) + 256 * g;
     // Rows of 2 * WIDTH bytes in this half's Q tile: piece c of row r, where Q goes and outputs pass through.
     uint8_t* q_tile = gbase + L::OFF_Q + g * L::Q_TILE;
     auto staged = [&](int row, int c) { return reinterpret_cast<uint4*>(q_tile + (c >> 3) * L::Q_HALF + row * 128 + 16 * ((c & 7) ^ (row & 7))); };
@@ -639,7 +643,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
       }
       copy_wait<0>();                                // (a wait that gave up leaves none of its own copies in flight)
     } else {
-      int pages[N_CHUNK], s_page = -1;               // of tile `ahead`: the page of each chunk's row, and of the key whose scales this thread fetches
+      // of tile `ahead`: the page of each chunk's row, and of the key whose scales this thread fetches
+      int pages[N_CHUNK], s_page = -1;
       auto page_of = [&](int key) -> int { return key < ahead.s.len ? __ldg(a.table + ahead.b * a.table_st + (key >> a.page_shift)) : -1; };
       auto fetch_pages = [&]() {
 #pragma unroll
