@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "sageattention", "libsage_b200.so")
 SOURCES = ["sage_capi.cu", "sage_prologue.cu", "sage_attn_sm100.cu", "sage_cache.cu", "sage_cache_attn.cu", "sage_cache_tree.cu"]
-HEADERS = ["sage_common.cuh", "sage_internal.h", "sage_cache_attn.cuh", os.path.join("..", "..", "include", "sage_b200.h")]
+HEADERS = ["sage_common.cuh", "sage_internal.h", "sage_ptx.cuh", "sage_cache_attn.cuh", os.path.join("..", "..", "include", "sage_b200.h")]
 
 
 def nvcc_path() -> str:

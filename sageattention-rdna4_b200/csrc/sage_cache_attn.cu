@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
   enter_line(a, cur, line.begin(stretch), line.begin(stretch + 1), before, ROWS, CA_KEYS);
   if (cur.left <= 0) return;
   Cursor ahead = cur;                                // the step whose loads are issued next
-  const uint32_t ring = smem_addr(smem) + warp * STAGES * L::STAGE;
+  const uint32_t ring = smem_u32(smem) + warp * STAGES * L::STAGE;
 
   // The 32 keys of the step at `ahead` into stage s.  Lane l copies piece l % PIECES of rows l / PIECES + i * RPI;
   // (row & 7) of the swizzle is that of the lane's first row, but for a change of one bit in every other copy.
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
       for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[blk][e] = fast_ex2(fmaf(s[blk][nb][e], row_c[nb][e & 1], -m[nb][e & 1]));
+          p[blk][e] = ex2(fmaf(s[blk][nb][e], row_c[nb][e & 1], -m[nb][e & 1]));
           w[blk][e] = p[blk][e] * (sv[blk][e >> 1] * nf[nb][e & 1]);
           p_top = fmaxf(p_top, p[blk][e]);
           w_top = fmaxf(w_top, w[blk][e]);
@@ -308,11 +308,11 @@ __global__ void __launch_bounds__(CA_THREADS, CTAS_PER_SM) cache_attn_kernel(con
           for (int sh = 4; sh < 32; sh <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, sh));
           if (!(top > m[nb][x] + LIMIT_LOG2 || big > LIMIT)) top = m[nb][x];
           const bool move = top != m[nb][x] || big > LIMIT;
-          const float fade = fast_ex2(m[nb][x] - top);
+          const float fade = ex2(m[nb][x] - top);
           big = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float v = fast_ex2(fmaf(s[i >> 1][nb][2 * (i & 1) + x], row_c[nb][x], -top));
+            const float v = ex2(fmaf(s[i >> 1][nb][2 * (i & 1) + x], row_c[nb][x], -top));
             p[i >> 1][2 * (i & 1) + x] = v;
             if (s[i >> 1][nb][2 * (i & 1) + x] != -INFINITY) big = fmaxf(big, v * sv[i >> 1][i & 1]);
           }
@@ -503,12 +503,12 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
       float up = top;
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j) up = fmaxf(up, ml[j].x);
-      const float fade = fast_ex2(top - up);
+      const float fade = ex2(top - up);
       acc.x *= fade; acc.y *= fade; acc.z *= fade; acc.w *= fade; sum *= fade;
       top = up;
 #pragma unroll
       for (int j = 0; j < AT_ONCE; ++j) {
-        const float weight = fast_ex2(ml[j].x - top);
+        const float weight = ex2(ml[j].x - top);
         sum = fmaf(ml[j].y, weight, sum);
         acc.x = fmaf(v[j].x, weight, acc.x); acc.y = fmaf(v[j].y, weight, acc.y); acc.z = fmaf(v[j].z, weight, acc.z); acc.w = fmaf(v[j].w, weight, acc.w);
       }
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(CC_THREADS) cache_combine_kernel(const CacheAt
 #pragma unroll
       for (int w = 0; w < CC_WARPS; ++w) top = fmaxf(top, ml_s[w].x);
 #pragma unroll
-      for (int w = 0; w < CC_WARPS; ++w) { weight[w] = fast_ex2(ml_s[w].x - top); sum = fmaf(ml_s[w].y, weight[w], sum); }
+      for (int w = 0; w < CC_WARPS; ++w) { weight[w] = ex2(ml_s[w].x - top); sum = fmaf(ml_s[w].y, weight[w], sum); }
       const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
       if (tid < a.D) {
         float v = 0.f;

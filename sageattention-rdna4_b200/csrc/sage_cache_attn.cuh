@@ -6,6 +6,7 @@
 
 #include "sage_common.cuh"
 #include "sage_internal.h"
+#include "sage_ptx.cuh"
 
 namespace sage {
 
@@ -194,12 +195,6 @@ __device__ __forceinline__ void add_carrying(float& sum, float& carry, float x) 
   carry = (t - sum) - y;
   sum = t;
 }
-__device__ __forceinline__ float fast_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   const int bytes = there ? 16 : 0;                  // 0: filled with zeros, nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");

@@ -42,9 +42,6 @@ namespace sage {
 
 namespace {
 
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -91,12 +88,6 @@ __device__ __forceinline__ void drain_wait(uint32_t bar, const Watch& w, int cod
 }
 enum { CODE_LOAD = 1, CODE_MMA = 2, CODE_SOFTMAX = 4 };   // the bits of the framework's status words
 
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Descriptors of operands in shared memory have the same upper word throughout (rows of 128 bytes, swizzled, eight of
 // them 1024 bytes apart); of the lower one the address moves, by constants within a tile.
 constexpr uint32_t DESC_HIGH = (1024u >> 4) | (1u << 14) | (2u << 29);
@@ -122,22 +113,15 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
       ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr) : "memory");
 }
-__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ void sts_f32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
 
 // Descriptors of 128-byte rows in the 128-byte swizzle, 8-row groups 1024 bytes apart: as a K-major operand, and as
 // an MN-major one whose next 64 columns lie `lead` bytes further.
@@ -215,8 +199,8 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
   enter_line(a, cur, line.begin(blockIdx.x), line.begin(blockIdx.x + 1), before, ROWS, KT);
   if (cur.left <= 0) return;
 
-  const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u, bar0 = base + L::OFF_BAR;
-  uint8_t* gbase = smem_raw + (base - smem_addr(smem_raw));
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, bar0 = base + L::OFF_BAR;
+  uint8_t* gbase = smem_raw + (base - smem_u32(smem_raw));
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(gbase + L::OFF_MISC);   // [0] TMEM address, [1] abort
   const Watch watch = {misc + 1, status_host};
   auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
@@ -404,7 +388,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
           if (__any_sync(0xffffffffu, top > m + LIMIT_LOG2)) {
             // the maximum moves; the sum and the accumulator follow
             top = top > m + LIMIT_LOG2 ? top - TOP_LOG2 : m;           // (each row by itself)
-            const float fade = fast_ex2(m - top);
+            const float fade = ex2(m - top);
             m = top;
             l *= fade;
             l_carry *= fade;
@@ -434,7 +418,7 @@ cache_tree_kernel(const CacheAttnKArgs a, int32_t* status_host) {
               const float4 lv = lv4[j], rv = rv4[j];
               const float2 u = __ffma2_rn(x2[2 * j], c2, __fadd2_rn(make_float2(lv.x, lv.y), nm2));
               const float2 v = __ffma2_rn(x2[2 * j + 1], c2, __fadd2_rn(make_float2(lv.z, lv.w), nm2));
-              const float2 w = make_float2(fast_ex2(u.x), fast_ex2(u.y)), z = make_float2(fast_ex2(v.x), fast_ex2(v.y));
+              const float2 w = make_float2(ex2(u.x), ex2(u.y)), z = make_float2(ex2(v.x), ex2(v.y));
               l2 = __ffma2_rn(w, make_float2(rv.x, rv.y), l2);
               l2 = __ffma2_rn(z, make_float2(rv.z, rv.w), l2);
               pw[2 * i] = pack2<__half>(w.x, w.y);
